@@ -1,0 +1,430 @@
+// Attention over packed sequences with grouped heads (fh_attention_packed_fwd) and its gradients (fh_attention_packed_grad).
+// Forward: attention_rows_kernel of fh_attention_rows.h over dense keys and values.
+//
+// Gradients, with D = sum_d dout out, p = exp(scale q.k - lse), dp = dout.v, ds = p (dp - D):
+//   dq = scale sum_u ds k_u,  dk = scale sum_r ds q_r,  dv = sum_r p dout_r,
+// the sums over r running over the rows of every head of the group. Two kernels, each forming p and dp again from q, k, v and
+// dout (7 products instead of the 5 that one kernel with atomic sums of dq would need), so that every sum has one owner and one
+// order: results do not depend on scheduling, and no fp32 copy of dq is needed.
+//   attention_dq_kernel:  32 rows per wave as in the forward; D is formed from its rows and kept for the second kernel.
+//   attention_dkv_kernel: 32 keys per wave, keys and values in registers, blocks of 32 rows of q and dout in LDS.
+// p and ds are rounded to the storage type as operands of the second products; everything else is fp32.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "fh_attention_rows.h"
+
+namespace fh {
+namespace {
+
+using namespace attn;
+
+struct GradArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* out;
+  const uint16_t* dout;
+  uint16_t* dq;
+  uint16_t* dk;
+  uint16_t* dv;
+  const float* lse;
+  float* delta;  // [tokens, heads]
+  const int32_t* cu;
+  int64_t ldq, ldk, ldv, ldo;
+  int tokens, batch, heads, kv_heads, dh;
+  Divider group;
+  int causal;
+  float scale;
+  int slots;
+};
+
+template <typename T, int DH, int W>
+__global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs a) {
+  constexpr int BYTES = kBlock * DH * 2;
+  constexpr int ROWS = 32 * W, SHIFT = __builtin_ctz(ROWS);
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int slot = a.slots - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
+  const int group = static_cast<int>(a.group.d);
+  int first_slot = 0;
+  const int b = find_sequence(a.cu, a.batch, a.tokens, group, SHIFT, slot, first_slot);
+  if (b < 0) return;
+  const Span seq = sequence(a.cu, b, a.tokens);
+  const int keys = seq.end - seq.begin, rows = keys * group;
+  const int tile0 = (slot - first_slot) * ROWS;
+  if (tile0 >= rows) return;
+  auto limit = [&](int r) { return a.causal ? divide(min(r, rows - 1), a.group) : keys - 1; };
+  const int kend = limit(tile0 + ROWS - 1) + 1;
+
+  const int r0 = tile0 + wave * 32, r = r0 + l32;
+  const bool live = r < rows;
+  const int lim = limit(r), lim_low = limit(r0), lim_high = limit(r0 + 31);
+  const int token = divide(min(r, rows - 1), a.group);
+  const int head = kv_head * group + (min(r, rows - 1) - token * group);
+  const int64_t trow = seq.begin + token;
+
+  u32x4_t qf[DH / 16], gf[DH / 16];
+  float delta = 0.0f;
+  {
+    const uint16_t* qr = a.q + trow * a.ldq + static_cast<int64_t>(head) * a.dh;
+    const int64_t oat = trow * a.ldo + static_cast<int64_t>(head) * a.dh;
+#pragma unroll
+    for (int s = 0; s < DH / 16; ++s) {
+      const int d = 16 * s + 8 * hi;
+      const bool ok = live && d < a.dh;
+      qf[s] = load_chunk(qr + d, ok);
+      gf[s] = load_chunk(a.dout + oat + d, ok);
+      const u32x4_t ov = load_chunk(a.out + oat + d, ok);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        delta = __builtin_fmaf(load_lo<T>(gf[s][j]), load_lo<T>(ov[j]), delta);
+        delta = __builtin_fmaf(load_hi<T>(gf[s][j]), load_hi<T>(ov[j]), delta);
+      }
+    }
+  }
+  delta = half_sum(delta);
+  const int64_t stat = trow * a.heads + head;
+  if (live && hi == 0) a.delta[stat] = delta;
+  const float lse2 = live ? a.lse[stat] * kLog2e : 0.0f;
+  const float c = a.scale * kLog2e;
+
+  f32x16_t acc[DH / 32];
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt) clear(acc[dt]);
+
+  // keys and values as the forward stages them
+  RowsArgs kv{};
+  kv.k = a.k;
+  kv.v = a.v;
+  kv.ldk = a.ldk;
+  kv.ldv = a.ldv;
+  kv.dh = a.dh;
+  KvStage<T, DH, kDense, W * 64> stage;
+  const TileReader<DH> tiles(lds, lane);
+  stage.load(kv, seq.begin, nullptr, kv_head, 0, kend, tid);
+  stage.store(lds, lds + BYTES, tid);
+  __syncthreads();
+  int buf = 0;
+  for (int kb = 0; kb < kend; kb += kBlock) {
+    const bool more = kb + kBlock < kend;
+    if (more) stage.load(kv, seq.begin, nullptr, kv_head, kb + kBlock, kend, tid);
+    if (kb <= lim_high) {
+      const int kbuf = buf * 2 * BYTES, vbuf = kbuf + BYTES;
+      const bool edge = kb + kBlock - 1 > lim_low;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x16_t s, dp;
+        clear(s);
+        clear(dp);
+#pragma unroll
+        for (int i = 0; i < DH / 16; ++i) {
+          mfma32<T>(tiles.rows(kbuf, 32 * t, i), qf[i], s);
+          mfma32<T>(tiles.rows(vbuf, 32 * t, i), gf[i], dp);
+        }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -lse2));
+          s[x] = p * (dp[x] - delta);
+        }
+        if (edge) {
+#pragma unroll
+          for (int x = 0; x < 16; ++x) s[x] = kb + 32 * t + result_row(x, hi) <= lim ? s[x] : 0.0f;
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const u32x4_t ds = pack_slice<T>(s, hf);
+#pragma unroll
+          for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(tiles.columns(kbuf, 32 * t + 16 * hf, dt), ds, acc[dt]);
+        }
+      }
+    }
+    if (more) {
+      unsigned char* next = lds + (buf ^ 1) * 2 * BYTES;
+      stage.store(next, next + BYTES, tid);
+    }
+    __syncthreads();
+    buf ^= 1;
+  }
+  if (live) store_row<T, DH>(a.dq + trow * a.ldq + static_cast<int64_t>(head) * a.dh, acc, a.scale, hi, a.dh);
+}
+
+constexpr int kGradRows = 32;  // rows of q and dout per block
+
+template <typename T, int DH, int W>
+__global__ __launch_bounds__(W * 64, 1) void attention_dkv_kernel(const GradArgs a) {
+  constexpr int BYTES = kGradRows * DH * 2;
+  constexpr int KEYS = 32 * W, SHIFT = __builtin_ctz(KEYS);
+  constexpr int CH = DH / 8, PASS = W * 64 / CH, N = (kGradRows + PASS - 1) / PASS;
+  static_assert(kGradRows % PASS == 0, "whole passes");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
+  __shared__ float stats[2][2][kGradRows];  // per buffer: lse (base 2), D
+
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int slot = static_cast<int>(blockIdx.x) / a.kv_heads;  // a causal sequence's first keys are seen by most rows
+  const int group = static_cast<int>(a.group.d);
+  int first_slot = 0;
+  const int b = find_sequence(a.cu, a.batch, a.tokens, 1, SHIFT, slot, first_slot);
+  if (b < 0) return;
+  const Span seq = sequence(a.cu, b, a.tokens);
+  const int keys = seq.end - seq.begin, rows = keys * group;
+  const int tile0 = (slot - first_slot) * KEYS;
+  if (tile0 >= keys) return;
+
+  const int k0 = tile0 + wave * 32, key = k0 + l32;
+  const bool live = key < keys;
+  const int64_t krow = seq.begin + (live ? key : 0);
+  const int64_t col = static_cast<int64_t>(kv_head) * a.dh;
+  u32x4_t kf[DH / 16], vf[DH / 16];
+#pragma unroll
+  for (int s = 0; s < DH / 16; ++s) {
+    const int d = 16 * s + 8 * hi;
+    kf[s] = load_chunk(a.k + krow * a.ldk + col + d, live && d < a.dh);
+    vf[s] = load_chunk(a.v + krow * a.ldv + col + d, live && d < a.dh);
+  }
+  // rows that see key u: r >= u * group (causal)
+  const int rbegin = a.causal ? tile0 * group / kGradRows * kGradRows : 0;
+  const int my_first = a.causal ? key * group : 0;
+
+  const int chunk = tid % CH, srow = tid / CH;
+  const bool inside = chunk * 8 < a.dh;
+  u32x4_t qs[N], gs[N];
+  float stat = 0.0f;
+  auto load = [&](int rb) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = rb + srow + n * PASS;
+      const int token = divide(min(r, rows - 1), a.group);
+      const int head = kv_head * group + (min(r, rows - 1) - token * group);
+      const int64_t trow = seq.begin + token;
+      const int64_t c0 = static_cast<int64_t>(head) * a.dh + chunk * 8;
+      qs[n] = load_chunk(a.q + trow * a.ldq + c0, inside && r < rows);
+      gs[n] = load_chunk(a.dout + trow * a.ldo + c0, inside && r < rows);
+    }
+    if (tid < 2 * kGradRows) {
+      const int r = rb + (tid & (kGradRows - 1));
+      stat = 0.0f;
+      if (r < rows) {
+        const int token = divide(r, a.group);
+        const int64_t at = (seq.begin + token) * static_cast<int64_t>(a.heads) + kv_head * group + (r - token * group);
+        stat = tid < kGradRows ? a.lse[at] * kLog2e : a.delta[at];
+      }
+    }
+  };
+  auto store = [&](int buf) {
+    unsigned char* qb = lds + buf * 2 * BYTES;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int at = tile_at<DH>(srow + n * PASS, chunk);
+      *reinterpret_cast<u32x4_t*>(qb + at) = qs[n];
+      *reinterpret_cast<u32x4_t*>(qb + BYTES + at) = gs[n];
+    }
+    if (tid < 2 * kGradRows) stats[buf][tid / kGradRows][tid & (kGradRows - 1)] = stat;
+  };
+
+  f32x16_t dk[DH / 32], dv[DH / 32];
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt) {
+    clear(dk[dt]);
+    clear(dv[dt]);
+  }
+  const float c = a.scale * kLog2e;
+  const TileReader<DH> tiles(lds, lane);
+  load(rbegin);
+  store(0);
+  __syncthreads();
+  int buf = 0;
+  for (int rb = rbegin; rb < rows; rb += kGradRows) {
+    const bool more = rb + kGradRows < rows;
+    if (more) load(rb + kGradRows);
+    // the wave's first key is seen from row k0 * group on
+    if (!a.causal || rb + kGradRows > k0 * group) {
+      const int qbuf = buf * 2 * BYTES, gbuf = qbuf + BYTES;
+      f32x16_t s, dp;
+      clear(s);
+      clear(dp);
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i) {
+        mfma32<T>(tiles.rows(qbuf, 0, i), kf[i], s);
+        mfma32<T>(tiles.rows(gbuf, 0, i), vf[i], dp);
+      }
+      const bool edge = a.causal && rb < (k0 + 31) * group;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 ls = *reinterpret_cast<const float4*>(&stats[buf][0][8 * q + 4 * hi]);
+        const float4 dl = *reinterpret_cast<const float4*>(&stats[buf][1][8 * q + 4 * hi]);
+        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dd[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int x = 4 * q + j;
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -lv[j]));
+          float d = p * (dp[x] - dd[j]);
+          if (edge) {
+            const bool seen = rb + result_row(x, hi) >= my_first;
+            p = seen ? p : 0.0f;
+            d = seen ? d : 0.0f;
+          }
+          s[x] = p;
+          dp[x] = d;
+        }
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const u32x4_t p = pack_slice<T>(s, hf), ds = pack_slice<T>(dp, hf);
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt) {
+          mfma32<T>(tiles.columns(gbuf, 16 * hf, dt), p, dv[dt]);
+          mfma32<T>(tiles.columns(qbuf, 16 * hf, dt), ds, dk[dt]);
+        }
+      }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  }
+  if (live) {
+    store_row<T, DH>(a.dk + krow * a.ldk + col, dk, a.scale, hi, a.dh);
+    store_row<T, DH>(a.dv + krow * a.ldv + col, dv, 1.0f, hi, a.dh);
+  }
+}
+
+fh_status check_packed(const char* fn, const fh_packed_attention* g) {
+  const std::string f(fn);
+  if (g == nullptr) return fail(FH_INVALID_ARGUMENT, f + ": null descriptor");
+  if (g->dtype != FH_BF16 && g->dtype != FH_F16) return fail(FH_UNIMPLEMENTED, f + ": needs bf16 or f16");
+  if (g->dh < 8 || g->dh > 128 || g->dh % 8 != 0) return fail(FH_UNIMPLEMENTED, f + ": head dim must be a multiple of 8 up to 128");
+  if (g->tokens < 0 || g->batch < 0) return fail(FH_INVALID_ARGUMENT, f + ": negative tokens or batch");
+  if (g->heads < 1 || g->kv_heads < 1 || g->heads % g->kv_heads != 0)
+    return fail(FH_INVALID_ARGUMENT, f + ": heads must be a multiple of kv_heads");
+  if (g->causal != 0 && g->causal != 1) return fail(FH_INVALID_ARGUMENT, f + ": causal must be 0 or 1");
+  if (!(g->scale > 0.0f) || !std::isfinite(g->scale)) return fail(FH_INVALID_ARGUMENT, f + ": scale must be positive and finite");
+  if (g->heads > 65535 || g->tokens > 0x7fffffff || g->batch > 0x3fffffff ||
+      (g->tokens + 256) * g->heads + g->batch * g->kv_heads > 0x7fffffff)
+    return fail(FH_INVALID_ARGUMENT, f + ": more than 2^31 rows (tokens x heads)");
+  if (g->q_stride < g->heads * g->dh || g->out_stride < g->heads * g->dh || g->k_stride < g->kv_heads * g->dh ||
+      g->v_stride < g->kv_heads * g->dh)
+    return fail(FH_INVALID_ARGUMENT, f + ": a row stride is shorter than its row");
+  if ((g->q_stride | g->k_stride | g->v_stride | g->out_stride) % 8 != 0)
+    return fail(FH_INVALID_ARGUMENT, f + ": row strides must be multiples of 8 elements");
+  return FH_OK;
+}
+
+// workgroups of `tile`-row tiles with per_token rows a token
+int64_t slots_for(const fh_packed_attention& g, int64_t per_token, int64_t tile) { return g.tokens * per_token / tile + g.batch; }
+
+}  // namespace
+}  // namespace fh
+
+using namespace fh;
+
+extern "C" fh_status fh_attention_packed_fwd(const fh_packed_attention* g, const void* q, const void* k, const void* v,
+                                             const int32_t* cu_seqlens, void* out, float* lse, void* stream) {
+  const char* fn = "fh_attention_packed_fwd";
+  if (fh_status st = check_packed(fn, g); st != FH_OK) return st;
+  if (g->tokens == 0 || g->batch == 0) return FH_OK;
+  if (!q || !k || !v || !out || !cu_seqlens) return fail(FH_INVALID_ARGUMENT, std::string(fn) + ": null pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return fail(FH_INVALID_ARGUMENT, std::string(fn) + ": q, k, v and out must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(cu_seqlens) | reinterpret_cast<uintptr_t>(lse)) % 4 != 0)
+    return fail(FH_INVALID_ARGUMENT, std::string(fn) + ": cu_seqlens and lse must be 4-byte aligned");
+  RowsArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.ldq = g->q_stride;
+  a.ldo = g->out_stride;
+  a.cu = cu_seqlens;
+  a.tokens = static_cast<int>(g->tokens);
+  a.batch = static_cast<int>(g->batch);
+  a.heads = static_cast<int>(g->heads);
+  a.kv_heads = static_cast<int>(g->kv_heads);
+  a.dh = static_cast<int>(g->dh);
+  a.group = make_divider(static_cast<uint32_t>(g->heads / g->kv_heads));
+  a.causal = g->causal;
+  a.scale = g->scale;
+  a.splits = 1;
+  a.k = k;
+  a.v = v;
+  a.ldk = g->k_stride;
+  a.ldv = g->v_stride;
+  constexpr int W = 4;
+  a.slots = static_cast<int>(slots_for(*g, a.group.d, 32 * W));
+  const dim3 grid(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads));
+  auto launch = [&]<typename T, int DH>() {
+    hipLaunchKernelGGL((attention_rows_kernel<T, DH, kDense, W>), grid, dim3(W * 64), 0, static_cast<hipStream_t>(stream), a);
+  };
+  if (g->dtype == FH_BF16) {
+    if (g->dh <= 64) launch.template operator()<bf16_t, 64>(); else launch.template operator()<bf16_t, 128>();
+  } else {
+    if (g->dh <= 64) launch.template operator()<f16_t, 64>(); else launch.template operator()<f16_t, 128>();
+  }
+  return launch_status("attention_rows_kernel launch");
+}
+
+extern "C" int64_t fh_attention_packed_grad_workspace(const fh_packed_attention* g) {
+  if (check_packed("fh_attention_packed_grad_workspace", g) != FH_OK) return -1;
+  return g->tokens * g->heads * 4;
+}
+
+extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, const void* q, const void* k, const void* v,
+                                              const int32_t* cu_seqlens, const void* out, const float* lse, const void* dout,
+                                              void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes,
+                                              void* stream) {
+  const std::string fn = "fh_attention_packed_grad";
+  if (fh_status st = check_packed(fn.c_str(), g); st != FH_OK) return st;
+  if (g->tokens == 0 || g->batch == 0) return FH_OK;
+  if (!q || !k || !v || !cu_seqlens || !out || !lse || !dout || !dq || !dk || !dv || !workspace)
+    return fail(FH_INVALID_ARGUMENT, fn + ": null pointer");
+  for (const void* p : {q, k, v, out, dout, static_cast<const void*>(dq), static_cast<const void*>(dk),
+                        static_cast<const void*>(dv), static_cast<const void*>(workspace)})
+    if (!aligned16(p)) return fail(FH_INVALID_ARGUMENT, fn + ": tensors and the workspace must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(cu_seqlens) | reinterpret_cast<uintptr_t>(lse)) % 4 != 0)
+    return fail(FH_INVALID_ARGUMENT, fn + ": cu_seqlens and lse must be 4-byte aligned");
+  if (workspace_bytes < fh_attention_packed_grad_workspace(g)) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
+  GradArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<const uint16_t*>(out);
+  a.dout = static_cast<const uint16_t*>(dout);
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  a.lse = lse;
+  a.delta = static_cast<float*>(workspace);
+  a.cu = cu_seqlens;
+  a.ldq = g->q_stride;
+  a.ldk = g->k_stride;
+  a.ldv = g->v_stride;
+  a.ldo = g->out_stride;
+  a.tokens = static_cast<int>(g->tokens);
+  a.batch = static_cast<int>(g->batch);
+  a.heads = static_cast<int>(g->heads);
+  a.kv_heads = static_cast<int>(g->kv_heads);
+  a.dh = static_cast<int>(g->dh);
+  a.group = make_divider(static_cast<uint32_t>(g->heads / g->kv_heads));
+  a.causal = g->causal;
+  a.scale = g->scale;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  constexpr int W = 4;
+  auto launch = [&]<typename T, int DH>() {
+    a.slots = static_cast<int>(slots_for(*g, a.group.d, 32 * W));
+    hipLaunchKernelGGL((attention_dq_kernel<T, DH, W>), dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads)),
+                       dim3(W * 64), 0, s, a);
+    if (fh_status st = launch_status("attention_dq_kernel launch"); st != FH_OK) return st;
+    a.slots = static_cast<int>(slots_for(*g, 1, 32 * W));
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DH, W>), dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads)),
+                       dim3(W * 64), 0, s, a);
+    return launch_status("attention_dkv_kernel launch");
+  };
+  if (g->dtype == FH_BF16)
+    return g->dh <= 64 ? launch.template operator()<bf16_t, 64>() : launch.template operator()<bf16_t, 128>();
+  return g->dh <= 64 ? launch.template operator()<f16_t, 64>() : launch.template operator()<f16_t, 128>();
+}

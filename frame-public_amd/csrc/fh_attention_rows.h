@@ -1,0 +1,339 @@
+// Attention of packed query rows over keys and values that are packed rows themselves (kDense), or rows of a paged cache in 16 bits
+// (kPaged) or e4m3 (kE4m3). For row r of a sequence with last visible key lim(r):
+//   s_u = scale q . k_u (u <= lim),  m = max s,  l = sum exp(s - m),  out = sum exp(s - m) v / l,  lse = m + log l
+// in one pass over blocks of 64 keys with a running m and l (fp32, base 2). A wave owns 32 rows; its workgroup's W waves share the
+// blocks in LDS, two buffers, the next block on its way in registers while this one is used. Scores are formed transposed
+// (K Q^T), so a lane holds one row's scores: maximum and sum stay in the lane but for one exchange of the halves, and the
+// probabilities, rounded to the storage type, are in place as the operand of V^T P^T.
+// The accumulators are scaled again only when a row's maximum grows by more than 8 (base 2) over the one in use: sums and
+// probabilities then stay within 2^8 of their usual range, which fp32 and the rounding to 16 bits do not notice.
+// Masked scores are -inf by selection, never by addition, and rows of keys that are not there are zeros in LDS, so nothing that
+// lies behind a sequence's end, on an unused part of a page or on a page number out of range reaches a result.
+#pragma once
+
+#include "fh_attention_tile.h"
+
+namespace fh {
+namespace attn {
+
+enum KvSource : int { kDense = 0, kPaged = 1, kE4m3 = 2 };
+
+constexpr int kBlock = 64;  // keys per block
+
+struct RowsArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  float* lse;  // [tokens, heads] or null
+  int64_t ldq, ldo;
+  const int32_t* cu;
+  int tokens, batch, heads, kv_heads, dh;
+  Divider group;
+  int causal;
+  float scale;
+  int slots;
+  // splits > 1: part z of each row's keys goes to part_out [splits][tokens * heads][dh] (normalised) and part_lse (base 2)
+  int splits;
+  float* part_out;
+  float* part_lse;
+  // keys and values
+  const void* k;
+  const void* v;
+  int64_t ldk, ldv;  // kDense: elements between tokens
+  const uint8_t* k_scale;
+  const uint8_t* v_scale;
+  const int32_t* table;
+  const int32_t* kv_lens;
+  int64_t table_stride;
+  int pages, page_shift;
+};
+
+// 8 e4m3 values times a power of two (the fp32 `scale`), as 8 values of T: exact in bf16; in f16 exact but below its smallest normal
+// value and past its largest, where the values of f16 rows that such a scale was made for do not lie.
+template <typename T>
+__device__ __forceinline__ u32x4_t widen_e4m3(const u32x2_t& w, float scale) {
+  u32x4_t o;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (std::is_same_v<T, bf16_t>) {
+      o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, false));
+      o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, true));
+    } else {
+      o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], scale, false));
+      o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], scale, true));
+    }
+  }
+  return o;
+}
+
+// One block of keys and values on its way from memory to LDS: thread t carries chunk t % CH of rows t / CH + n PASS.
+template <typename T, int DH, int SRC, int THREADS>
+struct KvStage {
+  static constexpr int CH = DH / 8, PASS = THREADS / CH, N = kBlock / PASS;
+  using Raw = std::conditional_t<SRC == kE4m3, u32x2_t, u32x4_t>;
+  Raw k[N], v[N];
+  uint32_t scales[N];  // kE4m3: the key's scale byte and the value's
+  uint64_t there;      // kPaged, kE4m3: keys of the block that exist
+
+  __device__ __forceinline__ void load(const RowsArgs& a, int begin, const int32_t* table, int kv_head, int kb, int kend, int tid) {
+    const int chunk = tid % CH, row0 = tid / CH;
+    const bool inside = chunk * 8 < a.dh;
+    if constexpr (SRC != kDense) {
+      const int key = kb + (tid & 63);
+      const bool ok = key < kend && static_cast<uint32_t>(table[key >> a.page_shift]) < static_cast<uint32_t>(a.pages);
+      there = __ballot(ok);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int key = kb + row0 + n * PASS;
+      if constexpr (SRC == kDense) {
+        const int64_t row = begin + key;
+        const int64_t col = static_cast<int64_t>(kv_head) * a.dh + chunk * 8;
+        const bool ok = inside && key < kend;
+        k[n] = load_chunk(static_cast<const uint16_t*>(a.k) + row * a.ldk + col, ok);
+        v[n] = load_chunk(static_cast<const uint16_t*>(a.v) + row * a.ldv + col, ok);
+      } else {
+        const int page = key < kend ? table[key >> a.page_shift] : -1;
+        const bool ok = inside && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
+        const int64_t slot = (static_cast<int64_t>(page) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+        const int64_t row = slot * a.kv_heads + kv_head;
+        const int64_t at = row * a.dh + chunk * 8;
+        if constexpr (SRC == kPaged) {
+          k[n] = load_chunk(static_cast<const uint16_t*>(a.k) + at, ok);
+          v[n] = load_chunk(static_cast<const uint16_t*>(a.v) + at, ok);
+        } else {
+          k[n] = u32x2_t{0, 0};
+          v[n] = u32x2_t{0, 0};
+          scales[n] = 0x7f7fu;
+          if (ok) {
+            k[n] = *reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(a.k) + at);
+            v[n] = *reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(a.v) + at);
+            scales[n] = a.k_scale[row] | (static_cast<uint32_t>(a.v_scale[row]) << 8);
+          }
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(unsigned char* kbuf, unsigned char* vbuf, int tid) const {
+    const int chunk = tid % CH, row0 = tid / CH;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int at = tile_at<DH>(row0 + n * PASS, chunk);
+      u32x4_t kw, vw;
+      if constexpr (SRC == kE4m3) {
+        kw = widen_e4m3<T>(k[n], __uint_as_float((scales[n] & 0xffu) << 23));
+        vw = widen_e4m3<T>(v[n], __uint_as_float((scales[n] >> 8) << 23));
+      } else {
+        kw = k[n];
+        vw = v[n];
+      }
+      *reinterpret_cast<u32x4_t*>(kbuf + at) = kw;
+      *reinterpret_cast<u32x4_t*>(vbuf + at) = vw;
+    }
+  }
+};
+
+template <typename T, int DH, int SRC, int W>
+__global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArgs a) {
+  constexpr int BYTES = kBlock * DH * 2;  // one block of keys, or of values
+  constexpr int ROWS = 32 * W;
+  static_assert((ROWS & (ROWS - 1)) == 0, "rows per workgroup: a power of two");
+  constexpr int SHIFT = __builtin_ctz(ROWS);
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Neighbouring workgroups take neighbouring key heads of one slot: with the dispatch order over the 8 XCDs, an XCD sees few heads'
+  // keys and values at a time. The last slots, a causal sequence's longest, go first.
+  const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int slot = a.slots - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
+  const int group = static_cast<int>(a.group.d);
+  int first_slot = 0;
+  const int b = find_sequence(a.cu, a.batch, a.tokens, group, SHIFT, slot, first_slot);
+  if (b < 0) return;
+  const Span seq = sequence(a.cu, b, a.tokens);
+  const int new_rows = seq.end - seq.begin;
+  const int rows = new_rows * group;
+  const int tile0 = (slot - first_slot) * ROWS;
+  if (tile0 >= rows) return;
+
+  // keys of the sequence, and where its first row stands among them
+  int keys = new_rows, first = 0;
+  const int32_t* table = nullptr;
+  if constexpr (SRC != kDense) {
+    // a length past what the block table's row can hold is taken as that
+    const int64_t cap = a.table_stride << a.page_shift;
+    keys = max(a.kv_lens[b], 0);
+    if (keys > cap) keys = static_cast<int>(cap);
+    first = keys - new_rows;
+    table = a.table + b * a.table_stride;
+  }
+  auto limit = [&](int r) {  // last visible key of row r
+    return a.causal ? min(first + divide(min(r, rows - 1), a.group), keys - 1) : keys - 1;
+  };
+  // this part's keys
+  int kbegin = 0, kend = limit(tile0 + ROWS - 1) + 1;
+  if (a.splits > 1) {
+    const int blocks = (kend + kBlock - 1) / kBlock;
+    const int per = (blocks + a.splits - 1) / a.splits;
+    kbegin = static_cast<int>(blockIdx.z) * per * kBlock;
+    kend = min(kend, kbegin + per * kBlock);
+  }
+
+  const int r0 = tile0 + wave * 32, r = r0 + l32;
+  const bool live = r < rows;
+  const int lim = limit(r);
+  const int lim_low = limit(r0), lim_high = limit(r0 + 31);  // rows are in order of their tokens
+  const int token = divide(min(r, rows - 1), a.group);
+  const int head = kv_head * group + (min(r, rows - 1) - token * group);
+  const int64_t trow = seq.begin + token;
+
+  u32x4_t qf[DH / 16];
+  {
+    const uint16_t* qr = a.q + trow * a.ldq + static_cast<int64_t>(head) * a.dh;
+#pragma unroll
+    for (int s = 0; s < DH / 16; ++s) qf[s] = load_chunk(qr + 16 * s + 8 * hi, live && 16 * s + 8 * hi < a.dh);
+  }
+
+  const float c = a.scale * kLog2e;
+  float m = -__builtin_inff(), l = 0.0f;
+  f32x16_t o[DH / 32];
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt) clear(o[dt]);
+
+  KvStage<T, DH, SRC, W * 64> stage;
+  const TileReader<DH> tiles(lds, lane);
+  uint64_t there = ~uint64_t{0};
+  if (kbegin < kend) {
+    stage.load(a, seq.begin, table, kv_head, kbegin, kend, tid);
+    stage.store(lds, lds + BYTES, tid);
+    if constexpr (SRC != kDense) there = stage.there;
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int kb = kbegin; kb < kend; kb += kBlock) {
+    const bool more = kb + kBlock < kend;
+    if (more) stage.load(a, seq.begin, table, kv_head, kb + kBlock, kend, tid);
+    if (kb <= lim_high) {
+      const int kbuf = buf * 2 * BYTES, vbuf = kbuf + BYTES;
+      f32x16_t s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        clear(s[t]);
+#pragma unroll
+        for (int i = 0; i < DH / 16; ++i) mfma32<T>(tiles.rows(kbuf, 32 * t, i), qf[i], s[t]);
+      }
+      if (kb + kBlock - 1 > lim_low || there != ~uint64_t{0}) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const int u = 32 * t + result_row(x, hi);
+            const bool seen = kb + u <= lim && (SRC == kDense || ((there >> u) & 1) != 0);
+            s[t][x] = seen ? s[t][x] : -__builtin_inff();
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) top = fmaxf(top, s[t][x]);
+      top = half_max(top) * c;
+      if (__any(top > m + 8.0f)) {
+        const float next = fmaxf(m, top);
+        const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= f;
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[dt][x] *= f;
+      }
+      const float ms = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          s[t][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], c, -ms));
+          l += s[t][x];
+        }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const u32x4_t p = pack_slice<T>(s[t], hf);
+#pragma unroll
+          for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(tiles.columns(vbuf, 32 * t + 16 * hf, dt), p, o[dt]);
+        }
+    }
+    if (more) {
+      unsigned char* next = lds + (buf ^ 1) * 2 * BYTES;
+      stage.store(next, next + BYTES, tid);
+      if constexpr (SRC != kDense) there = stage.there;
+    }
+    __syncthreads();
+    buf ^= 1;
+  }
+
+  l = half_sum(l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // rows without a visible key: zeros, lse -inf
+  const float lse2 = l == 0.0f ? -__builtin_inff() : m + __log2f(l);
+  if (!live) return;
+  if (a.splits > 1) {
+    const int64_t row = (static_cast<int64_t>(blockIdx.z) * a.tokens + trow) * a.heads + head;
+    if (hi == 0) a.part_lse[row] = lse2;
+    float* p = a.part_out + row * a.dh;
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = 32 * dt + 8 * q + 4 * hi;
+        if (d < a.dh)
+          *reinterpret_cast<float4*>(p + d) =
+              make_float4(o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv, o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv);
+      }
+    return;
+  }
+  store_row<T, DH>(a.out + trow * a.ldo + static_cast<int64_t>(head) * a.dh, o, inv, hi, a.dh);
+  if (a.lse != nullptr && hi == 0) a.lse[trow * a.heads + head] = lse2 * kLn2;
+}
+
+// The parts' weighted sum: out = sum_z w_z out_z / sum_z w_z, w_z = 2^(lse_z - max lse). One wave per (token, head), 4 values a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_kernel(const RowsArgs a) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
+  if (row >= rows) return;
+  const int64_t token = row / a.heads;
+  // rows outside the sequences stay as they are
+  if (token < a.cu[0] || token >= a.cu[a.batch]) return;
+  const int lane = threadIdx.x & 63;
+  float top = -__builtin_inff();
+  for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_lse[z * rows + row]);
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int d = lane * 4;
+  for (int z = 0; z < a.splits; ++z) {
+    const float w = __builtin_amdgcn_exp2f(a.part_lse[z * rows + row] - ref);
+    sum += w;
+    if (w != 0.0f && d < a.dh) {
+      const float4 p = *reinterpret_cast<const float4*>(a.part_out + (z * rows + row) * a.dh + d);
+      acc[0] += w * p.x;
+      acc[1] += w * p.y;
+      acc[2] += w * p.z;
+      acc[3] += w * p.w;
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (d < a.dh) {
+    u32x2_t w;
+    w[0] = store2<T>(acc[0] * inv, acc[1] * inv);
+    w[1] = store2<T>(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<u32x2_t*>(a.out + token * a.ldo + (row - token * a.heads) * a.dh + d) = w;
+  }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace attn
+}  // namespace fh

@@ -1,0 +1,182 @@
+// What the attention kernels over packed sequences and over a paged cache share: where a row of a tile comes from, LDS tiles that
+// serve both row and transposed fragments, and the 32-row products on v_mfma_f32_32x32x16.
+//
+// Rows. The query rows of one key head are taken together: row r of a sequence is its token r / group, head
+// kv_head * group + r % group, so the heads that share keys and values share every tile of them, and a lane (one row of a 32-row
+// tile) carries its own last visible key.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "fh_common.h"
+#include "fh_mfma16.h"
+
+namespace fh {
+namespace attn {
+
+using namespace mfma16;
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// r / d for 0 <= r < 2^31 as (r * mul) >> shift: with 2^(l-1) < d <= 2^l, mul = ceil(2^(31+l) / d) exceeds the quotient by less
+// than d / 2^(31+l), which times r stays below one step of 1/d.
+struct Divider {
+  uint32_t d, mul, shift;
+};
+inline Divider make_divider(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t{1} << l) < d) ++l;
+  return {d, static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), 31 + l};
+}
+__device__ __forceinline__ int divide(int r, const Divider& v) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(r)) * v.mul) >> v.shift);
+}
+
+// cu_seqlens is device data: whatever it holds, a sequence's rows stay within the tensors' rows.
+struct Span {
+  int begin, end;
+};
+__device__ __forceinline__ Span sequence(const int32_t* cu, int b, int rows) {
+  const int s = min(max(cu[b], 0), rows);
+  return {s, min(max(cu[b + 1], s), rows)};
+}
+
+// Work slots. The tiles of `tile` rows (rows = tokens * per_token) of all sequences are numbered without knowing the lengths on the
+// host: sequence b's begin at slot(b) = floor(cu[b] * per_token / tile) + b, which leaves room for its ceil(length / tile) tiles
+// before slot(b + 1). Slots that no tile takes end at once. Every wave looks 64 sequences up at a time.
+// Host: floor(rows * per_token / tile) + batch slots.
+__device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, int rows, int per_token, int tile_shift, int slot,
+                                             int& first_slot) {
+  const int lane = threadIdx.x & 63;
+  int found = 0;
+  for (int base = 0; base < batch; base += 64) {
+    const int b = base + lane;
+    bool before = false;
+    if (b < batch) {
+      const int64_t at = static_cast<int64_t>(min(max(cu[b], 0), rows)) * per_token;
+      before = (at >> tile_shift) + b <= slot;
+    }
+    const uint64_t m = __ballot(before);
+    found += __popcll(m);
+    if (m != ~uint64_t{0}) break;
+  }
+  if (found == 0) return -1;
+  const int b = __builtin_amdgcn_readfirstlane(found - 1);
+  const int64_t at = static_cast<int64_t>(min(max(cu[b], 0), rows)) * per_token;
+  first_slot = static_cast<int>(at >> tile_shift) + b;
+  return b;
+}
+
+// LDS tiles: rows of DH 16-bit values, 16-byte chunks XORed with swz(row). 16 rows' equal chunks (a row fragment read: lane -> row
+// l % 32, 16 bytes) fall on 16 different 16-byte columns of the 64 banks, and the 64-byte windows of 4 consecutive rows (a transposed
+// read) on 4 different ones, so both kinds of read are free of conflicts.
+template <int DH>
+__device__ __forceinline__ int swz(int row) {
+  if constexpr (DH == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+  return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+}
+template <int DH>
+__device__ __forceinline__ int tile_at(int row, int chunk) {
+  return row * (DH * 2) + ((chunk ^ swz<DH>(row)) << 4);
+}
+
+// Fragments of a tile in LDS. rows(): rows row0 .. row0 + 31 (lane l: row l % 32), slice s of 16 values (lane half: 8 of them).
+// columns(): the transposed operand: lane l: column 32 dt + l % 32, the 8 rows row0 + 4 (l / 32) + {0..3, 8..11} of a 16-row slice,
+// which is the order in which a 32x32 product's result holds its rows.
+template <int DH>
+struct TileReader {
+  const unsigned char* base;
+  int row_off, row_x, col_off[2], col_x[2];
+  __device__ __forceinline__ explicit TileReader(const unsigned char* lds, int lane) : base(lds) {
+    const int l32 = lane & 31, hi = lane >> 5;
+    row_off = l32 * (DH * 2);
+    row_x = swz<DH>(l32) ^ hi;
+    const int g = lane >> 4, rr = lane & 15, qd = rr & 3, e = rr >> 2;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const int row = 8 * part + 4 * (g >> 1) + e;
+      col_off[part] = row * (DH * 2) + (qd & 1) * 8;
+      col_x[part] = swz<DH>(row) ^ (2 * (g & 1) + (qd >> 1));
+    }
+  }
+  __device__ __forceinline__ u32x4_t rows(int buffer, int row0, int s) const {
+    return *reinterpret_cast<const u32x4_t*>(base + buffer + row0 * (DH * 2) + row_off + ((row_x ^ (2 * s)) << 4));
+  }
+  __device__ __forceinline__ u32x4_t columns(int buffer, int row0, int dt) const {
+    const u32x2_t a = read(buffer, row0, dt, 0), b = read(buffer, row0, dt, 1);
+    return u32x4_t{a[0], a[1], b[0], b[1]};
+  }
+
+ private:
+  __device__ __forceinline__ u32x2_t read(int buffer, int row0, int dt, int part) const {
+    const unsigned char* p = base + buffer + row0 * (DH * 2) + col_off[part] + ((col_x[part] ^ (4 * dt)) << 4);
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((FH_LDS s16x4_t*)(p)));
+  }
+};
+
+// max / sum of a lane's value and the other half's (same row of a 32x32 result, the other 16 of its values)
+__device__ __forceinline__ void both_halves(float v, float& low, float& high) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  low = __uint_as_float(r[0]);
+  high = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float half_max(float v) {
+  float a, b;
+  both_halves(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float v) {
+  float a, b;
+  both_halves(v, a, b);
+  return a + b;
+}
+
+__device__ __forceinline__ void clear(f32x16_t& a) {
+#pragma unroll
+  for (int x = 0; x < 16; ++x) a[x] = 0.0f;
+}
+
+// Slice hf (16 of its rows) of a 32x32 result rounded to T, as the operand of the next product.
+template <typename T>
+__device__ __forceinline__ u32x4_t pack_slice(const f32x16_t& p, int hf) {
+  u32x4_t w;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = store2<T>(p[8 * hf + 2 * j], p[8 * hf + 2 * j + 1]);
+  return w;
+}
+
+// Row x of lane half hi in a 32x32 result.
+__device__ __forceinline__ constexpr int result_row(int x, int hi) { return 8 * (x / 4) + 4 * hi + x % 4; }
+
+// A 16-byte chunk of 8 values at p when `there`, else zeros.
+__device__ __forceinline__ u32x4_t load_chunk(const uint16_t* p, bool there) {
+  u32x4_t v{0, 0, 0, 0};
+  if (there) v = *reinterpret_cast<const u32x4_t*>(p);
+  return v;
+}
+
+// A lane's transposed accumulators (DH / 32 tiles of [32 values of d][32 rows]) as one row of 16-bit values at `row`; dh values are
+// kept (dh % 8 == 0, so 4-value pieces are whole).
+template <typename T, int DH>
+__device__ __forceinline__ void store_row(uint16_t* row, const f32x16_t (&acc)[DH / 32], float scale, int hi, int dh) {
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * dt + 8 * q + 4 * hi;
+      if (d < dh) {
+        u32x2_t w;
+        w[0] = store2<T>(acc[dt][4 * q] * scale, acc[dt][4 * q + 1] * scale);
+        w[1] = store2<T>(acc[dt][4 * q + 2] * scale, acc[dt][4 * q + 3] * scale);
+        *reinterpret_cast<u32x2_t*>(row + d) = w;
+      }
+    }
+}
+
+}  // namespace attn
+}  // namespace fh

@@ -1,0 +1,196 @@
+// The paged key/value cache: fh_kv_cache_write puts new tokens' rows at their positions, fh_kv_cache_read brings rows back.
+// e4m3: a row (one token, one head) is stored as e4m3 values and one E8M0 byte, its scale: the least power of two p >= 2^-126 with
+// max|row| <= 448 p, and 1 for a row of zeros. A power of two costs the 3-bit fraction nothing against any other scale and is
+// undone exactly: the cached value e4m3 * p is a bf16 value, so attention needs no further rounding of it. Values that are not
+// finite become NaN, and the maximum is taken over the others.
+// Both kernels move 16 bytes of the tensors' side per lane, a row in DH / 8 lanes (8 or 16, power of two, for the maximum's shuffles);
+// they are bound by memory, and by the launch for a step's few rows.
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "fh_attention_rows.h"
+#include "fh_paged_cache.h"
+
+namespace fh {
+namespace {
+
+using namespace attn;
+
+struct CacheArgs {
+  void* k;  // the cache
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  uint16_t* xk;  // the packed rows
+  uint16_t* xv;
+  int64_t ldk, ldv;
+  const int32_t* cu;
+  const int32_t* table;
+  const int32_t* kv_lens;
+  int64_t table_stride;
+  int tokens, batch, kv_heads, dh, pages, page_shift;
+};
+
+// The cache row of packed row `token` (its slot), or -1: outside the sequences, past the block table, a page that does not exist.
+// New tokens stand at the end of their sequence (WRITE), rows that are read at its beginning.
+template <bool WRITE>
+__device__ __forceinline__ int64_t slot_of(const CacheArgs& a, int token, bool& in_sequence) {
+  // the first sequence that ends after the token
+  int lo = 0, hi = a.batch;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid + 1] > token) hi = mid; else lo = mid + 1;
+  }
+  in_sequence = lo < a.batch && a.cu[lo] <= token;
+  if (!in_sequence) return -1;
+  const Span seq = sequence(a.cu, lo, a.tokens);
+  const int64_t cap = a.table_stride << a.page_shift;
+  int64_t len = max(a.kv_lens[lo], 0);
+  if (len > cap) len = cap;
+  const int64_t position = token - seq.begin + (WRITE ? len - (seq.end - seq.begin) : 0);
+  if (position < 0 || position >= len) return -1;
+  const int page = a.table[lo * a.table_stride + (position >> a.page_shift)];
+  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) return -1;
+  return (static_cast<int64_t>(page) << a.page_shift) + (position & ((1 << a.page_shift) - 1));
+}
+
+// Exponent byte of the least power of two p with top <= 448 p: 448 = 1.75 * 2^8.
+__device__ __forceinline__ uint32_t scale_byte(float top) {
+  const uint32_t u = __float_as_uint(top);
+  if (u == 0) return 127;
+  const int e = static_cast<int>(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return static_cast<uint32_t>(max(e, 1));
+}
+
+// 8 values of T over 2^(byte - 127), to e4m3 (nearest even; the quotients lie within its range)
+template <typename T>
+__device__ __forceinline__ u32x2_t narrow_e4m3(const float (&v)[8], uint32_t byte) {
+  const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte); byte 1 .. 247
+  u32x2_t w{0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = v[4 * i + j] * inv;
+    int p = 0;
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], p, false);
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], p, true);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (!(__builtin_fabsf(v[4 * i + j]) < __builtin_inff())) p = (p & ~(0xff << (8 * j))) | (0x7f << (8 * j));
+    w[i] = static_cast<uint32_t>(p);
+  }
+  return w;
+}
+
+// One row (token, head) of keys or values per LANES lanes. blockIdx.y: 0 keys, 1 values.
+template <typename T, int LANES, bool E4M3, bool WRITE>
+__global__ __launch_bounds__(256) void kv_cache_kernel(const CacheArgs a) {
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;
+  const int chunk = threadIdx.x % LANES;
+  const int64_t token = row / a.kv_heads;
+  const bool inside = token < a.tokens;
+  const int head = static_cast<int>(row - token * a.kv_heads);
+  const bool values = blockIdx.y != 0;
+  bool in_sequence = false;
+  const int64_t slot = inside ? slot_of<WRITE>(a, static_cast<int>(token), in_sequence) : -1;
+  const bool there = slot >= 0 && chunk * 8 < a.dh;
+  const int64_t crow = slot * a.kv_heads + head;
+  uint16_t* x = (values ? a.xv + token * a.ldv : a.xk + token * a.ldk) + static_cast<int64_t>(head) * a.dh + chunk * 8;
+  void* cache = values ? a.v : a.k;
+  uint8_t* scales = values ? a.v_scale : a.k_scale;
+  if constexpr (WRITE) {
+    const u32x4_t w = load_chunk(x, there);
+    if constexpr (!E4M3) {
+      if (there) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(cache) + crow * a.dh + chunk * 8) = w;
+    } else {
+      float v[8];
+      unpack_vec<T>(uint4{w[0], w[1], w[2], w[3]}, v);
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float s = __builtin_fabsf(v[j]);
+        if (s < __builtin_inff()) top = fmaxf(top, s);
+      }
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+      if (there) {
+        const uint32_t byte = scale_byte(top);
+        *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(cache) + crow * a.dh + chunk * 8) = narrow_e4m3<T>(v, byte);
+        if (chunk == 0) scales[crow] = static_cast<uint8_t>(byte);
+      }
+    }
+  } else {
+    u32x4_t w{0, 0, 0, 0};  // positions without a cached row read as zeros
+    if (there) {
+      if constexpr (E4M3)
+        w = widen_e4m3<T>(*reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(cache) + crow * a.dh + chunk * 8),
+                          __uint_as_float(static_cast<uint32_t>(scales[crow]) << 23));
+      else
+        w = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(cache) + crow * a.dh + chunk * 8);
+    }
+    if (in_sequence && chunk * 8 < a.dh) *reinterpret_cast<u32x4_t*>(x) = w;
+  }
+}
+
+template <bool WRITE>
+fh_status run(const std::string& fn, const fh_paged_cache* c, void* k, int64_t k_stride, void* v, int64_t v_stride, int64_t tokens,
+              const int32_t* cu_seqlens, void* stream) {
+  if (fh_status st = check_paged_cache(fn, c); st != FH_OK) return st;
+  if (tokens < 0 || tokens > 0x7fffffff) return fail(FH_INVALID_ARGUMENT, fn + ": bad tokens");
+  if (tokens == 0 || c->batch == 0) return FH_OK;
+  if (!k || !v || !cu_seqlens) return fail(FH_INVALID_ARGUMENT, fn + ": null pointer");
+  if (!aligned16(k) || !aligned16(v)) return fail(FH_INVALID_ARGUMENT, fn + ": k and v must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(cu_seqlens) % 4 != 0) return fail(FH_INVALID_ARGUMENT, fn + ": cu_seqlens must be 4-byte aligned");
+  if (k_stride < c->kv_heads * c->dh || v_stride < c->kv_heads * c->dh || (k_stride | v_stride) % 8 != 0)
+    return fail(FH_INVALID_ARGUMENT, fn + ": row strides must be multiples of 8 elements, no shorter than a row");
+  CacheArgs a{};
+  a.k = c->k;
+  a.v = c->v;
+  a.k_scale = c->k_scale;
+  a.v_scale = c->v_scale;
+  a.xk = static_cast<uint16_t*>(k);
+  a.xv = static_cast<uint16_t*>(v);
+  a.ldk = k_stride;
+  a.ldv = v_stride;
+  a.cu = cu_seqlens;
+  a.table = c->block_table;
+  a.kv_lens = c->kv_lens;
+  a.table_stride = c->table_stride;
+  a.tokens = static_cast<int>(tokens);
+  a.batch = static_cast<int>(c->batch);
+  a.kv_heads = static_cast<int>(c->kv_heads);
+  a.dh = static_cast<int>(c->dh);
+  a.pages = static_cast<int>(c->pages);
+  a.page_shift = page_shift(c->page_size);
+  auto launch = [&]<typename T, int LANES, bool E4M3>() {
+    const int64_t blocks = (tokens * c->kv_heads * LANES + 255) / 256;
+    if (blocks > 0x7fffffff) return fail(FH_INVALID_ARGUMENT, fn + ": too many rows");
+    hipLaunchKernelGGL((kv_cache_kernel<T, LANES, E4M3, WRITE>), dim3(static_cast<uint32_t>(blocks), 2), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), a);
+    return launch_status("kv_cache_kernel launch");
+  };
+  auto typed = [&]<typename T>() {
+    if (c->cache_dtype == FH_E4M3)
+      return c->dh <= 64 ? launch.template operator()<T, 8, true>() : launch.template operator()<T, 16, true>();
+    return c->dh <= 64 ? launch.template operator()<T, 8, false>() : launch.template operator()<T, 16, false>();
+  };
+  return c->dtype == FH_BF16 ? typed.template operator()<bf16_t>() : typed.template operator()<f16_t>();
+}
+
+}  // namespace
+}  // namespace fh
+
+using namespace fh;
+
+extern "C" fh_status fh_kv_cache_write(const fh_paged_cache* cache, const void* k, int64_t k_stride, const void* v,
+                                       int64_t v_stride, int64_t tokens, const int32_t* cu_seqlens, void* stream) {
+  return run<true>("fh_kv_cache_write", cache, const_cast<void*>(k), k_stride, const_cast<void*>(v), v_stride, tokens, cu_seqlens,
+                   stream);
+}
+
+extern "C" fh_status fh_kv_cache_read(const fh_paged_cache* cache, void* k, int64_t k_stride, void* v, int64_t v_stride,
+                                      int64_t tokens, const int32_t* cu_seqlens, void* stream) {
+  return run<false>("fh_kv_cache_read", cache, k, k_stride, v, v_stride, tokens, cu_seqlens, stream);
+}

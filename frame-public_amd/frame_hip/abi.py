@@ -18,6 +18,7 @@ KERNELS_LIB = os.path.join(LIB_DIR, "libframe_hip_kernels.so")
 
 FH_OK = 0
 F32, F16, BF16 = 0, 2, 3
+E4M3 = 16  # cache type only (fh_paged_cache)
 EW_ADD, EW_MUL, EW_RELU, EW_SQUARE, EW_GELU = 1, 2, 3, 4, 5
 GEMM_ANY_ORDER = 1
 H2H, H2D, D2H, D2D = 0, 1, 2, 3
@@ -36,6 +37,21 @@ class FrameHipError(RuntimeError):
 class Epilogue(ctypes.Structure):
     _fields_ = [("nseg", c_int32), ("round_between", c_int32), ("ops", c_uint8 * MAX_SEGMENTS),
                 ("ins", c_void_p * MAX_SEGMENTS)]
+
+
+class PackedAttention(ctypes.Structure):
+    """fh_packed_attention: the sequences, heads and strides of attention over packed rows."""
+    _fields_ = [("dtype", c_int32), ("causal", c_int32), ("tokens", c_int64), ("batch", c_int64), ("heads", c_int64),
+                ("kv_heads", c_int64), ("dh", c_int64), ("q_stride", c_int64), ("k_stride", c_int64),
+                ("v_stride", c_int64), ("out_stride", c_int64), ("scale", c_float)]
+
+
+class PagedCache(ctypes.Structure):
+    """fh_paged_cache: a paged cache of keys and values, its block table and the cached lengths."""
+    _fields_ = [("dtype", c_int32), ("cache_dtype", c_int32), ("pages", c_int64), ("page_size", c_int64),
+                ("kv_heads", c_int64), ("dh", c_int64), ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p),
+                ("v_scale", c_void_p), ("batch", c_int64), ("block_table", c_void_p), ("table_stride", c_int64),
+                ("kv_lens", c_void_p)]
 
 
 _lib = None
@@ -96,6 +112,16 @@ _SIGS = {
     "fh_attention_grad_workspace": (c_int64, [c_int64, c_int64, c_int64]),
     "fh_attention_grad": (c_int32, [c_int32] + [c_void_p] * 8 + [c_int64] * 5 + [c_float, c_void_p]),
     "fh_attention_supported": (c_int32, [c_int32, c_int64, c_int64]),
+    "fh_attention_packed_fwd": (c_int32, [POINTER(PackedAttention)] + [c_void_p] * 7),
+    "fh_attention_packed_grad_workspace": (c_int64, [POINTER(PackedAttention)]),
+    "fh_attention_packed_grad": (c_int32, [POINTER(PackedAttention)] + [c_void_p] * 11 + [c_int64, c_void_p]),
+    "fh_kv_cache_write": (c_int32, [POINTER(PagedCache), c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                    c_void_p]),
+    "fh_kv_cache_read": (c_int32, [POINTER(PagedCache), c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                   c_void_p]),
+    "fh_attention_paged_workspace": (c_int64, [POINTER(PagedCache), c_int64, c_int64, c_int64, c_int64]),
+    "fh_attention_paged": (c_int32, [POINTER(PagedCache), c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                                     c_float, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
     "fh_softmax_rows": (c_int32, [c_int32, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
     "fh_layer_norm_rows": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float,
                                      c_void_p]),

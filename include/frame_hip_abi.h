@@ -40,6 +40,9 @@ typedef enum fh_status {
 
 /* Equal to frame::DTypeCode ordinals (reference: include/frame/core/dtype.h:17-29). */
 typedef enum fh_dtype { FH_F32 = 0, FH_F16 = 2, FH_BF16 = 3 } fh_dtype;
+/* What a key/value cache may hold besides FH_F16 and FH_BF16: OCP e4m3 with a power-of-two scale per row (fh_kv_cache_write). No
+ * tensor of a graph has this type, so the code lies outside frame::DTypeCode's. */
+#define FH_E4M3 16
 
 /* Elementwise sub-op codes understood by fh_ew_program and the GEMM/conv epilogues.
  * add/mul/relu/square are the reference's fusable ops (reference: src/ops/schemas/elementwise.cpp:667-707);
@@ -320,6 +323,80 @@ int64_t fh_attention_grad_workspace(int64_t batch, int64_t seq, int64_t heads);
 fh_status fh_attention_grad(int32_t dtype, const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk,
                             void* dv, void* workspace, int64_t workspace_bytes, int64_t batch, int64_t seq, int64_t heads,
                             int64_t dh, float scale, void* stream);
+
+/* ---- attention over packed sequences, with grouped heads ----
+ * `batch` sequences lie row after row in tensors of `tokens` rows: sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1] - 1 (device
+ * memory, batch + 1 values, not decreasing; a length may be 0). A row holds `heads` heads of dh values (q, out), or kv_heads (k, v);
+ * head h reads key head h / (heads / kv_heads). The strides are elements between rows, so q, k and v may be columns of one
+ * projection's output. Rows outside the sequences are neither read nor written, and cu_seqlens values out of range are taken as 0 or
+ * `tokens`. bf16 / f16, dh a multiple of 8 up to 128, strides multiples of 8 elements, tensors 16-byte aligned.
+ * No counterpart in the reference, whose attention has one length, no mask and as many key heads as heads
+ * (src/nn/layers.cpp:1014-1080); unlike fh_attention_fwd these round no intermediate as a graph of single ops would: scores,
+ * softmax and sums are fp32, and only the probabilities (and in the gradients their derivatives) are rounded to the storage type,
+ * as operands of the second product. */
+typedef struct fh_packed_attention {
+  int32_t dtype;
+  int32_t causal; /* 1: row t of a sequence sees its rows 0 .. t; 0: all of them */
+  int64_t tokens, batch, heads, kv_heads, dh;
+  int64_t q_stride, k_stride, v_stride, out_stride;
+  float scale; /* of the scores, e.g. 1/sqrt(dh); positive */
+} fh_packed_attention;
+
+/* out = softmax(scale q k^T) v per head, and the natural logarithm of the softmax's sum in lse ([tokens, heads] fp32; may be NULL),
+ * which the gradients read. A value of the sequence itself that is not finite may reach other rows of that sequence (never of
+ * another), also rows that do not see it. */
+fh_status fh_attention_packed_fwd(const fh_packed_attention* geom, const void* q, const void* k, const void* v,
+                                  const int32_t* cu_seqlens, void* out, float* lse, void* stream);
+
+/* Gradients with respect to q, k and v for the output gradient dout, from the forward's operands, out and lse. dout has out's
+ * stride; dq, dk and dv have q's, k's and v's. Deterministic. The workspace holds one fp32 per (row, head). */
+int64_t fh_attention_packed_grad_workspace(const fh_packed_attention* geom);
+fh_status fh_attention_packed_grad(const fh_packed_attention* geom, const void* q, const void* k, const void* v,
+                                   const int32_t* cu_seqlens, const void* out, const float* lse, const void* dout, void* dq,
+                                   void* dk, void* dv, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- a paged cache of keys and values, and attention over it ----
+ * The cache is [pages, page_size, kv_heads, dh] for keys and for values; position p of sequence b is row p % page_size of page
+ * block_table[b * table_stride + p / page_size]. kv_lens[b] positions are cached, this call's new tokens among them (a length past
+ * table_stride * page_size is taken as that). block_table and kv_lens are device memory. A page number outside [0, pages) is
+ * a page that does not exist: nothing is written to it, it reads as zeros, and attention leaves its positions out.
+ * page_size is a power of two; cache_dtype is the tensors' dtype or FH_E4M3, which adds an E8M0 byte per (row, head): the value is
+ * e4m3 * 2^(byte - 127). No counterpart in the reference. */
+typedef struct fh_paged_cache {
+  int32_t dtype;       /* of the tensors: FH_BF16 or FH_F16 */
+  int32_t cache_dtype; /* dtype, or FH_E4M3 */
+  int64_t pages, page_size, kv_heads, dh;
+  void* k;
+  void* v;
+  uint8_t* k_scale; /* [pages, page_size, kv_heads], FH_E4M3 only */
+  uint8_t* v_scale;
+  int64_t batch;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* kv_lens;
+} fh_paged_cache;
+
+/* Writes packed rows (sequences as cu_seqlens says, see fh_packed_attention) into the cache: the n new tokens of sequence b go to
+ * positions kv_lens[b] - n .. kv_lens[b] - 1; rows whose position would be negative are skipped. FH_E4M3: each (row, head) is divided
+ * by the least power of two p, 2^-126 or more, with max|row| <= 448 p (1 for a row of zeros), and rounded to nearest even; values
+ * that are not finite become NaN and do not count for the maximum. Two sequences whose new tokens share a page's row leave either's
+ * values there, possibly of both mixed. */
+fh_status fh_kv_cache_write(const fh_paged_cache* cache, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                            int64_t tokens, const int32_t* cu_seqlens, void* stream);
+
+/* Reads positions 0 .. n - 1 of each sequence into the n packed rows that cu_seqlens gives it; positions that are not cached read as
+ * zeros. */
+fh_status fh_kv_cache_read(const fh_paged_cache* cache, void* k, int64_t k_stride, void* v, int64_t v_stride, int64_t tokens,
+                           const int32_t* cu_seqlens, void* stream);
+
+/* Attention of the new tokens over the cache: token i of the n new ones of sequence b sees positions 0 .. kv_lens[b] - n + i (the
+ * cache holds the new tokens' keys and values already, see fh_kv_cache_write). Rows that see nothing are zeros. n = 1 is a
+ * decoding step. max_new and max_keys are the longest n and kv_lens that are expected: they choose how the work is cut, and
+ * any lengths give the same results up to rounding. The workspace query takes the same numbers; 0 bytes: may be NULL. */
+int64_t fh_attention_paged_workspace(const fh_paged_cache* cache, int64_t tokens, int64_t heads, int64_t max_new, int64_t max_keys);
+fh_status fh_attention_paged(const fh_paged_cache* cache, const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                             int64_t tokens, int64_t heads, const int32_t* cu_seqlens, float scale, int64_t max_new,
+                             int64_t max_keys, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* 2-D pooling, NCHW. mode 0 = max (-inf padding, first max wins), 1 = average (include padding).
  * geom = {N, C, H, W, KH, KW, stride_h, stride_w, pad_h, pad_w}.
