@@ -90,7 +90,6 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   }
   delta = half_sum(delta);
   const int64_t stat = trow * a.heads + head;
-  if (live && hi == 0) a.delta[stat] = delta;
   const float lse2 = live ? a.lse[stat] * kLog2e : 0.0f;
   const float c = a.scale * kLog2e;
 
@@ -105,8 +104,17 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   kv.ldk = a.ldk;
   kv.ldv = a.ldv;
   kv.dh = a.dh;
-  KvStage<T, DH, kDense, W * 64> stage;
+  KvStage<T, DH, kDense, W * 64, kBlock> stage;
   const TileReader<DH> tiles(lds, lane);
+  auto scores = [&](int kbuf, int vbuf, int t, f32x16_t& s, f32x16_t& dp) {  // q k and dout v for 32 keys
+    clear(s);
+    clear(dp);
+#pragma unroll
+    for (int i = 0; i < DH / 16; ++i) {
+      mfma32<T>(tiles.rows(kbuf, 32 * t, i), qf[i], s);
+      mfma32<T>(tiles.rows(vbuf, 32 * t, i), gf[i], dp);
+    }
+  };
   stage.load(kv, seq.begin, nullptr, kv_head, 0, kend, tid);
   stage.store(lds, lds + BYTES, tid);
   __syncthreads();
@@ -117,16 +125,30 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
     if (kb <= lim_high) {
       const int kbuf = buf * 2 * BYTES, vbuf = kbuf + BYTES;
       const bool edge = kb + kBlock - 1 > lim_low;
+      if (lim_high < kBlock) {
+        // Rows that see one block: D = sum p dp / sum p from the block itself, as a difference from the first key's dp. D from the
+        // rounded output is off by a rounding of every out, which counts beside dp - D where a row sees few keys; and where it sees
+        // one, dp - D has to vanish.
+        float d0 = 0.0f, d = 0.0f, sum = 0.0f, unused;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f32x16_t s, dp;
+          scores(kbuf, vbuf, t, s, dp);
+          if (t == 0) both_halves(dp[0], d0, unused);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const bool seen = 32 * t + result_row(x, hi) <= lim;
+            const float p = seen ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -lse2)) : 0.0f;
+            sum += p;
+            d = seen ? __builtin_fmaf(p, dp[x] - d0, d) : d;
+          }
+        }
+        delta = d0 + half_sum(d) / half_sum(sum);
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f32x16_t s, dp;
-        clear(s);
-        clear(dp);
-#pragma unroll
-        for (int i = 0; i < DH / 16; ++i) {
-          mfma32<T>(tiles.rows(kbuf, 32 * t, i), qf[i], s);
-          mfma32<T>(tiles.rows(vbuf, 32 * t, i), gf[i], dp);
-        }
+        scores(kbuf, vbuf, t, s, dp);
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -lse2));
@@ -151,6 +173,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
     __syncthreads();
     buf ^= 1;
   }
+  if (live && hi == 0) a.delta[stat] = delta;
   if (live) store_row<T, DH>(a.dq + trow * a.ldq + static_cast<int64_t>(head) * a.dh, acc, a.scale, hi, a.dh);
 }
 
@@ -308,6 +331,8 @@ fh_status check_packed(const char* fn, const fh_packed_attention* g) {
   if (g->heads > 65535 || g->tokens > 0x7fffffff || g->batch > 0x3fffffff ||
       (g->tokens + 256) * g->heads + g->batch * g->kv_heads > 0x7fffffff)
     return fail(FH_INVALID_ARGUMENT, f + ": more than 2^31 rows (tokens x heads)");
+  if (g->tokens * g->heads / 128 + (g->batch + 1) * g->kv_heads > kMaxBlocks)
+    return fail(FH_INVALID_ARGUMENT, f + ": more rows than one launch takes");
   if (g->q_stride < g->heads * g->dh || g->out_stride < g->heads * g->dh || g->k_stride < g->kv_heads * g->dh ||
       g->v_stride < g->kv_heads * g->dh)
     return fail(FH_INVALID_ARGUMENT, f + ": a row stride is shorter than its row");

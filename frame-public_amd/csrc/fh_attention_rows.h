@@ -31,8 +31,8 @@ struct RowsArgs {
   int causal;
   float scale;
   int slots;
-  // splits > 1: part z of each row's keys goes to part_out [splits][tokens * heads][dh] (normalised) and part_lse (base 2)
-  int splits;
+  // splits > 1: part z of a longer sequence's keys goes to part_out [splits][tokens * heads][dh] (normalised) and part_lse (base 2)
+  int splits, part_keys;
   float* part_out;
   float* part_lse;
   // keys and values
@@ -65,22 +65,46 @@ __device__ __forceinline__ u32x4_t widen_e4m3(const u32x2_t& w, float scale) {
   return o;
 }
 
-// One block of keys and values on its way from memory to LDS: thread t carries chunk t % CH of rows t / CH + n PASS.
-template <typename T, int DH, int SRC, int THREADS>
+// One block of BK keys and values on its way from memory to LDS: thread t carries chunk t % CH of rows t / CH + n PASS. Of a paged
+// cache, lane j holds the page of key j % BK, looked up one block ahead, and its scales; the threads that carry the row take them from
+// that lane.
+template <typename T, int DH, int SRC, int THREADS, int BK>
 struct KvStage {
-  static constexpr int CH = DH / 8, PASS = THREADS / CH, N = kBlock / PASS;
+  static constexpr int CH = DH / 8, PASS = THREADS / CH, N = BK / PASS;
+  static_assert(BK % PASS == 0 && BK <= 64, "whole passes, a lane per key");
   using Raw = std::conditional_t<SRC == kE4m3, u32x2_t, u32x4_t>;
   Raw k[N], v[N];
-  uint32_t scales[N];  // kE4m3: the key's scale byte and the value's
-  uint64_t there;      // kPaged, kE4m3: keys of the block that exist
+  int page;         // of this lane's key in the block that load() takes next; -1: none
+  uint32_t scales;  // kE4m3: of this lane's key in the block on its way: the key's byte, the value's
+  uint64_t there;   // kPaged, kE4m3: keys of that block that exist
 
+  __device__ __forceinline__ void look_up(const RowsArgs& a, const int32_t* table, int kb, int kend, int tid) {
+    if constexpr (SRC != kDense) {
+      const int key = kb + (tid & (BK - 1));
+      page = key < kend ? table[key >> a.page_shift] : -1;
+    }
+  }
+
+  // STEP: from this block to the next that this stage takes
+  template <int STEP = BK>
   __device__ __forceinline__ void load(const RowsArgs& a, int begin, const int32_t* table, int kv_head, int kb, int kend, int tid) {
     const int chunk = tid % CH, row0 = tid / CH;
     const bool inside = chunk * 8 < a.dh;
+    const int in_page = (1 << a.page_shift) - 1;
+    auto cache_row = [&](int p, int key) {
+      return ((static_cast<int64_t>(p) << a.page_shift) + (key & in_page)) * a.kv_heads + kv_head;
+    };
     if constexpr (SRC != kDense) {
-      const int key = kb + (tid & 63);
-      const bool ok = key < kend && static_cast<uint32_t>(table[key >> a.page_shift]) < static_cast<uint32_t>(a.pages);
-      there = __ballot(ok);
+      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) page = -1;
+      there = __ballot(page >= 0);
+      if constexpr (BK < 64) there |= ~uint64_t{0} << BK;
+    }
+    if constexpr (SRC == kE4m3) {
+      scales = 0x7f7fu;
+      if (page >= 0) {
+        const int64_t row = cache_row(page, kb + (tid & (BK - 1)));
+        scales = a.k_scale[row] | (static_cast<uint32_t>(a.v_scale[row]) << 8);
+      }
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -92,26 +116,23 @@ struct KvStage {
         k[n] = load_chunk(static_cast<const uint16_t*>(a.k) + row * a.ldk + col, ok);
         v[n] = load_chunk(static_cast<const uint16_t*>(a.v) + row * a.ldv + col, ok);
       } else {
-        const int page = key < kend ? table[key >> a.page_shift] : -1;
-        const bool ok = inside && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
-        const int64_t slot = (static_cast<int64_t>(page) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-        const int64_t row = slot * a.kv_heads + kv_head;
-        const int64_t at = row * a.dh + chunk * 8;
+        const int p = __shfl(page, row0 + n * PASS, 64);
+        const bool ok = inside && p >= 0;
+        const int64_t at = cache_row(p, key) * a.dh + chunk * 8;
         if constexpr (SRC == kPaged) {
           k[n] = load_chunk(static_cast<const uint16_t*>(a.k) + at, ok);
           v[n] = load_chunk(static_cast<const uint16_t*>(a.v) + at, ok);
         } else {
           k[n] = u32x2_t{0, 0};
           v[n] = u32x2_t{0, 0};
-          scales[n] = 0x7f7fu;
           if (ok) {
             k[n] = *reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(a.k) + at);
             v[n] = *reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(a.v) + at);
-            scales[n] = a.k_scale[row] | (static_cast<uint32_t>(a.v_scale[row]) << 8);
           }
         }
       }
     }
+    look_up(a, table, kb + STEP, kend, tid);
   }
 
   __device__ __forceinline__ void store(unsigned char* kbuf, unsigned char* vbuf, int tid) const {
@@ -121,8 +142,9 @@ struct KvStage {
       const int at = tile_at<DH>(row0 + n * PASS, chunk);
       u32x4_t kw, vw;
       if constexpr (SRC == kE4m3) {
-        kw = widen_e4m3<T>(k[n], __uint_as_float((scales[n] & 0xffu) << 23));
-        vw = widen_e4m3<T>(v[n], __uint_as_float((scales[n] >> 8) << 23));
+        const uint32_t sc = __shfl(scales, row0 + n * PASS, 64);
+        kw = widen_e4m3<T>(k[n], __uint_as_float((sc & 0xffu) << 23));
+        vw = widen_e4m3<T>(v[n], __uint_as_float((sc >> 8) << 23));
       } else {
         kw = k[n];
         vw = v[n];
@@ -133,154 +155,78 @@ struct KvStage {
   }
 };
 
-template <typename T, int DH, int SRC, int W>
-__global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArgs a) {
-  constexpr int BYTES = kBlock * DH * 2;  // one block of keys, or of values
-  constexpr int ROWS = 32 * W;
-  static_assert((ROWS & (ROWS - 1)) == 0, "rows per workgroup: a power of two");
-  constexpr int SHIFT = __builtin_ctz(ROWS);
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
-
-  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // Neighbouring workgroups take neighbouring key heads of one slot: with the dispatch order over the 8 XCDs, an XCD sees few heads'
-  // keys and values at a time. The last slots, a causal sequence's longest, go first.
-  const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
-  const int slot = a.slots - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
-  const int group = static_cast<int>(a.group.d);
-  int first_slot = 0;
-  const int b = find_sequence(a.cu, a.batch, a.tokens, group, SHIFT, slot, first_slot);
-  if (b < 0) return;
-  const Span seq = sequence(a.cu, b, a.tokens);
-  const int new_rows = seq.end - seq.begin;
-  const int rows = new_rows * group;
-  const int tile0 = (slot - first_slot) * ROWS;
-  if (tile0 >= rows) return;
-
-  // keys of the sequence, and where its first row stands among them
-  int keys = new_rows, first = 0;
-  const int32_t* table = nullptr;
-  if constexpr (SRC != kDense) {
-    // a length past what the block table's row can hold is taken as that
-    const int64_t cap = a.table_stride << a.page_shift;
-    keys = max(a.kv_lens[b], 0);
-    if (keys > cap) keys = static_cast<int>(cap);
-    first = keys - new_rows;
-    table = a.table + b * a.table_stride;
-  }
-  auto limit = [&](int r) {  // last visible key of row r
-    return a.causal ? min(first + divide(min(r, rows - 1), a.group), keys - 1) : keys - 1;
-  };
-  // this part's keys
-  int kbegin = 0, kend = limit(tile0 + ROWS - 1) + 1;
-  if (a.splits > 1) {
-    const int blocks = (kend + kBlock - 1) / kBlock;
-    const int per = (blocks + a.splits - 1) / a.splits;
-    kbegin = static_cast<int>(blockIdx.z) * per * kBlock;
-    kend = min(kend, kbegin + per * kBlock);
-  }
-
-  const int r0 = tile0 + wave * 32, r = r0 + l32;
-  const bool live = r < rows;
-  const int lim = limit(r);
-  const int lim_low = limit(r0), lim_high = limit(r0 + 31);  // rows are in order of their tokens
-  const int token = divide(min(r, rows - 1), a.group);
-  const int head = kv_head * group + (min(r, rows - 1) - token * group);
-  const int64_t trow = seq.begin + token;
-
-  u32x4_t qf[DH / 16];
-  {
-    const uint16_t* qr = a.q + trow * a.ldq + static_cast<int64_t>(head) * a.dh;
-#pragma unroll
-    for (int s = 0; s < DH / 16; ++s) qf[s] = load_chunk(qr + 16 * s + 8 * hi, live && 16 * s + 8 * hi < a.dh);
-  }
-
-  const float c = a.scale * kLog2e;
-  float m = -__builtin_inff(), l = 0.0f;
+// The running softmax of a wave's 32 rows over blocks of NT 32-key tiles in LDS, and the accumulators of the output.
+template <typename T, int DH>
+struct RowState {
+  float m = -__builtin_inff(), l = 0.0f;  // l: the lane half's share
   f32x16_t o[DH / 32];
+  __device__ __forceinline__ RowState() {
 #pragma unroll
-  for (int dt = 0; dt < DH / 32; ++dt) clear(o[dt]);
-
-  KvStage<T, DH, SRC, W * 64> stage;
-  const TileReader<DH> tiles(lds, lane);
-  uint64_t there = ~uint64_t{0};
-  if (kbegin < kend) {
-    stage.load(a, seq.begin, table, kv_head, kbegin, kend, tid);
-    stage.store(lds, lds + BYTES, tid);
-    if constexpr (SRC != kDense) there = stage.there;
+    for (int dt = 0; dt < DH / 32; ++dt) clear(o[dt]);
   }
-  __syncthreads();
-  int buf = 0;
-  for (int kb = kbegin; kb < kend; kb += kBlock) {
-    const bool more = kb + kBlock < kend;
-    if (more) stage.load(a, seq.begin, table, kv_head, kb + kBlock, kend, tid);
-    if (kb <= lim_high) {
-      const int kbuf = buf * 2 * BYTES, vbuf = kbuf + BYTES;
-      f32x16_t s[2];
+
+  // keys kb .. of the block at kbuf / vbuf; MASK: by `lim` (the lane's last visible key) and the block's `there` bits
+  template <int NT>
+  __device__ __forceinline__ void block(const TileReader<DH>& tiles, int kbuf, int vbuf, const u32x4_t (&qf)[DH / 16], float c,
+                                        int kb, bool masked, int lim, uint64_t there, int hi) {
+    f32x16_t s[NT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        clear(s[t]);
+    for (int t = 0; t < NT; ++t) {
+      clear(s[t]);
 #pragma unroll
-        for (int i = 0; i < DH / 16; ++i) mfma32<T>(tiles.rows(kbuf, 32 * t, i), qf[i], s[t]);
-      }
-      if (kb + kBlock - 1 > lim_low || there != ~uint64_t{0}) {
+      for (int i = 0; i < DH / 16; ++i) mfma32<T>(tiles.rows(kbuf, 32 * t, i), qf[i], s[t]);
+    }
+    if (masked) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const int u = 32 * t + result_row(x, hi);
-            const bool seen = kb + u <= lim && (SRC == kDense || ((there >> u) & 1) != 0);
-            s[t][x] = seen ? s[t][x] : -__builtin_inff();
-          }
-      }
-      float top = s[0][0];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) top = fmaxf(top, s[t][x]);
-      top = half_max(top) * c;
-      if (__any(top > m + 8.0f)) {
-        const float next = fmaxf(m, top);
-        const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - next);
-        m = next;
-        l *= f;
-#pragma unroll
-        for (int dt = 0; dt < DH / 32; ++dt)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[dt][x] *= f;
-      }
-      const float ms = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          s[t][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], c, -ms));
-          l += s[t][x];
-        }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const u32x4_t p = pack_slice<T>(s[t], hf);
-#pragma unroll
-          for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(tiles.columns(vbuf, 32 * t + 16 * hf, dt), p, o[dt]);
+          const int u = 32 * t + result_row(x, hi);
+          s[t][x] = kb + u <= lim && ((there >> u) & 1) != 0 ? s[t][x] : -__builtin_inff();
         }
     }
-    if (more) {
-      unsigned char* next = lds + (buf ^ 1) * 2 * BYTES;
-      stage.store(next, next + BYTES, tid);
-      if constexpr (SRC != kDense) there = stage.there;
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) top = fmaxf(top, s[t][x]);
+    top = half_max(top) * c;
+    if (__any(top > m + 8.0f)) {
+      const float next = fmaxf(m, top);
+      const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[dt][x] *= f;
     }
-    __syncthreads();
-    buf ^= 1;
+    const float ms = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        s[t][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], c, -ms));
+        l += s[t][x];
+      }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const u32x4_t p = pack_slice<T>(s[t], hf);
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(tiles.columns(vbuf, 32 * t + 16 * hf, dt), p, o[dt]);
+      }
   }
 
-  l = half_sum(l);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // rows without a visible key: zeros, lse -inf
-  const float lse2 = l == 0.0f ? -__builtin_inff() : m + __log2f(l);
-  if (!live) return;
-  if (a.splits > 1) {
-    const int64_t row = (static_cast<int64_t>(blockIdx.z) * a.tokens + trow) * a.heads + head;
+  // rows without a visible key: zeros, lse -inf
+  __device__ __forceinline__ void finish(float& inv, float& lse2) {
+    const float sum = half_sum(l);
+    inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    lse2 = sum == 0.0f ? -__builtin_inff() : m + __log2f(sum);
+  }
+
+  __device__ __forceinline__ void write_part(const RowsArgs& a, int64_t row, float inv, float lse2, int hi) const {
     if (hi == 0) a.part_lse[row] = lse2;
     float* p = a.part_out + row * a.dh;
 #pragma unroll
@@ -292,45 +238,130 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
           *reinterpret_cast<float4*>(p + d) =
               make_float4(o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv, o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv);
       }
+  }
+};
+
+// The tile of rows that a workgroup takes and the keys that they see.
+struct RowTile {
+  Span seq;
+  int rows;         // of the sequence and key head
+  int tile0;        // the tile's first row
+  int keys, first;  // keys of the sequence, and the place of its first row among them
+  const int32_t* table;
+
+  // false: no tile at this slot
+  template <int SRC>
+  __device__ __forceinline__ bool find(const RowsArgs& a, int slot, int shift) {
+    const int group = static_cast<int>(a.group.d);
+    int first_slot = 0;
+    const int b = find_sequence(a.cu, a.batch, a.tokens, group, shift, slot, first_slot);
+    if (b < 0) return false;
+    seq = sequence(a.cu, b, a.tokens);
+    const int new_rows = seq.end - seq.begin;
+    rows = new_rows * group;
+    tile0 = (slot - first_slot) << shift;
+    if (tile0 >= rows) return false;
+    keys = new_rows;
+    first = 0;
+    table = nullptr;
+    if constexpr (SRC != kDense) {
+      // a length past what the block table's row can hold is taken as that
+      const int64_t cap = a.table_stride << a.page_shift;
+      keys = max(a.kv_lens[b], 0);
+      if (keys > cap) keys = static_cast<int>(cap);
+      first = keys - new_rows;
+      table = a.table + b * a.table_stride;
+    }
+    return true;
+  }
+  __device__ __forceinline__ int limit(const RowsArgs& a, int r) const {  // last visible key of row r
+    return a.causal ? min(first + divide(min(r, rows - 1), a.group), keys - 1) : keys - 1;
+  }
+  // Parts: z takes keys z * part .. (z + 1) * part - 1, the last part all that follow. False: nothing for this part to write (a
+  // sequence that the first part covers is written whole by it; the join goes by the same rule).
+  __device__ __forceinline__ bool part(const RowsArgs& a, int z, int& kbegin, int& kend, bool& whole) const {
+    whole = a.splits == 1 || keys <= a.part_keys;
+    if (whole) return z == 0;
+    kbegin = z * a.part_keys;
+    if (z + 1 < a.splits) kend = min(kend, kbegin + a.part_keys);
+    return kbegin < keys;
+  }
+};
+
+template <typename T, int DH, int SRC, int W>
+__global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArgs a) {
+  constexpr int BYTES = kBlock * DH * 2;  // one block of keys, or of values
+  constexpr int ROWS = 32 * W;
+  static_assert((ROWS & (ROWS - 1)) == 0, "rows per workgroup: a power of two");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Neighbouring workgroups take neighbouring key heads of one slot: with the dispatch order over the 8 XCDs, an XCD sees few heads'
+  // keys and values at a time. The last slots, a causal sequence's longest, go first.
+  const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int slot = a.slots - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
+  RowTile tile;
+  if (!tile.find<SRC>(a, slot, __builtin_ctz(ROWS))) return;
+  int kbegin = 0, kend = tile.limit(a, tile.tile0 + ROWS - 1) + 1;
+  bool whole;
+  if (!tile.part(a, static_cast<int>(blockIdx.z), kbegin, kend, whole)) return;
+
+  const int r0 = tile.tile0 + wave * 32, r = r0 + l32;
+  const bool live = r < tile.rows;
+  const int lim = tile.limit(a, r);
+  const int lim_low = tile.limit(a, r0), lim_high = tile.limit(a, r0 + 31);  // rows are in order of their tokens
+  const int token = divide(min(r, tile.rows - 1), a.group);
+  const int group = static_cast<int>(a.group.d);
+  const int head = kv_head * group + (min(r, tile.rows - 1) - token * group);
+  const int64_t trow = tile.seq.begin + token;
+
+  u32x4_t qf[DH / 16];
+  {
+    const uint16_t* qr = a.q + trow * a.ldq + static_cast<int64_t>(head) * a.dh;
+#pragma unroll
+    for (int s = 0; s < DH / 16; ++s) qf[s] = load_chunk(qr + 16 * s + 8 * hi, live && 16 * s + 8 * hi < a.dh);
+  }
+
+  const float c = a.scale * kLog2e;
+  RowState<T, DH> state;
+  KvStage<T, DH, SRC, W * 64, kBlock> stage;
+  const TileReader<DH> tiles(lds, lane);
+  uint64_t there = ~uint64_t{0};
+  if (kbegin < kend) {
+    stage.look_up(a, tile.table, kbegin, kend, tid);
+    stage.load(a, tile.seq.begin, tile.table, kv_head, kbegin, kend, tid);
+    stage.store(lds, lds + BYTES, tid);
+    if constexpr (SRC != kDense) there = stage.there;
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int kb = kbegin; kb < kend; kb += kBlock) {
+    const bool more = kb + kBlock < kend;
+    if (more) stage.load(a, tile.seq.begin, tile.table, kv_head, kb + kBlock, kend, tid);
+    if (kb <= lim_high) {
+      const int kbuf = buf * 2 * BYTES;
+      state.template block<2>(tiles, kbuf, kbuf + BYTES, qf, c, kb, kb + kBlock - 1 > lim_low || there != ~uint64_t{0}, lim, there,
+                              hi);
+    }
+    if (more) {
+      unsigned char* next = lds + (buf ^ 1) * 2 * BYTES;
+      stage.store(next, next + BYTES, tid);
+      if constexpr (SRC != kDense) there = stage.there;
+    }
+    __syncthreads();
+    buf ^= 1;
+  }
+
+  float inv, lse2;
+  state.finish(inv, lse2);
+  if (!live) return;
+  if (!whole) {
+    state.write_part(a, (static_cast<int64_t>(blockIdx.z) * a.tokens + trow) * a.heads + head, inv, lse2, hi);
     return;
   }
-  store_row<T, DH>(a.out + trow * a.ldo + static_cast<int64_t>(head) * a.dh, o, inv, hi, a.dh);
+  store_row<T, DH>(a.out + trow * a.ldo + static_cast<int64_t>(head) * a.dh, state.o, inv, hi, a.dh);
   if (a.lse != nullptr && hi == 0) a.lse[trow * a.heads + head] = lse2 * kLn2;
-}
-
-// The parts' weighted sum: out = sum_z w_z out_z / sum_z w_z, w_z = 2^(lse_z - max lse). One wave per (token, head), 4 values a lane.
-template <typename T>
-__global__ __launch_bounds__(256) void attention_join_kernel(const RowsArgs a) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
-  if (row >= rows) return;
-  const int64_t token = row / a.heads;
-  // rows outside the sequences stay as they are
-  if (token < a.cu[0] || token >= a.cu[a.batch]) return;
-  const int lane = threadIdx.x & 63;
-  float top = -__builtin_inff();
-  for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_lse[z * rows + row]);
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
-  float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int d = lane * 4;
-  for (int z = 0; z < a.splits; ++z) {
-    const float w = __builtin_amdgcn_exp2f(a.part_lse[z * rows + row] - ref);
-    sum += w;
-    if (w != 0.0f && d < a.dh) {
-      const float4 p = *reinterpret_cast<const float4*>(a.part_out + (z * rows + row) * a.dh + d);
-      acc[0] += w * p.x;
-      acc[1] += w * p.y;
-      acc[2] += w * p.z;
-      acc[3] += w * p.w;
-    }
-  }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (d < a.dh) {
-    u32x2_t w;
-    w[0] = store2<T>(acc[0] * inv, acc[1] * inv);
-    w[1] = store2<T>(acc[2] * inv, acc[3] * inv);
-    *reinterpret_cast<u32x2_t*>(a.out + token * a.ldo + (row - token * a.heads) * a.dh + d) = w;
-  }
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -21,6 +21,7 @@ using namespace mfma16;
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int64_t kMaxBlocks = 0xffffff;  // of 256 threads: a grid dimension holds fewer than 2^32 threads
 constexpr float kLn2 = 0.69314718055994530942f;
 
 // r / d for 0 <= r < 2^31 as (r * mul) >> shift: with 2^(l-1) < d <= 2^l, mul = ceil(2^(31+l) / d) exceeds the quotient by less

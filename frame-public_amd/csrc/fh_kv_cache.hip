@@ -166,7 +166,7 @@ fh_status run(const std::string& fn, const fh_paged_cache* c, void* k, int64_t k
   a.page_shift = page_shift(c->page_size);
   auto launch = [&]<typename T, int LANES, bool E4M3>() {
     const int64_t blocks = (tokens * c->kv_heads * LANES + 255) / 256;
-    if (blocks > 0x7fffffff) return fail(FH_INVALID_ARGUMENT, fn + ": too many rows");
+    if (blocks > kMaxBlocks) return fail(FH_INVALID_ARGUMENT, fn + ": too many rows");
     hipLaunchKernelGGL((kv_cache_kernel<T, LANES, E4M3, WRITE>), dim3(static_cast<uint32_t>(blocks), 2), dim3(256), 0,
                        static_cast<hipStream_t>(stream), a);
     return launch_status("kv_cache_kernel launch");

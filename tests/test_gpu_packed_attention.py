@@ -180,6 +180,17 @@ def test_packed_gradients(hip, case):
         ref.check(ref.values(g, p.dtype)[p.inside], total[p.inside], ref.rounded(total, tol, p.dtype)[p.inside], "d" + name)
 
 
+@pytest.mark.parametrize("dtype,dh", [(BF16, 128), (F16, 64)])
+def test_packed_gradients_of_single_tokens(hip, dtype, dh):
+    # a softmax over one key has no derivative: dq and dk are zeros, not the noise of dp - D
+    say(f"packed gradients of single tokens dtype={dtype} dh={dh}")
+    p = Packed(hip, dtype, [1, 1, 0, 1], 4, 2, dh, 1)
+    dq, dk, dv = p.backward(*p.forward())
+    assert not (dq & 0x7fff).any() and not (dk & 0x7fff).any()
+    total, tol = p.want_grads()
+    ref.check(ref.values(dv, dtype), total[2], ref.rounded(total[2], tol[2], dtype), "dv")
+
+
 @pytest.mark.parametrize("std,scale", [(4.0, 0.125), (1.0, 1e-6), (0.01, 3.0)])
 def test_packed_score_ranges(hip, std, scale):
     # wide scores (most probabilities vanish, the running maximum moves often), all but equal ones, tiny inputs
