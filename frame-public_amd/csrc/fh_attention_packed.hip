@@ -7,10 +7,11 @@
 // dout (7 products instead of the 5 that one kernel with atomic sums of dq would need), so that every sum has one owner and one
 // order: results do not depend on scheduling, and no fp32 copy of dq is needed.
 //   attention_dq_kernel:  32 rows per wave as in the forward; D is formed from its rows and kept for the second kernel.
-//   attention_dkv_kernel: 32 keys per wave, keys and values in registers, blocks of 32 rows of q and dout in LDS.
+//   attention_dkv_kernel: 32 keys per wave, keys and values in registers, blocks of 64 rows of q and dout in LDS.
 // p and ds are rounded to the storage type as operands of the second products; everything else is fp32.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -39,7 +40,11 @@ struct GradArgs {
   int causal;
   float scale;
   int slots;
+  int parts;    // of the rows of a key tile
+  float* part;  // parts > 1: [parts][dv, dk][tokens][kv_heads * dh]
 };
+
+constexpr int kWholeBlocks = 24;  // key tiles of no more blocks of rows are not cut
 
 template <typename T, int DH, int W>
 __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs a) {
@@ -177,19 +182,37 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   if (live) store_row<T, DH>(a.dq + trow * a.ldq + static_cast<int64_t>(head) * a.dh, acc, a.scale, hi, a.dh);
 }
 
-constexpr int kGradRows = 32;  // rows of q and dout per block
+constexpr int kGradRows = 64;  // rows of q and dout per block
+constexpr int kGradKeys = 128;
 
-template <typename T, int DH, int W>
-__global__ __launch_bounds__(W * 64, 1) void attention_dkv_kernel(const GradArgs a) {
-  constexpr int BYTES = kGradRows * DH * 2;
-  constexpr int KEYS = 32 * W, SHIFT = __builtin_ctz(KEYS);
-  constexpr int CH = DH / 8, PASS = W * 64 / CH, N = (kGradRows + PASS - 1) / PASS;
+// The rows [begin, end) that part z of a key tile sums over, in whole blocks; `whole`: the first part takes them all.
+struct RowRange {
+  int begin, end;
+  bool whole;
+};
+__device__ __forceinline__ RowRange row_range(const GradArgs& a, int tile0, int rows, int z) {
+  const int first = a.causal ? tile0 * static_cast<int>(a.group.d) / kGradRows : 0;  // rows that see key u: r >= u * group
+  const int blocks = (rows + kGradRows - 1) / kGradRows - first;
+  if (a.parts == 1 || blocks <= kWholeBlocks) return {first * kGradRows, z == 0 ? rows : 0, true};
+  const int per = (blocks + a.parts - 1) / a.parts;
+  return {(first + z * per) * kGradRows, min(rows, (first + (z + 1) * per) * kGradRows), false};
+}
+
+// 128 keys per workgroup of 8 waves: waves w and w + 4 own the same 32 keys and sit on one SIMD; the first sums dv (two products:
+// q k and p dout), the second dk (three: q k, dout v and ds q). Forming q k twice leaves each wave one accumulator, which is what lets
+// two waves share a SIMD's registers and hide each other's waits; with both sums in one wave (400 registers, one wave per SIMD) the
+// same work took more than twice as long.
+template <typename T, int DH>
+__global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a) {
+  constexpr int BYTES = kGradRows * DH * 2, SHIFT = __builtin_ctz(kGradKeys);
+  constexpr int CH = DH / 8, PASS = 512 / CH, N = kGradRows / PASS;
   static_assert(kGradRows % PASS == 0, "whole passes");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
-  __shared__ float stats[2][2][kGradRows];  // per buffer: lse (base 2), D
+  __shared__ __attribute__((aligned(16))) float stats[2][2][kGradRows];  // per buffer: lse (base 2), D
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool for_dk = wave >= 4;
   const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
   const int slot = static_cast<int>(blockIdx.x) / a.kv_heads;  // a causal sequence's first keys are seen by most rows
   const int group = static_cast<int>(a.group.d);
@@ -198,10 +221,12 @@ __global__ __launch_bounds__(W * 64, 1) void attention_dkv_kernel(const GradArgs
   if (b < 0) return;
   const Span seq = sequence(a.cu, b, a.tokens);
   const int keys = seq.end - seq.begin, rows = keys * group;
-  const int tile0 = (slot - first_slot) * KEYS;
+  const int tile0 = (slot - first_slot) * kGradKeys;
   if (tile0 >= keys) return;
+  const RowRange range = row_range(a, tile0, rows, static_cast<int>(blockIdx.z));
+  if (range.whole && blockIdx.z != 0) return;
 
-  const int k0 = tile0 + wave * 32, key = k0 + l32;
+  const int k0 = tile0 + (wave & 3) * 32, key = k0 + l32;
   const bool live = key < keys;
   const int64_t krow = seq.begin + (live ? key : 0);
   const int64_t col = static_cast<int64_t>(kv_head) * a.dh;
@@ -212,8 +237,6 @@ __global__ __launch_bounds__(W * 64, 1) void attention_dkv_kernel(const GradArgs
     kf[s] = load_chunk(a.k + krow * a.ldk + col + d, live && d < a.dh);
     vf[s] = load_chunk(a.v + krow * a.ldv + col + d, live && d < a.dh);
   }
-  // rows that see key u: r >= u * group (causal)
-  const int rbegin = a.causal ? tile0 * group / kGradRows * kGradRows : 0;
   const int my_first = a.causal ? key * group : 0;
 
   const int chunk = tid % CH, srow = tid / CH;
@@ -252,69 +275,117 @@ __global__ __launch_bounds__(W * 64, 1) void attention_dkv_kernel(const GradArgs
     if (tid < 2 * kGradRows) stats[buf][tid / kGradRows][tid & (kGradRows - 1)] = stat;
   };
 
-  f32x16_t dk[DH / 32], dv[DH / 32];
+  f32x16_t acc[DH / 32];
 #pragma unroll
-  for (int dt = 0; dt < DH / 32; ++dt) {
-    clear(dk[dt]);
-    clear(dv[dt]);
-  }
+  for (int dt = 0; dt < DH / 32; ++dt) clear(acc[dt]);
   const float c = a.scale * kLog2e;
   const TileReader<DH> tiles(lds, lane);
-  load(rbegin);
-  store(0);
+  if (range.begin < range.end) {
+    load(range.begin);
+    store(0);
+  }
   __syncthreads();
   int buf = 0;
-  for (int rb = rbegin; rb < rows; rb += kGradRows) {
-    const bool more = rb + kGradRows < rows;
+  for (int rb = range.begin; rb < range.end; rb += kGradRows) {
+    const bool more = rb + kGradRows < range.end;
     if (more) load(rb + kGradRows);
-    // the wave's first key is seen from row k0 * group on
-    if (!a.causal || rb + kGradRows > k0 * group) {
-      const int qbuf = buf * 2 * BYTES, gbuf = qbuf + BYTES;
-      f32x16_t s, dp;
-      clear(s);
-      clear(dp);
+    const int qbuf = buf * 2 * BYTES, gbuf = qbuf + BYTES;
 #pragma unroll
-      for (int i = 0; i < DH / 16; ++i) {
-        mfma32<T>(tiles.rows(qbuf, 0, i), kf[i], s);
-        mfma32<T>(tiles.rows(gbuf, 0, i), vf[i], dp);
-      }
-      const bool edge = a.causal && rb < (k0 + 31) * group;
+    for (int t = 0; t < kGradRows / 32; ++t) {
+      const int r0 = rb + 32 * t;
+      // the wave's first key is seen from row k0 * group on
+      if (a.causal && r0 + 32 <= k0 * group) continue;
+      const bool edge = a.causal && r0 < (k0 + 31) * group;
+      f32x16_t s;
+      clear(s);
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i) mfma32<T>(tiles.rows(qbuf, 32 * t, i), kf[i], s);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float4 ls = *reinterpret_cast<const float4*>(&stats[buf][0][8 * q + 4 * hi]);
-        const float4 dl = *reinterpret_cast<const float4*>(&stats[buf][1][8 * q + 4 * hi]);
-        const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dd[4] = {dl.x, dl.y, dl.z, dl.w};
+        const float4 ls = *reinterpret_cast<const float4*>(&stats[buf][0][32 * t + 8 * q + 4 * hi]);
+        const float lv[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int x = 4 * q + j;
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -lv[j]));
-          float d = p * (dp[x] - dd[j]);
-          if (edge) {
-            const bool seen = rb + result_row(x, hi) >= my_first;
-            p = seen ? p : 0.0f;
-            d = seen ? d : 0.0f;
-          }
-          s[x] = p;
-          dp[x] = d;
+        for (int j = 0; j < 4; ++j) s[4 * q + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + j], c, -lv[j]));
+      }
+      int operand = gbuf;
+      if (for_dk) {
+        operand = qbuf;
+        f32x16_t dp;
+        clear(dp);
+#pragma unroll
+        for (int i = 0; i < DH / 16; ++i) mfma32<T>(tiles.rows(gbuf, 32 * t, i), vf[i], dp);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 dl = *reinterpret_cast<const float4*>(&stats[buf][1][32 * t + 8 * q + 4 * hi]);
+          const float dd[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[4 * q + j] *= dp[4 * q + j] - dd[j];
         }
+      }
+      if (edge) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[x] = r0 + result_row(x, hi) >= my_first ? s[x] : 0.0f;
       }
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const u32x4_t p = pack_slice<T>(s, hf), ds = pack_slice<T>(dp, hf);
+        const u32x4_t p = pack_slice<T>(s, hf);
 #pragma unroll
-        for (int dt = 0; dt < DH / 32; ++dt) {
-          mfma32<T>(tiles.columns(gbuf, 16 * hf, dt), p, dv[dt]);
-          mfma32<T>(tiles.columns(qbuf, 16 * hf, dt), ds, dk[dt]);
-        }
+        for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(tiles.columns(operand, 32 * t + 16 * hf, dt), p, acc[dt]);
       }
     }
     if (more) store(buf ^ 1);
     __syncthreads();
     buf ^= 1;
   }
-  if (live) {
-    store_row<T, DH>(a.dk + krow * a.ldk + col, dk, a.scale, hi, a.dh);
-    store_row<T, DH>(a.dv + krow * a.ldv + col, dv, 1.0f, hi, a.dh);
+  if (!live) return;
+  const float factor = for_dk ? a.scale : 1.0f;
+  if (range.whole) {
+    store_row<T, DH>(for_dk ? a.dk + krow * a.ldk + col : a.dv + krow * a.ldv + col, acc, factor, hi, a.dh);
+    return;
+  }
+  float* p = a.part + ((static_cast<int64_t>(blockIdx.z) * 2 + for_dk) * a.tokens + krow) * a.kv_heads * a.dh + col;
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * dt + 8 * q + 4 * hi;
+      if (d < a.dh)
+        *reinterpret_cast<float4*>(p + d) = make_float4(acc[dt][4 * q] * factor, acc[dt][4 * q + 1] * factor,
+                                                        acc[dt][4 * q + 2] * factor, acc[dt][4 * q + 3] * factor);
+    }
+}
+
+// dk and dv of the key tiles whose rows were cut into parts: the parts' sum, in their order. One wave per key row of all heads.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_dkv_join_kernel(const GradArgs a) {
+  const int token = static_cast<int>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (token >= a.tokens) return;
+  const int b = sequence_of(a.cu, a.batch, token);
+  if (b < 0) return;
+  const Span seq = sequence(a.cu, b, a.tokens);
+  if (token < seq.begin || token >= seq.end) return;
+  const int rows = (seq.end - seq.begin) * static_cast<int>(a.group.d);
+  const int tile0 = (token - seq.begin) / kGradKeys * kGradKeys;
+  if (row_range(a, tile0, rows, 0).whole) return;
+  const int width = a.kv_heads * a.dh;
+  const int64_t stride = static_cast<int64_t>(a.tokens) * width;
+  for (int i = (threadIdx.x & 63) * 4; i < 2 * width; i += 256) {
+    const int which = i >= width;  // 0: dv, 1: dk
+    const int d = i - which * width;
+    const float* p = a.part + which * stride + static_cast<int64_t>(token) * width + d;
+    float4 t = *reinterpret_cast<const float4*>(p);
+    for (int z = 1; z < a.parts; ++z) {
+      const float4 y = *reinterpret_cast<const float4*>(p + z * 2 * stride);
+      t.x += y.x;
+      t.y += y.y;
+      t.z += y.z;
+      t.w += y.w;
+    }
+    u32x2_t w;
+    w[0] = store2<T>(t.x, t.y);
+    w[1] = store2<T>(t.z, t.w);
+    uint16_t* out = which ? a.dk + token * a.ldk : a.dv + token * a.ldv;
+    *reinterpret_cast<u32x2_t*>(out + d) = w;
   }
 }
 
@@ -331,7 +402,7 @@ fh_status check_packed(const char* fn, const fh_packed_attention* g) {
   if (g->heads > 65535 || g->tokens > 0x7fffffff || g->batch > 0x3fffffff ||
       (g->tokens + 256) * g->heads + g->batch * g->kv_heads > 0x7fffffff)
     return fail(FH_INVALID_ARGUMENT, f + ": more than 2^31 rows (tokens x heads)");
-  if (g->tokens * g->heads / 128 + (g->batch + 1) * g->kv_heads > kMaxBlocks)
+  if (g->tokens * g->heads / 128 + (g->batch + 1) * g->kv_heads > kMaxBlocks / 2)
     return fail(FH_INVALID_ARGUMENT, f + ": more rows than one launch takes");
   if (g->q_stride < g->heads * g->dh || g->out_stride < g->heads * g->dh || g->k_stride < g->kv_heads * g->dh ||
       g->v_stride < g->kv_heads * g->dh)
@@ -343,6 +414,17 @@ fh_status check_packed(const char* fn, const fh_packed_attention* g) {
 
 // workgroups of `tile`-row tiles with per_token rows a token
 int64_t slots_for(const fh_packed_attention& g, int64_t per_token, int64_t tile) { return g.tokens * per_token / tile + g.batch; }
+
+int64_t delta_bytes(const fh_packed_attention& g) { return (g.tokens * g.heads * 4 + 15) / 16 * 16; }
+
+// A key tile's rows are cut into parts where the tiles are few: a causal sequence's first keys are seen by all of its rows, so the
+// longest tile would otherwise outlast the others by twice their mean.
+int64_t grad_parts(const fh_packed_attention& g) {
+  const int64_t tiles = (g.tokens + kGradKeys - 1) / kGradKeys * g.kv_heads, cus = device_cu_count();
+  const int64_t blocks = g.tokens * (g.heads / g.kv_heads) / kGradRows;
+  if (tiles >= 3 * cus || blocks <= kWholeBlocks) return 1;
+  return std::max<int64_t>(1, std::min<int64_t>((3 * cus + tiles - 1) / tiles, 4));
+}
 
 }  // namespace
 }  // namespace fh
@@ -395,7 +477,8 @@ extern "C" fh_status fh_attention_packed_fwd(const fh_packed_attention* g, const
 
 extern "C" int64_t fh_attention_packed_grad_workspace(const fh_packed_attention* g) {
   if (check_packed("fh_attention_packed_grad_workspace", g) != FH_OK) return -1;
-  return g->tokens * g->heads * 4;
+  const int64_t parts = grad_parts(*g);
+  return delta_bytes(*g) + (parts > 1 ? parts * 2 * g->tokens * g->kv_heads * g->dh * 4 : 0);
 }
 
 extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, const void* q, const void* k, const void* v,
@@ -424,6 +507,8 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
   a.dv = static_cast<uint16_t*>(dv);
   a.lse = lse;
   a.delta = static_cast<float*>(workspace);
+  a.parts = static_cast<int>(grad_parts(*g));
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(*g));
   a.cu = cu_seqlens;
   a.ldq = g->q_stride;
   a.ldk = g->k_stride;
@@ -444,10 +529,13 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
     hipLaunchKernelGGL((attention_dq_kernel<T, DH, W>), dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads)),
                        dim3(W * 64), 0, s, a);
     if (fh_status st = launch_status("attention_dq_kernel launch"); st != FH_OK) return st;
-    a.slots = static_cast<int>(slots_for(*g, 1, 32 * W));
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DH, W>), dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads)),
-                       dim3(W * 64), 0, s, a);
-    return launch_status("attention_dkv_kernel launch");
+    a.slots = static_cast<int>(slots_for(*g, 1, kGradKeys));
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DH>),
+                       dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads), 1, static_cast<uint32_t>(a.parts)),
+                       dim3(512), 0, s, a);
+    if (fh_status st = launch_status("attention_dkv_kernel launch"); st != FH_OK || a.parts == 1) return st;
+    hipLaunchKernelGGL((attention_dkv_join_kernel<T>), dim3(static_cast<uint32_t>((g->tokens + 3) / 4)), dim3(256), 0, s, a);
+    return launch_status("attention_dkv_join_kernel launch");
   };
   if (g->dtype == FH_BF16)
     return g->dh <= 64 ? launch.template operator()<bf16_t, 64>() : launch.template operator()<bf16_t, 128>();

@@ -129,15 +129,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const RowsArgs a) {
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
   if (row >= rows) return;
   const int token = static_cast<int>(row / a.heads);
-  // the last sequence that begins at the token or before it
-  int found = 0;
-  for (int base = 0; base < a.batch; base += 64) {
-    const int i = base + static_cast<int>(threadIdx.x & 63);
-    const uint64_t m = __ballot(i < a.batch && a.cu[min(i, a.batch)] <= token);
-    found += __popcll(m);
-    if (m != ~uint64_t{0}) break;
-  }
-  const int b = __builtin_amdgcn_readfirstlane(found - 1);
+  const int b = sequence_of(a.cu, a.batch, token);
   if (b < 0) return;
   const Span seq = sequence(a.cu, b, a.tokens);
   if (token < seq.begin || token >= seq.end) return;  // rows outside the sequences stay as they are

@@ -73,6 +73,18 @@ __device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, int r
   return b;
 }
 
+// The last sequence that begins at `token` or before it (the one that holds it, if any does), or -1.
+__device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int token) {
+  int found = 0;
+  for (int base = 0; base < batch; base += 64) {
+    const int i = base + static_cast<int>(threadIdx.x & 63);
+    const uint64_t m = __ballot(i < batch && cu[min(i, batch)] <= token);
+    found += __popcll(m);
+    if (m != ~uint64_t{0}) break;
+  }
+  return __builtin_amdgcn_readfirstlane(found - 1);
+}
+
 // LDS tiles: rows of DH 16-bit values, 16-byte chunks XORed with swz(row). 16 rows' equal chunks (a row fragment read: lane -> row
 // l % 32, 16 bytes) fall on 16 different 16-byte columns of the 64 banks, and the 64-byte windows of 4 consecutive rows (a transposed
 // read) on 4 different ones, so both kinds of read are free of conflicts.
