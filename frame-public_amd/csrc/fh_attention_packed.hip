@@ -58,9 +58,8 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   const int slot = a.slots - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
   const int group = static_cast<int>(a.group.d);
   int first_slot = 0;
-  const int b = find_sequence(a.cu, a.batch, a.tokens, group, SHIFT, slot, first_slot);
-  if (b < 0) return;
-  const Span seq = sequence(a.cu, b, a.tokens);
+  Span seq;
+  if (find_sequence(a.cu, a.batch, a.tokens, group, SHIFT, slot, first_slot, seq) < 0) return;
   const int keys = seq.end - seq.begin, rows = keys * group;
   const int tile0 = (slot - first_slot) * ROWS;
   if (tile0 >= rows) return;
@@ -217,9 +216,8 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
   const int slot = static_cast<int>(blockIdx.x) / a.kv_heads;  // a causal sequence's first keys are seen by most rows
   const int group = static_cast<int>(a.group.d);
   int first_slot = 0;
-  const int b = find_sequence(a.cu, a.batch, a.tokens, 1, SHIFT, slot, first_slot);
-  if (b < 0) return;
-  const Span seq = sequence(a.cu, b, a.tokens);
+  Span seq;
+  if (find_sequence(a.cu, a.batch, a.tokens, 1, SHIFT, slot, first_slot, seq) < 0) return;
   const int keys = seq.end - seq.begin, rows = keys * group;
   const int tile0 = (slot - first_slot) * kGradKeys;
   if (tile0 >= keys) return;

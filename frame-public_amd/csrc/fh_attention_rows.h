@@ -254,9 +254,8 @@ struct RowTile {
   __device__ __forceinline__ bool find(const RowsArgs& a, int slot, int shift) {
     const int group = static_cast<int>(a.group.d);
     int first_slot = 0;
-    const int b = find_sequence(a.cu, a.batch, a.tokens, group, shift, slot, first_slot);
+    const int b = find_sequence(a.cu, a.batch, a.tokens, group, shift, slot, first_slot, seq);
     if (b < 0) return false;
-    seq = sequence(a.cu, b, a.tokens);
     const int new_rows = seq.end - seq.begin;
     rows = new_rows * group;
     tile0 = (slot - first_slot) << shift;

@@ -52,25 +52,29 @@ __device__ __forceinline__ Span sequence(const int32_t* cu, int b, int rows) {
 // before slot(b + 1). Slots that no tile takes end at once. Every wave looks 64 sequences up at a time.
 // Host: floor(rows * per_token / tile) + batch slots.
 __device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, int rows, int per_token, int tile_shift, int slot,
-                                             int& first_slot) {
+                                             int& first_slot, Span& seq) {
   const int lane = threadIdx.x & 63;
-  int found = 0;
+  int found = 0, begin = 0, end = 0;
   for (int base = 0; base < batch; base += 64) {
     const int b = base + lane;
     bool before = false;
+    int s = 0, e = 0;
     if (b < batch) {
-      const int64_t at = static_cast<int64_t>(min(max(cu[b], 0), rows)) * per_token;
-      before = (at >> tile_shift) + b <= slot;
+      s = min(max(cu[b], 0), rows);
+      e = min(max(cu[b + 1], s), rows);
+      before = ((static_cast<int64_t>(s) * per_token) >> tile_shift) + b <= slot;
     }
-    const uint64_t m = __ballot(before);
-    found += __popcll(m);
-    if (m != ~uint64_t{0}) break;
+    const int n = __popcll(__ballot(before));
+    if (n > 0) {
+      begin = __builtin_amdgcn_readlane(s, n - 1);
+      end = __builtin_amdgcn_readlane(e, n - 1);
+    }
+    found += n;
+    if (n < 64) break;
   }
-  if (found == 0) return -1;
-  const int b = __builtin_amdgcn_readfirstlane(found - 1);
-  const int64_t at = static_cast<int64_t>(min(max(cu[b], 0), rows)) * per_token;
-  first_slot = static_cast<int>(at >> tile_shift) + b;
-  return b;
+  seq = {begin, end};
+  first_slot = static_cast<int>((static_cast<int64_t>(begin) * per_token) >> tile_shift) + found - 1;
+  return found - 1;
 }
 
 // The last sequence that begins at `token` or before it (the one that holds it, if any does), or -1.

@@ -7,6 +7,7 @@
 // they are bound by memory, and by the launch for a step's few rows.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "fh_attention_rows.h"
@@ -84,53 +85,89 @@ __device__ __forceinline__ u32x2_t narrow_e4m3(const float (&v)[8], uint32_t byt
   return w;
 }
 
-// One row (token, head) of keys or values per LANES lanes. blockIdx.y: 0 keys, 1 values.
+// A workgroup takes `per` tokens: their cache rows are looked up once, a thread each, then their rows (token, head) move LANES lanes
+// a row, keys and values by the same thread, kUnroll rows of both in flight.
+constexpr int kUnroll = 4, kMostTokens = 32;
+
 template <typename T, int LANES, bool E4M3, bool WRITE>
-__global__ __launch_bounds__(256) void kv_cache_kernel(const CacheArgs a) {
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;
+__global__ __launch_bounds__(256) void kv_cache_kernel(const CacheArgs a, int per, Divider by_heads) {
+  __shared__ int64_t slots[kMostTokens];
+  __shared__ int owned[kMostTokens];
+  const int t0 = static_cast<int>(blockIdx.x) * per;
+  const int count = min(per, a.tokens - t0);
+  if (static_cast<int>(threadIdx.x) < count) {
+    bool in_sequence;
+    slots[threadIdx.x] = slot_of<WRITE>(a, t0 + static_cast<int>(threadIdx.x), in_sequence);
+    owned[threadIdx.x] = in_sequence;
+  }
+  __syncthreads();
+  constexpr int ROWS = 256 / LANES;
   const int chunk = threadIdx.x % LANES;
-  const int64_t token = row / a.kv_heads;
-  const bool inside = token < a.tokens;
-  const int head = static_cast<int>(row - token * a.kv_heads);
-  const bool values = blockIdx.y != 0;
-  bool in_sequence = false;
-  const int64_t slot = inside ? slot_of<WRITE>(a, static_cast<int>(token), in_sequence) : -1;
-  const bool there = slot >= 0 && chunk * 8 < a.dh;
-  const int64_t crow = slot * a.kv_heads + head;
-  uint16_t* x = (values ? a.xv + token * a.ldv : a.xk + token * a.ldk) + static_cast<int64_t>(head) * a.dh + chunk * 8;
-  void* cache = values ? a.v : a.k;
-  uint8_t* scales = values ? a.v_scale : a.k_scale;
-  if constexpr (WRITE) {
-    const u32x4_t w = load_chunk(x, there);
-    if constexpr (!E4M3) {
-      if (there) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(cache) + crow * a.dh + chunk * 8) = w;
-    } else {
-      float v[8];
-      unpack_vec<T>(uint4{w[0], w[1], w[2], w[3]}, v);
-      float top = 0.0f;
+  const bool inside = chunk * 8 < a.dh;
+  const int rows = count * a.kv_heads;
+  for (int r0 = static_cast<int>(threadIdx.x) / LANES; r0 < (rows + ROWS - 1) / ROWS * ROWS; r0 += kUnroll * ROWS) {
+    bool there[kUnroll], mine[kUnroll];
+    int64_t at[kUnroll], crow[kUnroll], xk[kUnroll], xv[kUnroll];
+    u32x4_t w[kUnroll][2];
+    u32x2_t c[kUnroll][2];
+    uint32_t byte[kUnroll][2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float s = __builtin_fabsf(v[j]);
-        if (s < __builtin_inff()) top = fmaxf(top, s);
-      }
+    for (int u = 0; u < kUnroll; ++u) {
+      const int r = min(r0 + u * ROWS, rows - 1), t = divide(r, by_heads), head = r - t * a.kv_heads;
+      const bool row = r0 + u * ROWS < rows;
+      mine[u] = row && inside && owned[t];
+      there[u] = row && inside && slots[t] >= 0;
+      crow[u] = slots[t] * a.kv_heads + head;
+      at[u] = crow[u] * a.dh + chunk * 8;
+      const int64_t col = static_cast<int64_t>(head) * a.dh + chunk * 8;
+      xk[u] = (t0 + t) * a.ldk + col;
+      xv[u] = (t0 + t) * a.ldv + col;
+      if constexpr (WRITE) {
+        w[u][0] = load_chunk(a.xk + xk[u], there[u]);
+        w[u][1] = load_chunk(a.xv + xv[u], there[u]);
+      } else if constexpr (E4M3) {
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-      if (there) {
-        const uint32_t byte = scale_byte(top);
-        *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(cache) + crow * a.dh + chunk * 8) = narrow_e4m3<T>(v, byte);
-        if (chunk == 0) scales[crow] = static_cast<uint8_t>(byte);
+        for (int i = 0; i < 2; ++i) {
+          c[u][i] = u32x2_t{0, 0};
+          byte[u][i] = 127;
+          if (there[u]) {
+            c[u][i] = *reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(i ? a.v : a.k) + at[u]);
+            byte[u][i] = (i ? a.v_scale : a.k_scale)[crow[u]];
+          }
+        }
+      } else {
+        w[u][0] = load_chunk(static_cast<const uint16_t*>(a.k) + at[u], there[u]);
+        w[u][1] = load_chunk(static_cast<const uint16_t*>(a.v) + at[u], there[u]);
       }
     }
-  } else {
-    u32x4_t w{0, 0, 0, 0};  // positions without a cached row read as zeros
-    if (there) {
-      if constexpr (E4M3)
-        w = widen_e4m3<T>(*reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(cache) + crow * a.dh + chunk * 8),
-                          __uint_as_float(static_cast<uint32_t>(scales[crow]) << 23));
-      else
-        w = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(cache) + crow * a.dh + chunk * 8);
-    }
-    if (in_sequence && chunk * 8 < a.dh) *reinterpret_cast<u32x4_t*>(x) = w;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (!WRITE) {
+          // positions without a cached row read as zeros
+          if constexpr (E4M3) w[u][i] = widen_e4m3<T>(c[u][i], __uint_as_float(byte[u][i] << 23));
+          if (mine[u]) *reinterpret_cast<u32x4_t*>(i ? a.xv + xv[u] : a.xk + xk[u]) = w[u][i];
+        } else if constexpr (!E4M3) {
+          if (there[u]) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(i ? a.v : a.k) + at[u]) = w[u][i];
+        } else {
+          float v[8];
+          unpack_vec<T>(uint4{w[u][i][0], w[u][i][1], w[u][i][2], w[u][i][3]}, v);
+          float top = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float s = __builtin_fabsf(v[j]);
+            if (s < __builtin_inff()) top = fmaxf(top, s);
+          }
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+          const uint32_t scale = scale_byte(top);
+          if (there[u]) {
+            *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(i ? a.v : a.k) + at[u]) = narrow_e4m3<T>(v, scale);
+            if (chunk == 0) (i ? a.v_scale : a.k_scale)[crow[u]] = static_cast<uint8_t>(scale);
+          }
+        }
+      }
   }
 }
 
@@ -165,10 +202,12 @@ fh_status run(const std::string& fn, const fh_paged_cache* c, void* k, int64_t k
   a.pages = static_cast<int>(c->pages);
   a.page_shift = page_shift(c->page_size);
   auto launch = [&]<typename T, int LANES, bool E4M3>() {
-    const int64_t blocks = (tokens * c->kv_heads * LANES + 255) / 256;
+    // a few tokens per workgroup once every CU has several of them
+    const int64_t per = std::min<int64_t>(kMostTokens, std::max<int64_t>(1, tokens / (8 * device_cu_count())));
+    const int64_t blocks = (tokens + per - 1) / per;
     if (blocks > kMaxBlocks) return fail(FH_INVALID_ARGUMENT, fn + ": too many rows");
-    hipLaunchKernelGGL((kv_cache_kernel<T, LANES, E4M3, WRITE>), dim3(static_cast<uint32_t>(blocks), 2), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL((kv_cache_kernel<T, LANES, E4M3, WRITE>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), a, static_cast<int>(per), make_divider(static_cast<uint32_t>(c->kv_heads)));
     return launch_status("kv_cache_kernel launch");
   };
   auto typed = [&]<typename T>() {
