@@ -387,6 +387,13 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const GradArgs 
   }
 }
 
+// One wave per row that no sequence covers.
+__global__ __launch_bounds__(256) void packed_clear_kernel(const int32_t* cu, int batch, uint4* x, int rows, int64_t chunks) {
+  const int row = static_cast<int>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= rows || (row >= cu[0] && row < cu[batch])) return;
+  for (int64_t i = threadIdx.x & 63; i < chunks; i += 64) x[row * chunks + i] = uint4{0, 0, 0, 0};
+}
+
 fh_status check_packed(const char* fn, const fh_packed_attention* g) {
   const std::string f(fn);
   if (g == nullptr) return fail(FH_INVALID_ARGUMENT, f + ": null descriptor");
@@ -493,7 +500,7 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
     if (!aligned16(p)) return fail(FH_INVALID_ARGUMENT, fn + ": tensors and the workspace must be 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(cu_seqlens) | reinterpret_cast<uintptr_t>(lse)) % 4 != 0)
     return fail(FH_INVALID_ARGUMENT, fn + ": cu_seqlens and lse must be 4-byte aligned");
-  if (workspace_bytes < fh_attention_packed_grad_workspace(g)) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
+  if (workspace_bytes < g->tokens * g->heads * 4) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
   GradArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);
@@ -505,7 +512,7 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
   a.dv = static_cast<uint16_t*>(dv);
   a.lse = lse;
   a.delta = static_cast<float*>(workspace);
-  a.parts = static_cast<int>(grad_parts(*g));
+  a.parts = workspace_bytes < fh_attention_packed_grad_workspace(g) ? 1 : static_cast<int>(grad_parts(*g));
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(*g));
   a.cu = cu_seqlens;
   a.ldq = g->q_stride;
@@ -538,4 +545,16 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
   if (g->dtype == FH_BF16)
     return g->dh <= 64 ? launch.template operator()<bf16_t, 64>() : launch.template operator()<bf16_t, 128>();
   return g->dh <= 64 ? launch.template operator()<f16_t, 64>() : launch.template operator()<f16_t, 128>();
+}
+
+extern "C" fh_status fh_packed_clear(const int32_t* cu_seqlens, int64_t batch, void* x, int64_t rows, int64_t row_bytes, void* stream) {
+  const std::string fn = "fh_packed_clear";
+  if (batch < 0 || batch > 0x3fffffff || rows < 0 || rows > 4 * kMaxBlocks || row_bytes < 0 || row_bytes % 16 != 0)
+    return fail(FH_INVALID_ARGUMENT, fn + ": bad batch, rows or row_bytes");
+  if (rows == 0 || row_bytes == 0) return FH_OK;
+  if (!cu_seqlens || !x || !aligned16(x) || reinterpret_cast<uintptr_t>(cu_seqlens) % 4 != 0)
+    return fail(FH_INVALID_ARGUMENT, fn + ": null or unaligned pointer");
+  hipLaunchKernelGGL(packed_clear_kernel, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                     cu_seqlens, static_cast<int>(batch), static_cast<uint4*>(x), static_cast<int>(rows), row_bytes / 16);
+  return launch_status("packed_clear_kernel launch");
 }

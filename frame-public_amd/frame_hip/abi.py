@@ -115,6 +115,7 @@ _SIGS = {
     "fh_attention_packed_fwd": (c_int32, [POINTER(PackedAttention)] + [c_void_p] * 7),
     "fh_attention_packed_grad_workspace": (c_int64, [POINTER(PackedAttention)]),
     "fh_attention_packed_grad": (c_int32, [POINTER(PackedAttention)] + [c_void_p] * 11 + [c_int64, c_void_p]),
+    "fh_packed_clear": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p]),
     "fh_kv_cache_write": (c_int32, [POINTER(PagedCache), c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                     c_void_p]),
     "fh_kv_cache_read": (c_int32, [POINTER(PagedCache), c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,

@@ -16,8 +16,8 @@ import numpy as np
 
 from . import synth
 
-F32, F16, BF16 = 0, 2, 3
-DTYPE_NAME = {F32: "float32", F16: "float16", BF16: "bfloat16"}
+F32, F16, BF16, I32 = 0, 2, 3, 6
+DTYPE_NAME = {F32: "float32", F16: "float16", BF16: "bfloat16", I32: "int32"}
 
 
 def _fmt_double(x: float) -> str:
@@ -114,6 +114,12 @@ class Graph:
 
     def softmax(self, a):
         return self.op("softmax", [a], a.shape)
+
+    def packed_attention(self, q, k, v, cu_seqlens, heads, kv_heads, causal=True, scale=None):
+        """Attention over sequences packed row after row: sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1] - 1 (int32)."""
+        scale = 1.0 / math.sqrt(q.shape[1] // heads) if scale is None else scale
+        return self.op("packed_attention", [q, k, v, cu_seqlens], q.shape,
+                       {"heads": int(heads), "kv_heads": int(kv_heads), "causal": bool(causal), "scale": float(scale)})
 
     def layer_norm(self, x, g, b, eps=1e-5):
         return self.op("layer_norm", [x, g, b], x.shape, {"eps": float(eps)})
@@ -389,6 +395,27 @@ def transformer_block(batch=8, seq=512, d_model=1024, heads=16, ffn=4096, dtype=
         g.output(g.mse_loss(y, g.input(dtype, (rows, d_model))))
     else:
         g.output(y)
+    return g, shapes
+
+
+def decoder_block(tokens, batch, d_model=1024, heads=16, kv_heads=4, ffn=4096, dtype=BF16, device="hip", train=False):
+    """The pre-LN block with causal attention over packed sequences and grouped heads: `batch` sequences of any lengths in
+    `tokens` rows, given by the second input, cu_seqlens (int32 [batch + 1]). Returns the graph and the parameters' shapes;
+    train=True adds a target input after them and outputs mse_loss(y, target)."""
+    g = Graph(device)
+    dh = d_model // heads
+    x, cu = g.input(dtype, (tokens, d_model)), g.input(I32, (batch + 1,))
+    names = ["ln1_g", "ln1_b", "wq", "wk", "wv", "wo", "ln2_g", "ln2_b", "w1", "w2"]
+    shapes = [(d_model,), (d_model,), (d_model, d_model), (d_model, kv_heads * dh), (d_model, kv_heads * dh),
+              (d_model, d_model), (d_model,), (d_model,), (d_model, ffn), (ffn, d_model)]
+    p = {n: g.input(dtype, s) for n, s in zip(names, shapes)}
+    h1 = g.layer_norm(x, p["ln1_g"], p["ln1_b"])
+    q, k, v = (g.matmul(h1, p[w]) for w in ("wq", "wk", "wv"))
+    attn = g.packed_attention(q, k, v, cu, heads, kv_heads)
+    h = g.add(g.matmul(attn, p["wo"]), x)
+    h2 = g.layer_norm(h, p["ln2_g"], p["ln2_b"])
+    y = g.add(g.matmul(g.gelu(g.matmul(h2, p["w1"])), p["w2"]), h)
+    g.output(g.mse_loss(y, g.input(dtype, (tokens, d_model))) if train else y)
     return g, shapes
 
 

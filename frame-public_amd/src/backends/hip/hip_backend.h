@@ -223,6 +223,11 @@ inline constexpr std::string_view kAttentionOp = "hip_attention_internal";
 // attention_grad(q, k, v, dout) -> dq, dk, dv, workspace (the same attributes; see fh_attention_grad).
 inline constexpr std::string_view kAttentionGradOp = "hip_attention_grad_internal";
 
+// packed_attention(q, k, v, cu_seqlens) -> out, lse [tokens, heads] fp32, where a gradient of it reads the latter.
+inline constexpr std::string_view kPackedAttentionOp = "hip_packed_attention_internal";
+// packed_attention_grad_internal with the forward's lse: (q, k, v, cu_seqlens, y, lse, gy) -> gq, gk, gv, workspace.
+inline constexpr std::string_view kPackedAttentionGradOp = "hip_packed_attention_grad_internal";
+
 // The graph HipBackend::compile plans for `graph` (already through the pass pipeline): attention, epilogue
 // (opt_level >= 1) and channels-last conv lowering applied to a copy. Host-only; used by compile and by
 // frame_hip_lowered_text.

@@ -1344,6 +1344,76 @@ Status lower_attention_grads(ir::Graph& g) {
   return Status::ok();
 }
 
+// A packed_attention whose gradient the graph holds hands it the softmax's log-sum-exps: both become their internal forms, the
+// gradient with a planned workspace of the size fh_attention_packed_grad asks for. At every opt level; a gradient whose forward the
+// graph does not hold stays as it is and forms them itself.
+Status lower_packed_attention(ir::Graph& g) {
+  auto forward_of = [](const ir::Node* n) -> const ir::Node* {
+    if (n->op() != "packed_attention_grad_internal" || n->inputs().size() != 6) return nullptr;
+    const ir::Node* f = n->inputs()[4]->producer();
+    if (f == nullptr || f->op() != "packed_attention" || f->attrs() != n->attrs()) return nullptr;
+    for (size_t i = 0; i < 4; ++i)
+      if (f->inputs()[i] != n->inputs()[i]) return nullptr;
+    const DTypeCode d = n->inputs()[0]->type().dtype.code();
+    return d == DTypeCode::kBFloat16 || d == DTypeCode::kFloat16 ? f : nullptr;
+  };
+  std::unordered_set<const ir::Node*> forwards;
+  for (const ir::Node* n : g.topological_order())
+    if (const ir::Node* f = forward_of(n)) forwards.insert(f);
+  if (forwards.empty()) return Status::ok();
+
+  std::unordered_map<const ir::Value*, ir::Value*> map;
+  std::unordered_map<const ir::Node*, ir::Value*> lse;
+  ir::Graph out{std::string(g.name())};
+  for (const ir::Node* n : g.topological_order()) {
+    if (n->op() == ir::kGraphInputOp) {
+      Result<ir::Value*> v = out.add_graph_input(n->outputs()[0].type());
+      if (!v.is_ok()) return v.status();
+      map[&n->outputs()[0]] = v.value();
+      continue;
+    }
+    std::vector<ir::Value*> ins;
+    for (const ir::Value* v : n->inputs()) ins.push_back(map.at(v));
+    std::vector<ir::TensorType> types;
+    for (const ir::Value& o : n->outputs()) types.push_back(o.type());
+    std::string op(n->op());
+    const ir::Node* f = forward_of(n);
+    if (forwards.count(n)) {
+      op = std::string(kPackedAttentionOp);
+      ir::TensorType t = n->inputs()[0]->type();
+      t.dtype = DType::of<float>();
+      t.shape = Shape({t.shape.dim(0), *n->attr<int64_t>("heads")});
+      types.push_back(t);
+    } else if (f != nullptr) {
+      op = std::string(kPackedAttentionGradOp);
+      ins.insert(ins.begin() + 5, lse.at(f));
+      const Shape &q = n->inputs()[0]->type().shape, &k = n->inputs()[1]->type().shape;
+      fh_packed_attention p{};
+      p.dtype = static_cast<int32_t>(n->inputs()[0]->type().dtype.code());
+      p.tokens = q.dim(0);
+      p.batch = n->inputs()[3]->type().shape.numel() - 1;
+      p.heads = *n->attr<int64_t>("heads");
+      p.kv_heads = *n->attr<int64_t>("kv_heads");
+      p.dh = q.dim(1) / p.heads;
+      p.q_stride = p.out_stride = q.dim(1);
+      p.k_stride = p.v_stride = k.dim(1);
+      p.scale = static_cast<float>(*n->attr<double>("scale"));
+      // (a geometry that the kernels refuse is named when the step runs)
+      const int64_t bytes = std::max<int64_t>(fh_attention_packed_grad_workspace(&p), 4);
+      types[3].dtype = DType::of<float>();
+      types[3].shape = Shape({(bytes + 3) / 4});
+    }
+    Result<ir::Node*> c = out.create_node(std::move(op), std::move(ins), std::move(types));
+    if (!c.is_ok()) return c.status();
+    for (const auto& [k, v] : n->attrs()) c.value()->set_attr(k, v);
+    for (size_t i = 0; i < n->outputs().size(); ++i) map[&n->outputs()[i]] = c.value()->output(static_cast<int32_t>(i));
+    if (forwards.count(n)) lse[n] = c.value()->output(1);
+  }
+  for (const ir::Value* o : g.outputs()) FRAME_RETURN_IF_ERROR(out.mark_output(map.at(o)));
+  g = std::move(out);
+  return Status::ok();
+}
+
 // Replaces every matched attention decomposition by one kAttentionOp node. Nodes of a decomposition whose
 // results are also used outside it (or are graph outputs) keep the decomposition as it is. The graph is rebuilt in
 // topological order without the nodes the rewrite leaves unused (the shared scale constant among them).
@@ -2005,6 +2075,7 @@ Status lower_grouped_gemms(ir::Graph& g) {
 Result<ir::Graph> lower_for_hip(const ir::Graph& graph, int32_t opt_level) {
   Result<ir::Graph> source = ir::clone_graph(graph);
   if (!source.is_ok()) return source.status();
+  FRAME_RETURN_IF_ERROR(lower_packed_attention(source.value()));
   if (opt_level >= 1) FRAME_RETURN_IF_ERROR(lower_attention_grads(source.value()));
   Result<ir::Graph> work = lower_matmul_grads(source.value(), opt_level);
   if (!work.is_ok()) return work.status();

@@ -47,6 +47,7 @@ Status arity(const KernelContext& ctx, const std::string& op, size_t n_in, size_
 bool same_elem_type(const Tensor& a, const Tensor& b) { return a.dtype() == b.dtype(); }
 bool same_elem_type(const Tensor& a, DType b) { return a.dtype() == b; }
 size_t elem_bytes(const Tensor& t) { return t.dtype().itemsize(); }
+bool alike(const Tensor& a, const Tensor& b) { return a.shape() == b.shape() && same_elem_type(a, b); }
 
 Status same_dtype(const KernelContext& ctx, const std::string& op) {
   const DType d = ctx.outputs[0].dtype();
@@ -620,6 +621,116 @@ Status attention_grad_kernel(KernelContext& ctx) {
   return Status::ok();
 }
 
+// ---- attention over packed sequences ----
+
+// The descriptor of a packed_attention node's tensors (dense rows) from q's and k's shapes, cu_seqlens' length and the attributes.
+Status packed_geometry(const KernelContext& ctx, const std::string& op, fh_packed_attention& g) {
+  const auto* heads = attr<int64_t>(ctx, "heads");
+  const auto* kv_heads = attr<int64_t>(ctx, "kv_heads");
+  const auto* causal = attr<bool>(ctx, "causal");
+  const auto* scale = attr<double>(ctx, "scale");
+  if (!heads || !kv_heads || !causal || !scale) return invalid(op, "missing heads/kv_heads/causal/scale attributes");
+  const Tensor &q = ctx.inputs[0], &k = ctx.inputs[1], &v = ctx.inputs[2], &cu = ctx.inputs[3];
+  if (*heads < 1 || q.shape().rank() != 2 || k.shape().rank() != 2 || q.shape().dim(1) % *heads != 0)
+    return invalid(op, "expects q [tokens, heads * dh]");
+  const int64_t dh = q.shape().dim(1) / *heads;
+  const Shape kv({q.shape().dim(0), *kv_heads * dh});
+  if (k.shape() != kv || v.shape() != kv) return invalid(op, "expects k and v [tokens, kv_heads * dh]");
+  if (!same_elem_type(k, q) || !same_elem_type(v, q)) return invalid(op, "q, k and v differ in element type");
+  if (!same_elem_type(cu, DType::of<std::int32_t>()) || cu.shape().rank() != 1 || cu.numel() < 1)
+    return invalid(op, "expects cu_seqlens int32 [batch + 1]");
+  Result<int32_t> dt = float_code(op, q.dtype());
+  if (!dt.is_ok()) return dt.status();
+  g.dtype = dt.value();
+  g.causal = *causal ? 1 : 0;
+  g.tokens = q.shape().dim(0);
+  g.batch = cu.numel() - 1;
+  g.heads = *heads;
+  g.kv_heads = *kv_heads;
+  g.dh = dh;
+  g.q_stride = g.out_stride = q.shape().dim(1);
+  g.k_stride = g.v_stride = k.shape().dim(1);
+  g.scale = static_cast<float>(*scale);
+  return Status::ok();
+}
+
+// A graph's tensors are whole: rows outside the sequences are zeros.
+Status clear_outside(const KernelContext& ctx, const std::string& op, Tensor& t, int64_t batch) {
+  FRAME_HIP_RETURN_IF_ERROR(
+      fh_packed_clear(static_cast<const int32_t*>(ctx.inputs[3].raw_data()), batch, t.raw_data(), t.shape().dim(0),
+                      t.shape().dim(1) * static_cast<int64_t>(elem_bytes(t)), stream_handle(ctx)),
+      "op '" + op + "' (hip)");
+  return Status::ok();
+}
+
+Status packed_forward(const KernelContext& ctx, const std::string& op, const fh_packed_attention& g, Tensor& out, float* lse) {
+  if (!alike(out, ctx.inputs[0]))
+    return invalid(op, "out must be of q's shape and dtype");
+  FRAME_HIP_RETURN_IF_ERROR(fh_attention_packed_fwd(&g, ctx.inputs[0].raw_data(), ctx.inputs[1].raw_data(),
+                                                    ctx.inputs[2].raw_data(),
+                                                    static_cast<const int32_t*>(ctx.inputs[3].raw_data()), out.raw_data(), lse,
+                                                    stream_handle(ctx)),
+                            "op '" + op + "' (hip)");
+  return Status::ok();
+}
+
+// WithLse: the compiled graph's form, whose second output a gradient reads.
+template <bool WithLse>
+Status packed_attention_kernel(KernelContext& ctx) {
+  const std::string op(WithLse ? kPackedAttentionOp : "packed_attention");
+  FRAME_RETURN_IF_ERROR(arity(ctx, op, 4, WithLse ? 2 : 1));
+  fh_packed_attention g{};
+  FRAME_RETURN_IF_ERROR(packed_geometry(ctx, op, g));
+  float* lse = nullptr;
+  if (WithLse) {
+    if (ctx.outputs[1].numel() != g.tokens * g.heads || elem_bytes(ctx.outputs[1]) != 4) return invalid(op, "lse must be fp32 [tokens, heads]");
+    lse = static_cast<float*>(ctx.outputs[1].raw_data());
+  }
+  FRAME_RETURN_IF_ERROR(packed_forward(ctx, op, g, ctx.outputs[0], lse));
+  return clear_outside(ctx, op, ctx.outputs[0], g.batch);
+}
+
+// WithLse: inputs q, k, v, cu_seqlens, y, lse, gy and a workspace as the fourth output. Otherwise (a node launched by itself)
+// q, k, v, cu_seqlens, y, gy: the log-sum-exps are formed again, by a forward whose output lands in gq's room, and they and the
+// workspace (its least, one fp32 per row and head) share the fourth output.
+template <bool WithLse>
+Status packed_attention_grad_kernel(KernelContext& ctx) {
+  const std::string op(WithLse ? kPackedAttentionGradOp : "packed_attention_grad_internal");
+  FRAME_RETURN_IF_ERROR(arity(ctx, op, WithLse ? 7 : 6, 4));
+  fh_packed_attention g{};
+  FRAME_RETURN_IF_ERROR(packed_geometry(ctx, op, g));
+  const Tensor &y = ctx.inputs[4], &gy = ctx.inputs[WithLse ? 6 : 5];
+  for (const Tensor* t : {&y, &gy})
+    if (!alike(*t, ctx.inputs[0]))
+      return invalid(op, "y and gy must be of q's shape and dtype");
+  for (size_t i = 0; i < 3; ++i)
+    if (!alike(ctx.outputs[i], ctx.inputs[i]))
+      return invalid(op, "gq, gk and gv must be of q's, k's and v's shape and dtype");
+  Tensor& scratch = ctx.outputs[3];
+  const int64_t stat = g.tokens * g.heads * 4;  // bytes of one fp32 per (row, head)
+  int64_t room = scratch.numel() * static_cast<int64_t>(elem_bytes(scratch));
+  char* ws = static_cast<char*>(scratch.raw_data());
+  const float* lse = nullptr;
+  if (WithLse) {
+    if (ctx.inputs[5].numel() != g.tokens * g.heads || elem_bytes(ctx.inputs[5]) != 4) return invalid(op, "lse must be fp32 [tokens, heads]");
+    lse = static_cast<const float*>(ctx.inputs[5].raw_data());
+  } else {
+    if (room < 2 * stat) return invalid(op, "stats must hold two fp32 values per (row, head)");
+    float* formed = reinterpret_cast<float*>(ws + stat);
+    FRAME_RETURN_IF_ERROR(packed_forward(ctx, op, g, ctx.outputs[0], formed));
+    lse = formed;
+    room = stat;
+  }
+  FRAME_HIP_RETURN_IF_ERROR(
+      fh_attention_packed_grad(&g, ctx.inputs[0].raw_data(), ctx.inputs[1].raw_data(), ctx.inputs[2].raw_data(),
+                               static_cast<const int32_t*>(ctx.inputs[3].raw_data()), y.raw_data(), lse, gy.raw_data(),
+                               ctx.outputs[0].raw_data(), ctx.outputs[1].raw_data(), ctx.outputs[2].raw_data(), ws, room,
+                               stream_handle(ctx)),
+      "op '" + op + "' (hip)");
+  for (size_t i = 0; i < 3; ++i) FRAME_RETURN_IF_ERROR(clear_outside(ctx, op, ctx.outputs[i], g.batch));
+  return Status::ok();
+}
+
 Status layer_norm_kernel(KernelContext& ctx) {
   FRAME_RETURN_IF_ERROR(arity(ctx, "layer_norm", 3, 1));
   FRAME_RETURN_IF_ERROR(same_dtype(ctx, "layer_norm"));
@@ -1124,6 +1235,10 @@ FRAME_REGISTER_KERNEL(kPackFilterC8Op, kHipBackendName, &pack_filter_c8_kernel);
 FRAME_REGISTER_KERNEL("softmax", kHipBackendName, &softmax_kernel);
 FRAME_REGISTER_KERNEL(kAttentionOp, kHipBackendName, &attention_kernel);
 FRAME_REGISTER_KERNEL(kAttentionGradOp, kHipBackendName, &attention_grad_kernel);
+FRAME_REGISTER_KERNEL("packed_attention", kHipBackendName, &packed_attention_kernel<false>);
+FRAME_REGISTER_KERNEL(kPackedAttentionOp, kHipBackendName, &packed_attention_kernel<true>);
+FRAME_REGISTER_KERNEL("packed_attention_grad_internal", kHipBackendName, &packed_attention_grad_kernel<false>);
+FRAME_REGISTER_KERNEL(kPackedAttentionGradOp, kHipBackendName, &packed_attention_grad_kernel<true>);
 FRAME_REGISTER_KERNEL("layer_norm", kHipBackendName, &layer_norm_kernel);
 FRAME_REGISTER_KERNEL("max_pool2d", kHipBackendName, &pool_kernel<0>);
 FRAME_REGISTER_KERNEL("avg_pool2d", kHipBackendName, &pool_kernel<1>);

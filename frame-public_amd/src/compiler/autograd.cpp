@@ -1,6 +1,8 @@
 // Reverse-mode differentiation over the IR (reference: src/compiler/autograd.cpp:118-450). The training graph is
 // built in the same node order as the reference's (clone, seed, then per forward node in reverse topological order:
-// its gradient micrograph, then one accumulating add per already-seen input), so its IR text is identical.
+// its gradient micrograph, then one accumulating add per already-seen input), so its IR text is identical. Inputs of an integer or
+// bool type (packed_attention's cu_seqlens; no op of the reference has one) have no gradient: a micrograph has one output per
+// floating-point input.
 #include <frame/compiler/autograd.h>
 
 #include <cmath>
@@ -73,6 +75,18 @@ Result<ir::Node*> splat(ir::Graph& g, const ir::TensorType& t, double v) {
   return ops::create_node_with_inferred_types(g, ops::kConstantOpName, t.device, attrs);
 }
 
+bool differentiable(const ir::TensorType& t) {
+  switch (t.dtype.code()) {
+    case DTypeCode::kFloat32:
+    case DTypeCode::kFloat64:
+    case DTypeCode::kFloat16:
+    case DTypeCode::kBFloat16:
+      return true;
+    default:
+      return false;
+  }
+}
+
 }  // namespace
 
 Result<ir::Graph> build_backward_graph(const ir::Graph& forward, int32_t loss_output_index,
@@ -98,6 +112,9 @@ Result<ir::Graph> build_backward_graph(const ir::Graph& forward, int32_t loss_ou
     if (!seen.insert(idx).second)
       return Status::make(ErrorCode::kInvalidArgument,
                           "compiler::build_backward_graph: wrt_input_indices entry " + std::to_string(idx) + " is duplicated");
+    if (!differentiable(forward.inputs()[static_cast<size_t>(idx)]->type()))
+      return Status::make(ErrorCode::kInvalidArgument, "compiler::build_backward_graph: wrt_input_indices entry " +
+                                                           std::to_string(idx) + " is not of a floating-point type");
   }
 
   ValueMap clone_map;
@@ -147,20 +164,23 @@ Result<ir::Graph> build_backward_graph(const ir::Graph& forward, int32_t loss_ou
       return Status::make(micro.status().code(), "compiler::build_backward_graph: op '" + op +
                                                      "' GradientFn failed: " + std::string(micro.status().message()));
     const size_t n = node->inputs().size(), m = node->outputs().size();
+    std::vector<ir::Value*> floats;
+    for (ir::Value* v : node->inputs())
+      if (differentiable(v->type())) floats.push_back(v);
     if (micro.value().inputs().size() != n + 2 * m)
       return internal("op '" + op + "' gradient micrograph declared " + std::to_string(micro.value().inputs().size()) +
                       " graph input(s), expected " + std::to_string(n + 2 * m) + " ([x.., y.., gy..])");
-    if (micro.value().outputs().size() != n)
+    if (micro.value().outputs().size() != floats.size())
       return Status::make(ErrorCode::kInvalidArgument,
                           "compiler::build_backward_graph: op '" + op + "' gradient micrograph produced " +
                               std::to_string(micro.value().outputs().size()) + " graph output(s), expected " +
-                              std::to_string(n) + " (one gradient per input)");
+                              std::to_string(floats.size()) + " (one gradient per input)");
     std::vector<ir::Value*> bound(node->inputs().begin(), node->inputs().end());
     for (size_t j = 0; j < m; ++j) bound.push_back(node->output(static_cast<int32_t>(j)));
     bound.insert(bound.end(), gys.begin(), gys.end());
     Result<std::vector<ir::Value*>> gx = splice(training, micro.value(), bound);
     if (!gx.is_ok()) return gx.status();
-    for (size_t i = 0; i < n; ++i) FRAME_RETURN_IF_ERROR(accumulate(training, grad, node->inputs()[i], gx.value()[i]));
+    for (size_t i = 0; i < floats.size(); ++i) FRAME_RETURN_IF_ERROR(accumulate(training, grad, floats[i], gx.value()[i]));
   }
 
   for (int32_t idx : wrt_input_indices) {

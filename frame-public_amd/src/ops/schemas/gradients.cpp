@@ -9,7 +9,7 @@
 //   reshape / transpose / slice / concat gradients   src/ops/schemas/shape.cpp:60-410
 //   softmax / layer_norm gradients and their row-statistics helpers   src/ops/schemas/sequence.cpp:255-615
 //   sigmoid / tanh / rsqrt gradients   src/ops/schemas/elementwise.cpp:401-660
-// gelu and gelu_grad_internal are this build's own (the reference has no gelu).
+// gelu, packed_attention and their gradient ops are this build's own (the reference has neither).
 // Only first-order gradients are registered: the gradient-only ops carry no GradientFn here, so differentiating
 // a training graph a second time reports kUnimplemented naming the op.
 #include "gradients.h"
@@ -62,10 +62,16 @@ class Micro {
     return v.is_ok() ? v.value() : nullptr;
   }
   ir::Value* op(std::string_view name, std::vector<ir::Value*> ins, const AttrMap& attrs = {}) {
-    if (!st_.is_ok()) return nullptr;
+    return op_outputs(name, std::move(ins), 1, attrs)[0];
+  }
+  // the first `count` outputs of a node
+  std::vector<ir::Value*> op_outputs(std::string_view name, std::vector<ir::Value*> ins, int32_t count, const AttrMap& attrs = {}) {
+    std::vector<ir::Value*> out(static_cast<size_t>(count), nullptr);
+    if (!st_.is_ok()) return out;
     Result<ir::Node*> n = create_node_with_inferred_types(g_, name, std::move(ins), attrs);
     if (!n.is_ok()) st_ = n.status();
-    return n.is_ok() ? n.value()->output(0) : nullptr;
+    for (int32_t i = 0; n.is_ok() && i < count; ++i) out[static_cast<size_t>(i)] = n.value()->output(i);
+    return out;
   }
   ir::Value* splat_shape(const ir::TensorType& like, const Shape& shape, double v) {
     ir::TensorType t = like;
@@ -460,6 +466,57 @@ Result<ir::Graph> softmax_gradient(const NodeContext& c) {
   return m.finish({m.op("mul", {sm, diff})});
 }
 
+Result<std::vector<Shape>> packed_attention_shapes(const NodeContext& c) {
+  const std::string op(c.op);
+  const auto &q = c.input_types[0], &k = c.input_types[1], &v = c.input_types[2], &cu = c.input_types[3];
+  const auto* heads = c.attr<int64_t>("heads");
+  const auto* kv_heads = c.attr<int64_t>("kv_heads");
+  const auto* scale = c.attr<double>("scale");
+  if (heads == nullptr || kv_heads == nullptr || scale == nullptr || c.attr<bool>("causal") == nullptr)
+    return bad(op, "is missing one of the required attributes 'heads', 'kv_heads', 'causal' (bool), 'scale' (double)");
+  if (*heads < 1 || *kv_heads < 1 || *heads % *kv_heads != 0)
+    return bad(op, "requires heads to be a positive multiple of kv_heads, got " + std::to_string(*heads) + " and " +
+                       std::to_string(*kv_heads));
+  if (!(*scale > 0.0)) return bad(op, "attribute 'scale' must be positive");
+  if (q.shape.rank() != 2 || k.shape.rank() != 2 || v.shape.rank() != 2)
+    return bad(op, "requires q, k and v to be rank-2 [tokens, heads * dh]");
+  FRAME_RETURN_IF_ERROR(same_dtype(op, q, k, "q", "k"));
+  FRAME_RETURN_IF_ERROR(same_dtype(op, q, v, "q", "v"));
+  if (!(cu.dtype == DType(DTypeCode::kInt32)) || cu.shape.rank() != 1 || cu.shape.dim(0) < 1)
+    return bad(op, "requires cu_seqlens to be int32 rank-1 [batch + 1], got '" + std::string(cu.dtype.name()) + "' " +
+                       cu.shape.to_string());
+  if (q.shape.dim(1) < 1 || q.shape.dim(1) % *heads != 0)
+    return bad(op, "requires q's second dimension to be a positive multiple of heads, got " + q.shape.to_string());
+  const Shape kv({q.shape.dim(0), q.shape.dim(1) / *heads * *kv_heads});
+  if (!(k.shape == kv) || !(v.shape == kv))
+    return bad(op, "requires k and v to be " + kv.to_string() + ", got " + k.shape.to_string() + " and " + v.shape.to_string());
+  return std::vector<Shape>{q.shape};
+}
+
+Shapes infer_packed_attention_grad(const NodeContext& c) {
+  const std::string op = "packed_attention_grad_internal";
+  if (c.input_types.size() != 6) return bad(op, "expects 6 inputs, got " + std::to_string(c.input_types.size()));
+  Shapes out = packed_attention_shapes(c);
+  if (!out.is_ok()) return out;
+  const auto& q = c.input_types[0];
+  for (size_t i = 4; i < 6; ++i) {
+    FRAME_RETURN_IF_ERROR(same_dtype(op, q, c.input_types[i], "q", i == 4 ? "y" : "gy"));
+    if (!(c.input_types[i].shape == q.shape))
+      return bad(op, "requires y and gy of q's shape " + q.shape.to_string() + ", got " + c.input_types[i].shape.to_string());
+  }
+  const Shape& kv = c.input_types[1].shape;
+  return std::vector<Shape>{q.shape, kv, kv, Shape({q.shape.dim(0), 4 * *c.attr<int64_t>("heads")})};
+}
+
+// One node for the three gradients; cu_seqlens, an integer input, has none.
+Result<ir::Graph> packed_attention_gradient(const NodeContext& c) {
+  FRAME_RETURN_IF_ERROR(expect(c, 4, "4 inputs (q, k, v, cu_seqlens)"));
+  Micro m("packed_attention_gradient");
+  Fwd f = forward_inputs(m, c);
+  return m.finish(m.op_outputs("packed_attention_grad_internal", {f.x[0], f.x[1], f.x[2], f.x[3], f.y, f.gy}, 3,
+                               pick(c, {"heads", "kv_heads", "causal", "scale"})));
+}
+
 // layer_norm (reference: src/ops/schemas/sequence.cpp:479-615): mean / variance / rsqrt recomputed from x, then
 // gx = r * ((a - mean(a)) - xhat * mean(a * xhat)) with a = gamma * gy; ggamma = sum(gy * xhat, axis 0);
 // gbeta = sum(gy, axis 0).
@@ -697,6 +754,23 @@ FRAME_REGISTER_OP("mse_loss_grad_internal")
     .input("gy", "upstream gradient of mse_loss's scalar output")
     .output("gpred", "2 * gy / numel * (pred - target)")
     .shape_infer(&fs::infer_mse_loss_grad);
+
+FRAME_REGISTER_OP("packed_attention_grad_internal")
+    .input("q", "packed_attention's inputs")
+    .input("k", "")
+    .input("v", "")
+    .input("cu_seqlens", "")
+    .input("y", "its output")
+    .input("gy", "upstream gradient of y")
+    .attr("heads", AttrType::kInt64, true)
+    .attr("kv_heads", AttrType::kInt64, true)
+    .attr("causal", AttrType::kBool, true)
+    .attr("scale", AttrType::kDouble, true)
+    .output("gq", "gradient w.r.t. q; rows outside the sequences are zeros, as in gk and gv")
+    .output("gk", "gradient w.r.t. k")
+    .output("gv", "gradient w.r.t. v")
+    .output("stats", "scratch of two fp32 values per (row, head), [tokens, 4 * heads] in 16-bit elements")
+    .shape_infer(&fs::infer_packed_attention_grad);
 
 FRAME_REGISTER_OP("gelu_grad_internal")
     .input("x", "gelu's original input")

@@ -2,6 +2,8 @@
 // Gradient micrographs of the forward ops (defined in gradients.cpp, attached to the schemas in schemas.cpp).
 // Each returns a graph with inputs [x.., y.., gy..] and one output per forward input, as
 // compiler::build_backward_graph expects.
+#include <vector>
+
 #include <frame/ir/graph.h>
 #include <frame/ops/op_schema.h>
 
@@ -25,5 +27,10 @@ Result<ir::Graph> sigmoid_gradient(const NodeContext& ctx);
 Result<ir::Graph> tanh_gradient(const NodeContext& ctx);
 Result<ir::Graph> rsqrt_gradient(const NodeContext& ctx);
 Result<ir::Graph> gelu_gradient(const NodeContext& ctx);
+Result<ir::Graph> packed_attention_gradient(const NodeContext& ctx);
+
+// The output shape of packed_attention on the context's first four inputs (q, k, v, cu_seqlens) and attributes, or what is wrong
+// with them; its gradient op takes the same.
+Result<std::vector<Shape>> packed_attention_shapes(const NodeContext& ctx);
 
 }  // namespace frame::ops::schemas

@@ -9,6 +9,8 @@
 //   fused chain  src/ops/schemas/fused_elementwise.cpp:24-51
 // gelu has no counterpart in the reference: it is this build's addition (0.5*x*(1+erf(x/sqrt(2)))), declared
 // elementwise and fusable so operator_fusion can merge bias-add + gelu into one fused group.
+// packed_attention has none either: attention over sequences of different lengths in one tensor's rows, with grouped heads and an
+// optional causal mask, as one op (the reference unrolls attention of one length per batch and head, src/nn/layers.cpp:1014-1080).
 #include <cstdint>
 #include <numeric>
 #include <string>
@@ -269,6 +271,11 @@ Shapes infer_constant(const NodeContext& c) {
   return std::vector<Shape>{*s};
 }
 
+Shapes infer_packed_attention(const NodeContext& c) {
+  FRAME_RETURN_IF_ERROR(expect_inputs(c, 4));
+  return frame::ops::schemas::packed_attention_shapes(c);
+}
+
 Shapes infer_fused(const NodeContext& c) {
   if (c.input_types.empty()) return bad("fused_elementwise_internal", "expects at least 1 input, got 0");
   if (c.attrs == nullptr) return bad("fused_elementwise_internal", "requires non-null attrs");
@@ -351,6 +358,19 @@ FRAME_REGISTER_OP("conv2d")
 
 FRAME_REGISTER_OP("softmax").input("x", "rank-2 [N, D]").output("out", "softmax along the last axis").shape_infer(&infer_softmax)
     .gradient(&frame::ops::schemas::softmax_gradient);
+
+FRAME_REGISTER_OP("packed_attention")
+    .input("q", "rank-2 [tokens, heads * dh]")
+    .input("k", "rank-2 [tokens, kv_heads * dh]")
+    .input("v", "rank-2 [tokens, kv_heads * dh]")
+    .input("cu_seqlens", "int32 rank-1 [batch + 1]: sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1] - 1")
+    .attr("heads", AttrType::kInt64, true)
+    .attr("kv_heads", AttrType::kInt64, true)
+    .attr("causal", AttrType::kBool, true)
+    .attr("scale", AttrType::kDouble, true)
+    .output("out", "softmax(scale q k^T) v per sequence and head; rows outside the sequences are zeros")
+    .shape_infer(&infer_packed_attention)
+    .gradient(&frame::ops::schemas::packed_attention_gradient);
 
 FRAME_REGISTER_OP("layer_norm")
     .input("x", "rank-2 [N, D]")

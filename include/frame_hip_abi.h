@@ -349,11 +349,15 @@ fh_status fh_attention_packed_fwd(const fh_packed_attention* geom, const void* q
                                   const int32_t* cu_seqlens, void* out, float* lse, void* stream);
 
 /* Gradients with respect to q, k and v for the output gradient dout, from the forward's operands, out and lse. dout has out's
- * stride; dq, dk and dv have q's, k's and v's. Deterministic. The workspace holds one fp32 per (row, head). */
+ * stride; dq, dk and dv have q's, k's and v's. Deterministic. tokens * heads * 4 bytes of workspace are enough; with all that the
+ * query returns, the rows that a long causal sequence's first keys sum over may be cut into parts. */
 int64_t fh_attention_packed_grad_workspace(const fh_packed_attention* geom);
 fh_status fh_attention_packed_grad(const fh_packed_attention* geom, const void* q, const void* k, const void* v,
                                    const int32_t* cu_seqlens, const void* out, const float* lse, const void* dout, void* dq,
                                    void* dk, void* dv, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Zeros in the rows of x [rows, row_bytes] (dense; row_bytes a multiple of 16) that no sequence of cu_seqlens covers. */
+fh_status fh_packed_clear(const int32_t* cu_seqlens, int64_t batch, void* x, int64_t rows, int64_t row_bytes, void* stream);
 
 /* ---- a paged cache of keys and values, and attention over it ----
  * The cache is [pages, page_size, kv_heads, dh] for keys and for values; position p of sequence b is row p % page_size of page

@@ -308,6 +308,26 @@ Status mse_loss_grad_kernel(ops::KernelContext& c) {
             "mse_loss_grad");
 }
 
+// packed_attention (inputs q, k, v, cu_seqlens) and its gradients (.., y, gy; the scratch output is left alone)
+template <bool Grad>
+Status packed_attention_kernel(ops::KernelContext& c) {
+  const int64_t heads = *attr<int64_t>(c, "heads"), kv_heads = *attr<int64_t>(c, "kv_heads");
+  const Shape& q = c.inputs[0].shape();
+  const int64_t tokens = q.dim(0), dh = q.dim(1) / heads, batch = c.inputs[3].numel() - 1;
+  const int causal = *attr<bool>(c, "causal") ? 1 : 0;
+  const double scale = *attr<double>(c, "scale");
+  const auto* cu = static_cast<const int32_t*>(c.inputs[3].raw_data());
+  const int dt = dcode(c.outputs[0].dtype());
+  if (Grad)
+    return rc(oracle_packed_attention_grad(dt, c.inputs[0].raw_data(), c.inputs[1].raw_data(), c.inputs[2].raw_data(), cu,
+                                           c.inputs[5].raw_data(), c.outputs[0].raw_data(), c.outputs[1].raw_data(),
+                                           c.outputs[2].raw_data(), tokens, batch, heads, kv_heads, dh, causal, scale),
+              "packed_attention_grad");
+  return rc(oracle_packed_attention(dt, c.inputs[0].raw_data(), c.inputs[1].raw_data(), c.inputs[2].raw_data(), cu,
+                                    c.outputs[0].raw_data(), tokens, batch, heads, kv_heads, dh, causal, scale),
+            "packed_attention");
+}
+
 }  // namespace oracle_cpu
 
 FRAME_REGISTER_BACKEND(frame::kCpuBackendName, oracle_cpu::CpuBackend);
@@ -341,5 +361,7 @@ FRAME_REGISTER_KERNEL("max_pool2d_grad_internal", frame::kCpuBackendName, &oracl
 FRAME_REGISTER_KERNEL("avg_pool2d_grad_internal", frame::kCpuBackendName, &oracle_cpu::pool_grad_kernel<1>);
 FRAME_REGISTER_KERNEL("sum", frame::kCpuBackendName, &oracle_cpu::sum_kernel);
 FRAME_REGISTER_KERNEL("sum_grad_internal", frame::kCpuBackendName, &oracle_cpu::sum_grad_kernel);
+FRAME_REGISTER_KERNEL("packed_attention", frame::kCpuBackendName, &oracle_cpu::packed_attention_kernel<false>);
+FRAME_REGISTER_KERNEL("packed_attention_grad_internal", frame::kCpuBackendName, &oracle_cpu::packed_attention_kernel<true>);
 FRAME_REGISTER_KERNEL("mse_loss", frame::kCpuBackendName, &oracle_cpu::mse_loss_kernel);
 FRAME_REGISTER_KERNEL("mse_loss_grad_internal", frame::kCpuBackendName, &oracle_cpu::mse_loss_grad_kernel);

@@ -5,6 +5,8 @@
 // Compiled with -ffp-contract=off: the reference's a*b+c is a multiply followed by an add.
 #include "cpu_kernels.h"
 
+#include <algorithm>
+#include <limits>
 #include <cmath>
 #include <cstring>
 #include <vector>
@@ -696,6 +698,106 @@ int oracle_mse_loss(int dtype, const void* pred, const void* target, void* out, 
       acc += diff * diff;
     }
     static_cast<S*>(out)[0] = D::st(acc / static_cast<float>(numel));
+    return 0;
+  });
+}
+
+// packed_attention (this build's op): per sequence, head and row the probabilities in double, then fn(row, last key + 1, p).
+}  // extern "C"
+
+namespace {
+template <typename D, typename Fn>
+void packed_rows(const typename D::S* Q, const typename D::S* K, const int32_t* cu, int64_t tokens, int64_t batch, int64_t heads,
+                 int64_t kv_heads, int64_t dh, int causal, double scale, Fn&& fn) {
+  const int64_t wq = heads * dh, wk = kv_heads * dh;
+  std::vector<double> p;
+  for (int64_t b = 0; b < batch; ++b) {
+    const int64_t begin = std::clamp<int64_t>(cu[b], 0, tokens), end = std::clamp<int64_t>(cu[b + 1], begin, tokens);
+    for (int64_t h = 0; h < heads; ++h) {
+      const int64_t j = h / (heads / kv_heads);
+      for (int64_t t = begin; t < end; ++t) {
+        const int64_t last = causal ? t + 1 : end;
+        p.assign(static_cast<size_t>(last - begin), 0.0);
+        double top = -std::numeric_limits<double>::infinity(), sum = 0.0;
+        for (int64_t u = begin; u < last; ++u) {
+          double s = 0.0;
+          for (int64_t d = 0; d < dh; ++d)
+            s += static_cast<double>(D::ld(Q[t * wq + h * dh + d])) * static_cast<double>(D::ld(K[u * wk + j * dh + d]));
+          p[static_cast<size_t>(u - begin)] = s * scale;
+          top = std::max(top, s * scale);
+        }
+        for (double& x : p) {
+          x = std::exp(x - top);
+          sum += x;
+        }
+        for (double& x : p) x /= sum;
+        fn(t, h, j, begin, p);
+      }
+    }
+  }
+}
+}  // namespace
+
+extern "C" {
+
+int oracle_packed_attention(int dtype, const void* q, const void* k, const void* v, const int32_t* cu, void* out, int64_t tokens,
+                            int64_t batch, int64_t heads, int64_t kv_heads, int64_t dh, int causal, double scale) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return 1;
+  return with_dtype(dtype, [&](auto d0) {
+    using D = decltype(d0);
+    using S = typename D::S;
+    const S* V = static_cast<const S*>(v);
+    S* O = static_cast<S*>(out);
+    for (int64_t i = 0; i < tokens * heads * dh; ++i) O[i] = D::st(0.0f);
+    packed_rows<D>(static_cast<const S*>(q), static_cast<const S*>(k), cu, tokens, batch, heads, kv_heads, dh, causal, scale,
+                   [&](int64_t t, int64_t h, int64_t j, int64_t begin, const std::vector<double>& p) {
+                     for (int64_t d = 0; d < dh; ++d) {
+                       double y = 0.0;
+                       for (size_t u = 0; u < p.size(); ++u)
+                         y += p[u] * static_cast<double>(D::ld(V[((begin + static_cast<int64_t>(u)) * kv_heads + j) * dh + d]));
+                       O[(t * heads + h) * dh + d] = D::st(static_cast<float>(y));
+                     }
+                   });
+    return 0;
+  });
+}
+
+int oracle_packed_attention_grad(int dtype, const void* q, const void* k, const void* v, const int32_t* cu, const void* gy, void* dq,
+                                 void* dk, void* dv, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dh,
+                                 int causal, double scale) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return 1;
+  return with_dtype(dtype, [&](auto d0) {
+    using D = decltype(d0);
+    using S = typename D::S;
+    const S *Q = static_cast<const S*>(q), *K = static_cast<const S*>(k), *V = static_cast<const S*>(v), *G = static_cast<const S*>(gy);
+    std::vector<double> gq(static_cast<size_t>(tokens * heads * dh)), gk(static_cast<size_t>(tokens * kv_heads * dh)), gv(gk.size());
+    std::vector<double> dp;
+    packed_rows<D>(Q, K, cu, tokens, batch, heads, kv_heads, dh, causal, scale,
+                   [&](int64_t t, int64_t h, int64_t j, int64_t begin, const std::vector<double>& p) {
+                     const int64_t row = (t * heads + h) * dh;
+                     dp.assign(p.size(), 0.0);
+                     double total = 0.0;
+                     for (size_t u = 0; u < p.size(); ++u) {
+                       const int64_t at = ((begin + static_cast<int64_t>(u)) * kv_heads + j) * dh;
+                       for (int64_t d = 0; d < dh; ++d)
+                         dp[u] += static_cast<double>(D::ld(G[row + d])) * static_cast<double>(D::ld(V[at + d]));
+                       total += p[u] * dp[u];
+                     }
+                     for (size_t u = 0; u < p.size(); ++u) {
+                       const int64_t at = ((begin + static_cast<int64_t>(u)) * kv_heads + j) * dh;
+                       const double ds = p[u] * (dp[u] - total) * scale;
+                       for (int64_t d = 0; d < dh; ++d) {
+                         gq[static_cast<size_t>(row + d)] += ds * static_cast<double>(D::ld(K[at + d]));
+                         gk[static_cast<size_t>(at + d)] += ds * static_cast<double>(D::ld(Q[row + d]));
+                         gv[static_cast<size_t>(at + d)] += p[u] * static_cast<double>(D::ld(G[row + d]));
+                       }
+                     }
+                   });
+    for (size_t i = 0; i < gq.size(); ++i) static_cast<S*>(dq)[i] = D::st(static_cast<float>(gq[i]));
+    for (size_t i = 0; i < gk.size(); ++i) {
+      static_cast<S*>(dk)[i] = D::st(static_cast<float>(gk[i]));
+      static_cast<S*>(dv)[i] = D::st(static_cast<float>(gv[i]));
+    }
     return 0;
   });
 }

@@ -97,6 +97,14 @@ int oracle_sum_grad(int itemsize, const void* gy, void* gx, int rank, const int6
 int oracle_mse_loss(int dtype, const void* pred, const void* target, void* out, int64_t numel);
 int oracle_mse_loss_grad(int dtype, const void* pred, const void* target, const void* gy, void* out, int64_t numel);
 
+/* packed_attention and its gradients (no reference counterpart): sequences of rows cu[b] .. cu[b+1] - 1, head h on key head
+ * h / (heads / kv_heads), in double with one rounding at the end; rows outside the sequences are zeros. grads: dq, dk, dv of gy. */
+int oracle_packed_attention(int dtype, const void* q, const void* k, const void* v, const int32_t* cu, void* out, int64_t tokens,
+                            int64_t batch, int64_t heads, int64_t kv_heads, int64_t dh, int causal, double scale);
+int oracle_packed_attention_grad(int dtype, const void* q, const void* k, const void* v, const int32_t* cu, const void* gy, void* dq,
+                                 void* dk, void* dv, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dh,
+                                 int causal, double scale);
+
 #ifdef __cplusplus
 }
 #endif

@@ -116,6 +116,8 @@ def test_cache_calls_are_refused():
                 dict(os=260), dict(tokens=-1), dict(heads=3), dict(heads=0), dict(scale=0.0), dict(scale=float("nan")),
                 dict(new=-1), dict(keys=-1), dict(tokens=1 << 31)):
         assert paged(**bad) == INVALID, bad
+    c = cache(table_stride=1 << 16)
+    r = ctypes.byref(c)
     need = lib.fh_attention_paged_workspace(r, 4, 4, 1, 1 << 20)
     assert need > 0  # few rows over a long context: the keys are cut into parts
     assert paged(keys=1 << 20, n=need - 1) == INVALID
