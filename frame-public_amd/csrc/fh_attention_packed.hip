@@ -110,24 +110,26 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   kv.dh = a.dh;
   KvStage<T, DH, kDense, W * 64, kBlock> stage;
   const TileReader<DH> tiles(lds, lane);
-  auto scores = [&](int kbuf, int vbuf, int t, f32x16_t& s, f32x16_t& dp) {  // q k and dout v for 32 keys
+  auto scores = [&](const TileReader<DH>& kt, const TileReader<DH>& vt, int t, f32x16_t& s, f32x16_t& dp) {  // q k, dout v: 32 keys
     clear(s);
     clear(dp);
 #pragma unroll
     for (int i = 0; i < DH / 16; ++i) {
-      mfma32<T>(tiles.rows(kbuf, 32 * t, i), qf[i], s);
-      mfma32<T>(tiles.rows(vbuf, 32 * t, i), gf[i], dp);
+      mfma32<T>(kt.rows(32 * t, i), qf[i], s);
+      mfma32<T>(vt.rows(32 * t, i), gf[i], dp);
     }
   };
-  stage.load(kv, seq.begin, nullptr, kv_head, 0, kend, tid);
+  stage.start(kv, seq.begin, nullptr, kv_head, 0, kend, tid);
+  stage.load(kv, nullptr, kv_head, 0, kend, tid);
   stage.store(lds, lds + BYTES, tid);
+  settle();
   __syncthreads();
   int buf = 0;
   for (int kb = 0; kb < kend; kb += kBlock) {
     const bool more = kb + kBlock < kend;
-    if (more) stage.load(kv, seq.begin, nullptr, kv_head, kb + kBlock, kend, tid);
+    if (more) stage.load(kv, nullptr, kv_head, kb + kBlock, kend, tid);
     if (kb <= lim_high) {
-      const int kbuf = buf * 2 * BYTES, vbuf = kbuf + BYTES;
+      const TileReader<DH> kt = tiles.at(buf * 2 * BYTES), vt = kt.at(BYTES);
       const bool edge = kb + kBlock - 1 > lim_low;
       if (lim_high < kBlock) {
         // Rows that see one block: D = sum p dp / sum p from the block itself, as a difference from the first key's dp. D from the
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           f32x16_t s, dp;
-          scores(kbuf, vbuf, t, s, dp);
+          scores(kt, vt, t, s, dp);
           if (t == 0) both_halves(dp[0], d0, unused);
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f32x16_t s, dp;
-        scores(kbuf, vbuf, t, s, dp);
+        scores(kt, vt, t, s, dp);
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -lse2));
@@ -166,7 +168,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
         for (int hf = 0; hf < 2; ++hf) {
           const u32x4_t ds = pack_slice<T>(s, hf);
 #pragma unroll
-          for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(tiles.columns(kbuf, 32 * t + 16 * hf, dt), ds, acc[dt]);
+          for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(kt.columns(32 * t + 16 * hf, dt), ds, acc[dt]);
         }
       }
     }
@@ -282,12 +284,13 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
     load(range.begin);
     store(0);
   }
+  settle();
   __syncthreads();
   int buf = 0;
   for (int rb = range.begin; rb < range.end; rb += kGradRows) {
     const bool more = rb + kGradRows < range.end;
     if (more) load(rb + kGradRows);
-    const int qbuf = buf * 2 * BYTES, gbuf = qbuf + BYTES;
+    const TileReader<DH> qt = tiles.at(buf * 2 * BYTES), gt = qt.at(BYTES);
 #pragma unroll
     for (int t = 0; t < kGradRows / 32; ++t) {
       const int r0 = rb + 32 * t;
@@ -297,7 +300,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
       f32x16_t s;
       clear(s);
 #pragma unroll
-      for (int i = 0; i < DH / 16; ++i) mfma32<T>(tiles.rows(qbuf, 32 * t, i), kf[i], s);
+      for (int i = 0; i < DH / 16; ++i) mfma32<T>(qt.rows(32 * t, i), kf[i], s);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float4 ls = *reinterpret_cast<const float4*>(&stats[buf][0][32 * t + 8 * q + 4 * hi]);
@@ -305,13 +308,12 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[4 * q + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + j], c, -lv[j]));
       }
-      int operand = gbuf;
+      const TileReader<DH> operand = for_dk ? qt : gt;
       if (for_dk) {
-        operand = qbuf;
         f32x16_t dp;
         clear(dp);
 #pragma unroll
-        for (int i = 0; i < DH / 16; ++i) mfma32<T>(tiles.rows(gbuf, 32 * t, i), vf[i], dp);
+        for (int i = 0; i < DH / 16; ++i) mfma32<T>(gt.rows(32 * t, i), vf[i], dp);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float4 dl = *reinterpret_cast<const float4*>(&stats[buf][1][32 * t + 8 * q + 4 * hi]);
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
       for (int hf = 0; hf < 2; ++hf) {
         const u32x4_t p = pack_slice<T>(s, hf);
 #pragma unroll
-        for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(tiles.columns(operand, 32 * t + 16 * hf, dt), p, acc[dt]);
+        for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(operand.columns(32 * t + 16 * hf, dt), p, acc[dt]);
       }
     }
     if (more) store(buf ^ 1);

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
   unsigned char* mine = lds + wave * 2 * BYTES;
   KvStage<T, DH, SRC, 64, BK> stage;
   const int kfirst = kbegin + wave * BK;
-  stage.look_up(a, tile.table, kfirst, kend, lane);
+  stage.start(a, tile.seq.begin, tile.table, kv_head, kfirst, kend, lane);
   u32x4_t qf[DH / 16];
   {
     const uint16_t* qr = a.q + trow * a.ldq + static_cast<int64_t>(head) * a.dh;
@@ -63,12 +63,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
   const TileReader<DH> tiles(mine, lane);
   constexpr int STEP = kWaves * BK;
   if (kfirst < kend) {
-    stage.template load<STEP>(a, tile.seq.begin, tile.table, kv_head, kfirst, kend, lane);
+    settle();
+    stage.template load<STEP>(a, tile.table, kv_head, kfirst, kend, lane);
     for (int kb = kfirst; kb < kend; kb += STEP) {
       stage.store(mine, mine + BYTES, lane);
       const uint64_t there = stage.there;
-      if (kb + STEP < kend) stage.template load<STEP>(a, tile.seq.begin, tile.table, kv_head, kb + STEP, kend, lane);
-      state.template block<1>(tiles, 0, BYTES, qf, c, kb, kb + BK - 1 > lim_low || there != ~uint64_t{0}, lim, there, hi);
+      if (kb + STEP < kend) stage.template load<STEP>(a, tile.table, kv_head, kb + STEP, kend, lane);
+      state.template block<1>(tiles, tiles.at(BYTES), qf, c, kb, kb + BK - 1 > lim_low || there != ~uint64_t{0}, lim, there, hi);
     }
   }
 

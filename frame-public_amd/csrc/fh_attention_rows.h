@@ -77,6 +77,19 @@ struct KvStage {
   int page;         // of this lane's key in the block that load() takes next; -1: none
   uint32_t scales;  // kE4m3: of this lane's key in the block on its way: the key's byte, the value's
   uint64_t there;   // kPaged, kE4m3: keys of that block that exist
+  const uint16_t* kp;  // kDense: this thread's chunk of the block that load() takes next
+  const uint16_t* vp;
+
+  // before the first load(), with that block's kb
+  __device__ __forceinline__ void start(const RowsArgs& a, int begin, const int32_t* table, int kv_head, int kb, int kend, int tid) {
+    if constexpr (SRC == kDense) {
+      const int64_t row = begin + kb + tid / CH, col = static_cast<int64_t>(kv_head) * a.dh + tid % CH * 8;
+      kp = static_cast<const uint16_t*>(a.k) + row * a.ldk + col;
+      vp = static_cast<const uint16_t*>(a.v) + row * a.ldv + col;
+    } else {
+      look_up(a, table, kb, kend, tid);
+    }
+  }
 
   __device__ __forceinline__ void look_up(const RowsArgs& a, const int32_t* table, int kb, int kend, int tid) {
     if constexpr (SRC != kDense) {
@@ -87,9 +100,28 @@ struct KvStage {
 
   // STEP: from this block to the next that this stage takes
   template <int STEP = BK>
-  __device__ __forceinline__ void load(const RowsArgs& a, int begin, const int32_t* table, int kv_head, int kb, int kend, int tid) {
+  __device__ __forceinline__ void load(const RowsArgs& a, const int32_t* table, int kv_head, int kb, int kend, int tid) {
     const int chunk = tid % CH, row0 = tid / CH;
     const bool inside = chunk * 8 < a.dh;
+    if constexpr (SRC == kDense) {
+      if (kb + BK <= kend && a.dh == DH) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          k[n] = *reinterpret_cast<const u32x4_t*>(kp + n * PASS * a.ldk);
+          v[n] = *reinterpret_cast<const u32x4_t*>(vp + n * PASS * a.ldv);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const bool ok = inside && kb + row0 + n * PASS < kend;
+          k[n] = load_chunk(kp + n * PASS * a.ldk, ok);
+          v[n] = load_chunk(vp + n * PASS * a.ldv, ok);
+        }
+      }
+      kp += STEP * a.ldk;
+      vp += STEP * a.ldv;
+      return;
+    }
     const int in_page = (1 << a.page_shift) - 1;
     auto cache_row = [&](int p, int key) {
       return ((static_cast<int64_t>(p) << a.page_shift) + (key & in_page)) * a.kv_heads + kv_head;
@@ -109,13 +141,7 @@ struct KvStage {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int key = kb + row0 + n * PASS;
-      if constexpr (SRC == kDense) {
-        const int64_t row = begin + key;
-        const int64_t col = static_cast<int64_t>(kv_head) * a.dh + chunk * 8;
-        const bool ok = inside && key < kend;
-        k[n] = load_chunk(static_cast<const uint16_t*>(a.k) + row * a.ldk + col, ok);
-        v[n] = load_chunk(static_cast<const uint16_t*>(a.v) + row * a.ldv + col, ok);
-      } else {
+      if constexpr (SRC != kDense) {
         const int p = __shfl(page, row0 + n * PASS, 64);
         const bool ok = inside && p >= 0;
         const int64_t at = cache_row(p, key) * a.dh + chunk * 8;
@@ -165,16 +191,16 @@ struct RowState {
     for (int dt = 0; dt < DH / 32; ++dt) clear(o[dt]);
   }
 
-  // keys kb .. of the block at kbuf / vbuf; MASK: by `lim` (the lane's last visible key) and the block's `there` bits
+  // keys kb .. of the block that kt and vt read; masked: by `lim` (the lane's last visible key) and the block's `there` bits
   template <int NT>
-  __device__ __forceinline__ void block(const TileReader<DH>& tiles, int kbuf, int vbuf, const u32x4_t (&qf)[DH / 16], float c,
+  __device__ __forceinline__ void block(const TileReader<DH>& kt, const TileReader<DH>& vt, const u32x4_t (&qf)[DH / 16], float c,
                                         int kb, bool masked, int lim, uint64_t there, int hi) {
     f32x16_t s[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       clear(s[t]);
 #pragma unroll
-      for (int i = 0; i < DH / 16; ++i) mfma32<T>(tiles.rows(kbuf, 32 * t, i), qf[i], s[t]);
+      for (int i = 0; i < DH / 16; ++i) mfma32<T>(kt.rows(32 * t, i), qf[i], s[t]);
     }
     if (masked) {
 #pragma unroll
@@ -185,11 +211,11 @@ struct RowState {
           s[t][x] = kb + u <= lim && ((there >> u) & 1) != 0 ? s[t][x] : -__builtin_inff();
         }
     }
-    float top = s[0][0];
+    float top = -__builtin_inff();
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int x = 0; x < 16; ++x) top = fmaxf(top, s[t][x]);
+      for (int x = 0; x < 16; x += 2) top = max3(top, s[t][x], s[t][x + 1]);
     top = half_max(top) * c;
     if (__any(top > m + 8.0f)) {
       const float next = fmaxf(m, top);
@@ -215,7 +241,7 @@ struct RowState {
       for (int hf = 0; hf < 2; ++hf) {
         const u32x4_t p = pack_slice<T>(s[t], hf);
 #pragma unroll
-        for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(tiles.columns(vbuf, 32 * t + 16 * hf, dt), p, o[dt]);
+        for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(vt.columns(32 * t + 16 * hf, dt), p, o[dt]);
       }
   }
 
@@ -328,19 +354,20 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   const TileReader<DH> tiles(lds, lane);
   uint64_t there = ~uint64_t{0};
   if (kbegin < kend) {
-    stage.look_up(a, tile.table, kbegin, kend, tid);
-    stage.load(a, tile.seq.begin, tile.table, kv_head, kbegin, kend, tid);
+    stage.start(a, tile.seq.begin, tile.table, kv_head, kbegin, kend, tid);
+    stage.load(a, tile.table, kv_head, kbegin, kend, tid);
     stage.store(lds, lds + BYTES, tid);
     if constexpr (SRC != kDense) there = stage.there;
   }
+  settle();
   __syncthreads();
   int buf = 0;
   for (int kb = kbegin; kb < kend; kb += kBlock) {
     const bool more = kb + kBlock < kend;
-    if (more) stage.load(a, tile.seq.begin, tile.table, kv_head, kb + kBlock, kend, tid);
+    if (more) stage.load(a, tile.table, kv_head, kb + kBlock, kend, tid);
     if (kb <= lim_high) {
-      const int kbuf = buf * 2 * BYTES;
-      state.template block<2>(tiles, kbuf, kbuf + BYTES, qf, c, kb, kb + kBlock - 1 > lim_low || there != ~uint64_t{0}, lim, there,
+      const TileReader<DH> kt = tiles.at(buf * 2 * BYTES);
+      state.template block<2>(kt, kt.at(BYTES), qf, c, kb, kb + kBlock - 1 > lim_low || there != ~uint64_t{0}, lim, there,
                               hi);
     }
     if (more) {

@@ -105,36 +105,52 @@ __device__ __forceinline__ int tile_at(int row, int chunk) {
 // Fragments of a tile in LDS. rows(): rows row0 .. row0 + 31 (lane l: row l % 32), slice s of 16 values (lane half: 8 of them).
 // columns(): the transposed operand: lane l: column 32 dt + l % 32, the 8 rows row0 + 4 (l / 32) + {0..3, 8..11} of a 16-row slice,
 // which is the order in which a 32x32 product's result holds its rows.
+// A tile starts on a multiple of its row's length, so a slice or column tile is one XOR on the lane's byte address, and rows are
+// offsets in the instruction (a reader per buffer: at()).
 template <int DH>
 struct TileReader {
-  const unsigned char* base;
-  int row_off, row_x, col_off[2], col_x[2];
-  __device__ __forceinline__ explicit TileReader(const unsigned char* lds, int lane) : base(lds) {
+  uint32_t row_at, col_at[2];
+  __device__ __forceinline__ TileReader(const void* lds, int lane) {
+    const uint32_t base = lds_addr((const FH_LDS void*)lds);
     const int l32 = lane & 31, hi = lane >> 5;
-    row_off = l32 * (DH * 2);
-    row_x = swz<DH>(l32) ^ hi;
+    row_at = base + l32 * (DH * 2) + ((swz<DH>(l32) ^ hi) << 4);
     const int g = lane >> 4, rr = lane & 15, qd = rr & 3, e = rr >> 2;
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       const int row = 8 * part + 4 * (g >> 1) + e;
-      col_off[part] = row * (DH * 2) + (qd & 1) * 8;
-      col_x[part] = swz<DH>(row) ^ (2 * (g & 1) + (qd >> 1));
+      col_at[part] = base + row * (DH * 2) + (qd & 1) * 8 + ((swz<DH>(row) ^ (2 * (g & 1) + (qd >> 1))) << 4);
     }
   }
-  __device__ __forceinline__ u32x4_t rows(int buffer, int row0, int s) const {
-    return *reinterpret_cast<const u32x4_t*>(base + buffer + row0 * (DH * 2) + row_off + ((row_x ^ (2 * s)) << 4));
+  // the same fragments of the tile `bytes` further on (a multiple of the row's length)
+  __device__ __forceinline__ TileReader at(int bytes) const {
+    TileReader r = *this;
+    r.row_at += bytes;
+    r.col_at[0] += bytes;
+    r.col_at[1] += bytes;
+    return r;
   }
-  __device__ __forceinline__ u32x4_t columns(int buffer, int row0, int dt) const {
-    const u32x2_t a = read(buffer, row0, dt, 0), b = read(buffer, row0, dt, 1);
+  __device__ __forceinline__ u32x4_t rows(int row0, int s) const {
+    return *(reinterpret_cast<const FH_LDS u32x4_t*>(row_at ^ static_cast<uint32_t>(s << 5)) + row0 * (DH / 8));
+  }
+  __device__ __forceinline__ u32x4_t columns(int row0, int dt) const {
+    const u32x2_t a = read(row0, dt, 0), b = read(row0, dt, 1);
     return u32x4_t{a[0], a[1], b[0], b[1]};
   }
 
  private:
-  __device__ __forceinline__ u32x2_t read(int buffer, int row0, int dt, int part) const {
-    const unsigned char* p = base + buffer + row0 * (DH * 2) + col_off[part] + ((col_x[part] ^ (4 * dt)) << 4);
-    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((FH_LDS s16x4_t*)(p)));
+  __device__ __forceinline__ u32x2_t read(int row0, int dt, int part) const {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           reinterpret_cast<FH_LDS s16x4_t*>(col_at[part] ^ static_cast<uint32_t>(dt << 6)) +
+                                           row0 * (DH / 4)));
   }
 };
+
+// max(m, a, b) in one instruction: fmaxf on products' results would first canonicalise each of them
+__device__ __forceinline__ float max3(float m, float a, float b) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(m), "v"(a), "v"(b));
+  return r;
+}
 
 // max / sum of a lane's value and the other half's (same row of a 32x32 result, the other 16 of its values)
 __device__ __forceinline__ void both_halves(float v, float& low, float& high) {
@@ -169,6 +185,10 @@ __device__ __forceinline__ u32x4_t pack_slice(const f32x16_t& p, int hf) {
 
 // Row x of lane half hi in a 32x32 result.
 __device__ __forceinline__ constexpr int result_row(int x, int hi) { return 8 * (x / 4) + 4 * hi + x % 4; }
+
+// Every load so far has arrived. Before a loop whose loads run ahead of their use: without it the compiler, which cannot tell the
+// first iteration from the others, waits inside the loop for all loads in flight wherever it uses a value loaded before the loop.
+__device__ __forceinline__ void settle() { wait_vmcnt<0>(); }
 
 // A 16-byte chunk of 8 values at p when `there`, else zeros.
 __device__ __forceinline__ u32x4_t load_chunk(const uint16_t* p, bool there) {
