@@ -428,7 +428,9 @@ int64_t delta_bytes(const fh_packed_attention& g) { return (g.tokens * g.heads *
 // longest tile would otherwise outlast the others by twice their mean.
 int64_t grad_parts(const fh_packed_attention& g) {
   const int64_t tiles = (g.tokens + kGradKeys - 1) / kGradKeys * g.kv_heads, cus = device_cu_count();
-  const int64_t blocks = g.tokens * (g.heads / g.kv_heads) / kGradRows;
+  // rows of a sequence four times the mean length: the lengths themselves are on the device
+  const int64_t longest = std::min(g.tokens, 4 * g.tokens / std::max<int64_t>(g.batch, 1));
+  const int64_t blocks = longest * (g.heads / g.kv_heads) / kGradRows;
   if (tiles >= 3 * cus || blocks <= kWholeBlocks) return 1;
   return std::max<int64_t>(1, std::min<int64_t>((3 * cus + tiles - 1) / tiles, 4));
 }

@@ -1,8 +1,9 @@
 // Attention of new tokens over a paged cache (fh_attention_paged), in two forms chosen by the rows that a key head has to serve at
 // once (new tokens times the group's heads):
-//   up to 32, decoding steps: attention_keys_kernel. One tile of 32 rows, and the keys are shared out among the waves of the
-//     workgroup. Nothing but the cache's bytes counts: every wave keeps a block of 32 keys and values on its way in registers
-//     while it uses the last one from LDS of its own, so no wave ever waits for another.
+//   up to 32, decoding steps: attention_keys_kernel. Tiles of 16 rows, and the keys are shared out among the waves of the
+//     workgroup. Nothing but the cache's bytes counts: every wave keeps one or two blocks of 32 keys and values on their way in
+//     registers while it uses another from LDS of its own, so no wave ever waits for another. (With tiles of 32 rows, mostly empty, and one
+//     block on its way, 64 sequences' step over an e4m3 cache of 550 MB took 165 us, bound by the waits for memory.)
 //   more, chunks: attention_rows_kernel of fh_attention_rows.h, whose waves share the keys and own 32 rows each.
 // Both cut long contexts into parts (keys z * part_keys ..) where the tiles alone would leave CUs idle; attention_join_kernel sums the
 // parts, weighted by their log-sum-exps, in their order.
@@ -22,101 +23,169 @@ using namespace attn;
 
 constexpr int kWaves = 4;
 
-// Keys [kbegin, kend) in blocks of 32, block i to wave i % kWaves; then the waves' sums are joined through LDS.
+// Keys [kbegin, kend) in blocks of 32, block i to wave i % kWaves; then the waves' sums are joined through LDS. Products are
+// 16x16x32: scores transposed (a lane holds 8 keys of one row), probabilities in place as the operand of V^T P^T.
 template <typename T, int DH, int SRC>
 __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const RowsArgs a) {
-  constexpr int BK = 32, BYTES = BK * DH * 2;
+  constexpr int BK = 32, BYTES = BK * DH * 2, PITCH = DH + 4, ROWS = 16;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kWaves * 2 * BYTES];
-  __shared__ float stats[2][kWaves][32];
-  static_assert(2 * BYTES == 32 * DH * 4, "a wave's room holds its fp32 sums");
+  __shared__ float stats[2][kWaves][ROWS];
+  static_assert(ROWS * PITCH * 4 <= 2 * BYTES, "a wave's room holds its fp32 sums");
 
-  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
   const int slot = static_cast<int>(blockIdx.x) / a.kv_heads;
   RowTile tile;
-  if (!tile.find<SRC>(a, slot, 5)) return;
-  int kbegin = 0, kend = tile.limit(a, tile.tile0 + 31) + 1;
+  if (!tile.find<SRC>(a, slot, 4)) return;
+  int kbegin = 0, kend = tile.limit(a, tile.tile0 + ROWS - 1) + 1;
   bool whole;
   if (!tile.part(a, static_cast<int>(blockIdx.z), kbegin, kend, whole)) return;
 
-  const int r = tile.tile0 + l32;
-  const bool live = r < tile.rows;
-  const int lim = tile.limit(a, r), lim_low = tile.limit(a, tile.tile0);
-  const int token = divide(min(r, tile.rows - 1), a.group);
   const int group = static_cast<int>(a.group.d);
-  const int head = kv_head * group + (min(r, tile.rows - 1) - token * group);
-  const int64_t trow = tile.seq.begin + token;
+  const int lim = tile.limit(a, tile.tile0 + l16), lim_low = tile.limit(a, tile.tile0);
 
   unsigned char* mine = lds + wave * 2 * BYTES;
-  KvStage<T, DH, SRC, 64, BK> stage;
+  // blocks on their way: 16 KB a wave either way (two of 128 16-bit values would spill)
+  constexpr int DEPTH = SRC == kE4m3 || DH == 64 ? 2 : 1;
+  constexpr int STEP = DEPTH * kWaves * BK;  // between a stage's blocks
+  KvStage<T, DH, SRC, 64, BK> stages[DEPTH];
   const int kfirst = kbegin + wave * BK;
-  stage.start(a, tile.seq.begin, tile.table, kv_head, kfirst, kend, lane);
-  u32x4_t qf[DH / 16];
-  {
-    const uint16_t* qr = a.q + trow * a.ldq + static_cast<int64_t>(head) * a.dh;
 #pragma unroll
-    for (int s = 0; s < DH / 16; ++s) qf[s] = load_chunk(qr + 16 * s + 8 * hi, live && 16 * s + 8 * hi < a.dh);
+  for (int i = 0; i < DEPTH; ++i) stages[i].start(a, tile.seq.begin, tile.table, kv_head, kfirst + i * kWaves * BK, kend, lane);
+  u32x4_t qf[DH / 32];
+  {
+    const int r = min(tile.tile0 + l16, tile.rows - 1), token = divide(r, a.group), head = kv_head * group + r - token * group;
+    const uint16_t* qr = a.q + (tile.seq.begin + token) * a.ldq + static_cast<int64_t>(head) * a.dh;
+#pragma unroll
+    for (int s = 0; s < DH / 32; ++s) qf[s] = load_chunk(qr + 32 * s + 8 * g, 32 * s + 8 * g < a.dh);
   }
   const float c = a.scale * kLog2e;
-  RowState<T, DH> state;
-  const TileReader<DH> tiles(mine, lane);
-  constexpr int STEP = kWaves * BK;
-  if (kfirst < kend) {
-    settle();
-    stage.template load<STEP>(a, tile.table, kv_head, kfirst, kend, lane);
-    for (int kb = kfirst; kb < kend; kb += STEP) {
-      stage.store(mine, mine + BYTES, lane);
-      const uint64_t there = stage.there;
-      if (kb + STEP < kend) stage.template load<STEP>(a, tile.table, kv_head, kb + STEP, kend, lane);
-      state.template block<1>(tiles, tiles.at(BYTES), qf, c, kb, kb + BK - 1 > lim_low || there != ~uint64_t{0}, lim, there, hi);
+  float m = -__builtin_inff(), l = 0.0f;  // l: the lane's share
+  f32x4_t o[DH / 16];
+#pragma unroll
+  for (int dt = 0; dt < DH / 16; ++dt) o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const TileReader16<DH> tiles(mine, lane);
+
+  auto use = [&](int kb, uint64_t there) {  // the block in LDS
+    f32x4_t s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) mfma16x<T>(tiles.rows(16 * t, i), qf[i], s[t]);
+    }
+    if (kb + BK - 1 > lim_low || there != ~uint64_t{0}) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int u = 16 * t + 4 * g + x;
+          s[t][x] = kb + u <= lim && ((there >> u) & 1) != 0 ? s[t][x] : -__builtin_inff();
+        }
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int x = 0; x < 4; x += 2) top = max3(top, s[t][x], s[t][x + 1]);
+    top = quarter_max(top) * c;
+    if (__any(top > m + 8.0f)) {
+      const float next = fmaxf(m, top);
+      const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < DH / 16; ++dt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[dt][x] *= f;
+    }
+    const float ms = m == -__builtin_inff() ? 0.0f : m;
+    u32x4_t p;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[t][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], c, -ms));
+        l += s[t][x];
+      }
+      p[2 * t] = store2<T>(s[t][0], s[t][1]);
+      p[2 * t + 1] = store2<T>(s[t][2], s[t][3]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DH / 16; ++dt) mfma16x<T>(tiles.columns(BYTES, dt), p, o[dt]);
+  };
+
+  settle();
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i)
+    if (kfirst + i * kWaves * BK < kend)
+      stages[i].template load<STEP>(a, tile.table, kv_head, kfirst + i * kWaves * BK, kend, lane);
+  for (int kb = kfirst; kb < kend; kb += STEP) {
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      const int at = kb + i * kWaves * BK;
+      if (at < kend) {
+        stages[i].store(mine, mine + BYTES, lane);
+        const uint64_t there = stages[i].there;
+        if (at + STEP < kend) stages[i].template load<STEP>(a, tile.table, kv_head, at + STEP, kend, lane);
+        use(at, there);
+      }
     }
   }
 
-  // every wave's maximum and sum, then its accumulators at the common scale: wave w sums the rows' d in [w DH / 4, (w + 1) DH / 4)
-  const float sum = half_sum(state.l);
-  if (hi == 0) {
-    stats[0][wave][l32] = state.m;
-    stats[1][wave][l32] = sum;
+  // every wave's maximum and sum per row, and its accumulators at the common scale
+  const float sum = quarter_sum(l);
+  if (g == 0) {
+    stats[0][wave][l16] = m;
+    stats[1][wave][l16] = sum;
   }
   __syncthreads();
-  float top = stats[0][0][l32], total = 0.0f;
+  float top = stats[0][0][l16];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, stats[0][w][l32]);
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, stats[0][w][l16]);
+  const float f = __builtin_amdgcn_exp2f(m - (top == -__builtin_inff() ? 0.0f : top));
+  float* room = reinterpret_cast<float*>(mine);
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) total += stats[1][w][l32] * __builtin_amdgcn_exp2f(stats[0][w][l32] - ref);
-  const float f = __builtin_amdgcn_exp2f(state.m - ref);
-  float* room = reinterpret_cast<float*>(mine);  // [DH][32]: the rows of the transposed result, a lane per row
-#pragma unroll
-  for (int dt = 0; dt < DH / 32; ++dt)
-#pragma unroll
-    for (int x = 0; x < 16; ++x) room[(32 * dt + result_row(x, hi)) * 32 + l32] = state.o[dt][x] * f;
+  for (int dt = 0; dt < DH / 16; ++dt)
+    *reinterpret_cast<float4*>(room + l16 * PITCH + 16 * dt + 4 * g) =
+        make_float4(o[dt][0] * f, o[dt][1] * f, o[dt][2] * f, o[dt][3] * f);
   __syncthreads();
+
+  // 16 threads per row, DH / 16 values each
+  const int row = tid >> 4, d = (tid & 15) * (DH / 16), r = tile.tile0 + row;
+  if (r >= tile.rows) return;
+  float high = stats[0][0][row], total = 0.0f;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) high = fmaxf(high, stats[0][w][row]);
+  const float ref = high == -__builtin_inff() ? 0.0f : high;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) total += stats[1][w][row] * __builtin_amdgcn_exp2f(stats[0][w][row] - ref);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  const int token = divide(r, a.group);
+  const int64_t trow = tile.seq.begin + token, head = kv_head * group + r - token * group;
   const int64_t part_row = (static_cast<int64_t>(blockIdx.z) * a.tokens + trow) * a.heads + head;
-  if (live && !whole && wave == 0 && hi == 0)
-    a.part_lse[part_row] = total == 0.0f ? -__builtin_inff() : ref + __log2f(total);
-  const float* all = reinterpret_cast<const float*>(lds);
+  if (!whole && (tid & 15) == 0) a.part_lse[part_row] = total == 0.0f ? -__builtin_inff() : ref + __log2f(total);
 #pragma unroll
-  for (int i = 0; i < DH / 32; ++i) {  // 4 values a lane and step
-    const int d = wave * (DH / 4) + 8 * i + 4 * hi;
-    float y[4];
+  for (int i = 0; i < DH / 64; ++i) {  // 4 values at a time
+    const int at = d + 4 * i;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) v += all[w * (DH * 32) + (d + j) * 32 + l32];
-      y[j] = v * inv;
+    for (int w = 0; w < kWaves; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(lds + w * 2 * BYTES) + row * PITCH + at);
+      y.x += v.x;
+      y.y += v.y;
+      y.z += v.z;
+      y.w += v.w;
     }
-    if (live && d < a.dh) {
+    if (at < a.dh) {
       if (!whole) {
-        *reinterpret_cast<float4*>(a.part_out + part_row * a.dh + d) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<float4*>(a.part_out + part_row * a.dh + at) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
       } else {
         u32x2_t w;
-        w[0] = store2<T>(y[0], y[1]);
-        w[1] = store2<T>(y[2], y[3]);
-        *reinterpret_cast<u32x2_t*>(a.out + trow * a.ldo + static_cast<int64_t>(head) * a.dh + d) = w;
+        w[0] = store2<T>(y.x * inv, y.y * inv);
+        w[1] = store2<T>(y.z * inv, y.w * inv);
+        *reinterpret_cast<u32x2_t*>(a.out + trow * a.ldo + head * a.dh + at) = w;
       }
     }
   }
@@ -209,12 +278,13 @@ Plan plan(const fh_paged_cache& c, int64_t tokens, int64_t heads, int64_t max_ne
   max_keys = std::min(max_keys, c.table_stride * c.page_size);
   Plan p{};
   p.by_keys = max_new * group <= 32;
-  const int64_t rows = p.by_keys ? 32 : 32 * kWaves;
+  const int64_t rows = p.by_keys ? 16 : 32 * kWaves;
   p.slots = tokens * group / rows + c.batch;
-  // Tiles that the expected lengths make, and enough parts for 4 (by keys; 2 fit a CU) or 3 rounds of workgroups, so that sequences
-  // of different lengths even out; no part shorter than 8 (4) blocks.
+  // Tiles that the expected lengths make, and enough parts for 6 (by keys) or 3 rounds of the workgroups that fit the chip, so that
+  // sequences of different lengths even out; no part shorter than 8 blocks. (Two rounds by keys: the 64 sequences above 156 us
+  // instead of 139, the longest parts start last.)
   const int64_t tiles = std::max<int64_t>(1, c.kv_heads * std::min(p.slots, c.batch * ((max_new * group + rows - 1) / rows)));
-  const int64_t want = ((p.by_keys ? 4 : 6) * cus + tiles - 1) / tiles;
+  const int64_t want = ((p.by_keys ? 12 : 6) * cus + tiles - 1) / tiles;
   const int64_t least = p.by_keys ? 256 : 512;
   const int64_t parts = std::max<int64_t>(1, std::min({want, max_keys / least, int64_t{128}}));
   p.part_keys = std::max(least, ((max_keys + parts - 1) / parts + kBlock - 1) / kBlock * kBlock);

@@ -145,6 +145,34 @@ struct TileReader {
   }
 };
 
+// The same for 16x16x32 products. rows(): rows row0 .. row0 + 15 (lane l: row l % 16), slice s of 32 values (8 in each 16-lane group).
+// columns(): lane l: column 16 dt + l % 16, the rows 4 (l / 16) + {0..3, 16..19} of a 32-row tile: the order in which two results
+// of 16 rows hold them.
+template <int DH>
+struct TileReader16 {
+  uint32_t row_at, col_at;
+  __device__ __forceinline__ TileReader16(const void* lds, int lane) {
+    const uint32_t base = lds_addr((const FH_LDS void*)lds);
+    const int l16 = lane & 15, g = lane >> 4, qd = lane & 3, e = (lane >> 2) & 3;
+    row_at = base + l16 * (DH * 2) + ((swz<DH>(l16) ^ g) << 4);
+    const int row = 4 * g + e;
+    col_at = base + row * (DH * 2) + (qd & 1) * 8 + ((swz<DH>(row) ^ (qd >> 1)) << 4);
+  }
+  __device__ __forceinline__ u32x4_t rows(int row0, int s) const {
+    return *(reinterpret_cast<const FH_LDS u32x4_t*>(row_at ^ static_cast<uint32_t>(s << 6)) + row0 * (DH / 8));
+  }
+  __device__ __forceinline__ u32x4_t columns(int bytes, int dt) const {  // of the tile `bytes` further on
+    const uint32_t at = col_at ^ static_cast<uint32_t>(dt << 5);
+    const u32x2_t a = read(at + bytes), b = read(at + bytes + 16 * DH * 2);
+    return u32x4_t{a[0], a[1], b[0], b[1]};
+  }
+
+ private:
+  __device__ __forceinline__ static u32x2_t read(uint32_t at) {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<FH_LDS s16x4_t*>(at)));
+  }
+};
+
 // max(m, a, b) in one instruction: fmaxf on products' results would first canonicalise each of them
 __device__ __forceinline__ float max3(float m, float a, float b) {
   float r;
@@ -167,6 +195,16 @@ __device__ __forceinline__ float half_sum(float v) {
   float a, b;
   both_halves(v, a, b);
   return a + b;
+}
+
+// over the 4 lanes l, l + 16, l + 32, l + 48
+__device__ __forceinline__ float quarter_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
 __device__ __forceinline__ void clear(f32x16_t& a) {
