@@ -191,31 +191,25 @@ struct RowState {
     for (int dt = 0; dt < DH / 32; ++dt) clear(o[dt]);
   }
 
-  // keys kb .. of the block that kt and vt read; masked: by `lim` (the lane's last visible key) and the block's `there` bits
-  template <int NT>
-  __device__ __forceinline__ void block(const TileReader<DH>& kt, const TileReader<DH>& vt, const u32x4_t (&qf)[DH / 16], float c,
-                                        int kb, bool masked, int lim, uint64_t there, int hi) {
-    f32x16_t s[NT];
+  // One 32-key tile in four steps. raise(): takes the running maximum up to the tile's, and returns the reference of its
+  // exponentials; mixed(): exponentials, their sum, and the probabilities as the next product's operand; gather(): V^T P^T.
+  __device__ __forceinline__ static void scores(const TileReader<DH>& kt, int row0, const u32x4_t (&qf)[DH / 16], f32x16_t& s) {
+    clear(s);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      clear(s[t]);
+    for (int i = 0; i < DH / 16; ++i) mfma32<T>(kt.rows(row0, i), qf[i], s);
+  }
+  // key: the tile's first; there: bit u of the tile's keys that exist
+  __device__ __forceinline__ static void mask(f32x16_t& s, int key, int lim, uint32_t there, int hi) {
 #pragma unroll
-      for (int i = 0; i < DH / 16; ++i) mfma32<T>(kt.rows(32 * t, i), qf[i], s[t]);
+    for (int x = 0; x < 16; ++x) {
+      const int u = result_row(x, hi);
+      s[x] = key + u <= lim && ((there >> u) & 1) != 0 ? s[x] : -__builtin_inff();
     }
-    if (masked) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int u = 32 * t + result_row(x, hi);
-          s[t][x] = kb + u <= lim && ((there >> u) & 1) != 0 ? s[t][x] : -__builtin_inff();
-        }
-    }
+  }
+  __device__ __forceinline__ float raise(const f32x16_t& s, float c) {
     float top = -__builtin_inff();
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int x = 0; x < 16; x += 2) top = max3(top, s[t][x], s[t][x + 1]);
+    for (int x = 0; x < 16; x += 2) top = max3(top, s[x], s[x + 1]);
     top = half_max(top) * c;
     if (__any(top > m + 8.0f)) {
       const float next = fmaxf(m, top);
@@ -227,22 +221,44 @@ struct RowState {
 #pragma unroll
         for (int x = 0; x < 16; ++x) o[dt][x] *= f;
     }
-    const float ms = m == -__builtin_inff() ? 0.0f : m;
+    return m == -__builtin_inff() ? 0.0f : m;
+  }
+  // weigh the tile s (reference `ref`) into p while the next tile's scores are formed from kt: a product, then the exponentials of as
+  // many values as take its time, and so on in this order; fragments are read three products ahead. vf: the first half of the
+  // values that gather() multiplies, read on the way.
+  __device__ __forceinline__ void mixed(f32x16_t& s, float c, float ref, u32x4_t (&p)[2], const TileReader<DH>& kt, int row0,
+                                        const u32x4_t (&qf)[DH / 16], f32x16_t& next, const TileReader<DH>& vt, int vrow,
+                                        u32x4_t (&vf)[DH / 32]) {
+    constexpr int N = DH / 16, PER = 16 / N, AHEAD = 3;
+    u32x4_t kf[N];
+    clear(next);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < AHEAD; ++i) kf[i] = kt.rows(row0, i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        s[t][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], c, -ms));
-        l += s[t][x];
+    for (int i = 0; i < N; ++i) {
+      mfma32<T>(kf[i], qf[i], next);
+      if (i + AHEAD < N) kf[i + AHEAD] = kt.rows(row0, i + AHEAD);
+      if (i >= N - DH / 32) vf[i - (N - DH / 32)] = vt.columns(vrow, i - (N - DH / 32));
+#pragma unroll
+      for (int x = PER * i; x < PER * (i + 1); ++x) {
+        s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], c, -ref));
+        l += s[x];
       }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int x = PER * i; x < PER * (i + 1); x += 2) p[x / 8][x % 8 / 2] = store2<T>(s[x], s[x + 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  __device__ __forceinline__ void gather(const TileReader<DH>& vt, int row0, const u32x4_t (&p)[2], const u32x4_t (&vf)[DH / 32]) {
+    u32x4_t second[DH / 32];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const u32x4_t p = pack_slice<T>(s[t], hf);
+    for (int dt = 0; dt < DH / 32; ++dt) second[dt] = vt.columns(row0 + 16, dt);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(vt.columns(32 * t + 16 * hf, dt), p, o[dt]);
-      }
+    for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(vf[dt], p[0], o[dt]);
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(second[dt], p[1], o[dt]);
   }
 
   // rows without a visible key: zeros, lse -inf
@@ -352,7 +368,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   RowState<T, DH> state;
   KvStage<T, DH, SRC, W * 64, kBlock> stage;
   const TileReader<DH> tiles(lds, lane);
-  uint64_t there = ~uint64_t{0};
+  uint64_t there = ~uint64_t{0}, there_next = ~uint64_t{0};
   if (kbegin < kend) {
     stage.start(a, tile.seq.begin, tile.table, kv_head, kbegin, kend, tid);
     stage.load(a, tile.table, kv_head, kbegin, kend, tid);
@@ -361,21 +377,37 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   }
   settle();
   __syncthreads();
+  if (kbegin + kBlock < kend) stage.load(a, tile.table, kv_head, kbegin + kBlock, kend, tid);
+  f32x16_t s0, s1;
+  state.scores(tiles, 0, qf, s0);
   int buf = 0;
   for (int kb = kbegin; kb < kend; kb += kBlock) {
-    const bool more = kb + kBlock < kend;
-    if (more) stage.load(a, tile.table, kv_head, kb + kBlock, kend, tid);
-    if (kb <= lim_high) {
-      const TileReader<DH> kt = tiles.at(buf * 2 * BYTES);
-      state.template block<2>(kt, kt.at(BYTES), qf, c, kb, kb + kBlock - 1 > lim_low || there != ~uint64_t{0}, lim, there,
-                              hi);
+    const bool more = kb + kBlock < kend, mine = kb <= lim_high;
+    const bool edge = kb + kBlock - 1 > lim_low || there != ~uint64_t{0};
+    const TileReader<DH> kt = tiles.at(buf * 2 * BYTES), vt = kt.at(BYTES);
+    u32x4_t p[2], vf[DH / 32];
+    if (mine) {
+      if (edge) state.mask(s0, kb, lim, static_cast<uint32_t>(there), hi);
+      const float ref = state.raise(s0, c);
+      state.mixed(s0, c, ref, p, kt, 32, qf, s1, vt, 0, vf);
     }
+    __syncthreads();  // every wave has read the other buffer's last values
     if (more) {
       unsigned char* next = lds + (buf ^ 1) * 2 * BYTES;
       stage.store(next, next + BYTES, tid);
-      if constexpr (SRC != kDense) there = stage.there;
+      if constexpr (SRC != kDense) there_next = stage.there;
+      if (kb + 2 * kBlock < kend) stage.load(a, tile.table, kv_head, kb + 2 * kBlock, kend, tid);
     }
-    __syncthreads();
+    if (mine) state.gather(vt, 0, p, vf);
+    __syncthreads();  // the next block is in LDS
+    if (mine) {
+      if (edge) state.mask(s1, kb + 32, lim, static_cast<uint32_t>(there >> 32), hi);
+      const float ref = state.raise(s1, c);
+      // (after the last block: scores of nothing, unused)
+      state.mixed(s1, c, ref, p, tiles.at((buf ^ 1) * 2 * BYTES), 0, qf, s0, vt, 32, vf);
+      state.gather(vt, 32, p, vf);
+    }
+    there = there_next;
     buf ^= 1;
   }
 
