@@ -44,7 +44,7 @@ struct GradArgs {
   float* part;  // parts > 1: [parts][dv, dk][tokens][kv_heads * dh]
 };
 
-constexpr int kWholeBlocks = 24;  // key tiles of no more blocks of rows are not cut
+constexpr int kWholeBlocks = 32;  // key tiles of no more blocks of rows are not cut
 
 template <typename T, int DH, int W>
 __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs a) {
@@ -215,7 +215,8 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool for_dk = wave >= 4;
   const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
-  const int slot = static_cast<int>(blockIdx.x) / a.kv_heads;  // a causal sequence's first keys are seen by most rows
+  // the parts of a tile side by side: a causal sequence's first keys, seen by most rows, go first with all their parts
+  const int work = static_cast<int>(blockIdx.x) / a.kv_heads, slot = work / a.parts, z = work - slot * a.parts;
   const int group = static_cast<int>(a.group.d);
   int first_slot = 0;
   Span seq;
@@ -223,8 +224,8 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
   const int keys = seq.end - seq.begin, rows = keys * group;
   const int tile0 = (slot - first_slot) * kGradKeys;
   if (tile0 >= keys) return;
-  const RowRange range = row_range(a, tile0, rows, static_cast<int>(blockIdx.z));
-  if (range.whole && blockIdx.z != 0) return;
+  const RowRange range = row_range(a, tile0, rows, z);
+  if (range.whole && z != 0) return;
 
   const int k0 = tile0 + (wave & 3) * 32, key = k0 + l32;
   const bool live = key < keys;
@@ -298,9 +299,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
       if (a.causal && r0 + 32 <= k0 * group) continue;
       const bool edge = a.causal && r0 < (k0 + 31) * group;
       f32x16_t s;
-      clear(s);
-#pragma unroll
-      for (int i = 0; i < DH / 16; ++i) mfma32<T>(qt.rows(32 * t, i), kf[i], s);
+      row_product<T, DH, 3>(qt, 32 * t, kf, s);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float4 ls = *reinterpret_cast<const float4*>(&stats[buf][0][32 * t + 8 * q + 4 * hi]);
@@ -311,9 +310,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
       const TileReader<DH> operand = for_dk ? qt : gt;
       if (for_dk) {
         f32x16_t dp;
-        clear(dp);
-#pragma unroll
-        for (int i = 0; i < DH / 16; ++i) mfma32<T>(gt.rows(32 * t, i), vf[i], dp);
+        row_product<T, DH, 3>(gt, 32 * t, vf, dp);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float4 dl = *reinterpret_cast<const float4*>(&stats[buf][1][32 * t + 8 * q + 4 * hi]);
@@ -326,12 +323,11 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[x] = r0 + result_row(x, hi) >= my_first ? s[x] : 0.0f;
       }
+      u32x4_t columns[DH / 32], p[2];
+      read_columns<DH>(operand, 32 * t, columns);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const u32x4_t p = pack_slice<T>(s, hf);
-#pragma unroll
-        for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(operand.columns(32 * t + 16 * hf, dt), p, acc[dt]);
-      }
+      for (int hf = 0; hf < 2; ++hf) p[hf] = pack_slice<T>(s, hf);
+      column_product<T, DH>(operand, 32 * t, p, columns, acc);
     }
     if (more) store(buf ^ 1);
     __syncthreads();
@@ -343,7 +339,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
     store_row<T, DH>(for_dk ? a.dk + krow * a.ldk + col : a.dv + krow * a.ldv + col, acc, factor, hi, a.dh);
     return;
   }
-  float* p = a.part + ((static_cast<int64_t>(blockIdx.z) * 2 + for_dk) * a.tokens + krow) * a.kv_heads * a.dh + col;
+  float* p = a.part + ((static_cast<int64_t>(z) * 2 + for_dk) * a.tokens + krow) * a.kv_heads * a.dh + col;
 #pragma unroll
   for (int dt = 0; dt < DH / 32; ++dt)
 #pragma unroll
@@ -431,8 +427,8 @@ int64_t grad_parts(const fh_packed_attention& g) {
   // rows of a sequence four times the mean length: the lengths themselves are on the device
   const int64_t longest = std::min(g.tokens, 4 * g.tokens / std::max<int64_t>(g.batch, 1));
   const int64_t blocks = longest * (g.heads / g.kv_heads) / kGradRows;
-  if (tiles >= 3 * cus || blocks <= kWholeBlocks) return 1;
-  return std::max<int64_t>(1, std::min<int64_t>((3 * cus + tiles - 1) / tiles, 4));
+  if (tiles >= 2 * cus || blocks <= kWholeBlocks) return 1;
+  return std::max<int64_t>(1, std::min<int64_t>((2 * cus + tiles - 1) / tiles, 4));
 }
 
 }  // namespace
@@ -540,7 +536,7 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
     if (fh_status st = launch_status("attention_dq_kernel launch"); st != FH_OK) return st;
     a.slots = static_cast<int>(slots_for(*g, 1, kGradKeys));
     hipLaunchKernelGGL((attention_dkv_kernel<T, DH>),
-                       dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads), 1, static_cast<uint32_t>(a.parts)),
+                       dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads) * static_cast<uint32_t>(a.parts)),
                        dim3(512), 0, s, a);
     if (fh_status st = launch_status("attention_dkv_kernel launch"); st != FH_OK || a.parts == 1) return st;
     hipLaunchKernelGGL((attention_dkv_join_kernel<T>), dim3(static_cast<uint32_t>((g->tokens + 3) / 4)), dim3(256), 0, s, a);

@@ -191,13 +191,8 @@ struct RowState {
     for (int dt = 0; dt < DH / 32; ++dt) clear(o[dt]);
   }
 
-  // One 32-key tile in four steps. raise(): takes the running maximum up to the tile's, and returns the reference of its
-  // exponentials; mixed(): exponentials, their sum, and the probabilities as the next product's operand; gather(): V^T P^T.
-  __device__ __forceinline__ static void scores(const TileReader<DH>& kt, int row0, const u32x4_t (&qf)[DH / 16], f32x16_t& s) {
-    clear(s);
-#pragma unroll
-    for (int i = 0; i < DH / 16; ++i) mfma32<T>(kt.rows(row0, i), qf[i], s);
-  }
+  // One 32-key tile. raise(): takes the running maximum up to the tile's, and returns the reference of its exponentials; mixed():
+  // exponentials, their sum, and the probabilities as the operand of V^T P^T.
   // key: the tile's first; there: bit u of the tile's keys that exist
   __device__ __forceinline__ static void mask(f32x16_t& s, int key, int lim, uint32_t there, int hi) {
 #pragma unroll
@@ -225,7 +220,7 @@ struct RowState {
   }
   // weigh the tile s (reference `ref`) into p while the next tile's scores are formed from kt: a product, then the exponentials of as
   // many values as take its time, and so on in this order; fragments are read three products ahead. vf: the first half of the
-  // values that gather() multiplies, read on the way.
+  // values' fragments, read on the way.
   __device__ __forceinline__ void mixed(f32x16_t& s, float c, float ref, u32x4_t (&p)[2], const TileReader<DH>& kt, int row0,
                                         const u32x4_t (&qf)[DH / 16], f32x16_t& next, const TileReader<DH>& vt, int vrow,
                                         u32x4_t (&vf)[DH / 32]) {
@@ -250,17 +245,6 @@ struct RowState {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  __device__ __forceinline__ void gather(const TileReader<DH>& vt, int row0, const u32x4_t (&p)[2], const u32x4_t (&vf)[DH / 32]) {
-    u32x4_t second[DH / 32];
-#pragma unroll
-    for (int dt = 0; dt < DH / 32; ++dt) second[dt] = vt.columns(row0 + 16, dt);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(vf[dt], p[0], o[dt]);
-#pragma unroll
-    for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(second[dt], p[1], o[dt]);
-  }
-
   // rows without a visible key: zeros, lse -inf
   __device__ __forceinline__ void finish(float& inv, float& lse2) {
     const float sum = half_sum(l);
@@ -379,7 +363,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   __syncthreads();
   if (kbegin + kBlock < kend) stage.load(a, tile.table, kv_head, kbegin + kBlock, kend, tid);
   f32x16_t s0, s1;
-  state.scores(tiles, 0, qf, s0);
+  row_product<T, DH>(tiles, 0, qf, s0);
   int buf = 0;
   for (int kb = kbegin; kb < kend; kb += kBlock) {
     const bool more = kb + kBlock < kend, mine = kb <= lim_high;
@@ -398,14 +382,14 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
       if constexpr (SRC != kDense) there_next = stage.there;
       if (kb + 2 * kBlock < kend) stage.load(a, tile.table, kv_head, kb + 2 * kBlock, kend, tid);
     }
-    if (mine) state.gather(vt, 0, p, vf);
+    if (mine) column_product<T, DH>(vt, 0, p, vf, state.o);
     __syncthreads();  // the next block is in LDS
     if (mine) {
       if (edge) state.mask(s1, kb + 32, lim, static_cast<uint32_t>(there >> 32), hi);
       const float ref = state.raise(s1, c);
       // (after the last block: scores of nothing, unused)
       state.mixed(s1, c, ref, p, tiles.at((buf ^ 1) * 2 * BYTES), 0, qf, s0, vt, 32, vf);
-      state.gather(vt, 32, p, vf);
+      column_product<T, DH>(vt, 32, p, vf, state.o);
     }
     there = there_next;
     buf ^= 1;

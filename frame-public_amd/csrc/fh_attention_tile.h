@@ -221,6 +221,45 @@ __device__ __forceinline__ u32x4_t pack_slice(const f32x16_t& p, int hf) {
   return w;
 }
 
+// Products with their fragments read ahead, in this order: an LDS read takes as long as four products, and the compiler by itself places
+// each read one or two products before its use.
+// acc = rows row0 .. row0 + 31 of the tile times the fragments f
+template <typename T, int DH, int AHEAD = 4>
+__device__ __forceinline__ void row_product(const TileReader<DH>& tile, int row0, const u32x4_t (&f)[DH / 16], f32x16_t& acc) {
+  constexpr int N = DH / 16;
+  u32x4_t r[N];
+  clear(acc);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) r[i] = tile.rows(row0, i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    mfma32<T>(r[i], f[i], acc);
+    if (i + AHEAD < N) r[i + AHEAD] = tile.rows(row0, i + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+// the first 16 rows' fragments of column_product, to be read before the values are ready
+template <int DH>
+__device__ __forceinline__ void read_columns(const TileReader<DH>& tile, int row0, u32x4_t (&first)[DH / 32]) {
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt) first[dt] = tile.columns(row0, dt);
+  __builtin_amdgcn_sched_barrier(0);
+}
+// acc += (rows row0 .. row0 + 31 of the tile)^T times p, a 32x32 result as two packed slices
+template <typename T, int DH>
+__device__ __forceinline__ void column_product(const TileReader<DH>& tile, int row0, const u32x4_t (&p)[2],
+                                               const u32x4_t (&first)[DH / 32], f32x16_t (&acc)[DH / 32]) {
+  u32x4_t second[DH / 32];
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt) second[dt] = tile.columns(row0 + 16, dt);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(first[dt], p[0], acc[dt]);
+#pragma unroll
+  for (int dt = 0; dt < DH / 32; ++dt) mfma32<T>(second[dt], p[1], acc[dt]);
+}
+
 // Row x of lane half hi in a 32x32 result.
 __device__ __forceinline__ constexpr int result_row(int x, int hi) { return 8 * (x / 4) + 4 * hi + x % 4; }
 
