@@ -40,7 +40,8 @@ struct GradArgs {
   int causal;
   float scale;
   int slots;
-  int parts;    // of the rows of a key tile
+  int tile_keys;  // keys of a workgroup of the second kernel
+  int parts;      // of the rows of a key tile
   float* part;  // parts > 1: [parts][dv, dk][tokens][kv_heads * dh]
 };
 
@@ -184,7 +185,6 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
 }
 
 constexpr int kGradRows = 64;  // rows of q and dout per block
-constexpr int kGradKeys = 128;
 
 // The rows [begin, end) that part z of a key tile sums over, in whole blocks; `whole`: the first part takes them all.
 struct RowRange {
@@ -199,21 +199,21 @@ __device__ __forceinline__ RowRange row_range(const GradArgs& a, int tile0, int 
   return {(first + z * per) * kGradRows, min(rows, (first + (z + 1) * per) * kGradRows), false};
 }
 
-// 128 keys per workgroup of 8 waves: waves w and w + 4 own the same 32 keys and sit on one SIMD; the first sums dv (two products:
+// 32 PAIRS keys per workgroup of 2 PAIRS waves: waves w and w + PAIRS own the same 32 keys (with 4 pairs on one SIMD); the first sums dv (two products:
 // q k and p dout), the second dk (three: q k, dout v and ds q). Forming q k twice leaves each wave one accumulator, which is what lets
 // two waves share a SIMD's registers and hide each other's waits; with both sums in one wave (400 registers, one wave per SIMD) the
 // same work took more than twice as long.
-template <typename T, int DH>
-__global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a) {
-  constexpr int BYTES = kGradRows * DH * 2, SHIFT = __builtin_ctz(kGradKeys);
-  constexpr int CH = DH / 8, PASS = 512 / CH, N = kGradRows / PASS;
+template <typename T, int DH, int PAIRS>
+__global__ __launch_bounds__(PAIRS * 128, 2) void attention_dkv_kernel(const GradArgs a) {
+  constexpr int BYTES = kGradRows * DH * 2, KEYS = 32 * PAIRS, SHIFT = __builtin_ctz(KEYS);
+  constexpr int CH = DH / 8, PASS = PAIRS * 128 / CH, N = kGradRows / PASS;
   static_assert(kGradRows % PASS == 0, "whole passes");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
   __shared__ __attribute__((aligned(16))) float stats[2][2][kGradRows];  // per buffer: lse (base 2), D
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const bool for_dk = wave >= 4;
+  const bool for_dk = wave >= PAIRS;
   const int kv_head = static_cast<int>(blockIdx.x) % a.kv_heads;
   // the parts of a tile side by side: a causal sequence's first keys, seen by most rows, go first with all their parts
   const int work = static_cast<int>(blockIdx.x) / a.kv_heads, slot = work / a.parts, z = work - slot * a.parts;
@@ -222,12 +222,12 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_kernel(const GradArgs a)
   Span seq;
   if (find_sequence(a.cu, a.batch, a.tokens, 1, SHIFT, slot, first_slot, seq) < 0) return;
   const int keys = seq.end - seq.begin, rows = keys * group;
-  const int tile0 = (slot - first_slot) * kGradKeys;
+  const int tile0 = (slot - first_slot) * KEYS;
   if (tile0 >= keys) return;
   const RowRange range = row_range(a, tile0, rows, z);
   if (range.whole && z != 0) return;
 
-  const int k0 = tile0 + (wave & 3) * 32, key = k0 + l32;
+  const int k0 = tile0 + (wave & (PAIRS - 1)) * 32, key = k0 + l32;
   const bool live = key < keys;
   const int64_t krow = seq.begin + (live ? key : 0);
   const int64_t col = static_cast<int64_t>(kv_head) * a.dh;
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const GradArgs 
   const Span seq = sequence(a.cu, b, a.tokens);
   if (token < seq.begin || token >= seq.end) return;
   const int rows = (seq.end - seq.begin) * static_cast<int>(a.group.d);
-  const int tile0 = (token - seq.begin) / kGradKeys * kGradKeys;
+  const int tile0 = (token - seq.begin) / a.tile_keys * a.tile_keys;
   if (row_range(a, tile0, rows, 0).whole) return;
   const int width = a.kv_heads * a.dh;
   const int64_t stride = static_cast<int64_t>(a.tokens) * width;
@@ -422,8 +422,13 @@ int64_t delta_bytes(const fh_packed_attention& g) { return (g.tokens * g.heads *
 
 // A key tile's rows are cut into parts where the tiles are few: a causal sequence's first keys are seen by all of its rows, so the
 // longest tile would otherwise outlast the others by twice their mean.
+// Keys per workgroup: 128, or 64 where that leaves fewer than two workgroups a CU and the head dim's registers allow the longer
+// staging.
+int64_t grad_keys(const fh_packed_attention& g) {
+  return g.dh <= 64 && (g.tokens + 127) / 128 * g.kv_heads < 2 * device_cu_count() ? 64 : 128;
+}
 int64_t grad_parts(const fh_packed_attention& g) {
-  const int64_t tiles = (g.tokens + kGradKeys - 1) / kGradKeys * g.kv_heads, cus = device_cu_count();
+  const int64_t keys = grad_keys(g), tiles = (g.tokens + keys - 1) / keys * g.kv_heads, cus = device_cu_count();
   // rows of a sequence four times the mean length: the lengths themselves are on the device
   const int64_t longest = std::min(g.tokens, 4 * g.tokens / std::max<int64_t>(g.batch, 1));
   const int64_t blocks = longest * (g.heads / g.kv_heads) / kGradRows;
@@ -512,6 +517,7 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
   a.dv = static_cast<uint16_t*>(dv);
   a.lse = lse;
   a.delta = static_cast<float*>(workspace);
+  a.tile_keys = static_cast<int>(grad_keys(*g));
   a.parts = workspace_bytes < fh_attention_packed_grad_workspace(g) ? 1 : static_cast<int>(grad_parts(*g));
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(*g));
   a.cu = cu_seqlens;
@@ -534,10 +540,12 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
     hipLaunchKernelGGL((attention_dq_kernel<T, DH, W>), dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads)),
                        dim3(W * 64), 0, s, a);
     if (fh_status st = launch_status("attention_dq_kernel launch"); st != FH_OK) return st;
-    a.slots = static_cast<int>(slots_for(*g, 1, kGradKeys));
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DH>),
-                       dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads) * static_cast<uint32_t>(a.parts)),
-                       dim3(512), 0, s, a);
+    a.slots = static_cast<int>(slots_for(*g, 1, a.tile_keys));
+    const dim3 grid(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads) * static_cast<uint32_t>(a.parts));
+    if constexpr (DH == 64) {
+      if (a.tile_keys == 64) hipLaunchKernelGGL((attention_dkv_kernel<T, DH, 2>), grid, dim3(256), 0, s, a);
+    }
+    if (a.tile_keys == 128) hipLaunchKernelGGL((attention_dkv_kernel<T, DH, 4>), grid, dim3(512), 0, s, a);
     if (fh_status st = launch_status("attention_dkv_kernel launch"); st != FH_OK || a.parts == 1) return st;
     hipLaunchKernelGGL((attention_dkv_join_kernel<T>), dim3(static_cast<uint32_t>((g->tokens + 3) / 4)), dim3(256), 0, s, a);
     return launch_status("attention_dkv_join_kernel launch");
