@@ -203,7 +203,7 @@ fh_status run(const std::string& fn, const fh_paged_cache* c, void* k, int64_t k
   a.page_shift = page_shift(c->page_size);
   auto launch = [&]<typename T, int LANES, bool E4M3>() {
     // a few tokens per workgroup once every CU has several of them
-    const int64_t per = std::min<int64_t>(kMostTokens, std::max<int64_t>(1, tokens / (8 * device_cu_count())));
+    const int64_t per = std::min<int64_t>(kMostTokens, std::max<int64_t>(1, tokens / (4 * device_cu_count())));
     const int64_t blocks = (tokens + per - 1) / per;
     if (blocks > kMaxBlocks) return fail(FH_INVALID_ARGUMENT, fn + ": too many rows");
     hipLaunchKernelGGL((kv_cache_kernel<T, LANES, E4M3, WRITE>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0,
