@@ -3,8 +3,10 @@
 // max|row| <= 448 p, and 1 for a row of zeros. A power of two costs the 3-bit fraction nothing against any other scale and is
 // undone exactly: the cached value e4m3 * p is a bf16 value, so attention needs no further rounding of it. Values that are not
 // finite become NaN, and the maximum is taken over the others.
-// Both kernels move 16 bytes of the tensors' side per lane, a row in DH / 8 lanes (8 or 16, power of two, for the maximum's shuffles);
-// they are bound by memory, and by the launch for a step's few rows.
+// Both directions move 16 bytes of the tensors' side per lane, a row in DH / 8 lanes (8 or 16, power of two, for the maximum's
+// shuffles); they are bound by memory, and by the launch for a step's few rows. Measured, 8 heads of 128: 65,532 cached rows read
+// as bf16 89 us (404 MB, 4.55 TB/s; a copy reaches 5.13), 8,192 rows written 14.3 us (50 MB, 3.5 TB/s); one row in flight per
+// thread and a lookup per row: 154 and 16.7 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -23,7 +23,7 @@ inline fh_status check_paged_cache(const std::string& fn, const fh_paged_cache* 
   if (c->page_size < 1 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)) != 0)
     return fail(FH_UNIMPLEMENTED, fn + ": page size must be a power of two up to 65536");
   if (c->kv_heads < 1 || c->kv_heads > 65535 || c->batch < 0 || c->batch > 0x3fffffff || c->pages < 0 || c->pages > 0x7fffffff ||
-      c->table_stride < 0 || c->table_stride > 0x7fffffff / c->page_size)
+      c->table_stride < 0 || c->table_stride > 0x7fff0000 / c->page_size)  // (positions and a few blocks more fit 32 bits)
     return fail(FH_INVALID_ARGUMENT, fn + ": bad kv_heads, batch, pages or table_stride");
   if (c->batch == 0) return FH_OK;
   if (c->kv_lens == nullptr || (c->table_stride > 0 && c->block_table == nullptr) || (c->pages > 0 && (!c->k || !c->v)))
