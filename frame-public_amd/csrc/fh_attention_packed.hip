@@ -9,9 +9,9 @@
 //   attention_dq_kernel:  32 rows per wave as in the forward; D is formed from its rows and kept for the second kernel.
 //   attention_dkv_kernel: 32 keys per wave, keys and values in registers, blocks of 64 rows of q and dout in LDS.
 // p and ds are rounded to the storage type as operands of the second products; everything else is fp32.
-// Measured: 2897 + 1034 + 165 tokens, 32 heads over 8, 128 dims, causal, bf16: 422 us (dq 155, dk and dv 255, the parts' sum 12),
-// 460 TFLOP/s counted as 5 products, 644 as the 7 that are made; 3300 tokens in 8 sequences, 16 heads of 64: 48 us. Bound by the waits
-// of a tile's dependent steps (product, exponentials, product), which two waves per SIMD do not fill.
+// Measured: 2897 + 1034 + 165 tokens, 32 heads over 8, 128 dims, causal, bf16: 430 us (traced: dq 172, dk and dv 280, the
+// parts' sum 12), 452 TFLOP/s counted as 5 products, 633 as the 7 that are made; 3300 tokens in 8 sequences, 16 heads of 64: 48.5 us.
+// Bound by the waits of a tile's dependent steps (product, exponentials, product), which two waves per SIMD do not fill.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -55,6 +55,9 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   constexpr int BYTES = kBlock * DH * 2;
   constexpr int ROWS = 32 * W, SHIFT = __builtin_ctz(ROWS);
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
+  // The first key with a value that is not finite, of those that scrub() zeroes, per 8 columns: every score of a row that sees it, so every
+  // derivative, is not finite either.
+  __shared__ int first_bad[DH / 8];
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -66,7 +69,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   if (find_sequence(a.cu, a.batch, a.tokens, group, SHIFT, slot, first_slot, seq) < 0) return;
   const int keys = seq.end - seq.begin, rows = keys * group;
   const int tile0 = (slot - first_slot) * ROWS;
-  if (tile0 >= rows) return;
+  if (!tile_in(tile0, rows)) return;
   auto limit = [&](int r) { return a.causal ? divide(min(r, rows - 1), a.group) : keys - 1; };
   const int kend = limit(tile0 + ROWS - 1) + 1;
 
@@ -125,7 +128,19 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   };
   stage.start(kv, seq.begin, nullptr, kv_head, 0, kend, tid);
   stage.load(kv, nullptr, kv_head, 0, kend, tid);
+  const int common = limit(tile0);
+  const bool uneven = common != kend - 1;
+  auto look = [&](unsigned char* keys_at, int kb) {
+    if (uneven && kb + kBlock - 1 > common)
+      scrub<T, DH, stage.PASS>(keys_at, tid / stage.CH, tid % stage.CH, stage.k,
+                               [&](int row, int d, uint32_t) { atomicMin(&first_bad[d / 8], kb + row); });
+  };
+  if (uneven) {
+    if (tid < DH / 8) first_bad[tid] = 0x7fffffff;
+    __syncthreads();
+  }
   stage.store(lds, lds + BYTES, tid);
+  look(lds, 0);
   settle();
   __syncthreads();
   int buf = 0;
@@ -179,9 +194,21 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
     if (more) {
       unsigned char* next = lds + (buf ^ 1) * 2 * BYTES;
       stage.store(next, next + BYTES, tid);
+      look(next, kb + kBlock);
     }
     __syncthreads();
     buf ^= 1;
+  }
+  if (uneven) {
+    int first = first_bad[0];
+#pragma unroll
+    for (int i = 1; i < DH / 8; ++i) first = min(first, first_bad[i]);
+    if (lim >= first) {
+#pragma unroll
+      for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) acc[dt][x] = __builtin_nanf("");
+    }
   }
   if (live && hi == 0) a.delta[stat] = delta;
   if (live) store_row<T, DH>(a.dq + trow * a.ldq + static_cast<int64_t>(head) * a.dh, acc, a.scale, hi, a.dh);
@@ -208,12 +235,15 @@ __device__ __forceinline__ RowRange row_range(const GradArgs& a, int tile0, int 
 // of 400 registers 821 us; this form 255; p handed from the first wave to the second through LDS, four products and a barrier
 // more, 304.
 template <typename T, int DH, int PAIRS>
-__global__ __launch_bounds__(PAIRS * 128, 2) void attention_dkv_kernel(const GradArgs a) {
+__global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv_kernel(const GradArgs a) {
   constexpr int BYTES = kGradRows * DH * 2, KEYS = 32 * PAIRS, SHIFT = __builtin_ctz(KEYS);
   constexpr int CH = DH / 8, PASS = PAIRS * 128 / CH, N = kGradRows / PASS;
   static_assert(kGradRows % PASS == 0, "whole passes");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
   __shared__ __attribute__((aligned(16))) float stats[2][2][kGradRows];  // per buffer: lse (base 2), D
+  // Rows with values that are not finite, of those that scrub() zeroes: the last of q per 8 columns (its scores are not finite), the last in
+  // each column of dout (dv's; its D is not finite, which reaches dk by itself), and whether there is any.
+  __shared__ int last_q[DH / 8], last_dout[DH], any_bad;
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -227,7 +257,7 @@ __global__ __launch_bounds__(PAIRS * 128, 2) void attention_dkv_kernel(const Gra
   if (find_sequence(a.cu, a.batch, a.tokens, 1, SHIFT, slot, first_slot, seq) < 0) return;
   const int keys = seq.end - seq.begin, rows = keys * group;
   const int tile0 = (slot - first_slot) * KEYS;
-  if (tile0 >= keys) return;
+  if (!tile_in(tile0, keys)) return;
   const RowRange range = row_range(a, tile0, rows, z);
   if (range.whole && z != 0) return;
 
@@ -285,9 +315,22 @@ __global__ __launch_bounds__(PAIRS * 128, 2) void attention_dkv_kernel(const Gra
   for (int dt = 0; dt < DH / 32; ++dt) clear(acc[dt]);
   const float c = a.scale * kLog2e;
   const TileReader<DH> tiles(lds, lane);
+  // blocks of rows that some keys of the tile are not seen by
+  auto look = [&](int buf, int rb) {
+    if (a.causal && rb < (tile0 + KEYS - 1) * group) {
+      unsigned char* qb = lds + buf * 2 * BYTES;
+      scrub<T, DH, PASS>(qb, srow, chunk, qs, [&](int row, int d, uint32_t) { atomicMax(&last_q[d / 8], rb + row), any_bad = 1; });
+      scrub<T, DH, PASS>(qb + BYTES, srow, chunk, gs, [&](int row, int d, uint32_t) { atomicMax(&last_dout[d], rb + row), any_bad = 1; });
+    }
+  };
   if (range.begin < range.end) {
     load(range.begin);
+    if (tid < DH) last_dout[tid] = -1;
+    if (tid < DH / 8) last_q[tid] = -1;
+    if (tid == 0) any_bad = 0;
+    __syncthreads();
     store(0);
+    look(0, range.begin);
   }
   settle();
   __syncthreads();
@@ -333,11 +376,24 @@ __global__ __launch_bounds__(PAIRS * 128, 2) void attention_dkv_kernel(const Gra
       for (int hf = 0; hf < 2; ++hf) p[hf] = pack_slice<T>(s, hf);
       column_product<T, DH>(operand, 32 * t, p, columns, acc);
     }
-    if (more) store(buf ^ 1);
+    if (more) {
+      store(buf ^ 1);
+      look(buf ^ 1, rb + kGradRows);
+    }
     __syncthreads();
     buf ^= 1;
   }
   if (!live) return;
+  if (range.begin < range.end && a.causal && any_bad != 0) {
+    int last = last_q[0];
+#pragma unroll
+    for (int i = 1; i < DH / 8; ++i) last = max(last, last_q[i]);
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+      for (int x = 0; x < 16; ++x)
+        if (my_first <= max(last, last_dout[32 * dt + result_row(x, hi)])) acc[dt][x] = __builtin_nanf("");
+  }
   const float factor = for_dk ? a.scale : 1.0f;
   if (range.whole) {
     store_row<T, DH>(for_dk ? a.dk + krow * a.ldk + col : a.dv + krow * a.ldv + col, acc, factor, hi, a.dh);

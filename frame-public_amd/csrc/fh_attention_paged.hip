@@ -33,6 +33,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
   constexpr int BK = 32, BYTES = BK * DH * 2, PITCH = DH + 4, ROWS = 16;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kWaves * 2 * BYTES];
   __shared__ float stats[2][kWaves][ROWS];
+  __shared__ NotFinite<T, DH> bad;
   static_assert(ROWS * PITCH * 4 <= 2 * BYTES, "a wave's room holds its fp32 sums");
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
@@ -47,6 +48,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
 
   const int group = static_cast<int>(a.group.d);
   const int lim = tile.limit(a, tile.tile0 + l16), lim_low = tile.limit(a, tile.tile0);
+  const bool uneven = lim_low != tile.limit(a, tile.tile0 + ROWS - 1);  // rows of several tokens
+  if (uneven) {
+    bad.clear(tid);
+    __syncthreads();
+  }
 
   unsigned char* mine = lds + wave * 2 * BYTES;
   // blocks on their way: 16 KB a wave either way (two of 128 16-bit values would spill)
@@ -130,6 +136,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
       const int at = kb + i * kWaves * BK;
       if (at < kend) {
         stages[i].store(mine, mine + BYTES, lane);
+        if (uneven && at + BK - 1 > lim_low)
+          stages[i].scrub_values(mine + BYTES, lane, [&](int row, int d, uint32_t bits) { bad.note(at + row, d, bits); });
         const uint64_t there = stages[i].there;
         if (at + STEP < kend) stages[i].template load<STEP>(a, tile.table, kv_head, at + STEP, kend, lane);
         use(at, there);
@@ -181,6 +189,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
       y.z += v.z;
       y.w += v.w;
     }
+    if (uneven && bad.any != 0) {
+      const int seen = tile.limit(a, r);
+      y.x += bad.gain(at, seen);
+      y.y += bad.gain(at + 1, seen);
+      y.z += bad.gain(at + 2, seen);
+      y.w += bad.gain(at + 3, seen);
+    }
     if (at < a.dh) {
       if (!whole) {
         *reinterpret_cast<float4*>(a.part_out + part_row * a.dh + at) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
@@ -215,7 +230,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const RowsArgs a) {
   int keys = max(a.kv_lens[b], 0);
   if (keys > cap) keys = static_cast<int>(cap);
   if (keys <= a.part_keys) return;  // written whole
-  const int parts = min((keys + a.part_keys - 1) / a.part_keys, a.splits);
+  const int parts = min((keys - 1) / a.part_keys + 1, a.splits);
 
   const int lane = threadIdx.x & 63, half = lane >> 5, d = (lane & 31) * 4;
   float top = -__builtin_inff();

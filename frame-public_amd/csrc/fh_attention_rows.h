@@ -7,14 +7,15 @@
 // probabilities, rounded to the storage type, are in place as the operand of V^T P^T.
 // What bounds it at long sequences is the vector ALU: 16 rows of 32 keys' exponentials, sums, maxima and conversions take about
 // as long as the 16 products that go with them, so the code places a product between every few exponentials. Measured: 5003 +
-// 2318 + 871 tokens, 32 heads over 8, 128 dims, causal, bf16: 302 us, 845 TFLOP/s of visible pairs (a library product of 8192^3: 1,249);
+// 2318 + 871 tokens, 32 heads over 8, 128 dims, causal, bf16: 300 us, 850 TFLOP/s of visible pairs (a library product of 8192^3: 1,249);
 // products and exponentials in separate stretches 310 us; a wait for the next block at the loop's start 318; 256 rows per
-// workgroup 302; raised wave priority around the products 312-320. Eight sequences of 512, 16 heads of 64: 16.7 us, launch and the
+// workgroup 302; raised wave priority around the products 312-320. Eight sequences of 512, 16 heads of 64: 16.9 us, launch and the
 // latencies of a workgroup's up to eight dependent blocks.
 // The accumulators are scaled again only when a row's maximum grows by more than 8 (base 2) over the one in use: sums and
 // probabilities then stay within 2^8 of their usual range, which fp32 and the rounding to 16 bits do not notice.
 // Masked scores are -inf by selection, never by addition, and rows of keys that are not there are zeros in LDS, so nothing that
-// lies behind a sequence's end, on an unused part of a page or on a page number out of range reaches a result.
+// lies behind a sequence's end, on an unused part of a page or on a page number out of range reaches a result; and values that are not
+// finite reach the rows that see them only (scrub()).
 #pragma once
 
 #include "fh_attention_tile.h"
@@ -185,6 +186,20 @@ struct KvStage {
       *reinterpret_cast<u32x4_t*>(vbuf + at) = vw;
     }
   }
+
+  // after store(), before the next load()
+  template <typename Note>
+  __device__ __forceinline__ void scrub_values(unsigned char* vbuf, int tid, Note note) const {
+    const int chunk = tid % CH, row0 = tid / CH;
+    if constexpr (SRC == kE4m3) {
+      u32x4_t w[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) w[n] = *reinterpret_cast<const u32x4_t*>(vbuf + tile_at<DH>(row0 + n * PASS, chunk));
+      scrub<T, DH, PASS>(vbuf, row0, chunk, w, note);
+    } else {
+      scrub<T, DH, PASS>(vbuf, row0, chunk, v, note);
+    }
+  }
 };
 
 // The running softmax of a wave's 32 rows over blocks of NT 32-key tiles in LDS, and the accumulators of the output.
@@ -291,7 +306,7 @@ struct RowTile {
     const int new_rows = seq.end - seq.begin;
     rows = new_rows * group;
     tile0 = (slot - first_slot) << shift;
-    if (tile0 >= rows) return false;
+    if (!tile_in(tile0, rows)) return false;
     keys = new_rows;
     first = 0;
     table = nullptr;
@@ -325,6 +340,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   constexpr int ROWS = 32 * W;
   static_assert((ROWS & (ROWS - 1)) == 0, "rows per workgroup: a power of two");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
+  __shared__ NotFinite<T, DH> bad;
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -359,10 +375,22 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   KvStage<T, DH, SRC, W * 64, kBlock> stage;
   const TileReader<DH> tiles(lds, lane);
   uint64_t there = ~uint64_t{0}, there_next = ~uint64_t{0};
+  // rows of the tile see the keys up to `common`; blocks with others are looked through for values that are not finite
+  const int common = tile.limit(a, tile.tile0);
+  const bool uneven = kbegin < kend && common != tile.limit(a, tile.tile0 + ROWS - 1);
+  auto look = [&](unsigned char* values, int kb) {
+    if (uneven && kb + kBlock - 1 > common)
+      stage.scrub_values(values, tid, [&](int row, int d, uint32_t bits) { bad.note(kb + row, d, bits); });
+  };
   if (kbegin < kend) {
     stage.start(a, tile.seq.begin, tile.table, kv_head, kbegin, kend, tid);
     stage.load(a, tile.table, kv_head, kbegin, kend, tid);
+    if (uneven) {
+      bad.clear(tid);
+      __syncthreads();
+    }
     stage.store(lds, lds + BYTES, tid);
+    look(lds + BYTES, kbegin);
     if constexpr (SRC != kDense) there = stage.there;
   }
   settle();
@@ -385,6 +413,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
     if (more) {
       unsigned char* next = lds + (buf ^ 1) * 2 * BYTES;
       stage.store(next, next + BYTES, tid);
+      look(next + BYTES, kb + kBlock);
       if constexpr (SRC != kDense) there_next = stage.there;
       if (kb + 2 * kBlock < kend) stage.load(a, tile.table, kv_head, kb + 2 * kBlock, kend, tid);
     }
@@ -404,6 +433,12 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   float inv, lse2;
   state.finish(inv, lse2);
   if (!live) return;
+  if (uneven && bad.any != 0) {
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) state.o[dt][x] += bad.gain(32 * dt + result_row(x, hi), lim);
+  }
   if (!whole) {
     state.write_part(a, (static_cast<int64_t>(blockIdx.z) * a.tokens + trow) * a.heads + head, inv, lse2, hi);
     return;

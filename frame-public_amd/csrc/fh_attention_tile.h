@@ -51,6 +51,7 @@ __device__ __forceinline__ Span sequence(const int32_t* cu, int b, int rows) {
 // host: sequence b's begin at slot(b) = floor(cu[b] * per_token / tile) + b, which leaves room for its ceil(length / tile) tiles
 // before slot(b + 1). Slots that no tile takes end at once. Every wave looks 64 sequences up at a time.
 // Host: floor(rows * per_token / tile) + batch slots.
+// Where cu_seqlens decreases, the sequence found may begin behind the slot: tile_in() takes such a tile for none.
 __device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, int rows, int per_token, int tile_shift, int slot,
                                              int& first_slot, Span& seq) {
   const int lane = threadIdx.x & 63;
@@ -75,6 +76,10 @@ __device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, int r
   seq = {begin, end};
   first_slot = static_cast<int>((static_cast<int64_t>(begin) * per_token) >> tile_shift) + found - 1;
   return found - 1;
+}
+
+__device__ __forceinline__ bool tile_in(int first_row, int rows) {
+  return static_cast<uint32_t>(first_row) < static_cast<uint32_t>(rows);
 }
 
 // The last sequence that begins at `token` or before it (the one that holds it, if any does), or -1.
@@ -170,6 +175,59 @@ struct TileReader16 {
  private:
   __device__ __forceinline__ static u32x2_t read(uint32_t at) {
     return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<FH_LDS s16x4_t*>(at)));
+  }
+};
+
+// Values that are not finite, in a block of keys that some rows of a workgroup's tile see and others do not. A product sums over the whole
+// block, and 0 times NaN is NaN: so there they are replaced by zeros in LDS, and their places are noted, for the rows that do see them to
+// be given them at the end.
+template <typename T>
+constexpr uint32_t kExponent = std::is_same_v<T, bf16_t> ? 0x7f80 : 0x7c00;  // not finite: all of these bits
+// w: the chunks that this thread has written to rows row0, row0 + PASS .. of the tile in LDS; note(row, column, bits). 10 instructions per
+// chunk, in such blocks only. (No loop in the rare part, and none that the compiler makes for atomics on one address: either gives the
+// whole kernel 16 registers more, which cost the gradients with 64 dims a wave per SIMD, 53 us instead of 48.)
+template <typename T, int DH, int PASS, int N, typename Note>
+__device__ __forceinline__ void scrub(unsigned char* tile, int row0, int chunk, const u32x4_t (&w)[N], Note note) {
+  constexpr uint32_t ONES = kExponent<T>, LOW = ONES & (0u - ONES);
+  uint32_t carry = 0;  // into a value's sign bit: an exponent of ones
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) carry |= (w[n][j] & (ONES * 0x10001u)) + LOW * 0x10001u;
+  if ((carry & 0x80008000u) == 0) return;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    u32x4_t x = w[n];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bits = (x[j / 2] >> (16 * (j & 1))) & 0xffffu;
+      if ((bits & ONES) == ONES) {
+        note(row0 + n * PASS, chunk * 8 + j, bits);
+        x[j / 2] &= j & 1 ? 0xffffu : 0xffff0000u;
+      }
+    }
+    *reinterpret_cast<u32x4_t*>(tile + tile_at<DH>(row0 + n * PASS, chunk)) = x;
+  }
+}
+
+// The first key of each column of values that holds +inf or NaN, and that holds -inf or NaN.
+template <typename T, int DH>
+struct NotFinite {
+  int first[2][DH], any;
+  __device__ __forceinline__ void clear(int tid) {  // by 2 DH threads or more
+    if (tid < 2 * DH) first[tid / DH][tid % DH] = 0x7fffffff;
+    if (tid == 0) any = 0;
+  }
+  __device__ __forceinline__ void note(int key, int d, uint32_t bits) {
+    const bool nan = (bits & 0x7fffu) > kExponent<T>, negative = (bits & 0x8000u) != 0;
+    if (nan || !negative) atomicMin(&first[0][d], key);
+    if (nan || negative) atomicMin(&first[1][d], key);
+    any = 1;
+  }
+  // what column d's sum gains for a row that sees the keys up to lim
+  __device__ __forceinline__ float gain(int d, int lim) const {
+    const float plus = lim >= first[0][d] ? __builtin_inff() : 0.0f, minus = lim >= first[1][d] ? __builtin_inff() : 0.0f;
+    return plus - minus;
   }
 };
 

@@ -329,7 +329,7 @@ fh_status fh_attention_grad(int32_t dtype, const void* q, const void* k, const v
  * memory, batch + 1 values, not decreasing; a length may be 0). A row holds `heads` heads of dh values (q, out), or kv_heads (k, v);
  * head h reads key head h / (heads / kv_heads). The strides are elements between rows, so q, k and v may be columns of one
  * projection's output. Rows outside the sequences are neither read nor written, and cu_seqlens values out of range are taken as 0 or
- * `tokens`. bf16 / f16, dh a multiple of 8 up to 128, strides multiples of 8 elements, tensors 16-byte aligned.
+ * `tokens`. No output may overlap an input. bf16 / f16, dh a multiple of 8 up to 128, strides multiples of 8 elements, tensors 16-byte aligned.
  * No counterpart in the reference, whose attention has one length, no mask and as many key heads as heads
  * (src/nn/layers.cpp:1014-1080); unlike fh_attention_fwd these round no intermediate as a graph of single ops would: scores,
  * softmax and sums are fp32, and only the probabilities (and in the gradients their derivatives) are rounded to the storage type,
@@ -343,13 +343,13 @@ typedef struct fh_packed_attention {
 } fh_packed_attention;
 
 /* out = softmax(scale q k^T) v per head, and the natural logarithm of the softmax's sum in lse ([tokens, heads] fp32; may be NULL),
- * which the gradients read. A value of the sequence itself that is not finite may reach other rows of that sequence (never of
- * another), also rows that do not see it. */
+ * which the gradients read. A value that is not finite reaches the rows that see it and no others. */
 fh_status fh_attention_packed_fwd(const fh_packed_attention* geom, const void* q, const void* k, const void* v,
                                   const int32_t* cu_seqlens, void* out, float* lse, void* stream);
 
 /* Gradients with respect to q, k and v for the output gradient dout, from the forward's operands, out and lse. dout has out's
- * stride; dq, dk and dv have q's, k's and v's. Deterministic. tokens * heads * 4 bytes of workspace are enough; with all that the
+ * stride; dq, dk and dv have q's, k's and v's. Deterministic. What is not finite reaches the gradients of what it meets: a row of q or dout those of
+ * the keys that the row sees, a key or value those of the rows that see it. tokens * heads * 4 bytes of workspace are enough; with all that the
  * query returns, the rows that a long causal sequence's first keys sum over may be cut into parts. */
 int64_t fh_attention_packed_grad_workspace(const fh_packed_attention* geom);
 fh_status fh_attention_packed_grad(const fh_packed_attention* geom, const void* q, const void* k, const void* v,
@@ -396,8 +396,8 @@ fh_status fh_kv_cache_read(const fh_paged_cache* cache, void* k, int64_t k_strid
 /* Attention of the new tokens over the cache: token i of the n new ones of sequence b sees positions 0 .. kv_lens[b] - n + i (the
  * cache holds the new tokens' keys and values already, see fh_kv_cache_write). Rows that see nothing are zeros. n = 1 is a
  * decoding step. max_new and max_keys are the longest n and kv_lens that are expected: they choose how the work is cut, and
- * any lengths give the same results up to rounding. The workspace query takes the same numbers; 0 bytes: may be NULL. As in
- * fh_attention_packed_fwd, a cached value of a visible sequence's later position that is not finite may reach its other new rows. */
+ * any lengths give the same results up to rounding. The workspace query takes the same numbers; 0 bytes: may be NULL. A
+ * cached value that is not finite reaches the rows that see it and no others. */
 int64_t fh_attention_paged_workspace(const fh_paged_cache* cache, int64_t tokens, int64_t heads, int64_t max_new, int64_t max_keys);
 fh_status fh_attention_paged(const fh_paged_cache* cache, const void* q, int64_t q_stride, void* out, int64_t out_stride,
                              int64_t tokens, int64_t heads, const int32_t* cu_seqlens, float scale, int64_t max_new,

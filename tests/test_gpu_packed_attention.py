@@ -241,6 +241,73 @@ def test_packed_not_finite_values_stay_in_their_sequence(hip):
     ref.check(lse.astype(np.float64)[clean], want_lse[clean], lse_tol[clean], "lse")
 
 
+INF = {F16: 0x7c00, BF16: 0x7f80}
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dh", [(BF16, 4, 2, 64), (F16, 2, 2, 128), (BF16, 3, 1, 40)])
+@pytest.mark.parametrize("t", [0, 5, 64, 130, 298])
+def test_packed_not_finite_values_reach_the_rows_that_see_them(hip, dtype, heads, kv_heads, dh, t):
+    # token t of the second sequence holds values that are not finite, one tensor at a time: rows that do not see it keep every bit
+    say(f"packed NaN at token {t}, {heads} heads over {kv_heads} of {dh}")
+    p = Packed(hip, dtype, [70, 300], heads, kv_heads, dh, 1)
+    group, at = heads // kv_heads, int(p.cu[1]) + t
+    clean_out, clean_lse = p.forward()
+    clean = p.backward(clean_out, clean_lse)
+    later = np.zeros(p.rows, bool)
+    later[at:] = True
+    mine = np.arange(heads * dh) // dh < group  # the heads of key head 0
+    value = lambda a: ref.values(a, dtype)
+
+    def with_bad(name, row, col, bits):
+        kept = p.x[name].copy()
+        p.x[name][row, col] = bits
+        out, lse = p.forward()
+        grads = p.backward(out, lse)
+        p.x[name] = kept
+        return out, lse, grads
+
+    def check(got, want, affected, test, what):
+        assert np.array_equal(got[~affected], want[~affected]), what + ": changed where nothing sees the value"
+        assert test(value(got[affected])).all(), what
+
+    # a value: its column, and no score
+    for bits, test in ((NAN[dtype], np.isnan), (INF[dtype], np.isposinf), (INF[dtype] | 0x8000, np.isneginf)):
+        out, lse, grads = with_bad("v", at, 3, bits)
+        check(out, clean_out, later[:, None] & mine & (np.arange(heads * dh) % dh == 3), test, "out of v")
+        assert np.array_equal(lse, clean_lse)
+        # (rows that see key t alone have a derivative of zero times its value)
+        check(grads[0], clean[0], later[:, None] & mine, lambda y: ~np.isfinite(y), "dq of v")
+    # infinities of both signs, the second one token on
+    kept = p.x["v"].copy()
+    p.x["v"][at, 3], p.x["v"][at + 1, 3] = INF[dtype], INF[dtype] | 0x8000
+    out, _ = p.forward()
+    p.x["v"] = kept
+    assert np.isposinf(value(out[at:at + 1, 3])).all() and np.isnan(value(out[at + 1:, 3])).all() and np.array_equal(out[:at], clean_out[:at])
+    # a key: all of its rows' scores
+    out, lse, grads = with_bad("k", at, 3, NAN[dtype])
+    check(out, clean_out, later[:, None] & mine, np.isnan, "out of k")
+    check(grads[0], clean[0], later[:, None] & mine, np.isnan, "dq of k")
+    assert np.isnan(lse[at:, :group]).all() and np.array_equal(lse[:at], clean_lse[:at])
+    # a row of q: itself, and the keys that it sees
+    shared = np.arange(kv_heads * dh) < dh
+    seen = np.zeros(p.rows, bool)
+    seen[p.cu[1]:at + 1] = True
+    this = np.zeros(p.rows, bool)
+    this[at] = True
+    first = np.arange(heads * dh) < dh
+    out, lse, grads = with_bad("q", at, 3, NAN[dtype])
+    check(out, clean_out, this[:, None] & first, np.isnan, "out of q")
+    for i, rows, cols in ((0, this, first), (1, seen, shared), (2, seen, shared)):
+        check(grads[i], clean[i], rows[:, None] & cols, np.isnan, f"d{'qkv'[i]} of q")
+    # an output's gradient: its column of dv, all of dk
+    kept = p.x["dout"].copy()
+    p.x["dout"][at, 3] = NAN[dtype]
+    grads = p.backward(clean_out, clean_lse)
+    p.x["dout"] = kept
+    for i, rows, cols in ((0, this, first), (1, seen, shared), (2, seen, shared & (np.arange(kv_heads * dh) % dh == 3))):
+        check(grads[i], clean[i], rows[:, None] & cols, np.isnan, f"d{'qkv'[i]} of dout")
+
+
 def test_packed_bad_lengths_stay_in_bounds(hip):
     # cu_seqlens out of range or decreasing: values are taken into [0, tokens] and no memory outside is touched
     say("packed lengths out of range")
@@ -252,6 +319,22 @@ def test_packed_bad_lengths_stay_in_bounds(hip):
     p.cu = np.array([100, 60, 160], np.int32)  # the first sequence is empty; what the second holds is its own affair
     got, lse = p.forward()
     assert (got[:60] == KEEP).all()
+
+
+def test_packed_decreasing_lengths_stay_in_bounds(hip):
+    # a sequence behind one that begins further on: slots of tiles then find the latter, whose tiles begin behind them. Causal rows 0 .. 9
+    # are the same in both sequences that hold them, so every row is either right or untouched.
+    say("packed decreasing lengths")
+    p = Packed(hip, BF16, [500], 2, 2, 64, 1)
+    want, lse = p.forward()
+    grads = p.backward(want, lse)
+    p.cu, p.lens = np.array([0, 500, 0, 10], np.int32), [500, 0, 10]
+    got, _ = p.forward()
+    right, untouched = (got == want).all(axis=1), (got == KEEP).all(axis=1)
+    assert (right | untouched).all() and right[:128].all()
+    dq = p.backward(want, lse)[0]
+    right, untouched = (dq == grads[0]).all(axis=1), (dq == KEEP).all(axis=1)
+    assert (right | untouched).all() and right[:128].all()
 
 
 def test_packed_gradients_are_deterministic_and_replay(hip):
@@ -458,6 +541,28 @@ def test_paged_pages_that_do_not_exist(hip, number):
         p.upload()
         for keys in (64, 1 << 20):
             p.check_attend(p.attend(max_keys=keys)[0], "missing page")
+
+
+@pytest.mark.parametrize("cache_dtype", [BF16, E4M3])
+@pytest.mark.parametrize("past,new,bad", [(70, 5, 3), (0, 4, 2), (2000, 6, 5), (61, 90, 40), (1500, 130, 1)])
+def test_paged_not_finite_values_reach_the_rows_that_see_them(hip, cache_dtype, past, new, bad):
+    say(f"paged NaN at new token {bad} of {new} behind {past}, cache {cache_dtype}")
+    p = Paged(hip, BF16, cache_dtype, [past], [new], 4, 2, 64, 16)
+    p.fill_past()
+    p.put_new()
+    p.upload()
+    for keys in (64, 1 << 20):
+        clean, _ = p.attend(max_keys=keys)
+        at, nan = p.slot(0, past + bad), 0x7f if cache_dtype == E4M3 else NAN[BF16]
+        kept = p.vc[at + (0, 3)]
+        p.vc[at + (0, 3)] = nan
+        p.dev["vc"].upload(p.vc)
+        out, _ = p.attend(max_keys=keys)
+        p.vc[at + (0, 3)] = kept
+        p.dev["vc"].upload(p.vc)
+        affected = (np.arange(new)[:, None] >= bad) & (np.arange(256) < 128) & (np.arange(256) % 64 == 3)
+        assert np.array_equal(out[~affected], clean[~affected])
+        assert np.isnan(ref.values(out[affected], BF16)).all()
 
 
 def test_paged_lengths_past_the_table(hip):
