@@ -329,7 +329,8 @@ fh_status fh_attention_grad(int32_t dtype, const void* q, const void* k, const v
  * memory, batch + 1 values, not decreasing; a length may be 0). A row holds `heads` heads of dh values (q, out), or kv_heads (k, v);
  * head h reads key head h / (heads / kv_heads). The strides are elements between rows, so q, k and v may be columns of one
  * projection's output. Rows outside the sequences are neither read nor written, and cu_seqlens values out of range are taken as 0 or
- * `tokens`. No output may overlap an input. bf16 / f16, dh a multiple of 8 up to 128, strides multiples of 8 elements, tensors 16-byte aligned.
+ * `tokens`. No output may overlap an input. bf16 / f16, dh a multiple of 8 up to 128, strides multiples of 8 elements, tensors
+ * 16-byte aligned.
  * No counterpart in the reference, whose attention has one length, no mask and as many key heads as heads
  * (src/nn/layers.cpp:1014-1080); unlike fh_attention_fwd these round no intermediate as a graph of single ops would: scores,
  * softmax and sums are fp32, and only the probabilities (and in the gradients their derivatives) are rounded to the storage type,
@@ -348,9 +349,9 @@ fh_status fh_attention_packed_fwd(const fh_packed_attention* geom, const void* q
                                   const int32_t* cu_seqlens, void* out, float* lse, void* stream);
 
 /* Gradients with respect to q, k and v for the output gradient dout, from the forward's operands, out and lse. dout has out's
- * stride; dq, dk and dv have q's, k's and v's. Deterministic. What is not finite reaches the gradients of what it meets: a row of q or dout those of
- * the keys that the row sees, a key or value those of the rows that see it. tokens * heads * 4 bytes of workspace are enough; with all that the
- * query returns, the rows that a long causal sequence's first keys sum over may be cut into parts. */
+ * stride; dq, dk and dv have q's, k's and v's. Deterministic. What is not finite reaches the gradients of what it meets: a row of q or
+ * dout those of the keys that the row sees, a key or value those of the rows that see it. tokens * heads * 4 bytes of workspace are
+ * enough; with all that the query returns, the rows that a long causal sequence's first keys sum over may be cut into parts. */
 int64_t fh_attention_packed_grad_workspace(const fh_packed_attention* geom);
 fh_status fh_attention_packed_grad(const fh_packed_attention* geom, const void* q, const void* k, const void* v,
                                    const int32_t* cu_seqlens, const void* out, const float* lse, const void* dout, void* dq,

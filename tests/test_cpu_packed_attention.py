@@ -125,6 +125,14 @@ def test_cache_calls_are_refused():
     assert paged(keys=1 << 20, ws=P + 8, n=need) == INVALID
 
 
+def test_positions_fit_32_bits():
+    lib = abi.lib()
+    c = cache(table_stride=0x7fff0000 // 16)
+    assert lib.fh_attention_paged_workspace(ctypes.byref(c), 1, 2, 1, 1) >= 0
+    c.table_stride += 1
+    assert lib.fh_attention_paged_workspace(ctypes.byref(c), 1, 2, 1, 1) == -1
+
+
 def test_reference_gradients_are_the_differences():
     rng = np.random.default_rng(3)
     n, dh, scale = 7, 8, 0.4

@@ -662,6 +662,44 @@ def test_write_skips_what_has_no_place(hip):
         assert np.array_equal(d[n].download(want.shape, want.dtype), want), n
 
 
+@pytest.mark.parametrize("cache_dtype", [BF16, E4M3])
+def test_offsets_past_32_bits(hip, cache_dtype):
+    # 2^32 elements and more in front of the pages: the same results as in a small cache
+    say(f"a cache of more than 2^32 elements, cache {cache_dtype}")
+    total, new, heads, dh, page = 603, 3, 4, 128, 256
+    k, v = (synth.tensor(70 + i, (total, dh), BF16, "normal") for i in range(2))
+    q = synth.tensor(72, (new, heads * dh), BF16, "normal")
+    lib, item = hip.lib(), 1 if cache_dtype == E4M3 else 2
+    dk, dv, dq = (hip.to_device(x) for x in (k, v, q))
+    lens, cu_all, cu_new = hip.to_device(np.array([total], np.int32)), hip.to_device(starts([total])), hip.to_device(starts([new]))
+    got = []
+    for pages in (3, (1 << 17) + 3):
+        kc, vc = (hip.DeviceBuffer(pages * page * dh * item) for _ in range(2))
+        ks, vs = (hip.DeviceBuffer(pages * page) for _ in range(2))
+        table = hip.to_device(np.array([[pages - 1, 0, pages - 2]], np.int32))
+        c = hip.PagedCache(dtype=BF16, cache_dtype=cache_dtype, pages=pages, page_size=page, kv_heads=1, dh=dh, k=kc.value, v=vc.value,
+                           k_scale=ks.value, v_scale=vs.value, batch=1, block_table=table.value, table_stride=3, kv_lens=lens.value)
+        r = ctypes.byref(c)
+        hip.check(lib.fh_kv_cache_write(r, dk.value, dh, dv.value, dh, total, cu_all.value, None))
+        back = [hip.to_device(np.zeros((total, dh), np.uint16)) for _ in range(2)]
+        hip.check(lib.fh_kv_cache_read(r, back[0].value, dh, back[1].value, dh, total, cu_all.value, None))
+        got.append([b.download((total, dh), np.uint16) for b in back])
+        out = hip.to_device(np.zeros((new, heads * dh), np.uint16))
+        for max_new in (new, 64):  # both forms
+            need = lib.fh_attention_paged_workspace(r, new, heads, max_new, total)
+            ws = hip.DeviceBuffer(max(need, 16))
+            hip.check(lib.fh_attention_paged(r, dq.value, heads * dh, out.value, heads * dh, new, heads, cu_new.value,
+                                             float(np.float32(1 / np.sqrt(dh))), max_new, total, ws.value, need, None))
+            hip.check(lib.fh_device_synchronize())
+            got[-1].append(out.download((new, heads * dh), np.uint16))
+        for b in (kc, vc):
+            b.free()
+    for a, b in zip(*got):
+        assert a.any() and np.array_equal(a, b)
+    if cache_dtype == BF16:
+        assert np.array_equal(got[0][0], k) and np.array_equal(got[0][1], v)
+
+
 def test_a_prompt_then_tokens_one_by_one(hip):
     """A run as a server makes it: the prompt's keys and values into an e4m3 cache, then steps that write one token each and attend
     over the cache, every step captured once and replayed, against the packed forward over what the cache reads back as."""
