@@ -118,8 +118,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
         s[t][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], c, -ms));
         l += s[t][x];
       }
-      p[2 * t] = store2<T>(s[t][0], s[t][1]);
-      p[2 * t + 1] = store2<T>(s[t][2], s[t][3]);
+      p[2 * t] = operand2<T>(s[t][0], s[t][1]);
+      p[2 * t + 1] = operand2<T>(s[t][2], s[t][3]);
     }
 #pragma unroll
     for (int dt = 0; dt < DH / 16; ++dt) mfma16x<T>(tiles.columns(BYTES, dt), p, o[dt]);

@@ -262,7 +262,7 @@ struct RowState {
         l += s[x];
       }
 #pragma unroll
-      for (int x = PER * i; x < PER * (i + 1); x += 2) p[x / 8][x % 8 / 2] = store2<T>(s[x], s[x + 1]);
+      for (int x = PER * i; x < PER * (i + 1); x += 2) p[x / 8][x % 8 / 2] = operand2<T>(s[x], s[x + 1]);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
