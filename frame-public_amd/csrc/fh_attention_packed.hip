@@ -49,11 +49,13 @@ struct GradArgs {
 };
 
 constexpr int kWholeBlocks = 32;  // key tiles of no more blocks of rows are not cut
+constexpr int kLeastBlocks = 8;   // of a part
 
-template <typename T, int DH, int W>
+// KSHARE 2: two waves share 32 rows, each taking one 32-key tile of a block, and their sums are joined through LDS.
+template <typename T, int DH, int W, int KSHARE>
 __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs a) {
   constexpr int BYTES = kBlock * DH * 2;
-  constexpr int ROWS = 32 * W, SHIFT = __builtin_ctz(ROWS);
+  constexpr int ROWS = 32 * W / KSHARE, SHIFT = __builtin_ctz(ROWS);
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
   // The first key with a value that is not finite, of those that scrub() zeroes, per 8 columns: every score of a row that sees it, so every
   // derivative, is not finite either.
@@ -73,7 +75,8 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
   auto limit = [&](int r) { return a.causal ? divide(min(r, rows - 1), a.group) : keys - 1; };
   const int kend = limit(tile0 + ROWS - 1) + 1;
 
-  const int r0 = tile0 + wave * 32, r = r0 + l32;
+  const int share = wave / (W / KSHARE);
+  const int r0 = tile0 + wave % (W / KSHARE) * 32, r = r0 + l32;
   const bool live = r < rows;
   const int lim = limit(r), lim_low = limit(r0), lim_high = limit(r0 + 31);
   const int token = divide(min(r, rows - 1), a.group);
@@ -171,7 +174,8 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
         delta = d0 + half_sum(d) / half_sum(sum);
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int i = 0; i < 2 / KSHARE; ++i) {
+        const int t = KSHARE == 2 ? share : i;
         f32x16_t s, dp;
         scores(kt, vt, t, s, dp);
 #pragma unroll
@@ -210,23 +214,37 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
         for (int x = 0; x < 16; ++x) acc[dt][x] = __builtin_nanf("");
     }
   }
+  if constexpr (KSHARE == 2) {
+    float* room = reinterpret_cast<float*>(lds) + wave % (W / 2) * (DH / 2 * 64) + lane;
+    if (share == 1) {
+#pragma unroll
+      for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) room[(dt * 16 + x) * 64] = acc[dt][x];
+    }
+    __syncthreads();
+    if (share == 1) return;
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) acc[dt][x] += room[(dt * 16 + x) * 64];
+  }
   if (live && hi == 0) a.delta[stat] = delta;
   if (live) store_row<T, DH>(a.dq + trow * a.ldq + static_cast<int64_t>(head) * a.dh, acc, a.scale, hi, a.dh);
 }
 
 constexpr int kGradRows = 64;  // rows of q and dout per block
 
-// The rows [begin, end) that part z of a key tile sums over, in whole blocks; `whole`: the first part takes them all.
+// The rows [begin, end) that part z of a key tile sums over, in whole blocks, and the tile's number of parts.
 struct RowRange {
-  int begin, end;
-  bool whole;
+  int begin, end, parts;
 };
 __device__ __forceinline__ RowRange row_range(const GradArgs& a, int tile0, int rows, int z) {
   const int first = a.causal ? tile0 * static_cast<int>(a.group.d) / kGradRows : 0;  // rows that see key u: r >= u * group
   const int blocks = (rows + kGradRows - 1) / kGradRows - first;
-  if (a.parts == 1 || blocks <= kWholeBlocks) return {first * kGradRows, z == 0 ? rows : 0, true};
-  const int per = (blocks + a.parts - 1) / a.parts;
-  return {(first + z * per) * kGradRows, min(rows, (first + (z + 1) * per) * kGradRows), false};
+  if (a.parts == 1 || blocks <= kWholeBlocks) return {first * kGradRows, z == 0 ? rows : 0, 1};
+  const int per = max((blocks + a.parts - 1) / a.parts, kLeastBlocks);
+  return {(first + z * per) * kGradRows, min(rows, (first + (z + 1) * per) * kGradRows), (blocks + per - 1) / per};
 }
 
 // 32 PAIRS keys per workgroup of 2 PAIRS waves: waves w and w + PAIRS own the same 32 keys (with 4 pairs on one SIMD); the first
@@ -259,7 +277,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv
   const int tile0 = (slot - first_slot) * KEYS;
   if (!tile_in(tile0, keys)) return;
   const RowRange range = row_range(a, tile0, rows, z);
-  if (range.whole && z != 0) return;
+  if (z >= range.parts) return;
 
   const int k0 = tile0 + (wave & (PAIRS - 1)) * 32, key = k0 + l32;
   const bool live = key < keys;
@@ -395,7 +413,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv
         if (my_first <= max(last, last_dout[32 * dt + result_row(x, hi)])) acc[dt][x] = __builtin_nanf("");
   }
   const float factor = for_dk ? a.scale : 1.0f;
-  if (range.whole) {
+  if (range.parts == 1) {
     store_row<T, DH>(for_dk ? a.dk + krow * a.ldk + col : a.dv + krow * a.ldv + col, acc, factor, hi, a.dh);
     return;
   }
@@ -411,10 +429,14 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv
     }
 }
 
-// dk and dv of the key tiles whose rows were cut into parts: the parts' sum, in their order. One wave per key row of all heads.
+// dk and dv of the key tiles whose rows were cut into parts: the parts' sum, in their order. A wave takes 256 of a token's values, so
+// that what counts, the parts' loads, are 8 deep.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const GradArgs a) {
-  const int token = static_cast<int>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int width = a.kv_heads * a.dh, slices = (2 * width + 255) / 256;
+  const int64_t work = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int token = static_cast<int>(work / slices), i = (static_cast<int>(work - static_cast<int64_t>(token) * slices) * 64 +
+                                                         static_cast<int>(threadIdx.x & 63)) * 4;
   if (token >= a.tokens) return;
   const int b = sequence_of(a.cu, a.batch, token);
   if (b < 0) return;
@@ -422,15 +444,16 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const GradArgs 
   if (token < seq.begin || token >= seq.end) return;
   const int rows = (seq.end - seq.begin) * static_cast<int>(a.group.d);
   const int tile0 = (token - seq.begin) / a.tile_keys * a.tile_keys;
-  if (row_range(a, tile0, rows, 0).whole) return;
-  const int width = a.kv_heads * a.dh;
+  const int parts = row_range(a, tile0, rows, 0).parts;
+  if (parts == 1) return;
   const int64_t stride = static_cast<int64_t>(a.tokens) * width;
-  for (int i = (threadIdx.x & 63) * 4; i < 2 * width; i += 256) {
+  if (i < 2 * width) {
     const int which = i >= width;  // 0: dv, 1: dk
     const int d = i - which * width;
     const float* p = a.part + which * stride + static_cast<int64_t>(token) * width + d;
     float4 t = *reinterpret_cast<const float4*>(p);
-    for (int z = 1; z < a.parts; ++z) {
+#pragma unroll 8
+    for (int z = 1; z < parts; ++z) {
       const float4 y = *reinterpret_cast<const float4*>(p + z * 2 * stride);
       t.x += y.x;
       t.y += y.y;
@@ -438,8 +461,8 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const GradArgs 
       t.w += y.w;
     }
     u32x2_t w;
-    w[0] = store2<T>(t.x, t.y);
-    w[1] = store2<T>(t.z, t.w);
+    w[0] = narrow2<T>(t.x, t.y);
+    w[1] = narrow2<T>(t.z, t.w);
     uint16_t* out = which ? a.dk + token * a.ldk : a.dv + token * a.ldv;
     *reinterpret_cast<u32x2_t*>(out + d) = w;
   }
@@ -480,20 +503,31 @@ int64_t slots_for(const fh_packed_attention& g, int64_t per_token, int64_t tile)
 
 int64_t delta_bytes(const fh_packed_attention& g) { return (g.tokens * g.heads * 4 + 15) / 16 * 16; }
 
-// A key tile's rows are cut into parts where the tiles are few: a causal sequence's first keys are seen by all of its rows, so the
-// longest tile would otherwise outlast the others by twice their mean.
-// Keys per workgroup: 128, or 64 where that leaves fewer than two workgroups a CU and the head dim's registers allow the longer
+// Two waves share 32 rows where tiles of 128 rows leave CUs with fewer waves than hide the steps of a block: fewer than two workgroups a CU in
+// the forward (12 sequences of up to 1886 tokens, 4 heads over 2 of 64: 22.7 us instead of 34; one of 4000, 8 heads over 1 of 128: 74
+// instead of 95; 480 workgroups: 57 either way), one and a half for dq (8 heads of 128 over 2000 tokens 139 instead of 164 in all; 416
+// workgroups: 50.3 instead of 48.5, 1048: 485 instead of 430).
+int key_shares(const fh_packed_attention& g, bool gradients) {
+  const int64_t tiles = (g.tokens * (g.heads / g.kv_heads) + 127) / 128 * g.kv_heads, cus = device_cu_count();
+  return tiles < (gradients ? cus + cus / 2 : 2 * cus) ? 2 : 1;
+}
+
+// dk, dv. Keys per workgroup: 128, or 64 where that leaves fewer than two workgroups a CU and the head dim's registers allow the longer
 // staging.
 int64_t grad_keys(const fh_packed_attention& g) {
   return g.dh <= 64 && (g.tokens + 127) / 128 * g.kv_heads < 2 * device_cu_count() ? 64 : 128;
 }
+// A key tile's rows are cut into parts where the tiles are few: a causal sequence's first keys are seen by all of its rows, so the
+// longest tile would otherwise outlast the others by twice their mean. As many as fill the chip once (three workgroups of 64 keys a CU, or one
+// of 128), and at least enough to even the tiles out. 32 heads over 8 of 64, 2800 tokens: 3 parts 137 us in all, 2 161; 8 heads over 1, 1900
+// tokens: 8 parts 102, 4 143; 8 heads over 2 of 128, 2000 tokens: 8 parts 138, 16 178 (a second round).
 int64_t grad_parts(const fh_packed_attention& g) {
   const int64_t keys = grad_keys(g), tiles = (g.tokens + keys - 1) / keys * g.kv_heads, cus = device_cu_count();
   // rows of a sequence four times the mean length: the lengths themselves are on the device
   const int64_t longest = std::min(g.tokens, 4 * g.tokens / std::max<int64_t>(g.batch, 1));
   const int64_t blocks = longest * (g.heads / g.kv_heads) / kGradRows;
   if (tiles >= 2 * cus || blocks <= kWholeBlocks) return 1;
-  return std::max<int64_t>(1, std::min<int64_t>((2 * cus + tiles - 1) / tiles, 4));
+  return std::min<int64_t>(keys == 64 ? std::max<int64_t>(3 * cus / tiles, 3) : std::max<int64_t>(cus / tiles, 2), 8);
 }
 
 }  // namespace
@@ -532,10 +566,14 @@ extern "C" fh_status fh_attention_packed_fwd(const fh_packed_attention* g, const
   a.ldk = g->k_stride;
   a.ldv = g->v_stride;
   constexpr int W = 4;
-  a.slots = static_cast<int>(slots_for(*g, a.group.d, 32 * W));
+  const int share = key_shares(*g, false);
+  a.slots = static_cast<int>(slots_for(*g, a.group.d, 32 * W / share));
   const dim3 grid(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads));
   auto launch = [&]<typename T, int DH>() {
-    hipLaunchKernelGGL((attention_rows_kernel<T, DH, kDense, W>), grid, dim3(W * 64), 0, static_cast<hipStream_t>(stream), a);
+    if (share == 2)
+      hipLaunchKernelGGL((attention_rows_kernel<T, DH, kDense, W, 2>), grid, dim3(W * 64), 0, static_cast<hipStream_t>(stream), a);
+    else
+      hipLaunchKernelGGL((attention_rows_kernel<T, DH, kDense, W, 1>), grid, dim3(W * 64), 0, static_cast<hipStream_t>(stream), a);
   };
   if (g->dtype == FH_BF16) {
     if (g->dh <= 64) launch.template operator()<bf16_t, 64>(); else launch.template operator()<bf16_t, 128>();
@@ -596,9 +634,13 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
   hipStream_t s = static_cast<hipStream_t>(stream);
   constexpr int W = 4;
   auto launch = [&]<typename T, int DH>() {
-    a.slots = static_cast<int>(slots_for(*g, a.group.d, 32 * W));
-    hipLaunchKernelGGL((attention_dq_kernel<T, DH, W>), dim3(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads)),
-                       dim3(W * 64), 0, s, a);
+    const int share = key_shares(*g, true);
+    a.slots = static_cast<int>(slots_for(*g, a.group.d, 32 * W / share));
+    const dim3 tiles(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads));
+    if (share == 2)
+      hipLaunchKernelGGL((attention_dq_kernel<T, DH, W, 2>), tiles, dim3(W * 64), 0, s, a);
+    else
+      hipLaunchKernelGGL((attention_dq_kernel<T, DH, W, 1>), tiles, dim3(W * 64), 0, s, a);
     if (fh_status st = launch_status("attention_dq_kernel launch"); st != FH_OK) return st;
     a.slots = static_cast<int>(slots_for(*g, 1, a.tile_keys));
     const dim3 grid(static_cast<uint32_t>(a.slots) * static_cast<uint32_t>(a.kv_heads) * static_cast<uint32_t>(a.parts));
@@ -607,7 +649,8 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
     }
     if (a.tile_keys == 128) hipLaunchKernelGGL((attention_dkv_kernel<T, DH, 4>), grid, dim3(512), 0, s, a);
     if (fh_status st = launch_status("attention_dkv_kernel launch"); st != FH_OK || a.parts == 1) return st;
-    hipLaunchKernelGGL((attention_dkv_join_kernel<T>), dim3(static_cast<uint32_t>((g->tokens + 3) / 4)), dim3(256), 0, s, a);
+    const int64_t slices = (2 * g->kv_heads * g->dh + 255) / 256;
+    hipLaunchKernelGGL((attention_dkv_join_kernel<T>), dim3(static_cast<uint32_t>((g->tokens * slices + 3) / 4)), dim3(256), 0, s, a);
     return launch_status("attention_dkv_join_kernel launch");
   };
   if (g->dtype == FH_BF16)

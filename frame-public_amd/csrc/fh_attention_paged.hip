@@ -118,8 +118,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
         s[t][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], c, -ms));
         l += s[t][x];
       }
-      p[2 * t] = operand2<T>(s[t][0], s[t][1]);
-      p[2 * t + 1] = operand2<T>(s[t][2], s[t][3]);
+      p[2 * t] = narrow2<T>(s[t][0], s[t][1]);
+      p[2 * t + 1] = narrow2<T>(s[t][2], s[t][3]);
     }
 #pragma unroll
     for (int dt = 0; dt < DH / 16; ++dt) mfma16x<T>(tiles.columns(BYTES, dt), p, o[dt]);
@@ -201,8 +201,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
         *reinterpret_cast<float4*>(a.part_out + part_row * a.dh + at) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
       } else {
         u32x2_t w;
-        w[0] = store2<T>(y.x * inv, y.y * inv);
-        w[1] = store2<T>(y.z * inv, y.w * inv);
+        w[0] = narrow2<T>(y.x * inv, y.y * inv);
+        w[1] = narrow2<T>(y.z * inv, y.w * inv);
         *reinterpret_cast<u32x2_t*>(a.out + trow * a.ldo + head * a.dh + at) = w;
       }
     }
@@ -278,8 +278,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const RowsArgs a) {
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (half == 0 && d < a.dh) {
     u32x2_t w;
-    w[0] = store2<T>(acc[0] * inv, acc[1] * inv);
-    w[1] = store2<T>(acc[2] * inv, acc[3] * inv);
+    w[0] = narrow2<T>(acc[0] * inv, acc[1] * inv);
+    w[1] = narrow2<T>(acc[2] * inv, acc[3] * inv);
     *reinterpret_cast<u32x2_t*>(a.out + token * a.ldo + (row - static_cast<int64_t>(token) * a.heads) * a.dh + d) = w;
   }
 }
@@ -287,6 +287,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const RowsArgs a) {
 // How a call is cut: the form, the tiles' slots, and the parts of the keys.
 struct Plan {
   bool by_keys;
+  int shares;  // chunks: waves that share 32 rows
   int64_t slots, splits, part_keys;
 };
 
@@ -296,12 +297,16 @@ Plan plan(const fh_paged_cache& c, int64_t tokens, int64_t heads, int64_t max_ne
   max_keys = std::min(max_keys, c.table_stride * c.page_size);
   Plan p{};
   p.by_keys = max_new * group <= 32;
-  const int64_t rows = p.by_keys ? 16 : 32 * kWaves;
-  p.slots = tokens * group / rows + c.batch;
+  // chunks with few tiles, as in the forward over packed rows: two waves share 32 rows
+  auto tiles_of = [&](int64_t rows) {
+    p.slots = tokens * group / rows + c.batch;
+    return std::max<int64_t>(1, c.kv_heads * std::min(p.slots, c.batch * ((max_new * group + rows - 1) / rows)));
+  };
+  p.shares = p.by_keys || tiles_of(32 * kWaves) >= 2 * cus ? 1 : 2;
+  const int64_t tiles = tiles_of(p.by_keys ? 16 : 32 * kWaves / p.shares);
   // Tiles that the expected lengths make, and enough parts for 6 (by keys) or 3 rounds of the workgroups that fit the chip, so that
   // sequences of different lengths even out; no part shorter than 8 blocks. (Two rounds by keys: the 64 sequences above 156 us
   // instead of 139, the longest parts start last.)
-  const int64_t tiles = std::max<int64_t>(1, c.kv_heads * std::min(p.slots, c.batch * ((max_new * group + rows - 1) / rows)));
   const int64_t want = ((p.by_keys ? 12 : 6) * cus + tiles - 1) / tiles;
   const int64_t least = p.by_keys ? 256 : 512;
   const int64_t parts = std::max<int64_t>(1, std::min({want, max_keys / least, int64_t{128}}));
@@ -386,10 +391,14 @@ extern "C" fh_status fh_attention_paged(const fh_paged_cache* c, const void* q, 
       hipLaunchKernelGGL((attention_keys_kernel<T, DH, kE4m3>), grid, dim3(kWaves * 64), 0, s, a);
     else if (p.by_keys)
       hipLaunchKernelGGL((attention_keys_kernel<T, DH, kPaged>), grid, dim3(kWaves * 64), 0, s, a);
+    else if (c->cache_dtype == FH_E4M3 && p.shares == 2)
+      hipLaunchKernelGGL((attention_rows_kernel<T, DH, kE4m3, kWaves, 2>), grid, dim3(kWaves * 64), 0, s, a);
     else if (c->cache_dtype == FH_E4M3)
-      hipLaunchKernelGGL((attention_rows_kernel<T, DH, kE4m3, kWaves>), grid, dim3(kWaves * 64), 0, s, a);
+      hipLaunchKernelGGL((attention_rows_kernel<T, DH, kE4m3, kWaves, 1>), grid, dim3(kWaves * 64), 0, s, a);
+    else if (p.shares == 2)
+      hipLaunchKernelGGL((attention_rows_kernel<T, DH, kPaged, kWaves, 2>), grid, dim3(kWaves * 64), 0, s, a);
     else
-      hipLaunchKernelGGL((attention_rows_kernel<T, DH, kPaged, kWaves>), grid, dim3(kWaves * 64), 0, s, a);
+      hipLaunchKernelGGL((attention_rows_kernel<T, DH, kPaged, kWaves, 1>), grid, dim3(kWaves * 64), 0, s, a);
     if (fh_status st = launch_status("fh_attention_paged launch"); st != FH_OK || a.splits == 1) return st;
     const int64_t rows = tokens * heads;
     if (a.splits > 8)

@@ -262,9 +262,26 @@ struct RowState {
         l += s[x];
       }
 #pragma unroll
-      for (int x = PER * i; x < PER * (i + 1); x += 2) p[x / 8][x % 8 / 2] = operand2<T>(s[x], s[x + 1]);
+      for (int x = PER * i; x < PER * (i + 1); x += 2) p[x / 8][x % 8 / 2] = narrow2<T>(s[x], s[x + 1]);
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
+  // the sums of the wave whose `share` is 1 go into the other's, through room[.. * 64]
+  __device__ __forceinline__ void join(float* room, int share) {
+    if (share == 1) {
+      room[0] = m;
+      room[64] = l;
+#pragma unroll
+      for (int i = 0; i < DH / 2; ++i) room[(2 + i) * 64] = o[i / 16][i % 16];
+    }
+    __syncthreads();
+    if (share == 1) return;
+    const float other = room[0], top = fmaxf(m, other), ref = top == -__builtin_inff() ? 0.0f : top;
+    const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(other - ref);
+    m = top;
+    l = l * f + room[64] * g;
+#pragma unroll
+    for (int i = 0; i < DH / 2; ++i) o[i / 16][i % 16] = o[i / 16][i % 16] * f + room[(2 + i) * 64] * g;
   }
   // rows without a visible key: zeros, lse -inf
   __device__ __forceinline__ void finish(float& inv, float& lse2) {
@@ -334,10 +351,11 @@ struct RowTile {
   }
 };
 
-template <typename T, int DH, int SRC, int W>
+// KSHARE 2: two waves share 32 rows, each taking one 32-key tile of every block; their sums are joined through LDS.
+template <typename T, int DH, int SRC, int W, int KSHARE>
 __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArgs a) {
   constexpr int BYTES = kBlock * DH * 2;  // one block of keys, or of values
-  constexpr int ROWS = 32 * W;
+  constexpr int ROWS = 32 * W / KSHARE;
   static_assert((ROWS & (ROWS - 1)) == 0, "rows per workgroup: a power of two");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
   __shared__ NotFinite<T, DH> bad;
@@ -354,7 +372,8 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   bool whole;
   if (!tile.part(a, static_cast<int>(blockIdx.z), kbegin, kend, whole)) return;
 
-  const int r0 = tile.tile0 + wave * 32, r = r0 + l32;
+  const int share = wave / (W / KSHARE);
+  const int r0 = tile.tile0 + wave % (W / KSHARE) * 32, r = r0 + l32;
   const bool live = r < tile.rows;
   const int lim = tile.limit(a, r);
   const int lim_low = tile.limit(a, r0), lim_high = tile.limit(a, r0 + 31);  // rows are in order of their tokens
@@ -397,14 +416,14 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
   __syncthreads();
   if (kbegin + kBlock < kend) stage.load(a, tile.table, kv_head, kbegin + kBlock, kend, tid);
   f32x16_t s0, s1;
-  row_product<T, DH>(tiles, 0, qf, s0);
+  row_product<T, DH>(tiles, 32 * share, qf, s0);
   int buf = 0;
   for (int kb = kbegin; kb < kend; kb += kBlock) {
     const bool more = kb + kBlock < kend, mine = kb <= lim_high;
     const bool edge = kb + kBlock - 1 > lim_low || there != ~uint64_t{0};
     const TileReader<DH> kt = tiles.at(buf * 2 * BYTES), vt = kt.at(BYTES);
     u32x4_t p[2], vf[DH / 32];
-    if (mine) {
+    if (KSHARE == 1 && mine) {
       if (edge) state.mask(s0, kb, lim, static_cast<uint32_t>(there), hi);
       const float ref = state.raise(s0, c);
       state.mixed(s0, c, ref, p, kt, 32, qf, s1, vt, 0, vf);
@@ -417,9 +436,17 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
       if constexpr (SRC != kDense) there_next = stage.there;
       if (kb + 2 * kBlock < kend) stage.load(a, tile.table, kv_head, kb + 2 * kBlock, kend, tid);
     }
-    if (mine) column_product<T, DH>(vt, 0, p, vf, state.o);
+    if (KSHARE == 1 && mine) column_product<T, DH>(vt, 0, p, vf, state.o);
     __syncthreads();  // the next block is in LDS
-    if (mine) {
+    if (KSHARE == 2) {
+      if (mine) {
+        if (edge) state.mask(s0, kb + 32 * share, lim, static_cast<uint32_t>(there >> (32 * share)), hi);
+        const float ref = state.raise(s0, c);
+        state.mixed(s0, c, ref, p, tiles.at((buf ^ 1) * 2 * BYTES), 32 * share, qf, s1, vt, 32 * share, vf);
+        column_product<T, DH>(vt, 32 * share, p, vf, state.o);
+        s0 = s1;
+      }
+    } else if (mine) {
       if (edge) state.mask(s1, kb + 32, lim, static_cast<uint32_t>(there >> 32), hi);
       const float ref = state.raise(s1, c);
       // (after the last block: scores of nothing, unused)
@@ -430,6 +457,11 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
     buf ^= 1;
   }
 
+  if constexpr (KSHARE == 2) {
+    __syncthreads();  // the last block is used
+    state.join(reinterpret_cast<float*>(lds) + wave % (W / 2) * ((DH / 2 + 2) * 64) + lane, share);
+    if (share == 1) return;
+  }
   float inv, lse2;
   state.finish(inv, lse2);
   if (!live) return;

@@ -231,6 +231,16 @@ struct NotFinite {
   }
 };
 
+// Two values rounded to nearest even in one instruction for either type, a NaN to a NaN. (store2 gives an f16 NaN one set of bits, by a branch
+// per value: the forward of 7 sequences of 0 .. 200 tokens in f16 took 11.5 us with it instead of 7.5.)
+template <typename T>
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef std::conditional_t<std::is_same_v<T, bf16_t>, __bf16, _Float16> t;
+  typedef t t2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{lo, hi}, t2));
+}
+
 // max(m, a, b) in one instruction: fmaxf on products' results would first canonicalise each of them
 __device__ __forceinline__ float max3(float m, float a, float b) {
   float r;
@@ -270,22 +280,12 @@ __device__ __forceinline__ void clear(f32x16_t& a) {
   for (int x = 0; x < 16; ++x) a[x] = 0.0f;
 }
 
-// Two values as an operand of a product, rounded to nearest even in one instruction for either type. (store2 gives an f16 NaN one set of
-// bits, by a branch per value: gradients of 1446 tokens, 20 heads of 64 in f16 took 147 us with it.)
-template <typename T>
-__device__ __forceinline__ uint32_t operand2(float lo, float hi) {
-  typedef float f2 __attribute__((ext_vector_type(2)));
-  typedef std::conditional_t<std::is_same_v<T, bf16_t>, __bf16, _Float16> t;
-  typedef t t2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{lo, hi}, t2));
-}
-
 // Slice hf (16 of its rows) of a 32x32 result rounded to T, as the operand of the next product.
 template <typename T>
 __device__ __forceinline__ u32x4_t pack_slice(const f32x16_t& p, int hf) {
   u32x4_t w;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = operand2<T>(p[8 * hf + 2 * j], p[8 * hf + 2 * j + 1]);
+  for (int j = 0; j < 4; ++j) w[j] = narrow2<T>(p[8 * hf + 2 * j], p[8 * hf + 2 * j + 1]);
   return w;
 }
 
@@ -353,8 +353,8 @@ __device__ __forceinline__ void store_row(uint16_t* row, const f32x16_t (&acc)[D
       const int d = 32 * dt + 8 * q + 4 * hi;
       if (d < dh) {
         u32x2_t w;
-        w[0] = store2<T>(acc[dt][4 * q] * scale, acc[dt][4 * q + 1] * scale);
-        w[1] = store2<T>(acc[dt][4 * q + 2] * scale, acc[dt][4 * q + 3] * scale);
+        w[0] = narrow2<T>(acc[dt][4 * q] * scale, acc[dt][4 * q + 1] * scale);
+        w[1] = narrow2<T>(acc[dt][4 * q + 2] * scale, acc[dt][4 * q + 3] * scale);
         *reinterpret_cast<u32x2_t*>(row + d) = w;
       }
     }

@@ -247,14 +247,41 @@ INF = {F16: 0x7c00, BF16: 0x7f80}
 @pytest.mark.parametrize("dtype,heads,kv_heads,dh", [(BF16, 4, 2, 64), (F16, 2, 2, 128), (BF16, 3, 1, 40)])
 @pytest.mark.parametrize("t", [0, 5, 64, 130, 298])
 def test_packed_not_finite_values_reach_the_rows_that_see_them(hip, dtype, heads, kv_heads, dh, t):
+    check_not_finite(hip, dtype, heads, kv_heads, dh, t, [70, 300])
+
+
+# batches of more tiles than CUs, which the kernels cut otherwise than small ones
+MANY = [70, 300, 0, 1, 129] + [17, 64, 100, 95] * 15
+
+
+@pytest.mark.parametrize("t", [5, 130])
+@pytest.mark.parametrize("dtype,heads,kv_heads,dh", [(BF16, 16, 16, 64), (BF16, 32, 8, 128)])
+def test_packed_not_finite_values_among_many_sequences(hip, dtype, heads, kv_heads, dh, t):
+    check_not_finite(hip, dtype, heads, kv_heads, dh, t, MANY)
+
+
+@pytest.mark.parametrize("case", [(BF16, MANY, 16, 16, 64, 1, 0, 5, True), (F16, MANY, 32, 8, 128, 1, 3, 0, False),
+                                  (BF16, MANY, 16, 16, 80, 0, 0, 0, False), (F16, MANY, 28, 14, 40, 1, 0, 2, True)], ids=packed_id)
+def test_packed_many_sequences(hip, case):
+    say(f"packed, many sequences {case}")
+    p = Packed(hip, *case)
+    p.check_forward(*p.forward(), "many")
+    got = p.backward(*p.stored_forward())
+    want, tol = p.want_grads()
+    for name, a, w, t in zip("qkv", got, want, tol):
+        assert (a[~p.inside] == KEEP).all()
+        ref.check(ref.values(a, p.dtype)[p.inside], w[p.inside], t[p.inside], f"d{name}")
+
+
+def check_not_finite(hip, dtype, heads, kv_heads, dh, t, lens):
     # token t of the second sequence holds values that are not finite, one tensor at a time: rows that do not see it keep every bit
     say(f"packed NaN at token {t}, {heads} heads over {kv_heads} of {dh}")
-    p = Packed(hip, dtype, [70, 300], heads, kv_heads, dh, 1)
+    p = Packed(hip, dtype, lens, heads, kv_heads, dh, 1)
     group, at = heads // kv_heads, int(p.cu[1]) + t
     clean_out, clean_lse = p.forward()
     clean = p.backward(clean_out, clean_lse)
     later = np.zeros(p.rows, bool)
-    later[at:] = True
+    later[at:p.cu[2]] = True
     mine = np.arange(heads * dh) // dh < group  # the heads of key head 0
     value = lambda a: ref.values(a, dtype)
 
@@ -282,12 +309,13 @@ def test_packed_not_finite_values_reach_the_rows_that_see_them(hip, dtype, heads
     p.x["v"][at, 3], p.x["v"][at + 1, 3] = INF[dtype], INF[dtype] | 0x8000
     out, _ = p.forward()
     p.x["v"] = kept
-    assert np.isposinf(value(out[at:at + 1, 3])).all() and np.isnan(value(out[at + 1:, 3])).all() and np.array_equal(out[:at], clean_out[:at])
+    assert np.isposinf(value(out[at:at + 1, 3])).all() and np.isnan(value(out[at + 1:p.cu[2], 3])).all()
+    assert np.array_equal(out[:at], clean_out[:at]) and np.array_equal(out[p.cu[2]:], clean_out[p.cu[2]:])
     # a key: all of its rows' scores
     out, lse, grads = with_bad("k", at, 3, NAN[dtype])
     check(out, clean_out, later[:, None] & mine, np.isnan, "out of k")
     check(grads[0], clean[0], later[:, None] & mine, np.isnan, "dq of k")
-    assert np.isnan(lse[at:, :group]).all() and np.array_equal(lse[:at], clean_lse[:at])
+    assert np.isnan(lse[at:p.cu[2], :group]).all() and np.array_equal(lse[:at], clean_lse[:at])
     # a row of q: itself, and the keys that it sees
     shared = np.arange(kv_heads * dh) < dh
     seen = np.zeros(p.rows, bool)
@@ -529,6 +557,17 @@ def test_paged_rows_that_see_nothing(hip):
             out, _ = p.attend(max_keys=keys)
             p.check_attend(out, "empty rows")
             assert (out[p.cu[1]:p.cu[1] + 3] == 0).all() and (out[p.cu[2]:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,cache_dtype,dh", [(BF16, BF16, 128), (F16, E4M3, 64)])
+def test_paged_many_chunks(hip, dtype, cache_dtype, dh):
+    # more tiles than CUs
+    say(f"paged, many chunks, dh {dh}, cache {cache_dtype}")
+    p = Paged(hip, dtype, cache_dtype, [0, 100, 33, 7] * 15, [40, 33, 20, 70] * 15, 32, 8, dh, 16)
+    p.fill_past()
+    p.put_new()
+    p.upload()
+    p.check_attend(p.attend()[0], "many chunks")
 
 
 @pytest.mark.parametrize("number", [-1, 1 << 30])
