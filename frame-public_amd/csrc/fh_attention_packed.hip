@@ -9,8 +9,8 @@
 //   attention_dq_kernel:  32 rows per wave as in the forward; D is formed from its rows and kept for the second kernel.
 //   attention_dkv_kernel: 32 keys per wave, keys and values in registers, blocks of 64 rows of q and dout in LDS.
 // p and ds are rounded to the storage type as operands of the second products; everything else is fp32.
-// Measured: 2897 + 1034 + 165 tokens, 32 heads over 8, 128 dims, causal, bf16: 430 us (traced: dq 172, dk and dv 280, the
-// parts' sum 12), 452 TFLOP/s counted as 5 products, 633 as the 7 that are made; 3300 tokens in 8 sequences, 16 heads of 64: 48.5 us.
+// Measured: 2897 + 1034 + 165 tokens, 32 heads over 8, 128 dims, causal, bf16: 430 us (traced: dq 171, dk and dv 278, the
+// parts' sum 13), 452 TFLOP/s counted as 5 products, 633 as the 7 that are made; 3300 tokens in 8 sequences, 16 heads of 64: 48.5 us.
 // Bound by the waits of a tile's dependent steps (product, exponentials, product), which two waves per SIMD do not fill.
 #include <hip/hip_runtime.h>
 
@@ -259,8 +259,8 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv
   static_assert(kGradRows % PASS == 0, "whole passes");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * BYTES];
   __shared__ __attribute__((aligned(16))) float stats[2][2][kGradRows];  // per buffer: lse (base 2), D
-  // Rows with values that are not finite, of those that scrub() zeroes: the last of q per 8 columns (its scores are not finite), the last in
-  // each column of dout (dv's; its D is not finite, which reaches dk by itself), and whether there is any.
+  // Rows with values that are not finite, of those that scrub() zeroes: the last of q per 8 columns (its scores are not finite), the
+  // last in each column of dout (dv's; its D is not finite, which reaches dk by itself), and whether there is any.
   __shared__ int last_q[DH / 8], last_dout[DH], any_bad;
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
@@ -429,14 +429,16 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv
     }
 }
 
-// dk and dv of the key tiles whose rows were cut into parts: the parts' sum, in their order. A wave takes 256 of a token's values, so
-// that what counts, the parts' loads, are 8 deep.
+// dk and dv of the key tiles whose rows were cut into parts: the parts' sum, in their order. A wave takes 512 of a token's
+// values, two chains of loads a lane: with one, two parts of 4096 tokens, 8 heads of 128 take 2.5 us longer, with four, eight parts of
+// 1900 tokens, a head of 64, 2.7.
+constexpr int kJoin = 2;
+
 template <typename T>
 __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const GradArgs a) {
-  const int width = a.kv_heads * a.dh, slices = (2 * width + 255) / 256;
+  const int width = a.kv_heads * a.dh, slices = (2 * width + kJoin * 256 - 1) / (kJoin * 256);
   const int64_t work = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int token = static_cast<int>(work / slices), i = (static_cast<int>(work - static_cast<int64_t>(token) * slices) * 64 +
-                                                         static_cast<int>(threadIdx.x & 63)) * 4;
+  const int token = static_cast<int>(work / slices), slice = static_cast<int>(work - static_cast<int64_t>(token) * slices);
   if (token >= a.tokens) return;
   const int b = sequence_of(a.cu, a.batch, token);
   if (b < 0) return;
@@ -447,24 +449,38 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const GradArgs 
   const int parts = row_range(a, tile0, rows, 0).parts;
   if (parts == 1) return;
   const int64_t stride = static_cast<int64_t>(a.tokens) * width;
-  if (i < 2 * width) {
-    const int which = i >= width;  // 0: dv, 1: dk
-    const int d = i - which * width;
-    const float* p = a.part + which * stride + static_cast<int64_t>(token) * width + d;
-    float4 t = *reinterpret_cast<const float4*>(p);
-#pragma unroll 8
-    for (int z = 1; z < parts; ++z) {
-      const float4 y = *reinterpret_cast<const float4*>(p + z * 2 * stride);
-      t.x += y.x;
-      t.y += y.y;
-      t.z += y.z;
-      t.w += y.w;
+  float4 t[kJoin];
+  const float* p[kJoin];
+  int at[kJoin];
+  bool there[kJoin], for_dk[kJoin];
+#pragma unroll
+  for (int j = 0; j < kJoin; ++j) {
+    const int i = ((slice * kJoin + j) * 64 + static_cast<int>(threadIdx.x & 63)) * 4;  // dv's values, then dk's
+    there[j] = i < 2 * width;
+    for_dk[j] = i >= width;
+    at[j] = there[j] ? i - for_dk[j] * width : 0;
+    p[j] = a.part + (there[j] && for_dk[j] ? stride : 0) + static_cast<int64_t>(token) * width + at[j];
+    t[j] = *reinterpret_cast<const float4*>(p[j]);
+  }
+#pragma unroll 2
+  for (int z = 1; z < parts; ++z) {
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j) {
+      const float4 y = *reinterpret_cast<const float4*>(p[j] + z * 2 * stride);
+      t[j].x += y.x;
+      t[j].y += y.y;
+      t[j].z += y.z;
+      t[j].w += y.w;
     }
+  }
+#pragma unroll
+  for (int j = 0; j < kJoin; ++j) {
+    if (!there[j]) continue;
     u32x2_t w;
-    w[0] = narrow2<T>(t.x, t.y);
-    w[1] = narrow2<T>(t.z, t.w);
-    uint16_t* out = which ? a.dk + token * a.ldk : a.dv + token * a.ldv;
-    *reinterpret_cast<u32x2_t*>(out + d) = w;
+    w[0] = narrow2<T>(t[j].x, t[j].y);
+    w[1] = narrow2<T>(t[j].z, t[j].w);
+    uint16_t* out = for_dk[j] ? a.dk + token * a.ldk : a.dv + token * a.ldv;
+    *reinterpret_cast<u32x2_t*>(out + at[j]) = w;
   }
 }
 
@@ -503,24 +519,24 @@ int64_t slots_for(const fh_packed_attention& g, int64_t per_token, int64_t tile)
 
 int64_t delta_bytes(const fh_packed_attention& g) { return (g.tokens * g.heads * 4 + 15) / 16 * 16; }
 
-// Two waves share 32 rows where tiles of 128 rows leave CUs with fewer waves than hide the steps of a block: fewer than two workgroups a CU in
-// the forward (12 sequences of up to 1886 tokens, 4 heads over 2 of 64: 22.7 us instead of 34; one of 4000, 8 heads over 1 of 128: 74
-// instead of 95; 480 workgroups: 57 either way), one and a half for dq (8 heads of 128 over 2000 tokens 139 instead of 164 in all; 416
-// workgroups: 50.3 instead of 48.5, 1048: 485 instead of 430).
+// Two waves share 32 rows where tiles of 128 rows leave CUs with fewer waves than hide the steps of a block: fewer than two
+// workgroups a CU in the forward (12 sequences of up to 1886 tokens, 4 heads over 2 of 64: 22.7 us instead of 34; one of 4000, 8 heads
+// over 1 of 128: 74 instead of 95; 480 workgroups: 57 either way), one and a half for dq (8 heads of 128 over 2000 tokens: 139 instead
+// of 164 in all; 416 workgroups: 50.3 instead of 48.5; 1048: 485 instead of 430).
 int key_shares(const fh_packed_attention& g, bool gradients) {
   const int64_t tiles = (g.tokens * (g.heads / g.kv_heads) + 127) / 128 * g.kv_heads, cus = device_cu_count();
   return tiles < (gradients ? cus + cus / 2 : 2 * cus) ? 2 : 1;
 }
 
-// dk, dv. Keys per workgroup: 128, or 64 where that leaves fewer than two workgroups a CU and the head dim's registers allow the longer
-// staging.
+// dk, dv. Keys per workgroup: 128, or 64 where that leaves fewer than two workgroups a CU and the head dim's registers allow the
+// longer staging (3300 tokens in 8 sequences, 16 heads of 64: 48 us in all instead of 57).
 int64_t grad_keys(const fh_packed_attention& g) {
   return g.dh <= 64 && (g.tokens + 127) / 128 * g.kv_heads < 2 * device_cu_count() ? 64 : 128;
 }
 // A key tile's rows are cut into parts where the tiles are few: a causal sequence's first keys are seen by all of its rows, so the
-// longest tile would otherwise outlast the others by twice their mean. As many as fill the chip once (three workgroups of 64 keys a CU, or one
-// of 128), and at least enough to even the tiles out. 32 heads over 8 of 64, 2800 tokens: 3 parts 137 us in all, 2 161; 8 heads over 1, 1900
-// tokens: 8 parts 102, 4 143; 8 heads over 2 of 128, 2000 tokens: 8 parts 138, 16 178 (a second round).
+// longest tile would otherwise outlast the others by twice their mean. As many as fill the chip once (three workgroups of 64 keys a CU,
+// or one of 128), and at least enough to even the tiles out. 32 heads over 8 of 64, 2800 tokens: 3 parts 137 us in all, 2 161; 8 heads
+// over 1 of 64, 1900 tokens: 8 parts 102, 4 143; 8 heads over 2 of 128, 2000 tokens: 8 parts 138, 16 178 (a second round).
 int64_t grad_parts(const fh_packed_attention& g) {
   const int64_t keys = grad_keys(g), tiles = (g.tokens + keys - 1) / keys * g.kv_heads, cus = device_cu_count();
   // rows of a sequence four times the mean length: the lengths themselves are on the device
@@ -649,7 +665,7 @@ extern "C" fh_status fh_attention_packed_grad(const fh_packed_attention* g, cons
     }
     if (a.tile_keys == 128) hipLaunchKernelGGL((attention_dkv_kernel<T, DH, 4>), grid, dim3(512), 0, s, a);
     if (fh_status st = launch_status("attention_dkv_kernel launch"); st != FH_OK || a.parts == 1) return st;
-    const int64_t slices = (2 * g->kv_heads * g->dh + 255) / 256;
+    const int64_t slices = (2 * g->kv_heads * g->dh + kJoin * 256 - 1) / (kJoin * 256);
     hipLaunchKernelGGL((attention_dkv_join_kernel<T>), dim3(static_cast<uint32_t>((g->tokens * slices + 3) / 4)), dim3(256), 0, s, a);
     return launch_status("attention_dkv_join_kernel launch");
   };

@@ -10,7 +10,7 @@
 // 2318 + 871 tokens, 32 heads over 8, 128 dims, causal, bf16: 300 us, 850 TFLOP/s of visible pairs (a library product of 8192^3: 1,249);
 // products and exponentials in separate stretches 310 us; a wait for the next block at the loop's start 318; 256 rows per
 // workgroup 302; raised wave priority around the products 312-320. Eight sequences of 512, 16 heads of 64: 16.9 us, launch and the
-// latencies of a workgroup's up to eight dependent blocks.
+// latencies of a workgroup's up to eight dependent blocks. Where tiles are few, two waves share 32 rows and split each block's keys.
 // The accumulators are scaled again only when a row's maximum grows by more than 8 (base 2) over the one in use: sums and
 // probabilities then stay within 2^8 of their usual range, which fp32 and the rounding to 16 bits do not notice.
 // Masked scores are -inf by selection, never by addition, and rows of keys that are not there are zeros in LDS, so nothing that

@@ -231,8 +231,8 @@ struct NotFinite {
   }
 };
 
-// Two values rounded to nearest even in one instruction for either type, a NaN to a NaN. (store2 gives an f16 NaN one set of bits, by a branch
-// per value: the forward of 7 sequences of 0 .. 200 tokens in f16 took 11.5 us with it instead of 7.5.)
+// Two values rounded to nearest even in one instruction for either type, a NaN to a NaN. (store2 gives an f16 NaN one set of bits, by
+// a branch per value: the forward of 7 sequences of 0 .. 200 tokens in f16 took 11.5 us with it instead of 7.5.)
 template <typename T>
 __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
   typedef float f2 __attribute__((ext_vector_type(2)));

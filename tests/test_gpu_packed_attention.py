@@ -496,8 +496,8 @@ class Paged:
             slots = [self.slot(b, p) for p in range(max(total, 0))]
             there = np.array([s is not None for s in slots], bool)
             empty = np.zeros((self.kv_heads, self.dh))
-            keys = np.stack([self.row(self.kc, self.ks, s) if s else empty for s in slots]) if slots else np.zeros((0, self.kv_heads, self.dh))
-            vals = np.stack([self.row(self.vc, self.vs, s) if s else empty for s in slots]) if slots else np.zeros((0, self.kv_heads, self.dh))
+            keys, vals = (np.array([self.row(c, scales, s) if s else empty for s in slots]).reshape(-1, self.kv_heads, self.dh)
+                          for c, scales in ((self.kc, self.ks), (self.vc, self.vs)))
             seen = (np.arange(total)[None, :] <= total - n + np.arange(n)[:, None]) & there[None, :]
             rows = slice(self.cu[b], self.cu[b + 1])
             for h in range(self.heads if n else 0):
