@@ -241,12 +241,9 @@ __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{lo, hi}, t2));
 }
 
-// max(m, a, b) in one instruction: fmaxf on products' results would first canonicalise each of them
-__device__ __forceinline__ float max3(float m, float a, float b) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(m), "v"(a), "v"(b));
-  return r;
-}
+// max(m, a, b), one v_max3_f32; a NaN counts for nothing. (Not as inline assembly: a, b are products' results, and the compiler keeps the
+// wait states that the matrix unit needs before they are read only for instructions that it knows.)
+__device__ __forceinline__ float max3(float m, float a, float b) { return fmaxf(fmaxf(m, a), b); }
 
 // max / sum of a lane's value and the other half's (same row of a 32x32 result, the other 16 of its values)
 __device__ __forceinline__ void both_halves(float v, float& low, float& high) {
