@@ -522,12 +522,14 @@ __global__ __launch_bounds__(512, 1) void attention_split_kernel(const uint16_t*
     // ---- output: half h writes d tile h from its partial and its partner's (kv is free: every V read is done) ----
     float* xo = reinterpret_cast<float*>(kv);
     {
-      const int other = 1 - half;
+      // a choice between two results, not acc_o[1 - half]: the compiler keeps no wait states between a product and a register that an
+      // index chooses, and values were read before they were written (4 states behind the product: columns 0 and 4 wrong)
+      const f32x16_t give = half == 0 ? acc_o[1] : acc_o[0];
       float4* dst = reinterpret_cast<float4*>(xo + (wave * 64 + lane) * 16);
       barrier();  // every wave's V reads are complete before kv is overwritten
   #pragma unroll
       for (int x4 = 0; x4 < 4; ++x4)
-        dst[x4] = make_float4(acc_o[other][4 * x4], acc_o[other][4 * x4 + 1], acc_o[other][4 * x4 + 2], acc_o[other][4 * x4 + 3]);
+        dst[x4] = make_float4(give[4 * x4], give[4 * x4 + 1], give[4 * x4 + 2], give[4 * x4 + 3]);
     }
     barrier();
     const float4* src = reinterpret_cast<const float4*>(xo + ((wave ^ 4) * 64 + lane) * 16);

@@ -3,7 +3,7 @@
 A vector or memory instruction that reads the result of a v_mfma must stand a number of wait states behind it; the hardware does
 not hold it back. The compiler keeps the distance for every instruction that it knows, but it does not look into inline assembly. So the
 built code objects are looked through: from each product along every path (branches taken and not), an instruction counts one state and
-s_nop n counts n + 1.
+s_nop n counts n + 1. Nor does it look into reads of a register that an index chooses at run time (s_set_gpr_idx_on): those may be of any.
 """
 from __future__ import annotations
 
@@ -29,7 +29,7 @@ def registers(text):
 def functions(library, folder):
     """(name, [(address, instruction, branch target or None)]) of every function with a matrix product."""
     link = os.path.join(folder, "lib.so")  # the code objects are written beside the file that they come from
-    os.symlink(library, link)
+    os.symlink(os.path.abspath(library), link)
     subprocess.run([OBJDUMP, "--offloading", link], check=True, stdout=subprocess.DEVNULL)
     for path in sorted(glob.glob(link + ".*gfx950")):
         text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", path], check=True, stdout=subprocess.PIPE, text=True).stdout
@@ -50,7 +50,7 @@ def functions(library, folder):
             yield head.group(1), code
 
 
-def early_reads(code):
+def early_reads(code, by_index_only=False):
     """(product, reading instruction, states between them, states needed) of a function's code."""
     place = {at: i for i, (at, _, _) in enumerate(code)}
     found = set()
@@ -59,25 +59,27 @@ def early_reads(code):
             continue
         name, args = product.split(None, 1)
         need = STATES[name[len("v_mfma_f32_"):]]
-        paths, seen = [(i + 1, 0, frozenset(registers(args.split(",")[0])))], {}
+        paths, seen = [(i + 1, 0, frozenset(registers(args.split(",")[0])), False)], {}
         while paths:
-            j, states, live = paths.pop()
-            if j >= len(code) or states >= need or not live or seen.get((j, live), need) <= states:
+            j, states, live, indexed = paths.pop()
+            if j >= len(code) or states >= need or not live or seen.get((j, live, indexed), need) <= states:
                 continue
-            seen[j, live] = states
+            seen[j, live, indexed] = states
             _, op, to = code[j]
             name, _, args = op.partition(" ")
+            if name.startswith("s_set_gpr_idx"):
+                indexed = name == "s_set_gpr_idx_on"
             if READS.match(name) and not name.startswith("v_mfma"):
                 written, _, read = args.partition(",") if name.startswith("v_") else ("", "", args)
-                if registers(read) & live:
+                if indexed or not by_index_only and registers(read) & live:
                     found.add((product, op, states, need))
             if name.startswith("v_"):
                 live = live - registers(args.partition(",")[0])
             if name == "s_endpgm":
                 continue
             if to is not None:
-                paths.append((place[to], states + 1, live))
+                paths.append((place[to], states + 1, live, indexed))
                 if name == "s_branch":
                     continue
-            paths.append((j + 1, states + (int(args, 0) + 1 if name == "s_nop" else 1), live))
+            paths.append((j + 1, states + (int(args, 0) + 1 if name == "s_nop" else 1), live, indexed))
     return sorted(found)
