@@ -165,11 +165,11 @@ __global__ __launch_bounds__(W * 64, 2) void attention_kernel(const uint16_t* __
             for (int j = 0; j < 8; ++j) {
               const uint32_t sr = pack2<T>(acc[t][2 * j], acc[t][2 * j + 1]);  // round(S), two keys
               if constexpr (POW2) {
-                // max(mraw, a, b) in one instruction: fmaxf on the raw MFMA results would first canonicalise
-                // each of them (the compiler cannot prove an MFMA result is not a signalling NaN; it never is)
-                float mx;
-                asm("v_max3_f32 %0, %1, %2, %3" : "=v"(mx) : "v"(mraw), "v"(acc[t][2 * j]), "v"(acc[t][2 * j + 1]));
-                mraw = mx;
+                // one v_max3_f32. (Not as inline assembly: the compiler keeps the wait states that the matrix unit needs before its
+                // results are read only for instructions that it knows.) Taken here, before the products' registers go on: gathered at
+                // the end, f16 with 512 keys spills 696 bytes.
+                mraw = fmaxf(fmaxf(mraw, acc[t][2 * j]), acc[t][2 * j + 1]);
+                asm volatile("" : "+v"(mraw));
                 s2[2 * blk + t][j] = sr;
               } else {
                 const float a0 = lo16<T>(sr) * scale, a1 = hi16<T>(sr) * scale;
@@ -401,9 +401,8 @@ __global__ __launch_bounds__(512, 1) void attention_split_kernel(const uint16_t*
               for (int j = 0; j < 8; ++j) {
                 const uint32_t sr = pack2<T>(acc[2 * j], acc[2 * j + 1]);
                 if constexpr (POW2) {
-                  float mx;
-                  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(mx) : "v"(mraw), "v"(acc[2 * j]), "v"(acc[2 * j + 1]));
-                  mraw = mx;
+                  mraw = fmaxf(fmaxf(mraw, acc[2 * j]), acc[2 * j + 1]);
+                  asm volatile("" : "+v"(mraw));
                   s2[2 * i + t][j] = sr;
                 } else {
                   const float a0 = lo16<T>(sr) * scale, a1 = hi16<T>(sr) * scale;

@@ -1,14 +1,10 @@
 """No built kernel reads a matrix product's result too early (tests/mfma_waits.py)."""
 import os
-import re
 
 import pytest
 
 import mfma_waits as waits
 from frame_hip import abi
-
-# attention over packed sequences and over a paged cache
-KERNELS = re.compile(r"attention_(rows|keys|dq|dkv)_kernel")
 
 
 @pytest.fixture(scope="module")
@@ -19,12 +15,8 @@ def kernels(tmp_path_factory):
 
 
 def test_results_of_products_are_read_when_written(kernels):
-    early = {}
-    looked = [name for name in kernels if KERNELS.search(name)]
-    for name in looked:
-        if found := waits.early_reads(kernels[name]):
-            early[name] = found[:2]
-    assert len(looked) >= 32
+    early = {name: found[:2] for name, code in kernels.items() if (found := waits.early_reads(code))}
+    assert len(kernels) >= 100
     assert not early, early
 
 
