@@ -138,9 +138,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
         stages[i].store(mine, mine + BYTES, lane);
         if (uneven && at + BK - 1 > lim_low)
           stages[i].scrub_values(mine + BYTES, lane, [&](int row, int d, uint32_t bits) { bad.note(at + row, d, bits); });
+        hand_over();
         const uint64_t there = stages[i].there;
         if (at + STEP < kend) stages[i].template load<STEP>(a, tile.table, kv_head, at + STEP, kend, lane);
         use(at, there);
+        hand_over();
       }
     }
   }

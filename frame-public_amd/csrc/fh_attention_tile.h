@@ -332,6 +332,14 @@ __device__ __forceinline__ constexpr int result_row(int x, int hi) { return 8 * 
 // first iteration from the others, waits inside the loop for all loads in flight wherever it uses a value loaded before the loop.
 __device__ __forceinline__ void settle() { wait_vmcnt<0>(); }
 
+// LDS changes hands between the lanes of one wave: what they wrote before is there for the reads behind it, and what they read is read
+// before the writes behind it. The wave's LDS accesses run in their order, so this costs no instruction; it keeps the compiler, which
+// looks at one lane at a time, from moving them across.
+__device__ __forceinline__ void hand_over() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // A 16-byte chunk of 8 values at p when `there`, else zeros.
 __device__ __forceinline__ u32x4_t load_chunk(const uint16_t* p, bool there) {
   u32x4_t v{0, 0, 0, 0};
