@@ -8,7 +8,8 @@
 // order: results do not depend on scheduling, and no fp32 copy of dq is needed.
 //   attention_dq_kernel:  32 rows per wave as in the forward; D is formed from its rows and kept for the second kernel.
 //   attention_dkv_kernel: 32 keys per wave, keys and values in registers, blocks of 64 rows of q and dout in LDS.
-// p and ds are rounded to the storage type as operands of the second products; everything else is fp32.
+// p and ds are rounded to the storage type as operands of the second products, in f16 times a power of two that keeps them in its range
+// (OperandRange); everything else is fp32.
 // Measured: 2897 + 1034 + 165 tokens, 32 heads over 8, 128 dims, causal, bf16: 430 us (traced: dq 171, dk and dv 278, the
 // parts' sum 13), 452 TFLOP/s counted as 5 products, 633 as the 7 that are made; 3300 tokens in 8 sequences, 16 heads of 64: 48.5 us.
 // Bound by the waits of a tile's dependent steps (product, exponentials, product), which two waves per SIMD do not fill.
@@ -111,6 +112,8 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
 #pragma unroll
   for (int dt = 0; dt < DH / 32; ++dt) clear(acc[dt]);
 
+  OperandRange<T> range;
+
   // keys and values as the forward stages them
   RowsArgs kv{};
   kv.k = a.k;
@@ -187,6 +190,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
 #pragma unroll
           for (int x = 0; x < 16; ++x) s[x] = kb + 32 * t + result_row(x, hi) <= lim ? s[x] : 0.0f;
         }
+        range.fit(s, acc);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const u32x4_t ds = pack_slice<T>(s, hf);
@@ -203,6 +207,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_dq_kernel(const GradArgs 
     __syncthreads();
     buf ^= 1;
   }
+  range.undo(acc);
   if (uneven) {
     int first = first_bad[0];
 #pragma unroll
@@ -331,6 +336,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv
   f32x16_t acc[DH / 32];
 #pragma unroll
   for (int dt = 0; dt < DH / 32; ++dt) clear(acc[dt]);
+  OperandRange<T> operands;
   const float c = a.scale * kLog2e;
   const TileReader<DH> tiles(lds, lane);
   // blocks of rows that some keys of the tile are not seen by
@@ -388,6 +394,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[x] = r0 + result_row(x, hi) >= my_first ? s[x] : 0.0f;
       }
+      operands.fit(s, acc);
       u32x4_t columns[DH / 32], p[2];
       read_columns<DH>(operand, 32 * t, columns);
 #pragma unroll
@@ -401,6 +408,7 @@ __global__ __launch_bounds__(PAIRS * 128, PAIRS == 2 ? 3 : 2) void attention_dkv
     __syncthreads();
     buf ^= 1;
   }
+  operands.undo(acc);
   if (!live) return;
   if (range.begin < range.end && a.causal && any_bad != 0) {
     int last = last_q[0];

@@ -334,7 +334,7 @@ fh_status fh_attention_grad(int32_t dtype, const void* q, const void* k, const v
  * No counterpart in the reference, whose attention has one length, no mask and as many key heads as heads
  * (src/nn/layers.cpp:1014-1080); unlike fh_attention_fwd these round no intermediate as a graph of single ops would: scores,
  * softmax and sums are fp32, and only the probabilities (and in the gradients their derivatives) are rounded to the storage type,
- * as operands of the second product. A workspace, here and below, serves one call at a time. */
+ * as operands of the second product (in f16 gradients times a power of two, so that small and large ones keep their bits). A workspace, here and below, serves one call at a time. */
 typedef struct fh_packed_attention {
   int32_t dtype;
   int32_t causal; /* 1: row t of a sequence sees its rows 0 .. t; 0: all of them */

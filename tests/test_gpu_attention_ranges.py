@@ -1,10 +1,11 @@
-"""Attention where its numbers reach far: scores that rise and fall from block to block, against float64 (tests/attention_ref.py, which
-derives the bounds)."""
+"""Attention where its numbers reach far: scores that rise and fall from block to block, derivatives that f16 cannot hold as they are.
+Against float64 (tests/attention_ref.py, which derives the bounds)."""
 import numpy as np
 import pytest
 
+import attention_ref as ref
 from frame_hip import synth
-from test_gpu_packed_attention import BF16, E4M3, F16, Paged, say
+from test_gpu_packed_attention import BF16, E4M3, F16, Packed, Paged, say
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +36,62 @@ def test_paged_scores_that_move_between_blocks(hip, dtype, cache_dtype, dh, shap
         p.upload()
         for keys in (64, None, 1 << 20):
             p.check_attend(p.attend(max_keys=keys)[0], f"{shape}, cut for {keys}")
+
+
+# dtype, tokens, heads, key heads, dims, size of dout, of v, causal
+SPANS = [
+    (F16, [3000], 2, 1, 64, 2.0 ** -12, 1.0, 1),    # ds about 2^-25: nothing of it is a normal f16 value, most is below the smallest one
+    (F16, [1500, 700], 4, 2, 128, 2.0 ** -12, 1.0, 1),
+    (F16, [2100], 1, 1, 64, 1.0, 2.0 ** -14, 0),
+    (F16, [513, 1500], 3, 3, 80, 2.0 ** -9, 2.0 ** -6, 0),
+    (F16, [1000, 900], 2, 1, 64, 2.0 ** 8, 2.0 ** 7, 1),    # first rows: ds up to 2^18, past the largest f16 value, gradients too
+    (F16, [600, 40, 1], 2, 2, 128, 2.0 ** 8, 1.0, 1),
+    (F16, [400, 64] * 30, 8, 4, 64, 2.0 ** -12, 1.0, 1),    # more tiles than CUs
+    (F16, [400, 64] * 30, 32, 8, 128, 2.0 ** -12, 1.0, 1),
+    (BF16, [1500], 2, 1, 64, 2.0 ** -30, 1.0, 1),
+    (BF16, [700], 2, 1, 128, 2.0 ** 30, 2.0 ** 10, 0),
+]
+
+
+def spans_id(c):
+    return f"{'f16' if c[0] == F16 else 'bf16'}-{len(c[1])}x{max(c[1])}-h{c[2]}k{c[3]}d{c[4]}-dout{c[5]:.0e}-v{c[6]:.0e}{'c' if c[7] else ''}"
+
+
+@pytest.mark.parametrize("case", SPANS, ids=spans_id)
+def test_packed_gradients_hold_small_and_large_derivatives(hip, case):
+    # A derivative keeps its bits whatever its size: each is off by half a step of its own (ref.U), plus for f16 2^-34 of the largest one
+    # that it is summed with (a power of two takes the largest to 2^10 or more, and 2^-25 there is the least step's half: 2^-35, twice).
+    dtype, lens, heads, kv_heads, dh, dout, v, causal = case
+    say(f"packed gradients, dout {dout:g}, v {v:g}: {case}")
+    p = Packed(hip, dtype, lens, heads, kv_heads, dh, causal)
+    for name, size in (("dout", dout), ("v", v)):
+        p.x[name] = synth.to_storage((synth.to_float(p.x[name], dtype) * np.float32(size)).astype(np.float32), dtype)
+    got = p.backward(*p.stored_forward())
+    total = [np.zeros((p.rows, w)) for w in p.widths]
+    tol = [np.zeros((p.rows, w)) for w in p.widths]
+    u, out_step = ref.U[dtype], ref.TINY[dtype]
+    for rows, h, mine, shared, q, k, vh, g, seen in p.heads_of():
+        out, _, prob, _, _ = ref.attend(q, k, vh, seen, p.scale, dtype)
+        dp = g @ vh.T
+        ds = prob * (dp - (prob * dp).sum(1, keepdims=True))
+        E = ref.softmax_error(q, k, p.scale) + (k.shape[0] + 64) * 2.0 ** -24
+        # D from the stored output (off by its rounding, at least f16's least step) and from fp32 sums
+        off_d = ((u + 140 * 2.0 ** -24) * np.abs(g * out) + out_step * np.abs(g)).sum(1, keepdims=True)
+        off_ds = 1.02 * u * np.abs(ds) + prob * (1.02 * off_d + 140 * 2.0 ** -24 * (np.abs(g) @ np.abs(vh).T)) + 2 * E * np.abs(ds)
+        off_p = 1.02 * u * prob + 2 * E * prob
+        for i, (value, off, operand, factor) in enumerate(((ds, off_ds, k, p.scale), (ds.T, off_ds.T, q, p.scale),
+                                                          (prob.T, off_p.T, g, 1.0))):
+            off = off + 2.0 ** -34 * np.abs(value).max(1, keepdims=True) * (seen if i == 0 else seen.T)
+            at = (rows, mine if i == 0 else shared)
+            total[i][at] += factor * (value @ operand)
+            tol[i][at] += factor * (off + (value.shape[1] + 4) * 2.0 ** -24 * np.abs(value)) @ np.abs(operand)
+    for i, name in enumerate("qkv"):
+        bound = ref.rounded(total[i], tol[i], dtype)
+        want, have = total[i].copy(), ref.values(got[i], dtype)
+        if dtype == F16:  # past the largest value: infinite, next to it either
+            high = np.abs(want) > 65504
+            near = np.abs(np.abs(want) - 65520) <= bound
+            have[near & np.isinf(have)] = want[near & np.isinf(have)]
+            want[high & ~near] = np.inf * np.sign(want[high & ~near])
+        with np.errstate(invalid="ignore"):  # infinite minus infinite
+            ref.check(have, want, bound, "d" + name)
