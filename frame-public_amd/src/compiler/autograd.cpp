@@ -1,8 +1,8 @@
 // Reverse-mode differentiation over the IR (reference: src/compiler/autograd.cpp:118-450). The training graph is
 // built in the same node order as the reference's (clone, seed, then per forward node in reverse topological order:
-// its gradient micrograph, then one accumulating add per already-seen input), so its IR text is identical. Inputs of an integer or
-// bool type (packed_attention's cu_seqlens; no op of the reference has one) have no gradient: a micrograph has one output per
-// floating-point input.
+// its gradient micrograph, then one accumulating add per already-seen input), so its IR text is identical. A micrograph has one output
+// per input, as in the reference, or one per floating-point input: an op may give its integer or bool inputs no gradient
+// (packed_attention's cu_seqlens), and then such a graph input is refused as one to differentiate with respect to.
 #include <frame/compiler/autograd.h>
 
 #include <cmath>
@@ -112,9 +112,6 @@ Result<ir::Graph> build_backward_graph(const ir::Graph& forward, int32_t loss_ou
     if (!seen.insert(idx).second)
       return Status::make(ErrorCode::kInvalidArgument,
                           "compiler::build_backward_graph: wrt_input_indices entry " + std::to_string(idx) + " is duplicated");
-    if (!differentiable(forward.inputs()[static_cast<size_t>(idx)]->type()))
-      return Status::make(ErrorCode::kInvalidArgument, "compiler::build_backward_graph: wrt_input_indices entry " +
-                                                           std::to_string(idx) + " is not of a floating-point type");
   }
 
   ValueMap clone_map;
@@ -131,6 +128,7 @@ Result<ir::Graph> build_backward_graph(const ir::Graph& forward, int32_t loss_ou
       for (const ir::Value* v : (*it)->inputs()) chain.insert(v->producer());
 
   ValueMap grad;
+  std::unordered_set<const ir::Value*> without;  // values that an op on the way to the loss gives no gradient
   Result<ir::Node*> seed = splat(training, loss->type(), 1.0);
   if (!seed.is_ok()) return seed.status();
   FRAME_RETURN_IF_ERROR(accumulate(training, grad, loss, seed.value()->output(0)));
@@ -164,27 +162,33 @@ Result<ir::Graph> build_backward_graph(const ir::Graph& forward, int32_t loss_ou
       return Status::make(micro.status().code(), "compiler::build_backward_graph: op '" + op +
                                                      "' GradientFn failed: " + std::string(micro.status().message()));
     const size_t n = node->inputs().size(), m = node->outputs().size();
-    std::vector<ir::Value*> floats;
-    for (ir::Value* v : node->inputs())
-      if (differentiable(v->type())) floats.push_back(v);
+    std::vector<ir::Value*> given(node->inputs().begin(), node->inputs().end()), left_out;
+    if (micro.value().outputs().size() != n) {
+      given.clear();
+      for (ir::Value* v : node->inputs()) (differentiable(v->type()) ? given : left_out).push_back(v);
+    }
     if (micro.value().inputs().size() != n + 2 * m)
       return internal("op '" + op + "' gradient micrograph declared " + std::to_string(micro.value().inputs().size()) +
                       " graph input(s), expected " + std::to_string(n + 2 * m) + " ([x.., y.., gy..])");
-    if (micro.value().outputs().size() != floats.size())
+    if (micro.value().outputs().size() != given.size())
       return Status::make(ErrorCode::kInvalidArgument,
                           "compiler::build_backward_graph: op '" + op + "' gradient micrograph produced " +
                               std::to_string(micro.value().outputs().size()) + " graph output(s), expected " +
-                              std::to_string(floats.size()) + " (one gradient per input)");
+                              std::to_string(n) + " (one gradient per input)");
     std::vector<ir::Value*> bound(node->inputs().begin(), node->inputs().end());
     for (size_t j = 0; j < m; ++j) bound.push_back(node->output(static_cast<int32_t>(j)));
     bound.insert(bound.end(), gys.begin(), gys.end());
     Result<std::vector<ir::Value*>> gx = splice(training, micro.value(), bound);
     if (!gx.is_ok()) return gx.status();
-    for (size_t i = 0; i < floats.size(); ++i) FRAME_RETURN_IF_ERROR(accumulate(training, grad, floats[i], gx.value()[i]));
+    for (size_t i = 0; i < given.size(); ++i) FRAME_RETURN_IF_ERROR(accumulate(training, grad, given[i], gx.value()[i]));
+    without.insert(left_out.begin(), left_out.end());
   }
 
   for (int32_t idx : wrt_input_indices) {
     ir::Value* x = clone_map.at(forward.inputs()[static_cast<size_t>(idx)]);
+    if (without.count(x) != 0 && !differentiable(x->type()))
+      return Status::make(ErrorCode::kInvalidArgument, "compiler::build_backward_graph: wrt_input_indices entry " +
+                                                           std::to_string(idx) + " is not of a floating-point type");
     auto g = grad.find(x);
     ir::Value* out = nullptr;
     if (g != grad.end()) {
