@@ -5,6 +5,7 @@
 // (packed_attention's cu_seqlens), and then such a graph input is refused as one to differentiate with respect to.
 #include <frame/compiler/autograd.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <unordered_map>
@@ -128,7 +129,7 @@ Result<ir::Graph> build_backward_graph(const ir::Graph& forward, int32_t loss_ou
       for (const ir::Value* v : (*it)->inputs()) chain.insert(v->producer());
 
   ValueMap grad;
-  std::unordered_set<const ir::Value*> without;  // values that an op on the way to the loss gives no gradient
+  std::unordered_set<const ir::Value*> without;  // values that an op on the way to the loss gives no gradient, and what they are made of
   Result<ir::Node*> seed = splat(training, loss->type(), 1.0);
   if (!seed.is_ok()) return seed.status();
   FRAME_RETURN_IF_ERROR(accumulate(training, grad, loss, seed.value()->output(0)));
@@ -136,6 +137,12 @@ Result<ir::Graph> build_backward_graph(const ir::Graph& forward, int32_t loss_ou
   for (auto it = order.rbegin(); it != order.rend(); ++it) {
     ir::Node* node = *it;
     if (chain.count(node) == 0 || node->inputs().empty()) continue;
+    // a node whose results the loss depends on only as inputs that are left out passes that on to its own
+    if (std::all_of(node->outputs().begin(), node->outputs().end(),
+                    [&](const ir::Value& v) { return grad.count(&v) == 0 && without.count(&v) != 0; })) {
+      without.insert(node->inputs().begin(), node->inputs().end());
+      continue;
+    }
     const std::string op(node->op());
     const ops::OpSchema* schema = ops::OpRegistry::instance().find(op);
     if (schema == nullptr) return internal("op '" + op + "' is not registered");

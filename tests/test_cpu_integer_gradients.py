@@ -1,11 +1,13 @@
-"""Training graphs with integer tensors: graphs of nothing else, and integer inputs beside others."""
+"""Training graphs with integer tensors: graphs of nothing else, inputs that an op gives no gradient to, and what computes those."""
 import ctypes
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 import oracle_lib as orc
+import packed_graphs as pg
 from frame_hip import graphs, host
 
 BF16, I32 = 3, graphs.I32
@@ -44,6 +46,40 @@ def test_an_integer_input_beside_the_loss_has_zeros():
     g.output(total(g, g.mul(a, a)))
     back = host.backward(g.text(), 0, [1])
     assert "int32[2]" in back.splitlines()[-3]
+
+
+def attention(g, tokens, cu):
+    q, k, v = (g.input(BF16, (tokens, 16)) for _ in range(3))
+    return g.packed_attention(q, k, v, cu, 2, 2)
+
+
+def test_cu_seqlens_may_be_computed():
+    # a slice of a longer tensor: the nodes that make it lie on the way to the loss and have no gradient
+    tokens, cu = 9, np.array([-3, 0, 4, 9, 7], np.int32)
+    g = graphs.Graph("cpu")
+    longer = g.input(I32, (5,))
+    y = attention(g, tokens, g.slice(longer, 0, 1, 4))
+    g.output(total(g, g.mul(y, g.input(BF16, (tokens, 16)))))
+    back = host.backward(g.text(), 0, [1, 2, 3])
+    assert back.count(" packed_attention_grad_internal(") == 1 and "slice_grad" not in back
+    q, k, v, _, dout = pg.inputs(BF16, cu[1:4], tokens, 2, 2, 8)
+    outs = orc.run_graph_cpu(back, [cu, q, k, v, dout])
+    plain = host.backward(pg.attention_graph(BF16, tokens, 2, 2, 2, 8, loss=True).text(), 0, [0, 1, 2])
+    for a, b in zip(outs, orc.run_graph_cpu(plain, [q, k, v, cu[1:4], dout])):
+        assert np.array_equal(a, b)
+    with pytest.raises(host.FrameError, match="not of a floating-point type"):
+        host.backward(g.text(), 0, [0, 1])
+
+
+def test_computed_cu_seqlens_through_several_nodes():
+    tokens = 9
+    g = graphs.Graph("cpu")
+    parts = [g.input(I32, (n,)) for n in (2, 3)]
+    cu = g.slice(g.concat(parts, 0), 0, 0, 3)
+    y = attention(g, tokens, cu)
+    g.output(total(g, g.mul(y, y)))
+    back = host.backward(g.text(), 0, [2, 3, 4])
+    assert back.count(" packed_attention_grad_internal(") == 1
 
 
 PLUGIN = """
