@@ -167,18 +167,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attention_keys_kernel(const Ro
 
   // 16 threads per row, DH / 16 values each
   const int row = tid >> 4, d = (tid & 15) * (DH / 16), r = tile.tile0 + row;
-  if (r >= tile.rows) return;
   float high = stats[0][0][row], total = 0.0f;
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) high = fmaxf(high, stats[0][w][row]);
   const float ref = high == -__builtin_inff() ? 0.0f : high;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) total += stats[1][w][row] * __builtin_amdgcn_exp2f(stats[0][w][row] - ref);
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  float inv = 1.0f / total, lse2 = ref + __log2f(total);
+  if (__any(total == 0.0f)) {
+    const bool sees = tile.template sees<SRC>(a, kbegin, kend, tile.limit(a, r));
+    if (total == 0.0f) weigh_nothing(sees, whole, inv, lse2);
+  }
+  if (r >= tile.rows) return;
   const int token = divide(r, a.group);
   const int64_t trow = tile.seq.begin + token, head = kv_head * group + r - token * group;
   const int64_t part_row = (static_cast<int64_t>(blockIdx.z) * a.tokens + trow) * a.heads + head;
-  if (!whole && (tid & 15) == 0) a.part_lse[part_row] = total == 0.0f ? -__builtin_inff() : ref + __log2f(total);
+  if (!whole && (tid & 15) == 0) a.part_lse[part_row] = lse2;
 #pragma unroll
   for (int i = 0; i < DH / 64; ++i) {  // 4 values at a time
     const int at = d + 4 * i;
@@ -277,7 +281,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const RowsArgs a) {
     acc[2] = t.z;
     acc[3] = t.w;
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inv = sum == 0.0f ? 0.0f : top == kNoScore ? __builtin_nanf("") : 1.0f / sum;
   if (half == 0 && d < a.dh) {
     u32x2_t w;
     w[0] = narrow2<T>(acc[0] * inv, acc[1] * inv);

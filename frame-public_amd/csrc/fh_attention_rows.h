@@ -202,6 +202,14 @@ struct KvStage {
   }
 };
 
+// A row's factor and log-sum-exp (base 2) where its sum is 0. No key seen: zeros, and -inf. Keys seen, every score of them -inf: 0 / 0, so
+// NaN; as one of several parts zeros that weigh less than any finite score's, with kNoScore for the join to tell.
+constexpr float kNoScore = -3.402823466e38f;
+__device__ __forceinline__ void weigh_nothing(bool sees, bool whole, float& inv, float& lse2) {
+  inv = sees && whole ? __builtin_nanf("") : 0.0f;
+  lse2 = sees && !whole ? kNoScore : -__builtin_inff();
+}
+
 // The running softmax of a wave's 32 rows over blocks of NT 32-key tiles in LDS, and the accumulators of the output.
 template <typename T, int DH>
 struct RowState {
@@ -283,11 +291,16 @@ struct RowState {
 #pragma unroll
     for (int i = 0; i < DH / 2; ++i) o[i / 16][i % 16] = o[i / 16][i % 16] * f + room[(2 + i) * 64] * g;
   }
-  // rows without a visible key: zeros, lse -inf
-  __device__ __forceinline__ void finish(float& inv, float& lse2) {
+  // sees(): whether the lane's row sees a key, asked of the whole wave where a row's sum is 0
+  template <typename Sees>
+  __device__ __forceinline__ void finish(float& inv, float& lse2, bool whole, Sees sees) {
     const float sum = half_sum(l);
-    inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    lse2 = sum == 0.0f ? -__builtin_inff() : m + __log2f(sum);
+    inv = 1.0f / sum;
+    lse2 = m + __log2f(sum);
+    if (__any(sum == 0.0f)) {
+      const bool any = sees();
+      if (sum == 0.0f) weigh_nothing(any, whole, inv, lse2);
+    }
   }
 
   __device__ __forceinline__ void write_part(const RowsArgs& a, int64_t row, float inv, float lse2, int hi) const {
@@ -339,6 +352,18 @@ struct RowTile {
   }
   __device__ __forceinline__ int limit(const RowsArgs& a, int r) const {  // last visible key of row r
     return a.causal ? min(first + divide(min(r, rows - 1), a.group), keys - 1) : keys - 1;
+  }
+  // Whether any of the keys kbegin .. min(lim, kend - 1) exists; by a whole wave (lim is a lane's), 64 pages at a time.
+  template <int SRC>
+  __device__ __forceinline__ bool sees(const RowsArgs& a, int kbegin, int kend, int lim) const {
+    if constexpr (SRC == kDense) return kbegin <= min(lim, kend - 1);
+    const int pages = kbegin < kend ? ((kend - 1) >> a.page_shift) + 1 : 0;
+    for (int base = kbegin >> a.page_shift; base < pages; base += 64) {
+      const int i = base + static_cast<int>(threadIdx.x & 63);
+      const uint64_t there = __ballot(i < pages && static_cast<uint32_t>(table[min(i, pages - 1)]) < static_cast<uint32_t>(a.pages));
+      if (there != 0) return max((base + __builtin_ctzll(there)) << a.page_shift, kbegin) <= lim;  // the first one
+    }
+    return false;
   }
   // Parts: z takes keys z * part .. (z + 1) * part - 1, the last part all that follow. False: nothing for this part to write (a
   // sequence that the first part covers is written whole by it; the join goes by the same rule).
@@ -463,7 +488,7 @@ __global__ __launch_bounds__(W * 64, 2) void attention_rows_kernel(const RowsArg
     if (share == 1) return;
   }
   float inv, lse2;
-  state.finish(inv, lse2);
+  state.finish(inv, lse2, whole, [&] { return tile.template sees<SRC>(a, kbegin, kend, lim); });
   if (!live) return;
   if (uneven && bad.any != 0) {
 #pragma unroll

@@ -95,3 +95,81 @@ def test_packed_gradients_hold_small_and_large_derivatives(hip, case):
             want[high & ~near] = np.inf * np.sign(want[high & ~near])
         with np.errstate(invalid="ignore"):  # infinite minus infinite
             ref.check(have, want, bound, "d" + name)
+
+
+INF = {F16: 0x7c00, BF16: 0x7f80}
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dh", [(BF16, 4, 2, 64), (F16, 2, 2, 128)])
+@pytest.mark.parametrize("lens", [[70, 300], [70, 300, 100] * 30])
+def test_packed_rows_whose_scores_are_all_minus_infinity(hip, dtype, heads, kv_heads, dh, lens):
+    # an infinite value of q against keys of the other sign: 0 / 0 in the row's softmax, and nothing for any other row
+    say(f"packed scores of minus infinity, {heads} heads over {kv_heads} of {dh}, {len(lens)} sequences")
+    p = Packed(hip, dtype, lens, heads, kv_heads, dh, 1)
+    p.x["k"][:, 3] |= 0x8000
+    clean, _ = p.forward()
+    kept = p.x["q"].copy()
+    for t in (0, 1, 64, 299):
+        at = int(p.cu[1]) + t
+        p.x["q"][at, 3] = INF[dtype]
+        out, lse = p.forward()
+        p.x["q"] = kept.copy()
+        hit = np.zeros(out.shape, bool)
+        hit[at, :dh] = True
+        assert np.isnan(ref.values(out[hit], dtype)).all() and np.array_equal(out[~hit], clean[~hit])
+        assert not np.isfinite(lse[at, 0])
+
+
+@pytest.mark.parametrize("dtype,cache_dtype,dh", [(BF16, BF16, 64), (F16, E4M3, 128)])
+@pytest.mark.parametrize("past,new", [(70, 2), (1900, 3), (0, 1), (40, 90), (1500, 130)])
+def test_paged_rows_whose_scores_are_all_minus_infinity(hip, dtype, cache_dtype, dh, past, new):
+    say(f"paged scores of minus infinity, {new} tokens behind {past}, cache {cache_dtype}")
+    p = Paged(hip, dtype, cache_dtype, [past], [new], 4, 2, dh, 16)
+    p.fill_past()
+    p.put_new()
+    p.kc[..., 0, 3] |= 0x80 if cache_dtype == E4M3 else 0x8000  # key head 0's keys are negative there
+    p.upload()
+    row = new // 2
+    for keys in (64, 1 << 20):
+        clean, _ = p.attend(max_keys=keys)
+        p.check_attend(clean, "finite")
+        kept = p.q.copy()
+        p.q[row, 3] = INF[dtype]
+        p.dev["q"].upload(p.q)
+        out, _ = p.attend(max_keys=keys)
+        hit = np.zeros(out.shape, bool)
+        hit[row, :dh] = True
+        assert np.isnan(ref.values(out[hit], dtype)).all() and np.array_equal(out[~hit], clean[~hit])
+        # the same row over pages that do not exist sees nothing, and is zeros
+        p.dev["table"].upload(np.full_like(p.table, -1))
+        out, _ = p.attend(max_keys=keys)
+        assert not (out & 0x7fff).any()
+        p.dev["table"].upload(p.table)
+        p.q = kept
+        p.dev["q"].upload(p.q)
+
+
+@pytest.mark.parametrize("dtype,dh", [(BF16, 64), (F16, 128)])
+@pytest.mark.parametrize("past,new", [(1900, 3), (1500, 130), (100, 40)])
+def test_paged_keys_at_minus_infinity_weigh_nothing(hip, dtype, dh, past, new):
+    # whole parts of the context at minus infinity beside finite ones: the others' result
+    say(f"paged keys at minus infinity, {new} tokens behind {past}")
+    p = Paged(hip, dtype, dtype, [past], [new], 4, 2, dh, 16)
+    p.fill_past()
+    p.put_new()
+    p.q[:, 3::dh] &= 0x7fff  # positive there
+    finite = past * 2 // 3
+    for i in range(finite):
+        p.kc[p.slot(0, i)][:, 3] = INF[dtype] | 0x8000
+    p.upload()
+    slots = [p.slot(0, i) for i in range(past + new)]
+    keys, vals = (np.array([p.row(c, None, s) for s in slots]) for c in (p.kc, p.vc))
+    keys[:finite] = 0.0
+    seen = (np.arange(past + new)[None, :] <= past + np.arange(new)[:, None]) & (np.arange(past + new) >= finite)
+    for max_keys in (64, 1 << 20):
+        out, _ = p.attend(max_keys=max_keys)
+        for h in range(p.heads):
+            mine = slice(h * dh, (h + 1) * dh)
+            want, tol, *_ = ref.attend(ref.values(p.q[:, mine], dtype), keys[:, h // 2], vals[:, h // 2], seen,
+                                       float(np.float32(1 / np.sqrt(dh))), dtype)
+            ref.check(ref.values(out[:, mine], dtype), want, tol + 2.0 ** -20 * np.abs(want), f"head {h}")
