@@ -55,7 +55,7 @@ struct RowsArgs {
 };
 
 // 8 e4m3 values times a power of two (the fp32 `scale`), as 8 values of T: exact in bf16; in f16 exact but below its smallest normal
-// value and past its largest, where the values of f16 rows that such a scale was made for do not lie.
+// value, where the values of f16 rows that such a scale was made for do not lie; past T's largest value infinite, see below_infinity().
 template <typename T>
 __device__ __forceinline__ u32x4_t widen_e4m3(const u32x2_t& w, float scale) {
   u32x4_t o;
@@ -68,6 +68,19 @@ __device__ __forceinline__ u32x4_t widen_e4m3(const u32x2_t& w, float scale) {
       o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], scale, false));
       o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], scale, true));
     }
+  }
+  return o;
+}
+// The largest values of T (f16 63,488 and more, bf16 248 2^120) are nearest to 256 times their row's scale, which T cannot hold: widened,
+// they become its largest value. kTopScale: the byte of the least scale with such values.
+template <typename T>
+constexpr uint32_t kTopScale = std::is_same_v<T, bf16_t> ? 127 + 120 : 127 + 8;
+template <typename T>
+__device__ __forceinline__ u32x4_t below_infinity(u32x4_t o) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t size = o[i] & 0x7fff7fffu;
+    o[i] -= ((size & 0xffffu) == kExponent<T> ? 1u : 0u) + ((size >> 16) == kExponent<T> ? 0x10000u : 0u);
   }
   return o;
 }
@@ -184,6 +197,18 @@ struct KvStage {
       }
       *reinterpret_cast<u32x4_t*>(kbuf + at) = kw;
       *reinterpret_cast<u32x4_t*>(vbuf + at) = vw;
+    }
+    if constexpr (SRC == kE4m3) {
+      // rare, so looked for once per key (per chunk, on the way: 64 sequences' step 149 us instead of 142); in a loop only where a
+      // thread has more chunks than registers for them (the loop's own addresses spill in the 256-thread form)
+      if (__any((scales & 0xffu) >= kTopScale<T> || (scales >> 8) >= kTopScale<T>)) {
+#pragma unroll(N <= 4 ? N : 1)
+        for (int n = 0; n < N; ++n) {
+          const int at = tile_at<DH>(row0 + n * PASS, chunk);
+          *reinterpret_cast<u32x4_t*>(kbuf + at) = below_infinity<T>(*reinterpret_cast<const u32x4_t*>(kbuf + at));
+          *reinterpret_cast<u32x4_t*>(vbuf + at) = below_infinity<T>(*reinterpret_cast<const u32x4_t*>(vbuf + at));
+        }
+      }
     }
   }
 

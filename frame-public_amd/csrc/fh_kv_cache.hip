@@ -148,7 +148,10 @@ __global__ __launch_bounds__(256) void kv_cache_kernel(const CacheArgs a, int pe
       for (int i = 0; i < 2; ++i) {
         if constexpr (!WRITE) {
           // positions without a cached row read as zeros
-          if constexpr (E4M3) w[u][i] = widen_e4m3<T>(c[u][i], __uint_as_float(byte[u][i] << 23));
+          if constexpr (E4M3) {
+            w[u][i] = widen_e4m3<T>(c[u][i], __uint_as_float(byte[u][i] << 23));
+            if (byte[u][i] >= kTopScale<T>) w[u][i] = below_infinity<T>(w[u][i]);
+          }
           if (mine[u]) *reinterpret_cast<u32x4_t*>(i ? a.xv + xv[u] : a.xk + xk[u]) = w[u][i];
         } else if constexpr (!E4M3) {
           if (there[u]) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(i ? a.v : a.k) + at[u]) = w[u][i];

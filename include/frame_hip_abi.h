@@ -366,7 +366,7 @@ fh_status fh_packed_clear(const int32_t* cu_seqlens, int64_t batch, void* x, int
  * table_stride * page_size is taken as that). block_table and kv_lens are device memory. A page number outside [0, pages) is
  * a page that does not exist: nothing is written to it, it reads as zeros, and attention leaves its positions out.
  * page_size is a power of two; cache_dtype is the tensors' dtype or FH_E4M3, which adds an E8M0 byte per (row, head): the value is
- * e4m3 * 2^(byte - 127). No counterpart in the reference. */
+ * e4m3 * 2^(byte - 127), or dtype's largest where that is past it. No counterpart in the reference. */
 typedef struct fh_paged_cache {
   int32_t dtype;       /* of the tensors: FH_BF16 or FH_F16 */
   int32_t cache_dtype; /* dtype, or FH_E4M3 */

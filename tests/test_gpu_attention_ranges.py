@@ -5,7 +5,7 @@ import pytest
 
 import attention_ref as ref
 from frame_hip import synth
-from test_gpu_packed_attention import BF16, E4M3, F16, Packed, Paged, say
+from test_gpu_packed_attention import BF16, E4M3, F16, NAN, Packed, Paged, say
 
 pytestmark = pytest.mark.gpu
 
@@ -173,3 +173,37 @@ def test_paged_keys_at_minus_infinity_weigh_nothing(hip, dtype, dh, past, new):
             want, tol, *_ = ref.attend(ref.values(p.q[:, mine], dtype), keys[:, h // 2], vals[:, h // 2], seen,
                                        float(np.float32(1 / np.sqrt(dh))), dtype)
             ref.check(ref.values(out[:, mine], dtype), want, tol + 2.0 ** -20 * np.abs(want), f"head {h}")
+
+
+@pytest.mark.parametrize("dtype,dh", [(F16, 64), (F16, 128), (BF16, 64), (BF16, 128)])
+def test_e4m3_cache_keeps_the_largest_values_finite(hip, dtype, dh):
+    # The largest values of a type are nearest to 256 times their row's scale, which is past it (f16: 65536; bf16: 2^128): they come back as the largest
+    # there is, and attention over them is finite.
+    say(f"e4m3 cache of the largest values, dtype {dtype}, dh {dh}")
+    top = 0x7bff if dtype == F16 else 0x7f7f
+    rows = 40
+    bits = np.random.default_rng(5).integers(top - 3, top + 1, (rows, dh)).astype(np.uint16)
+    bits[:, ::2] |= 0x8000
+    bits[0, 1] = NAN[dtype]
+    # (bf16: over one row; the fp32 sum of more has no room for them)
+    for past, new in ((0, [rows]), (rows - 1, [1]), (rows - 6, [6])) if dtype == F16 else ((0, [1]),):
+        rows = past + sum(new)
+        bits = bits[:rows]
+        p = Paged(hip, dtype, E4M3, [past], new, 2, 1, dh, 16)
+        p.k[:] = 0
+        for c, s, all_rows in ((p.kc, p.ks, np.zeros_like(bits)), (p.vc, p.vs, bits)):
+            p.put(c, s, 0, 0, all_rows)
+        r = p.upload()
+        back = [hip.to_device(np.zeros((rows, dh), np.uint16)) for _ in range(2)]
+        cu = hip.to_device(np.array([0, rows], np.int32))
+        hip.check(hip.lib().fh_kv_cache_read(r, back[0].value, dh, back[1].value, dh, rows, cu.value, None))
+        got = back[1].download((rows, dh), np.uint16)
+        nan = (bits & 0x7fff) == NAN[dtype]
+        assert np.array_equal(got[~nan], top | (bits[~nan] & 0x8000)) and np.isnan(ref.values(got[nan], dtype)).all()
+        for max_new in (1, 64):  # both forms; equal scores, so the mean of the values
+            out, _ = p.attend(max_new=max_new)
+            out = ref.values(out, dtype)
+            want = np.where(np.arange(dh) % 2, 1.0, -1.0) * float(ref.values(np.array([top], np.uint16), dtype)[0])
+            keep = np.arange(2 * dh) % dh != 1
+            assert np.allclose(out[:, keep], np.tile(want, 2)[keep], rtol=4 * ref.U[dtype], atol=0)
+            assert np.isnan(out[:, ~keep]).all()
