@@ -10,9 +10,10 @@
 //   attention_dkv_kernel: 32 keys per wave, keys and values in registers, blocks of 64 rows of q and dout in LDS.
 // p and ds are rounded to the storage type as operands of the second products, in f16 times a power of two that keeps them in its range
 // (OperandRange); everything else is fp32.
-// Measured: 2897 + 1034 + 165 tokens, 32 heads over 8, 128 dims, causal, bf16: 430 us (traced: dq 171, dk and dv 278, the
-// parts' sum 13), 452 TFLOP/s counted as 5 products, 633 as the 7 that are made; 3300 tokens in 8 sequences, 16 heads of 64: 48.5 us.
-// Bound by the waits of a tile's dependent steps (product, exponentials, product), which two waves per SIMD do not fill.
+// Measured: 2897 + 1034 + 165 tokens, 32 heads over 8, 128 dims, causal, bf16: 425 to 433 us (traced: dq 164, dk and dv 248, the
+// parts' sum 12), 455 TFLOP/s counted as 5 products, 637 as the 7 that are made; f16 456; 3300 tokens in 8 sequences, 16 heads of 64: 48.5 us.
+// Bound by the waits of a tile's dependent steps (product, exponentials, product), which two waves per SIMD do not fill: the matrix
+// unit is busy for 116 k of 379 k cycles per SIMD in dq and 190 k of 604 k in dk and dv, the vector ALU for 97 k and 177 k.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -4,10 +4,12 @@
 //     workgroup. Nothing but the cache's bytes counts: every wave keeps one or two blocks of 32 keys and values on their way in
 //     registers while it uses another from LDS of its own, so no wave ever waits for another. (With tiles of 32 rows, mostly empty, and one
 //     block on its way, 64 sequences' step over an e4m3 cache of 550 MB took 165 us, bound by the waits for memory.)
-//     Measured, 32 heads over 8, 128 dims: that step 140 us (3.9 TB/s), one new token over 32768 keys of 16 bits 35.5 us (25 and 5.5
+//     Measured, 32 heads over 8, 128 dims: that step 142 us (3.9 TB/s), one new token over 32768 keys of 16 bits 35.5 us (26 and 5.3
 //     for the join; 134 MB).
 //   more, chunks: attention_rows_kernel of fh_attention_rows.h, whose waves share the keys and own 32 rows each. 2025 new tokens
-//     of 7 sequences over up to 8,192 keys: 230 us, 590 TFLOP/s; in one part per sequence 456 us, the longest sequence's tiles alone.
+//     of 7 sequences over up to 8,192 keys: 232 to 236 us, 580 TFLOP/s; in one part per sequence 456 us, the longest sequence's tiles alone.
+// The form is the call's, by its longest sequence. 60 sequences' one token beside a chunk of 512 over 2,048 keys, contexts of 127 to 8,191:
+// 180 us over an e4m3 cache (apart, in two calls, 73 + 59), 173 over 16 bits (124 + 54).
 // Both cut long contexts into parts (keys z * part_keys ..) where the tiles alone would leave CUs idle; attention_join_kernel sums the
 // parts, weighted by their log-sum-exps, in their order.
 #include <hip/hip_runtime.h>

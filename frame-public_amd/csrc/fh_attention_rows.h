@@ -5,12 +5,14 @@
 // blocks in LDS, two buffers, the next block on its way in registers while this one is used. Scores are formed transposed
 // (K Q^T), so a lane holds one row's scores: maximum and sum stay in the lane but for one exchange of the halves, and the
 // probabilities, rounded to the storage type, are in place as the operand of V^T P^T.
-// What bounds it at long sequences is the vector ALU: 16 rows of 32 keys' exponentials, sums, maxima and conversions take about
-// as long as the 16 products that go with them, so the code places a product between every few exponentials. Measured: 5003 +
-// 2318 + 871 tokens, 32 heads over 8, 128 dims, causal, bf16: 300 us, 850 TFLOP/s of visible pairs (a library product of 8192^3: 1,249);
-// products and exponentials in separate stretches 310 us; a wait for the next block at the loop's start 318; 256 rows per
-// workgroup 302; raised wave priority around the products 312-320. Eight sequences of 512, 16 heads of 64: 16.9 us, launch and the
-// latencies of a workgroup's up to eight dependent blocks. Where tiles are few, two waves share 32 rows and split each block's keys.
+// Measured: 5003 + 2318 + 871 tokens, 32 heads over 8, 128 dims, causal, bf16: 297 to 307 us, 830 to 860 TFLOP/s of visible pairs (a
+// library product of 8192^3: 1,249); f16 325. What bounds it at long sequences is that matrix and vector work, about as much of
+// each, overlap little: of 657 k cycles per SIMD the matrix unit is busy for 252 k and the vector ALU for 279 k, and the two waves of a
+// SIMD, of different workgroups, fall into no order in which one's products run beside the other's exponentials. Within a wave
+// the code places a product between every few exponentials; both in separate stretches 310 us; a wait for the next block at the
+// loop's start 318; 256 rows per workgroup 302; raised wave priority around the products 312-320. Eight sequences of 512, 16 heads of
+// 64: 16.8 us, launch and the latencies of a workgroup's up to eight dependent blocks. Where tiles are few, two waves share 32 rows and
+// split each block's keys.
 // The accumulators are scaled again only when a row's maximum grows by more than 8 (base 2) over the one in use: sums and
 // probabilities then stay within 2^8 of their usual range, which fp32 and the rounding to 16 bits do not notice.
 // Masked scores are -inf by selection, never by addition, and rows of keys that are not there are zeros in LDS, so nothing that

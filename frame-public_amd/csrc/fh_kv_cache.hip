@@ -5,7 +5,7 @@
 // finite become NaN, and the maximum is taken over the others.
 // Both directions move 16 bytes of the tensors' side per lane, a row in DH / 8 lanes (8 or 16, power of two, for the maximum's
 // shuffles); they are bound by memory, and by the launch for a step's few rows. Measured, 8 heads of 128: 65,532 cached rows read
-// as bf16 89 us (404 MB, 4.55 TB/s; a copy reaches 5.13), 8,192 rows written 14.3 us (50 MB, 3.5 TB/s); one row in flight per
+// as bf16 84 us (404 MB, 4.8 TB/s; a copy reaches 5.13), 8,192 rows written 14.3 us (50 MB, 3.5 TB/s); one row in flight per
 // thread and a lookup per row: 154 and 16.7 us.
 #include <hip/hip_runtime.h>
 

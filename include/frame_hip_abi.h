@@ -334,7 +334,8 @@ fh_status fh_attention_grad(int32_t dtype, const void* q, const void* k, const v
  * No counterpart in the reference, whose attention has one length, no mask and as many key heads as heads
  * (src/nn/layers.cpp:1014-1080); unlike fh_attention_fwd these round no intermediate as a graph of single ops would: scores,
  * softmax and sums are fp32, and only the probabilities (and in the gradients their derivatives) are rounded to the storage type,
- * as operands of the second product (in f16 gradients times a power of two, so that small and large ones keep their bits). A workspace, here and below, serves one call at a time. */
+ * as operands of the second product (in f16 gradients times a power of two, so that small and large ones keep their bits). The
+ * sums hold up to 2^8 times the values before they are divided: bf16 values near 2^119 over the number of keys overflow them. A workspace, here and below, serves one call at a time. */
 typedef struct fh_packed_attention {
   int32_t dtype;
   int32_t causal; /* 1: row t of a sequence sees its rows 0 .. t; 0: all of them */
@@ -344,7 +345,8 @@ typedef struct fh_packed_attention {
 } fh_packed_attention;
 
 /* out = softmax(scale q k^T) v per head, and the natural logarithm of the softmax's sum in lse ([tokens, heads] fp32; may be NULL),
- * which the gradients read. A value that is not finite reaches the rows that see it and no others. */
+ * which the gradients read. A value that is not finite reaches the rows that see it and no others; a row whose every score is
+ * -infinity is NaN. */
 fh_status fh_attention_packed_fwd(const fh_packed_attention* geom, const void* q, const void* k, const void* v,
                                   const int32_t* cu_seqlens, void* out, float* lse, void* stream);
 
@@ -397,7 +399,7 @@ fh_status fh_kv_cache_read(const fh_paged_cache* cache, void* k, int64_t k_strid
 /* Attention of the new tokens over the cache: token i of the n new ones of sequence b sees positions 0 .. kv_lens[b] - n + i (the
  * cache holds the new tokens' keys and values already, see fh_kv_cache_write). Rows that see nothing are zeros. n = 1 is a
  * decoding step. max_new and max_keys are the longest n and kv_lens that are expected: they choose how the work is cut, and
- * any lengths give the same results up to rounding. The workspace query takes the same numbers; 0 bytes: may be NULL. A
+ * any lengths give the same results up to rounding. A batch of single tokens beside a longer chunk may be faster as two calls. The workspace query takes the same numbers; 0 bytes: may be NULL. A
  * cached value that is not finite reaches the rows that see it and no others. */
 int64_t fh_attention_paged_workspace(const fh_paged_cache* cache, int64_t tokens, int64_t heads, int64_t max_new, int64_t max_keys);
 fh_status fh_attention_paged(const fh_paged_cache* cache, const void* q, int64_t q_stride, void* out, int64_t out_stride,
