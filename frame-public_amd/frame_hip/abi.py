@@ -54,6 +54,18 @@ class PagedCache(ctypes.Structure):
                 ("kv_lens", c_void_p)]
 
 
+class TokenEmbedding(ctypes.Structure):
+    """fh_token_embedding: the sizes of a table's lookup by token and of its gradient."""
+    _fields_ = [("dtype", c_int32), ("tokens", c_int64), ("vocab", c_int64), ("dim", c_int64), ("row_stride", c_int64),
+                ("scale", c_float)]
+
+
+class VocabLoss(ctypes.Structure):
+    """fh_vocab_loss: the sizes of softmax cross entropy over a vocabulary and of its gradients."""
+    _fields_ = [("dtype", c_int32), ("loss_dtype", c_int32), ("mean", c_int32), ("tokens", c_int64), ("vocab", c_int64),
+                ("dim", c_int64), ("x_stride", c_int64), ("w_stride", c_int64)]
+
+
 _lib = None
 
 # name -> (restype, argtypes)
@@ -157,6 +169,14 @@ _SIGS = {
     "fh_conv2d_nhwc_fwd_split": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, POINTER(c_int64), c_void_p,
                                            c_int32, c_int32, c_void_p, c_int64, c_void_p]),
     "fh_pool2d": (c_int32, [c_int32, c_int32, c_void_p, c_void_p, POINTER(c_int64), c_void_p]),
+    "fh_embedding_fwd": (c_int32, [POINTER(TokenEmbedding)] + [c_void_p] * 4),
+    "fh_embedding_grad_workspace": (c_int64, [POINTER(TokenEmbedding)]),
+    "fh_embedding_grad": (c_int32, [POINTER(TokenEmbedding)] + [c_void_p] * 5 + [c_int64, c_void_p]),
+    "fh_vocab_loss_workspace": (c_int64, [POINTER(VocabLoss)]),
+    "fh_vocab_loss_fwd": (c_int32, [POINTER(VocabLoss)] + [c_void_p] * 7 + [c_int64, c_void_p]),
+    "fh_vocab_loss_grad_workspace": (c_int64, [POINTER(VocabLoss)]),
+    "fh_vocab_loss_grad_least": (c_int64, [POINTER(VocabLoss)]),
+    "fh_vocab_loss_grad": (c_int32, [POINTER(VocabLoss)] + [c_void_p] * 8 + [c_int64, c_void_p]),
     "fh_permute": (c_int32, [c_int32, c_void_p, c_void_p, c_int32, POINTER(c_int64), POINTER(c_int64), c_void_p]),
     "fh_copy2d": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
     "fh_fill": (c_int32, [c_void_p, c_int32, c_uint64, c_int64, c_void_p]),

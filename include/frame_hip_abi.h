@@ -406,6 +406,53 @@ fh_status fh_attention_paged(const fh_paged_cache* cache, const void* q, int64_t
                              int64_t tokens, int64_t heads, const int32_t* cu_seqlens, float scale, int64_t max_new,
                              int64_t max_keys, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- the two ends of a language model: token embedding, and the loss over the vocabulary ----
+ * Ids and targets are int32 in device memory; one outside [0, vocab) names nothing: its embedding is a row of zeros, its row of dout
+ * reaches nothing, its row of x has no loss (that row of x, dx aside, may hold anything). No counterpart in the reference, whose tensors
+ * of integers no op reads and whose only loss is mse_loss (src/ops/schemas/loss.cpp:30-279). */
+typedef struct fh_token_embedding {
+  int32_t dtype; /* FH_F32, FH_F16 or FH_BF16 */
+  int64_t tokens, vocab, dim;
+  int64_t row_stride; /* elements between rows of out or dout; the table is dense [vocab, dim] */
+  float scale;
+} fh_token_embedding;
+
+/* out[t] = scale * table[ids[t]], rounded once. Any dim and alignment. */
+fh_status fh_embedding_fwd(const fh_token_embedding* geom, const void* table, const int32_t* ids, void* out, void* stream);
+
+/* dtable[v] = base[v] + scale * sum of dout[t] over the tokens with ids[t] = v, in fp32, rounded once; base NULL is zeros. base may be
+ * dtable itself: then rows that no token names are left as they are. The table's other gradient (tied weights: fh_vocab_loss_grad's dw)
+ * goes in that way. Deterministic: a sum's order depends on the ids alone. */
+int64_t fh_embedding_grad_workspace(const fh_token_embedding* geom);
+fh_status fh_embedding_grad(const fh_token_embedding* geom, const void* dout, const int32_t* ids, const void* base, void* dtable,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of the logits x w^T against one target per row, without keeping the logits: x [tokens, dim], w [vocab, dim]
+ * (the embedding's table where they are tied), rows x_stride and w_stride elements apart. Rows without a target (see above) do not count:
+ * no work is done for them. bf16 / f16, dim and strides multiples of 8, tensors 16-byte aligned, no output may overlap an input. */
+typedef struct fh_vocab_loss {
+  int32_t dtype;      /* of x, w, dx and dw: FH_BF16 or FH_F16 */
+  int32_t loss_dtype; /* of the loss and of its gradient, one value each: FH_F32 or dtype */
+  int32_t mean;       /* 1: the loss is the mean over the rows with a target, 0: their sum; no such row: 0, and gradients of zeros */
+  int64_t tokens, vocab, dim, x_stride, w_stride;
+} fh_vocab_loss;
+
+/* lse[t] = log sum_v exp(x[t] . w[v]), row_loss[t] = lse[t] - x[t] . w[target[t]] (both fp32, 0 for rows without a target; row_loss
+ * may be NULL), and the loss. The gradients read lse. */
+int64_t fh_vocab_loss_workspace(const fh_vocab_loss* geom);
+fh_status fh_vocab_loss_fwd(const fh_vocab_loss* geom, const void* x, const void* w, const int32_t* targets, void* loss, float* row_loss,
+                            float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients with respect to x and w for the loss' gradient dloss (device memory), from the forward's lse: dx rows without a target are
+ * zeros; dx and dw have x's and w's strides, and either may be NULL. The logits are formed again a piece of the vocabulary at a time; the
+ * derivatives (probability, less 1 at the target) are rounded to dtype as operands of the two products (f16: times 2^14), sums are
+ * fp32. Deterministic for one workspace size. The query returns the size for pieces that the kernels run well on; the least that is taken has
+ * room for 256 columns of derivatives: fh_vocab_loss_grad_least. */
+int64_t fh_vocab_loss_grad_workspace(const fh_vocab_loss* geom);
+int64_t fh_vocab_loss_grad_least(const fh_vocab_loss* geom);
+fh_status fh_vocab_loss_grad(const fh_vocab_loss* geom, const void* x, const void* w, const int32_t* targets, const float* lse,
+                             const void* dloss, void* dx, void* dw, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* 2-D pooling, NCHW. mode 0 = max (-inf padding, first max wins), 1 = average (include padding).
  * geom = {N, C, H, W, KH, KW, stride_h, stride_w, pad_h, pad_w}.
  * Replaces cudnnPoolingForward (reference: src/backends/cuda/kernels/pool.cpp:172-244);
