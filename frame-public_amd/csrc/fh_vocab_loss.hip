@@ -1,0 +1,596 @@
+// Softmax cross entropy over a vocabulary without keeping the logits (fh_vocab_loss_fwd) and its gradients (fh_vocab_loss_grad).
+//
+// With z = x w^T, lse = log sum_v exp z and one target per row:
+//   forward:   row_loss = lse - z[target]; a tile of logits leaves the maximum and the sum of its exponentials per row, which a second
+//              kernel joins over the tiles of the vocabulary.
+//   gradients: with g = exp(z - lse) - [v = target], dx = f g w and dw = f g^T x, f = dloss (/ count for the mean): a piece of
+//              the vocabulary at a time, whose logits are formed again, whose g is kept in the storage type (f16: times 2^14, so that
+//              probabilities down to 2^-28 keep their bits) and read by both products. f is left to the products' results.
+// Rows without a target are taken out first: a list of the others stands for x's rows (forward), or they are copied together (gradients,
+// where rows are also summed over, and what such rows hold must not reach the sums).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "fh_common.h"
+#include "fh_mfma16.h"
+
+namespace fh {
+namespace {
+
+using namespace mfma16;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// What g is multiplied by in the storage type.
+template <typename T>
+constexpr float kRaise = std::is_same_v<T, f16_t> ? 0x1p14f : 1.0f;
+
+struct LossArgs {
+  const uint16_t* x;
+  const uint16_t* w;
+  const int32_t* targets;
+  int64_t ldx, ldw;
+  int tokens, vocab, dim;
+  int mean, loss_dtype;
+  float* lse;
+  float* row_loss;
+  void* loss;
+  const void* dloss;
+  uint16_t* dx;
+  uint16_t* dw;
+  // workspace
+  int* count;        // rows with a target
+  int32_t* rows;     // which they are, in their order
+  float* at_target;  // their target's logit
+  float2* part;      // [column tiles][tokens]: maximum, sum of exp(z - maximum)
+  int tiles_n;
+  // gradients: the rows with a target copied together, their targets and log-sum-exps, a piece of g, fp32 sums of dx over the pieces
+  uint16_t* xc;
+  int32_t* targets_c;
+  float* lse_c;
+  uint16_t* g;
+  int64_t ldg;
+  float* dx_sum;
+  int first, last;  // columns of the piece
+  int first_piece, last_piece;
+};
+
+// ---- one tile of a product ----
+
+// An operand of a tile's product, rows r (of the tile's dimension) by k. Not KMAJOR: element (r, k) = p[row(r) * ld + k], row(r) = rows[r]
+// or r, r clamped to `last`. KMAJOR: p[k * ld + r], chunks of 8 r clamped to end at `last`. Zeros from k = `depth` on.
+struct Operand {
+  const uint16_t* p;
+  int64_t ld;
+  const int32_t* rows;
+  int last, depth;
+};
+
+// A workgroup's BM x BN tile of A B^T over k < K, by WAVES_M x WAVES_N waves; the wave's lane l holds rows 16 i + 4 (l / 16) + x, columns
+// 16 j + l % 16 of its part.
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool AK, bool BK_>
+struct Tile {
+  static constexpr int NT = WAVES_M * WAVES_N * 64;
+  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 16, TN = WN / 16;
+  static constexpr int LD = kBK + 8;
+  static constexpr int LDS = (BM + BN) * LD * 2;
+
+  template <int R, bool KMAJOR>
+  __device__ static void stage(uint16_t* to, const Operand& o, int r0, int k0) {
+    for (int i = threadIdx.x; i < R * 4; i += NT) {
+      u32x4_t v{0, 0, 0, 0};
+      if constexpr (KMAJOR) {
+        const int k = i / (R / 8), c = i % (R / 8) * 8;
+        if (k0 + k < o.depth) v = *reinterpret_cast<const u32x4_t*>(o.p + static_cast<int64_t>(k0 + k) * o.ld + min(r0 + c, o.last - 7));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[(c + e) * LD + k] = static_cast<uint16_t>(v[e / 2] >> (16 * (e & 1)));
+      } else {
+        const int r = min(r0 + i / 4, o.last), k = i % 4 * 8;
+        const int64_t row = o.rows != nullptr ? o.rows[r] : r;
+        if (k0 + k < o.depth) v = *reinterpret_cast<const u32x4_t*>(o.p + row * o.ld + k0 + k);
+        *reinterpret_cast<u32x4_t*>(to + (i / 4) * LD + k) = v;
+      }
+    }
+  }
+
+  __device__ static void product(unsigned char* lds, const Operand& a, const Operand& b, int m0, int n0, int K, f32x4_t (&acc)[TM][TN]) {
+    uint16_t* as = reinterpret_cast<uint16_t*>(lds);
+    uint16_t* bs = as + BM * LD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave / WAVES_N * WM, wn = wave % WAVES_N * WN;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = 0; k0 < K; k0 += kBK) {
+      __syncthreads();
+      stage<BM, AK>(as, a, m0, k0);
+      stage<BN, BK_>(bs, b, n0, k0);
+      __syncthreads();
+      u32x4_t fa[TM], fb[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const u32x4_t*>(as + (wm + 16 * i + (lane & 15)) * LD + 8 * (lane >> 4));
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const u32x4_t*>(bs + (wn + 16 * j + (lane & 15)) * LD + 8 * (lane >> 4));
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) mfma16x<T>(fa[i], fb[j], acc[i][j]);
+    }
+  }
+};
+
+// max and sum over the 16 lanes that share rows of a tile
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ float sum16(float v) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// A maximum that exponents can be taken against: of a row of -infinity, 0.
+__device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// ---- rows with a target ----
+
+// By one workgroup: the list of rows with a target and their number; the others' outputs. In the gradients (lse_c) also their targets
+// and log-sum-exps.
+__global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a) {
+  __shared__ int waves[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int each = (a.tokens + 1023) / 1024, begin = tid * each, end = min(a.tokens, begin + each);
+  auto has = [&](int t) { return a.targets[t] >= 0 && a.targets[t] < a.vocab; };
+  int n = 0;
+  for (int t = begin; t < end; ++t) n += has(t);
+  int scan = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(scan, o, 64);
+    if (lane >= o) scan += up;
+  }
+  if (lane == 63) waves[wave] = scan;
+  __syncthreads();
+  int at = scan - n;
+  for (int w = 0; w < wave; ++w) at += waves[w];
+  if (tid == 1023) *a.count = at + n;
+  for (int t = begin; t < end; ++t) {
+    if (has(t)) {
+      a.rows[at] = t;
+      if (a.lse_c != nullptr) {
+        a.targets_c[at] = a.targets[t];
+        a.lse_c[at] = a.lse[t];
+      }
+      ++at;
+    } else if (a.lse_c == nullptr) {
+      a.lse[t] = 0.0f;
+      if (a.row_loss != nullptr) a.row_loss[t] = 0.0f;
+    }
+  }
+}
+
+// ---- forward ----
+
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(const LossArgs a) {
+  using P = Tile<T, BM, BN, WAVES_M, WAVES_N, false, false>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::LDS];
+  __shared__ float2 joined[WAVES_N][BM];
+  const int count = *a.count;
+  const int tiles_m = (a.tokens + BM - 1) / BM;
+  const int m0 = static_cast<int>(blockIdx.x % tiles_m) * BM, tn = static_cast<int>(blockIdx.x / tiles_m), n0 = tn * BN;
+  if (m0 >= count) return;
+  f32x4_t acc[P::TM][P::TN];
+  P::product(lds, {a.x, a.ldx, a.rows, count - 1, a.dim}, {a.w, a.ldw, nullptr, a.vocab - 1, a.dim}, m0, n0, a.dim, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+  const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
+#pragma unroll
+  for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int row = wm + 16 * i + 4 * g + x, m = m0 + row;
+      const int target = a.targets[a.rows[min(m, count - 1)]];
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < P::TN; ++j) {
+        const int col = n0 + wn + 16 * j + r;
+        if (col < a.vocab) top = fmaxf(top, acc[i][j][x]);
+        if (col == target && m < count) a.at_target[m] = acc[i][j][x];
+      }
+      top = max16(top);
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < P::TN; ++j)
+        if (n0 + wn + 16 * j + r < a.vocab) sum += __builtin_amdgcn_exp2f((acc[i][j][x] - origin(top)) * kLog2e);
+      sum = sum16(sum);
+      if (r == 0) joined[wave % WAVES_N][row] = float2{top, sum};
+    }
+  __syncthreads();
+  for (int row = threadIdx.x; row < BM; row += P::NT) {
+    if (m0 + row >= count) break;
+    float top = joined[0][row].x, sum = 0.0f;
+    for (int w = 1; w < WAVES_N; ++w) top = fmaxf(top, joined[w][row].x);
+    for (int w = 0; w < WAVES_N; ++w) sum += joined[w][row].y * __builtin_amdgcn_exp2f((joined[w][row].x - origin(top)) * kLog2e);
+    a.part[static_cast<int64_t>(tn) * a.tokens + m0 + row] = float2{top, sum};
+  }
+}
+
+// 16 rows per workgroup, 16 threads each a share of the tiles.
+__global__ __launch_bounds__(256) void loss_join_kernel(const LossArgs a) {
+  __shared__ float2 shares[16][16];
+  const int row = threadIdx.x & 15, share = threadIdx.x >> 4;
+  const int count = *a.count, m = static_cast<int>(blockIdx.x) * 16 + row;
+  float top = -INFINITY, sum = 0.0f;
+  if (m < count)
+    for (int t = share; t < a.tiles_n; t += 16) {
+      const float2 p = a.part[static_cast<int64_t>(t) * a.tokens + m];
+      const float both = fmaxf(top, p.x), from = origin(both);
+      sum = sum * __builtin_amdgcn_exp2f((top - from) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - from) * kLog2e);
+      top = both;
+    }
+  shares[share][row] = float2{top, sum};
+  __syncthreads();
+  if (share != 0 || m >= count) return;
+  for (int s = 1; s < 16; ++s) top = fmaxf(top, shares[s][row].x);
+  float all = 0.0f;
+  for (int s = 0; s < 16; ++s) all += shares[s][row].y * __builtin_amdgcn_exp2f((shares[s][row].x - origin(top)) * kLog2e);
+  const float lse = origin(top) + logf(all);
+  const int t = a.rows[m];
+  a.lse[t] = lse;
+  a.at_target[m] = lse - a.at_target[m];
+  if (a.row_loss != nullptr) a.row_loss[t] = a.at_target[m];
+}
+
+// The loss, by one workgroup: the rows' losses in one order, in double.
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const LossArgs a) {
+  __shared__ double shares[1024];
+  const int tid = threadIdx.x, count = *a.count;
+  double sum = 0.0;
+  for (int m = tid; m < count; m += 1024) sum += a.at_target[m];
+  shares[tid] = sum;
+  __syncthreads();
+  for (int o = 512; o > 0; o >>= 1) {
+    if (tid < o) shares[tid] += shares[tid + o];
+    __syncthreads();
+  }
+  if (tid != 0) return;
+  const float loss = static_cast<float>(a.mean && count > 0 ? shares[0] / count : shares[0]);
+  if (a.loss_dtype == FH_F32) *static_cast<float*>(a.loss) = loss;
+  if (a.loss_dtype == FH_BF16) *static_cast<uint16_t*>(a.loss) = Io<bf16_t>::store(loss);
+  if (a.loss_dtype == FH_F16) *static_cast<uint16_t*>(a.loss) = Io<f16_t>::store(loss);
+}
+
+// ---- gradients ----
+
+// A wave per row: xc's row m is x's row rows[m]; rows behind the last, up to a multiple of 64, are zeros (dw sums over them); dx's rows
+// without a target are zeros.
+__global__ __launch_bounds__(256) void loss_gather_kernel(const LossArgs a) {
+  const int lane = threadIdx.x & 63, t = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int count = *a.count, end = (count + 63) / 64 * 64;
+  const u32x4_t zeros{0, 0, 0, 0};
+  if (t < end) {
+    const uint16_t* from = t < count ? a.x + a.rows[t] * a.ldx : nullptr;
+    for (int c = lane * 8; c < a.dim; c += 512)
+      *reinterpret_cast<u32x4_t*>(a.xc + static_cast<int64_t>(t) * a.dim + c) = from != nullptr ? *reinterpret_cast<const u32x4_t*>(from + c) : zeros;
+  }
+  if (a.dx != nullptr && t < a.tokens && !(a.targets[t] >= 0 && a.targets[t] < a.vocab))
+    for (int c = lane * 8; c < a.dim; c += 512) *reinterpret_cast<u32x4_t*>(a.dx + t * a.ldx + c) = zeros;
+}
+
+__device__ __forceinline__ float loss_factor(const LossArgs& a) {
+  const float d = a.loss_dtype == FH_F32    ? *static_cast<const float*>(a.dloss)
+                  : a.loss_dtype == FH_BF16 ? Io<bf16_t>::load(*static_cast<const uint16_t*>(a.dloss))
+                                            : Io<f16_t>::load(*static_cast<const uint16_t*>(a.dloss));
+  return a.mean ? d / static_cast<float>(*a.count) : d;
+}
+
+// g of a piece: columns first .. last - 1 of the vocabulary, zeros behind them and in rows without one up to the tile's end.
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(const LossArgs a) {
+  using P = Tile<T, BM, BN, WAVES_M, WAVES_N, false, false>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::LDS];
+  const int count = *a.count;
+  const int tiles_m = (a.tokens + BM - 1) / BM;
+  const int m0 = static_cast<int>(blockIdx.x % tiles_m) * BM, n0 = static_cast<int>(blockIdx.x / tiles_m) * BN;
+  if (m0 >= count) return;
+  f32x4_t acc[P::TM][P::TN];
+  P::product(lds, {a.xc, a.dim, nullptr, count - 1, a.dim}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.vocab - 1 - a.first, a.dim}, m0, n0, a.dim, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+  const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
+#pragma unroll
+  for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int m = m0 + wm + 16 * i + 4 * g + x, mc = min(m, count - 1);
+      const float lse = a.lse_c[mc];
+      const int target = a.targets_c[mc];
+#pragma unroll
+      for (int j = 0; j < P::TN; ++j) {
+        const int col = n0 + wn + 16 * j + r, v = a.first + col;
+        float d = __builtin_amdgcn_exp2f((acc[i][j][x] - lse) * kLog2e) - (v == target ? 1.0f : 0.0f);
+        if (m >= count || v >= a.last) d = 0.0f;
+        a.g[static_cast<int64_t>(m) * a.ldg + col] = Io<T>::store(d * kRaise<T>);
+      }
+    }
+}
+
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const LossArgs a) {
+  using P = Tile<T, BM, BN, WAVES_M, WAVES_N, false, true>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::LDS];
+  const int count = *a.count;
+  const int tiles_m = (a.tokens + BM - 1) / BM;
+  const int m0 = static_cast<int>(blockIdx.x % tiles_m) * BM, n0 = static_cast<int>(blockIdx.x / tiles_m) * BN;
+  if (m0 >= count) return;
+  const int depth = a.last - a.first;
+  f32x4_t acc[P::TM][P::TN];
+  P::product(lds, {a.g, a.ldg, nullptr, count - 1, static_cast<int>(a.ldg)}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.dim - 1, depth}, m0, n0, depth, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+  const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
+  const float f = loss_factor(a) / kRaise<T>;
+#pragma unroll
+  for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int m = m0 + wm + 16 * i + 4 * g + x;
+      if (m >= count) continue;
+#pragma unroll
+      for (int j = 0; j < P::TN; ++j) {
+        const int col = n0 + wn + 16 * j + r;
+        if (col >= a.dim) continue;
+        float v = acc[i][j][x];
+        float* sum = a.dx_sum + static_cast<int64_t>(m) * a.dim + col;
+        if (!a.first_piece) v += *sum;
+        if (a.last_piece)
+          a.dx[a.rows[m] * a.ldx + col] = Io<T>::store(v * f);
+        else
+          *sum = v;
+      }
+    }
+}
+
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const LossArgs a) {
+  using P = Tile<T, BM, BN, WAVES_M, WAVES_N, true, true>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::LDS];
+  const int count = *a.count, depth = (count + kBK - 1) / kBK * kBK;
+  const int tiles_n = (a.dim + BN - 1) / BN;
+  const int n0 = static_cast<int>(blockIdx.x % tiles_n) * BN, m0 = static_cast<int>(blockIdx.x / tiles_n) * BM;
+  f32x4_t acc[P::TM][P::TN];
+  P::product(lds, {a.g, a.ldg, nullptr, static_cast<int>(a.ldg) - 1, depth}, {a.xc, a.dim, nullptr, a.dim - 1, depth}, m0, n0, depth, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+  const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
+  const float f = count > 0 ? loss_factor(a) / kRaise<T> : 0.0f;
+#pragma unroll
+  for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int v = a.first + m0 + wm + 16 * i + 4 * g + x;
+      if (v >= a.last) continue;
+#pragma unroll
+      for (int j = 0; j < P::TN; ++j) {
+        const int col = n0 + wn + 16 * j + r;
+        if (col < a.dim) a.dw[v * a.ldw + col] = Io<T>::store(acc[i][j][x] * f);
+      }
+    }
+}
+
+// ---- host ----
+
+constexpr int kTile = 64;        // rows and columns of a workgroup's tile
+constexpr int kLeastPiece = 256;
+constexpr int64_t kPieceValues = int64_t{1} << 27;  // of g: 256 MB
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+fh_status check_loss(const std::string& fn, const fh_vocab_loss* g) {
+  if (g == nullptr) return fail(FH_INVALID_ARGUMENT, fn + ": null geometry");
+  if (g->dtype != FH_BF16 && g->dtype != FH_F16) return fail(FH_UNIMPLEMENTED, fn + ": dtype must be bf16 or f16");
+  if (g->loss_dtype != FH_F32 && g->loss_dtype != g->dtype) return fail(FH_INVALID_ARGUMENT, fn + ": loss_dtype must be f32 or dtype");
+  if (g->mean != 0 && g->mean != 1) return fail(FH_INVALID_ARGUMENT, fn + ": mean must be 0 or 1");
+  if (g->tokens < 0 || g->vocab < 1 || g->dim < 8) return fail(FH_INVALID_ARGUMENT, fn + ": bad tokens, vocab or dim");
+  if (g->dim % 8 != 0) return fail(FH_UNIMPLEMENTED, fn + ": dim must be a multiple of 8");
+  // tiles are counted in 32 bits
+  if (g->tokens > (1 << 24) || g->vocab > (1 << 24) || g->dim > (1 << 20) ||
+      up(g->tokens, kTile) / kTile * (up(std::max(g->vocab, g->dim), kTile) / kTile) > 0x7fffffff)
+    return fail(FH_INVALID_ARGUMENT, fn + ": too large");
+  for (int64_t ld : {g->x_stride, g->w_stride})
+    if (ld < g->dim || ld % 8 != 0 || ld > (int64_t{1} << 32))
+      return fail(FH_INVALID_ARGUMENT, fn + ": strides must be multiples of 8, dim at least");
+  return FH_OK;
+}
+
+struct Room {
+  int64_t bytes = 0;
+  int64_t take(int64_t n) {
+    const int64_t at = bytes;
+    bytes += up(n, 256);
+    return at;
+  }
+};
+struct ForwardRoom {
+  int64_t count, rows, at_target, part, bytes;
+};
+ForwardRoom forward_room(const fh_vocab_loss& g) {
+  Room r;
+  ForwardRoom f{};
+  f.count = r.take(4);
+  f.rows = r.take(4 * g.tokens);
+  f.at_target = r.take(4 * g.tokens);
+  f.part = r.take(8 * g.tokens * (up(g.vocab, kTile) / kTile));
+  f.bytes = r.bytes;
+  return f;
+}
+struct GradRoom {
+  int64_t count, rows, targets, lse, xc, dx_sum, g, bytes;
+  int64_t g_rows;
+};
+// with a piece of `columns`
+GradRoom grad_room(const fh_vocab_loss& g, int64_t columns) {
+  Room r;
+  GradRoom f{};
+  f.g_rows = up(g.tokens, 256);
+  f.count = r.take(4);
+  f.rows = r.take(4 * g.tokens);
+  f.targets = r.take(4 * g.tokens);
+  f.lse = r.take(4 * g.tokens);
+  f.xc = r.take(2 * f.g_rows * g.dim);
+  f.dx_sum = r.take(columns < g.vocab ? 4 * g.tokens * g.dim : 0);
+  f.g = r.take(2 * f.g_rows * columns);
+  f.bytes = r.bytes;
+  return f;
+}
+int64_t best_piece(const fh_vocab_loss& g) {
+  const int64_t all = up(g.vocab, kLeastPiece), rows = up(std::max<int64_t>(g.tokens, 1), 256);
+  return std::min(all, std::max<int64_t>(kPieceValues / rows / kLeastPiece * kLeastPiece, kLeastPiece));
+}
+// (one piece needs no sums between pieces)
+int64_t least_room(const fh_vocab_loss& g) { return std::min(grad_room(g, kLeastPiece).bytes, grad_room(g, best_piece(g)).bytes); }
+
+LossArgs loss_args(const fh_vocab_loss& g, const void* x, const void* w, const int32_t* targets) {
+  LossArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.w = static_cast<const uint16_t*>(w);
+  a.targets = targets;
+  a.ldx = g.x_stride;
+  a.ldw = g.w_stride;
+  a.tokens = static_cast<int>(g.tokens);
+  a.vocab = static_cast<int>(g.vocab);
+  a.dim = static_cast<int>(g.dim);
+  a.mean = g.mean;
+  a.loss_dtype = g.loss_dtype;
+  return a;
+}
+
+template <typename F>
+fh_status by_type(int32_t dtype, F&& f) {
+  return dtype == FH_BF16 ? f.template operator()<bf16_t>() : f.template operator()<f16_t>();
+}
+
+}  // namespace
+}  // namespace fh
+
+using namespace fh;
+
+extern "C" int64_t fh_vocab_loss_workspace(const fh_vocab_loss* g) {
+  if (check_loss("fh_vocab_loss_workspace", g) != FH_OK) return -1;
+  return forward_room(*g).bytes;
+}
+
+extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, const void* w, const int32_t* targets, void* loss,
+                                       float* row_loss, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  const std::string fn = "fh_vocab_loss_fwd";
+  if (fh_status st = check_loss(fn, g); st != FH_OK) return st;
+  if (!loss || !workspace || (g->tokens > 0 && (!x || !w || !targets || !lse))) return fail(FH_INVALID_ARGUMENT, fn + ": null pointer");
+  if (!aligned16(x) || !aligned16(w) || !aligned16(workspace))
+    return fail(FH_INVALID_ARGUMENT, fn + ": x, w and the workspace must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(targets) | reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(row_loss)) % 4 != 0 ||
+      reinterpret_cast<uintptr_t>(loss) % dtype_size(g->loss_dtype) != 0)
+    return fail(FH_INVALID_ARGUMENT, fn + ": targets, loss, row_loss and lse must be aligned to their elements");
+  const ForwardRoom room = forward_room(*g);
+  if (workspace_bytes < room.bytes) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
+  char* ws = static_cast<char*>(workspace);
+  LossArgs a = loss_args(*g, x, w, targets);
+  a.loss = loss;
+  a.row_loss = row_loss;
+  a.lse = lse;
+  a.count = reinterpret_cast<int*>(ws + room.count);
+  a.rows = reinterpret_cast<int32_t*>(ws + room.rows);
+  a.at_target = reinterpret_cast<float*>(ws + room.at_target);
+  a.part = reinterpret_cast<float2*>(ws + room.part);
+  a.tiles_n = static_cast<int>(up(g->vocab, kTile) / kTile);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, s, a);
+  if (fh_status st = launch_status("loss_rows_kernel launch"); st != FH_OK) return st;
+  if (g->tokens > 0) {
+    const fh_status st = by_type(g->dtype, [&]<typename T>() {
+      hipLaunchKernelGGL((loss_logits_kernel<T, kTile, kTile, 2, 2>), dim3(static_cast<uint32_t>(up(g->tokens, kTile) / kTile * a.tiles_n)),
+                         dim3(256), 0, s, a);
+      return launch_status("loss_logits_kernel launch");
+    });
+    if (st != FH_OK) return st;
+    hipLaunchKernelGGL(loss_join_kernel, dim3(static_cast<uint32_t>((g->tokens + 15) / 16)), dim3(256), 0, s, a);
+    if (fh_status st2 = launch_status("loss_join_kernel launch"); st2 != FH_OK) return st2;
+  }
+  hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, s, a);
+  return launch_status("loss_sum_kernel launch");
+}
+
+extern "C" int64_t fh_vocab_loss_grad_workspace(const fh_vocab_loss* g) {
+  if (check_loss("fh_vocab_loss_grad_workspace", g) != FH_OK) return -1;
+  return grad_room(*g, best_piece(*g)).bytes;
+}
+
+extern "C" int64_t fh_vocab_loss_grad_least(const fh_vocab_loss* g) {
+  if (check_loss("fh_vocab_loss_grad_least", g) != FH_OK) return -1;
+  return least_room(*g);
+}
+
+extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, const void* w, const int32_t* targets, const float* lse,
+                                        const void* dloss, void* dx, void* dw, void* workspace, int64_t workspace_bytes, void* stream) {
+  const std::string fn = "fh_vocab_loss_grad";
+  if (fh_status st = check_loss(fn, g); st != FH_OK) return st;
+  if (!dx && !dw) return FH_OK;
+  if (g->tokens == 0 && !dw) return FH_OK;
+  if (!workspace || !dloss || (g->tokens > 0 && (!x || !w || !targets || !lse))) return fail(FH_INVALID_ARGUMENT, fn + ": null pointer");
+  for (const void* p : {x, w, static_cast<const void*>(dx), static_cast<const void*>(dw), static_cast<const void*>(workspace)})
+    if (!aligned16(p)) return fail(FH_INVALID_ARGUMENT, fn + ": tensors and the workspace must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(targets) | reinterpret_cast<uintptr_t>(lse)) % 4 != 0 ||
+      reinterpret_cast<uintptr_t>(dloss) % dtype_size(g->loss_dtype) != 0)
+    return fail(FH_INVALID_ARGUMENT, fn + ": targets, lse and dloss must be aligned to their elements");
+  // the widest piece, up to the best, that the workspace has room for
+  int64_t columns = best_piece(*g);
+  if (workspace_bytes < grad_room(*g, columns).bytes) {
+    const GradRoom least = grad_room(*g, kLeastPiece);
+    if (workspace_bytes < least.bytes) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
+    // room beside the sums between pieces, which a piece of the whole vocabulary would not need
+    columns = std::min(columns, (workspace_bytes - least.g) / (2 * least.g_rows) / kLeastPiece * kLeastPiece);
+    if (columns >= g->vocab) columns = up(g->vocab, kLeastPiece) - kLeastPiece;
+  }
+  const GradRoom room = grad_room(*g, columns);
+  char* ws = static_cast<char*>(workspace);
+  LossArgs a = loss_args(*g, x, w, targets);
+  a.lse = const_cast<float*>(lse);
+  a.dloss = dloss;
+  a.dx = static_cast<uint16_t*>(dx);
+  a.dw = static_cast<uint16_t*>(dw);
+  a.count = reinterpret_cast<int*>(ws + room.count);
+  a.rows = reinterpret_cast<int32_t*>(ws + room.rows);
+  a.targets_c = reinterpret_cast<int32_t*>(ws + room.targets);
+  a.lse_c = reinterpret_cast<float*>(ws + room.lse);
+  a.xc = reinterpret_cast<uint16_t*>(ws + room.xc);
+  a.dx_sum = reinterpret_cast<float*>(ws + room.dx_sum);
+  a.g = reinterpret_cast<uint16_t*>(ws + room.g);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, s, a);
+  if (fh_status st = launch_status("loss_rows_kernel launch"); st != FH_OK) return st;
+  if (g->tokens > 0) {
+    hipLaunchKernelGGL(loss_gather_kernel, dim3(static_cast<uint32_t>(up(g->tokens, 64) / 4)), dim3(256), 0, s, a);
+    if (fh_status st = launch_status("loss_gather_kernel launch"); st != FH_OK) return st;
+  }
+  const int64_t tiles_m = up(g->tokens, kTile) / kTile, tiles_d = up(g->dim, kTile) / kTile;
+  return by_type(g->dtype, [&]<typename T>() {
+    for (int64_t first = 0; first < g->vocab; first += columns) {
+      a.first = static_cast<int>(first);
+      a.last = static_cast<int>(std::min(g->vocab, first + columns));
+      a.first_piece = first == 0;
+      a.last_piece = a.last == g->vocab;
+      a.ldg = up(a.last - a.first, kLeastPiece);
+      const int64_t tiles_v = a.ldg / kTile;
+      if (g->tokens > 0) {
+        hipLaunchKernelGGL((loss_derivative_kernel<T, kTile, kTile, 2, 2>), dim3(static_cast<uint32_t>(tiles_m * tiles_v)), dim3(256), 0, s, a);
+        if (fh_status st = launch_status("loss_derivative_kernel launch"); st != FH_OK) return st;
+        if (dx) hipLaunchKernelGGL((loss_dx_kernel<T, kTile, kTile, 2, 2>), dim3(static_cast<uint32_t>(tiles_m * tiles_d)), dim3(256), 0, s, a);
+        if (fh_status st = launch_status("loss_dx_kernel launch"); st != FH_OK) return st;
+      }
+      if (dw) hipLaunchKernelGGL((loss_dw_kernel<T, kTile, kTile, 2, 2>), dim3(static_cast<uint32_t>(tiles_v * tiles_d)), dim3(256), 0, s, a);
+      if (fh_status st = launch_status("loss_dw_kernel launch"); st != FH_OK) return st;
+    }
+    return FH_OK;
+  });
+}
