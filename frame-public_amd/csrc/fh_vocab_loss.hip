@@ -14,12 +14,12 @@
 #include <string>
 
 #include "fh_common.h"
-#include "fh_mfma16.h"
+#include "fh_tile_product.h"
 
 namespace fh {
 namespace {
 
-using namespace mfma16;
+using namespace tile;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -57,71 +57,6 @@ struct LossArgs {
   int first_piece, last_piece;
 };
 
-// ---- one tile of a product ----
-
-// An operand of a tile's product, rows r (of the tile's dimension) by k. Not KMAJOR: element (r, k) = p[row(r) * ld + k], row(r) = rows[r]
-// or r, r clamped to `last`. KMAJOR: p[k * ld + r], chunks of 8 r clamped to end at `last`. Zeros from k = `depth` on.
-struct Operand {
-  const uint16_t* p;
-  int64_t ld;
-  const int32_t* rows;
-  int last, depth;
-};
-
-// A workgroup's BM x BN tile of A B^T over k < K, by WAVES_M x WAVES_N waves; the wave's lane l holds rows 16 i + 4 (l / 16) + x, columns
-// 16 j + l % 16 of its part.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool AK, bool BK_>
-struct Tile {
-  static constexpr int NT = WAVES_M * WAVES_N * 64;
-  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 16, TN = WN / 16;
-  static constexpr int LD = kBK + 8;
-  static constexpr int LDS = (BM + BN) * LD * 2;
-
-  template <int R, bool KMAJOR>
-  __device__ static void stage(uint16_t* to, const Operand& o, int r0, int k0) {
-    for (int i = threadIdx.x; i < R * 4; i += NT) {
-      u32x4_t v{0, 0, 0, 0};
-      if constexpr (KMAJOR) {
-        const int k = i / (R / 8), c = i % (R / 8) * 8;
-        if (k0 + k < o.depth) v = *reinterpret_cast<const u32x4_t*>(o.p + static_cast<int64_t>(k0 + k) * o.ld + min(r0 + c, o.last - 7));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) to[(c + e) * LD + k] = static_cast<uint16_t>(v[e / 2] >> (16 * (e & 1)));
-      } else {
-        const int r = min(r0 + i / 4, o.last), k = i % 4 * 8;
-        const int64_t row = o.rows != nullptr ? o.rows[r] : r;
-        if (k0 + k < o.depth) v = *reinterpret_cast<const u32x4_t*>(o.p + row * o.ld + k0 + k);
-        *reinterpret_cast<u32x4_t*>(to + (i / 4) * LD + k) = v;
-      }
-    }
-  }
-
-  __device__ static void product(unsigned char* lds, const Operand& a, const Operand& b, int m0, int n0, int K, f32x4_t (&acc)[TM][TN]) {
-    uint16_t* as = reinterpret_cast<uint16_t*>(lds);
-    uint16_t* bs = as + BM * LD;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / WAVES_N * WM, wn = wave % WAVES_N * WN;
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = 0; k0 < K; k0 += kBK) {
-      __syncthreads();
-      stage<BM, AK>(as, a, m0, k0);
-      stage<BN, BK_>(bs, b, n0, k0);
-      __syncthreads();
-      u32x4_t fa[TM], fb[TN];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const u32x4_t*>(as + (wm + 16 * i + (lane & 15)) * LD + 8 * (lane >> 4));
-#pragma unroll
-      for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const u32x4_t*>(bs + (wn + 16 * j + (lane & 15)) * LD + 8 * (lane >> 4));
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) mfma16x<T>(fa[i], fb[j], acc[i][j]);
-    }
-  }
-};
-
 // max and sum over the 16 lanes that share rows of a tile
 __device__ __forceinline__ float max16(float v) {
 #pragma unroll
@@ -138,8 +73,8 @@ __device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.0f 
 
 // ---- rows with a target ----
 
-// By one workgroup: the list of rows with a target and their number; the others' outputs. In the gradients (lse_c) also their targets
-// and log-sum-exps.
+// By one workgroup: the list of rows with a target, their number and targets; the others' outputs, or (gradients: lse_c) the
+// log-sum-exps.
 __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a) {
   __shared__ int waves[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -161,10 +96,8 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a) {
   for (int t = begin; t < end; ++t) {
     if (has(t)) {
       a.rows[at] = t;
-      if (a.lse_c != nullptr) {
-        a.targets_c[at] = a.targets[t];
-        a.lse_c[at] = a.lse[t];
-      }
+      a.targets_c[at] = a.targets[t];
+      if (a.lse_c != nullptr) a.lse_c[at] = a.lse[t];
       ++at;
     } else if (a.lse_c == nullptr) {
       a.lse[t] = 0.0f;
@@ -177,40 +110,38 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a) {
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(const LossArgs a) {
-  using P = Tile<T, BM, BN, WAVES_M, WAVES_N, false, false>;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::LDS];
-  __shared__ float2 joined[WAVES_N][BM];
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, false, false, true, true>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
-  const int tiles_m = (a.tokens + BM - 1) / BM;
-  const int m0 = static_cast<int>(blockIdx.x % tiles_m) * BM, tn = static_cast<int>(blockIdx.x / tiles_m), n0 = tn * BN;
-  if (m0 >= count) return;
-  f32x4_t acc[P::TM][P::TN];
-  P::product(lds, {a.x, a.ldx, a.rows, count - 1, a.dim}, {a.w, a.ldw, nullptr, a.vocab - 1, a.dim}, m0, n0, a.dim, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-  const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
+  int tm, tn;
+  if (!place(blockIdx.x, (count + BM - 1) / BM, a.tiles_n, tm, tn)) return;
+  const int m0 = tm * BM, n0 = tn * BN;
+  typename P::Acc acc;
+  P::run(lds, {a.x, a.ldx, a.rows, count - 1, a.dim}, {a.w, a.ldw, nullptr, a.vocab - 1, a.dim}, m0, n0, (a.dim + kBK - 1) / kBK, acc);
+  float2(*joined)[BM] = reinterpret_cast<float2(*)[BM]>(lds);
+  const int g = P::lane() >> 4, r = P::lane() & 15, row0 = P::wave_row(), col0 = n0 + P::wave_column() + r;
 #pragma unroll
   for (int i = 0; i < P::TM; ++i)
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int row = wm + 16 * i + 4 * g + x, m = m0 + row;
-      const int target = a.targets[a.rows[min(m, count - 1)]];
+      const int row = row0 + 16 * i + 4 * g + x, m = m0 + row;
+      const int target = a.targets_c[min(m, count - 1)];
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < P::TN; ++j) {
-        const int col = n0 + wn + 16 * j + r;
-        if (col < a.vocab) top = fmaxf(top, acc[i][j][x]);
-        if (col == target && m < count) a.at_target[m] = acc[i][j][x];
+        if (col0 + 16 * j < a.vocab) top = fmaxf(top, acc[i][j][x]);
+        if (col0 + 16 * j == target && m < count) a.at_target[m] = acc[i][j][x];
       }
       top = max16(top);
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < P::TN; ++j)
-        if (n0 + wn + 16 * j + r < a.vocab) sum += __builtin_amdgcn_exp2f((acc[i][j][x] - origin(top)) * kLog2e);
+        if (col0 + 16 * j < a.vocab) sum += __builtin_amdgcn_exp2f((acc[i][j][x] - origin(top)) * kLog2e);
       sum = sum16(sum);
-      if (r == 0) joined[wave % WAVES_N][row] = float2{top, sum};
+      if (r == 0) joined[P::wave() % WAVES_N][row] = float2{top, sum};
     }
   __syncthreads();
-  for (int row = threadIdx.x; row < BM; row += P::NT) {
+  for (int row = threadIdx.x; row < BM; row += P::kThreads) {
     if (m0 + row >= count) break;
     float top = joined[0][row].x, sum = 0.0f;
     for (int w = 1; w < WAVES_N; ++w) top = fmaxf(top, joined[w][row].x);
@@ -288,100 +219,100 @@ __device__ __forceinline__ float loss_factor(const LossArgs& a) {
   return a.mean ? d / static_cast<float>(*a.count) : d;
 }
 
-// g of a piece: columns first .. last - 1 of the vocabulary, zeros behind them and in rows without one up to the tile's end.
+// g of a piece: columns first .. last - 1 of the vocabulary, zeros behind them and in the tile's rows that no row with a target is.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(const LossArgs a) {
-  using P = Tile<T, BM, BN, WAVES_M, WAVES_N, false, false>;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::LDS];
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, false, false, true, true>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
-  const int tiles_m = (a.tokens + BM - 1) / BM;
-  const int m0 = static_cast<int>(blockIdx.x % tiles_m) * BM, n0 = static_cast<int>(blockIdx.x / tiles_m) * BN;
-  if (m0 >= count) return;
-  f32x4_t acc[P::TM][P::TN];
-  P::product(lds, {a.xc, a.dim, nullptr, count - 1, a.dim}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.vocab - 1 - a.first, a.dim}, m0, n0, a.dim, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-  const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
+  int tm, tn;
+  if (!place(blockIdx.x, (count + BM - 1) / BM, static_cast<int>(a.ldg / BN), tm, tn)) return;
+  const int m0 = tm * BM, n0 = tn * BN;
+  typename P::Acc acc;
+  P::run(lds, {a.xc, a.dim, nullptr, count - 1, a.dim}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.vocab - 1 - a.first, a.dim}, m0, n0,
+         (a.dim + kBK - 1) / kBK, acc);
+  const int g = P::lane() >> 4, r = P::lane() & 15;
+  const int row0 = m0 + P::wave_row() + 4 * g, col0 = a.first + n0 + P::wave_column() + r;
+  float lse[P::TM][4];
+  int target[P::TM][4];
 #pragma unroll
   for (int i = 0; i < P::TM; ++i)
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int m = m0 + wm + 16 * i + 4 * g + x, mc = min(m, count - 1);
-      const float lse = a.lse_c[mc];
-      const int target = a.targets_c[mc];
-#pragma unroll
-      for (int j = 0; j < P::TN; ++j) {
-        const int col = n0 + wn + 16 * j + r, v = a.first + col;
-        float d = __builtin_amdgcn_exp2f((acc[i][j][x] - lse) * kLog2e) - (v == target ? 1.0f : 0.0f);
-        if (m >= count || v >= a.last) d = 0.0f;
-        a.g[static_cast<int64_t>(m) * a.ldg + col] = Io<T>::store(d * kRaise<T>);
-      }
+      const int m = min(row0 + 16 * i + x, count - 1);
+      lse[i][x] = a.lse_c[m];
+      target[i][x] = a.targets_c[m];
     }
+  P::store(
+      lds,
+      [&](int i, int x, int j) {
+        const int v = col0 + 16 * j;
+        const float d = __builtin_amdgcn_exp2f((acc[i][j][x] - lse[i][x]) * kLog2e) - (v == target[i][x] ? 1.0f : 0.0f);
+        return row0 + 16 * i + x < count && v < a.last ? d * kRaise<T> : 0.0f;
+      },
+      [&](int row, int c, const u32x4_t& v) { *reinterpret_cast<u32x4_t*>(a.g + static_cast<int64_t>(m0 + row) * a.ldg + n0 + c) = v; });
 }
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const LossArgs a) {
-  using P = Tile<T, BM, BN, WAVES_M, WAVES_N, false, true>;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::LDS];
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, false, true, false, true>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
-  const int tiles_m = (a.tokens + BM - 1) / BM;
-  const int m0 = static_cast<int>(blockIdx.x % tiles_m) * BM, n0 = static_cast<int>(blockIdx.x / tiles_m) * BN;
-  if (m0 >= count) return;
-  const int depth = a.last - a.first;
-  f32x4_t acc[P::TM][P::TN];
-  P::product(lds, {a.g, a.ldg, nullptr, count - 1, static_cast<int>(a.ldg)}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.dim - 1, depth}, m0, n0, depth, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-  const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
-  const float f = loss_factor(a) / kRaise<T>;
+  int tm, tn;
+  if (!place(blockIdx.x, (count + BM - 1) / BM, (a.dim + BN - 1) / BN, tm, tn)) return;
+  const int m0 = tm * BM, n0 = tn * BN, depth = a.last - a.first;
+  typename P::Acc acc;
+  P::run(lds, {a.g, a.ldg, nullptr, count - 1, depth}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.dim - 1, depth}, m0, n0,
+         (depth + kBK - 1) / kBK, acc);
+  const int g = P::lane() >> 4, r = P::lane() & 15;
+  const int row0 = m0 + P::wave_row() + 4 * g, col0 = n0 + P::wave_column() + r;
+  if (!a.first_piece || !a.last_piece) {
 #pragma unroll
-  for (int i = 0; i < P::TM; ++i)
+    for (int i = 0; i < P::TM; ++i)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int m = m0 + wm + 16 * i + 4 * g + x;
-      if (m >= count) continue;
+      for (int x = 0; x < 4; ++x) {
+        const int m = row0 + 16 * i + x;
+        if (m >= count) continue;
+        float* sum = a.dx_sum + static_cast<int64_t>(m) * a.dim + col0;
 #pragma unroll
-      for (int j = 0; j < P::TN; ++j) {
-        const int col = n0 + wn + 16 * j + r;
-        if (col >= a.dim) continue;
-        float v = acc[i][j][x];
-        float* sum = a.dx_sum + static_cast<int64_t>(m) * a.dim + col;
-        if (!a.first_piece) v += *sum;
-        if (a.last_piece)
-          a.dx[a.rows[m] * a.ldx + col] = Io<T>::store(v * f);
-        else
-          *sum = v;
+        for (int j = 0; j < P::TN; ++j) {
+          if (col0 + 16 * j >= a.dim) continue;
+          if (!a.first_piece) acc[i][j][x] += sum[16 * j];
+          if (!a.last_piece) sum[16 * j] = acc[i][j][x];
+        }
       }
-    }
+  }
+  if (!a.last_piece) return;
+  const float f = loss_factor(a) / kRaise<T>;
+  P::store(
+      lds, [&](int i, int x, int j) { return acc[i][j][x] * f; },
+      [&](int row, int c, const u32x4_t& v) {
+        if (m0 + row < count && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dx + a.rows[m0 + row] * a.ldx + n0 + c) = v;
+      });
 }
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const LossArgs a) {
-  using P = Tile<T, BM, BN, WAVES_M, WAVES_N, true, true>;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::LDS];
-  const int count = *a.count, depth = (count + kBK - 1) / kBK * kBK;
-  const int tiles_n = (a.dim + BN - 1) / BN;
-  const int n0 = static_cast<int>(blockIdx.x % tiles_n) * BN, m0 = static_cast<int>(blockIdx.x / tiles_n) * BM;
-  f32x4_t acc[P::TM][P::TN];
-  P::product(lds, {a.g, a.ldg, nullptr, static_cast<int>(a.ldg) - 1, depth}, {a.xc, a.dim, nullptr, a.dim - 1, depth}, m0, n0, depth, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-  const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, true, true, false, false>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
+  const int count = *a.count;
+  int tm, tn;
+  if (!place(blockIdx.x, static_cast<int>((a.last - a.first + BM - 1) / BM), (a.dim + BN - 1) / BN, tm, tn)) return;
+  const int m0 = tm * BM, n0 = tn * BN;
+  typename P::Acc acc;
+  P::run(lds, {a.g, a.ldg, nullptr, static_cast<int>(a.ldg) - 1, 0}, {a.xc, a.dim, nullptr, a.dim - 1, 0}, m0, n0, (count + kBK - 1) / kBK, acc);
   const float f = count > 0 ? loss_factor(a) / kRaise<T> : 0.0f;
-#pragma unroll
-  for (int i = 0; i < P::TM; ++i)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int v = a.first + m0 + wm + 16 * i + 4 * g + x;
-      if (v >= a.last) continue;
-#pragma unroll
-      for (int j = 0; j < P::TN; ++j) {
-        const int col = n0 + wn + 16 * j + r;
-        if (col < a.dim) a.dw[v * a.ldw + col] = Io<T>::store(acc[i][j][x] * f);
-      }
-    }
+  P::store(
+      lds, [&](int i, int x, int j) { return acc[i][j][x] * f; },
+      [&](int row, int c, const u32x4_t& v) {
+        const int64_t to = a.first + m0 + row;
+        if (to < a.last && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dw + to * a.ldw + n0 + c) = v;
+      });
 }
 
 // ---- host ----
 
-constexpr int kTile = 64;        // rows and columns of a workgroup's tile
+constexpr int kTile = 64;  // the smallest tile's rows and columns
 constexpr int kLeastPiece = 256;
 constexpr int64_t kPieceValues = int64_t{1} << 27;  // of g: 256 MB
 
@@ -397,12 +328,35 @@ fh_status check_loss(const std::string& fn, const fh_vocab_loss* g) {
   if (g->dim % 8 != 0) return fail(FH_UNIMPLEMENTED, fn + ": dim must be a multiple of 8");
   // tiles are counted in 32 bits
   if (g->tokens > (1 << 24) || g->vocab > (1 << 24) || g->dim > (1 << 20) ||
-      up(g->tokens, kTile) / kTile * (up(std::max(g->vocab, g->dim), kTile) / kTile) > 0x7fffffff)
+      up(g->tokens, kTile) / kTile * (up(std::max(g->vocab, g->dim), kLeastPiece) / kTile) > 0x7fffffff)
     return fail(FH_INVALID_ARGUMENT, fn + ": too large");
   for (int64_t ld : {g->x_stride, g->w_stride})
     if (ld < g->dim || ld % 8 != 0 || ld > (int64_t{1} << 32))
       return fail(FH_INVALID_ARGUMENT, fn + ": strides must be multiples of 8, dim at least");
   return FH_OK;
+}
+
+// The tile of a product of m rows and n columns: the largest that gives (nearly) every CU a workgroup, as in fh_gemm16.hip.
+struct Shape {
+  int m, n;
+};
+Shape tile_for(int64_t m, int64_t n) {
+  const int64_t cus = device_cu_count();
+  auto tiles = [&](int64_t bm, int64_t bn) { return up(m, bm) / bm * (up(n, bn) / bn); };
+  if (m >= 256 && n >= 256 && tiles(256, 256) * 4 >= cus * 3) return {256, 256};
+  if (m >= 128 && n >= 128 && tiles(128, 128) >= cus) return {128, 128};
+  if (n >= 128 && tiles(64, 128) >= cus) return {64, 128};
+  return {64, 64};
+}
+// launch<BM, BN, WAVES_M, WAVES_N>(workgroups) with the tile of m x n
+template <typename F>
+void by_tile(int64_t m, int64_t n, F&& launch) {
+  const Shape t = tile_for(m, n);
+  const dim3 grid(static_cast<uint32_t>(up(m, t.m) / t.m * (up(n, t.n) / t.n)));
+  if (t.m == 256) launch.template operator()<256, 256, 4, 2>(grid);
+  else if (t.m == 128) launch.template operator()<128, 128, 2, 4>(grid);
+  else if (t.n == 128) launch.template operator()<64, 128, 2, 2>(grid);
+  else launch.template operator()<64, 64, 2, 2>(grid);
 }
 
 struct Room {
@@ -414,15 +368,19 @@ struct Room {
   }
 };
 struct ForwardRoom {
-  int64_t count, rows, at_target, part, bytes;
+  int64_t count, rows, targets, at_target, part, bytes;
+  int64_t tiles_n;
 };
 ForwardRoom forward_room(const fh_vocab_loss& g) {
   Room r;
   ForwardRoom f{};
   f.count = r.take(4);
   f.rows = r.take(4 * g.tokens);
+  f.targets = r.take(4 * g.tokens);
   f.at_target = r.take(4 * g.tokens);
-  f.part = r.take(8 * g.tokens * (up(g.vocab, kTile) / kTile));
+  const int64_t columns = tile_for(g.tokens, g.vocab).n;
+  f.tiles_n = up(g.vocab, columns) / columns;
+  f.part = r.take(8 * g.tokens * f.tiles_n);
   f.bytes = r.bytes;
   return f;
 }
@@ -503,14 +461,16 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
   a.rows = reinterpret_cast<int32_t*>(ws + room.rows);
   a.at_target = reinterpret_cast<float*>(ws + room.at_target);
   a.part = reinterpret_cast<float2*>(ws + room.part);
-  a.tiles_n = static_cast<int>(up(g->vocab, kTile) / kTile);
+  a.targets_c = reinterpret_cast<int32_t*>(ws + room.targets);
+  a.tiles_n = static_cast<int>(room.tiles_n);
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, s, a);
   if (fh_status st = launch_status("loss_rows_kernel launch"); st != FH_OK) return st;
   if (g->tokens > 0) {
     const fh_status st = by_type(g->dtype, [&]<typename T>() {
-      hipLaunchKernelGGL((loss_logits_kernel<T, kTile, kTile, 2, 2>), dim3(static_cast<uint32_t>(up(g->tokens, kTile) / kTile * a.tiles_n)),
-                         dim3(256), 0, s, a);
+      by_tile(g->tokens, g->vocab, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+        hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
+      });
       return launch_status("loss_logits_kernel launch");
     });
     if (st != FH_OK) return st;
@@ -573,7 +533,6 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
     hipLaunchKernelGGL(loss_gather_kernel, dim3(static_cast<uint32_t>(up(g->tokens, 64) / 4)), dim3(256), 0, s, a);
     if (fh_status st = launch_status("loss_gather_kernel launch"); st != FH_OK) return st;
   }
-  const int64_t tiles_m = up(g->tokens, kTile) / kTile, tiles_d = up(g->dim, kTile) / kTile;
   return by_type(g->dtype, [&]<typename T>() {
     for (int64_t first = 0; first < g->vocab; first += columns) {
       a.first = static_cast<int>(first);
@@ -581,14 +540,21 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
       a.first_piece = first == 0;
       a.last_piece = a.last == g->vocab;
       a.ldg = up(a.last - a.first, kLeastPiece);
-      const int64_t tiles_v = a.ldg / kTile;
       if (g->tokens > 0) {
-        hipLaunchKernelGGL((loss_derivative_kernel<T, kTile, kTile, 2, 2>), dim3(static_cast<uint32_t>(tiles_m * tiles_v)), dim3(256), 0, s, a);
+        by_tile(g->tokens, a.ldg, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+          hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
+        });
         if (fh_status st = launch_status("loss_derivative_kernel launch"); st != FH_OK) return st;
-        if (dx) hipLaunchKernelGGL((loss_dx_kernel<T, kTile, kTile, 2, 2>), dim3(static_cast<uint32_t>(tiles_m * tiles_d)), dim3(256), 0, s, a);
+        if (dx)
+          by_tile(g->tokens, g->dim, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+            hipLaunchKernelGGL((loss_dx_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
+          });
         if (fh_status st = launch_status("loss_dx_kernel launch"); st != FH_OK) return st;
       }
-      if (dw) hipLaunchKernelGGL((loss_dw_kernel<T, kTile, kTile, 2, 2>), dim3(static_cast<uint32_t>(tiles_v * tiles_d)), dim3(256), 0, s, a);
+      if (dw)
+        by_tile(a.last - a.first, g->dim, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+          hipLaunchKernelGGL((loss_dw_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
+        });
       if (fh_status st = launch_status("loss_dw_kernel launch"); st != FH_OK) return st;
     }
     return FH_OK;

@@ -113,6 +113,9 @@ SHAPES = [  # tokens, vocab, dim, share of rows without a target, mean, pad
     (64, 64, 64, 0.0, 0, 0), (65, 65, 72, 0.0, 1, 0), (33, 257, 24, 0.5, 0, 16), (130, 1000, 128, 0.1, 1, 0), (256, 256, 256, 0.0, 1, 0),
     (257, 511, 264, 0.0, 1, 0), (333, 2003, 200, 0.4, 1, 8), (700, 300, 96, 0.2, 0, 0), (16, 3001, 1000, 0.0, 1, 0), (600, 1500, 512, 0.0, 1, 0),
     (1100, 1025, 136, 0.9, 1, 0),
+    # the larger tiles: of logits, of dx and dw, of both, and few rows of many columns
+    (2048, 8197, 40, 0.1, 1, 0), (2100, 2051, 6152, 0.3, 1, 0), (300, 11003, 24, 0.0, 1, 0), (800, 900, 5000, 0.0, 1, 0),
+    (60, 40000, 16, 0.0, 1, 0), (5, 70, 33000, 0.0, 1, 0),
 ]
 
 
