@@ -1,11 +1,13 @@
 // One workgroup's tile of a 16-bit matrix product A B^T with operands in either storage order, fp32 accumulation on
 // v_mfma_f32_16x16x32_{bf16,f16}: the main loop of kernels whose epilogue is not a stored matrix (fh_vocab_loss.hip).
 //
-// The data path is fh_gemm16.hip's (a ring of four LDS stages of 32 k that global_load_lds fills three stages ahead, XOR-swizzled chunks,
-// fragment reads between the products in fixed program order, one barrier per stage) with either operand in either order:
-//   rows:      element (r, k) at p[row(r) * ld + k]. A stage is [rows][32 k], 64 bytes a row; a fragment (8 k of one row per lane) is one
-//              ds_read_b128. row(r) may come from a list.
-//   columns:   element (r, k) at p[k * ld + r]. A stage is [32 k][rows], kept as in memory; a fragment is two transposing reads of 4 k each
+// A stage is 64 k of both operands. global_load_lds fills a ring of stages (16 bytes a lane, no registers between), chunks XOR-swizzled so
+// that the fragments' reads meet no bank twice; the reads and the loads stand between the products in fixed program order; one barrier
+// per stage. Either operand comes in either order:
+//   rows:      element (r, k) at p[row(r) * ld + k]. In LDS [rows][64 k], 128 bytes a row: a whole cache line per row and stage (with 64 bytes
+//              each line went from L2 to the CU twice, at 64 bytes a clock all that it has for two such operands). A fragment (8 k
+//              of one row per lane) is one ds_read_b128. row(r) may come from a list.
+//   columns:   element (r, k) at p[k * ld + r]. In LDS [64 k][rows], as in memory; a fragment is two transposing reads of 4 k each
 //              (ds_read_b64_tr_b16).
 #pragma once
 
@@ -20,6 +22,9 @@ namespace fh {
 namespace tile {
 
 using namespace mfma16;
+
+constexpr int kDepth = 64;  // k of a stage: two steps of 32
+constexpr int kStep = 32;
 
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 
@@ -63,26 +68,29 @@ __device__ __forceinline__ void tie(Fragments<TX, C>& f) {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// The swizzle of a row's 16-byte chunks (row order): two rows share the banks' 256 bytes, so rows 2 apart must differ.
+__device__ __forceinline__ int row_swizzle(int row) { return (row >> 1) & 7; }
+
 // One operand's way: R rows of the tile by NW waves' loads, TX blocks of 16 rows read by each wave. UNEVEN: the depth may end inside a stage.
 template <int R, int TX, bool COLUMNS, bool UNEVEN, int NW>
 struct Feed {
-  static constexpr int kBytes = R * kBK * 2;
+  static constexpr int kBytes = R * kDepth * 2;
   static constexpr int kLoads = kBytes / 1024 / NW;  // load instructions per wave and stage
   static constexpr int kChunks = R / 8;              // column order: 16-byte chunks of a row of k
   static_assert(kBytes / 1024 % NW == 0, "a stage's loads split evenly over the waves");
   static_assert(!COLUMNS || (kChunks >= 8 && kChunks <= 64), "rows in [64, 512]");
 
   const uint16_t* src[kLoads];
-  int64_t step;        // elements from a stage to the next
-  int first[kLoads];   // the lane's first k in a stage
+  int64_t step;       // elements from a stage to the next
+  int first[kLoads];  // the lane's first k in a stage
   int depth;
-  int off[COLUMNS ? TX : 1];  // where the lane reads, bytes within a stage
+  int off[COLUMNS ? TX : 2];  // where the lane reads, bytes within a stage: per block, or per step of 32 k
 
   // r0: the tile's first row; mine: the wave's first row in the tile
   __device__ __forceinline__ void init(const Operand& o, int r0, int mine, int wave, int lane) {
     depth = o.depth;
     if constexpr (COLUMNS) {
-      step = kBK * o.ld;
+      step = kDepth * o.ld;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int k = (wave * kLoads + j) * (64 / kChunks) + lane / kChunks;
@@ -98,58 +106,61 @@ struct Feed {
         off[i] = k * (R * 2) + ((row >> 3) ^ b_swizzle16<kChunks>(k)) * 16 + (row & 7) * 2;
       }
     } else {
-      step = kBK;
+      step = kDepth;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int in_tile = (wave * kLoads + j) * 16 + (lane >> 2), row = min(r0 + in_tile, o.last);
-        const int chunk = (lane & 3) ^ a_swizzle(in_tile);
+        const int in_tile = (wave * kLoads + j) * 8 + (lane >> 3), row = min(r0 + in_tile, o.last);
+        const int chunk = (lane & 7) ^ row_swizzle(in_tile);
         first[j] = chunk * 8;
         src[j] = o.p + static_cast<int64_t>(o.rows != nullptr ? o.rows[row] : row) * o.ld + chunk * 8;
       }
       const int row = mine + (lane & 15);
-      off[0] = row * 64 + (((lane >> 4) ^ a_swizzle(row)) * 16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) off[h] = row * (kDepth * 2) + (((lane >> 4) + 4 * h) ^ row_swizzle(row)) * 16;
     }
   }
   // load instruction J of stage kt to this operand's part of a stage
   template <int J>
   __device__ __forceinline__ void load(int kt, unsigned char* to, int wave) const {
     const uint16_t* from = src[J] + kt * step;
-    if constexpr (UNEVEN) from = first[J] < depth - kt * kBK ? from : reinterpret_cast<const uint16_t*>(&kZeros);
+    if constexpr (UNEVEN) from = first[J] < depth - kt * kDepth ? from : reinterpret_cast<const uint16_t*>(&kZeros);
     global_to_lds16(from, (FH_LDS void*)(to + (wave * kLoads + J) * 1024));
   }
-  // read instruction N of blocks I0, I0 + 1, .. of the stage part at `base`
-  template <int N, int I0, int TF>
+  // read instruction N of blocks I0, I0 + 1, .. for step H of the stage part at `base`
+  template <int N, int I0, int H, int TF>
   __device__ __forceinline__ void read(uint32_t base, Fragments<TF, COLUMNS>& f) const {
     if constexpr (COLUMNS) {
       if constexpr (N % 2 == 0)
-        f.low[N / 2] = lds_read_tr16_b64<0>(base + off[I0 + N / 2]);
+        f.low[N / 2] = lds_read_tr16_b64<H * kStep * R * 2>(base + off[I0 + N / 2]);
       else
-        f.high[N / 2] = lds_read_tr16_b64<4 * R * 2>(base + off[I0 + N / 2]);
+        f.high[N / 2] = lds_read_tr16_b64<(H * kStep + 4) * R * 2>(base + off[I0 + N / 2]);
     } else {
-      f.v[N] = lds_read_b128<(I0 + N) * 1024>(base + off[0]);
+      f.v[N] = lds_read_b128<(I0 + N) * 16 * kDepth * 2>(base + off[H]);
     }
   }
 };
 
-// The BM x BN tile at (m0, n0) of A B^T over k < 32 KT, by WAVES_M x WAVES_N waves. A wave's part begins at row WM (wave / WAVES_N), column
+// The BM x BN tile at (m0, n0) of A B^T over k < 64 KT, by WAVES_M x WAVES_N waves. A wave's part begins at row WM (wave / WAVES_N), column
 // WN (wave % WAVES_N); its lane l holds rows 16 i + 4 (l / 16) + x and column 16 j + l % 16 of it in acc[i][j][x]. On return all of the
 // workgroup's waves are past their last use of `lds` (kLds bytes, 1 KB aligned).
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool A_COLUMNS, bool B_COLUMNS, bool A_UNEVEN, bool B_UNEVEN>
+// A stage is two steps. Small wave tiles hold two full sets of fragments and take a step in one phase; large ones take it in two, over halves
+// of the B blocks. While a phase's products run the next phase's fragments are read; in the stage's last one, after a barrier behind which
+// the next stage is there and this one is read, the stage STAGES ahead is loaded into this one's place.
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, bool A_COLUMNS, bool B_COLUMNS, bool A_UNEVEN, bool B_UNEVEN>
 struct Product {
   static constexpr int kWaves = WAVES_M * WAVES_N, kThreads = kWaves * 64;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 16, TN = WN / 16;
   using FeedA = Feed<BM, TM, A_COLUMNS, A_UNEVEN, kWaves>;
   using FeedB = Feed<BN, TN, B_COLUMNS, B_UNEVEN, kWaves>;
-  static constexpr int kStage = FeedA::kBytes + FeedB::kBytes, kLds = kStages * kStage;
+  static constexpr int kStage = FeedA::kBytes + FeedB::kBytes, kLds = STAGES * kStage;
   static constexpr int kLoads = FeedA::kLoads + FeedB::kLoads;
-  // Small wave tiles hold two full sets of fragments and run a stage as one phase; large ones split it over halves of the B blocks.
   static constexpr bool kOne = (TM + 2 * TN) * 8 + TM * TN * 4 <= 160;
   static constexpr int TB = kOne ? TN : TN / 2;
   static constexpr int kReadsA = A_COLUMNS ? 2 * TM : TM, kReadsB = B_COLUMNS ? 2 * TB : TB;
   static constexpr int kProducts = TM * TB;  // of a phase
   // reads are spread over the first three quarters of a phase's products, loads over the first half
   static constexpr int kReadSpan = kProducts * 3 / 4 > 0 ? kProducts * 3 / 4 : 1, kLoadSpan = kProducts / 2 > 0 ? kProducts / 2 : 1;
-  static_assert(TM >= 1 && TN >= 2 && TN % 2 == 0 && 2 * kLoads <= 63, "tile shape");
+  static_assert(TM >= 1 && TN >= 2 && TN % 2 == 0 && STAGES >= 2 && (STAGES - 1) * kLoads <= 63, "tile shape");
   using Acc = f32x4_t[TM][TN];
   using SetA = Fragments<TM, A_COLUMNS>;
   using SetB = Fragments<TB, B_COLUMNS>;
@@ -172,27 +183,27 @@ struct Product {
     fb.init(b, n0, wave_column(), wave, lane);
     const uint32_t ring = lds_addr((const FH_LDS void*)lds);
 
-    // stages past the end load the last one again (nobody reads them), so that every step issues as many loads and the waits count right
-    auto load_one = [&]<int J>(int kt) {
-      unsigned char* to = lds + (kt & (kStages - 1)) * kStage;
+    // stages past the end load the last one again (nobody reads them), so that every stage issues as many loads and the waits count right
+    auto load_one = [&]<int J>(int kt, int slot) {
+      unsigned char* to = lds + slot * kStage;
       if constexpr (J < FeedA::kLoads)
         fa.template load<J>(min(kt, KT - 1), to, wave);
       else
         fb.template load<J - FeedA::kLoads>(min(kt, KT - 1), to + FeedA::kBytes, wave);
     };
     auto load_stage = [&](int kt) {
-      [&]<int... J>(std::integer_sequence<int, J...>) { (load_one.template operator()<J>(kt), ...); }(std::make_integer_sequence<int, kLoads>{});
+      [&]<int... J>(std::integer_sequence<int, J...>) { (load_one.template operator()<J>(kt, kt), ...); }(std::make_integer_sequence<int, kLoads>{});
     };
-    // read N of a stage's first set: A's blocks, then B's [0, TB)
-    auto read_set = [&]<int N>(uint32_t base, SetA& sa, SetB& sb) {
+    // read N of the first set of step H: A's blocks, then B's [0, TB)
+    auto read_set = [&]<int N, int H>(uint32_t base, SetA& sa, SetB& sb) {
       if constexpr (N < kReadsA)
-        fa.template read<N, 0, TM>(base, sa);
+        fa.template read<N, 0, H>(base, sa);
       else
-        fb.template read<N - kReadsA, 0, TB>(base + FeedA::kBytes, sb);
+        fb.template read<N - kReadsA, 0, H>(base + FeedA::kBytes, sb);
     };
-    // The products of B's blocks [J0, J0 + TB), between them (NEXT) the reads of the stage at `base` into (sa_n, sb_n) and the loads of
-    // stage load_kt, or the reads of the same stage's B blocks [TB, 2 TB) into sb_n.
-    auto phase = [&]<int J0, bool NEXT>(SetA& sa, SetB& sb, uint32_t base, SetA& sa_n, SetB& sb_n, int load_kt) {
+    // The products of B's blocks [J0, J0 + TB), between them (NEXT) the reads of the first set of step H of the stage at `base` into (sa_n, sb_n),
+    // or those of the same step's B blocks [TB, 2 TB) into sb_n; LOAD: and the loads of stage load_kt into `slot`.
+    auto phase = [&]<int J0, int H, bool NEXT, bool LOAD>(SetA& sa, SetB& sb, uint32_t base, SetA& sa_n, SetB& sb_n, int load_kt, int slot) {
       constexpr int reads = NEXT ? kReadsA + kReadsB : kReadsB;
       [&]<int... M_>(std::integer_sequence<int, M_...>) {
         (
@@ -202,14 +213,14 @@ struct Product {
               constexpr int r0 = mfma16::first(M_, reads, kReadSpan);
               [&]<int... R_>(std::integer_sequence<int, R_...>) {
                 if constexpr (NEXT)
-                  (read_set.template operator()<r0 + R_>(base, sa_n, sb_n), ...);
+                  (read_set.template operator()<r0 + R_, H>(base, sa_n, sb_n), ...);
                 else
-                  (fb.template read<r0 + R_, TB, TB>(base + FeedA::kBytes, sb_n), ...);
+                  (fb.template read<r0 + R_, TB, H>(base + FeedA::kBytes, sb_n), ...);
               }(std::make_integer_sequence<int, share(M_, reads, kReadSpan)>{});
-              if constexpr (NEXT) {
+              if constexpr (LOAD) {
                 constexpr int l0 = mfma16::first(M_, kLoads, kLoadSpan);
                 [&]<int... L_>(std::integer_sequence<int, L_...>) {
-                  (load_one.template operator()<l0 + L_>(load_kt), ...);
+                  (load_one.template operator()<l0 + L_>(load_kt, slot), ...);
                 }(std::make_integer_sequence<int, share(M_, kLoads, kLoadSpan)>{});
               }
               __builtin_amdgcn_sched_barrier(0);
@@ -217,54 +228,51 @@ struct Product {
             ...);
       }(std::make_integer_sequence<int, kProducts>{});
     };
-    auto barrier_next = [&] {
-      wait_vmcnt<kLoads>();  // this wave's part of stage kt + 1 is there (stage kt + 2 may be on its way)
+    auto ready = [&](SetA& sa, SetB& sb) {
+      wait_lds();
+      tie(sa);
+      tie(sb);
+    };
+    // this wave's reads of the stage are done (wait_lds before it) and its part of the next one is there; behind the barrier, everybody's
+    auto turn = [&] {
+      wait_vmcnt<(STAGES - 2) * kLoads>();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
-    // Stage kt with its first set in (sa, sb). The slot that is filled after the barrier held stage kt - 1, whose reads every wave waited
-    // for before it arrived there.
-    auto stage = [&](int kt, SetA& sa, SetA& sa_n, SetB& sb, SetB& sb_n) {
-      const uint32_t cur = ring + (kt & (kStages - 1)) * kStage, nxt = ring + ((kt + 1) & (kStages - 1)) * kStage;
-      if constexpr (kOne) {
-        barrier_next();
-        wait_lds();
-        tie(sa);
-        tie(sb);
-        phase.template operator()<0, true>(sa, sb, nxt, sa_n, sb_n, kt + kStages - 1);
-      } else {
-        wait_lds();
-        tie(sa);
-        tie(sb);
-        phase.template operator()<0, false>(sa, sb, cur, sa_n, sb_n, 0);
-        barrier_next();
-        wait_lds();
-        tie(sb_n);
-        phase.template operator()<TN - TB, true>(sa, sb_n, nxt, sa_n, sb, kt + kStages - 1);
-      }
-    };
 
     SetA sa0, sa1;
     SetB sb0, sb1;
-    load_stage(0);
-    load_stage(1);
-    load_stage(2);
-    wait_vmcnt<2 * kLoads>();
+    [&]<int... S_>(std::integer_sequence<int, S_...>) { (load_stage(S_), ...); }(std::make_integer_sequence<int, STAGES>{});
+    wait_vmcnt<(STAGES - 1) * kLoads>();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     [&]<int... N_>(std::integer_sequence<int, N_...>) {
-      (read_set.template operator()<N_>(ring, sa0, sb0), ...);
+      (read_set.template operator()<N_, 0>(ring, sa0, sb0), ...);
     }(std::make_integer_sequence<int, kReadsA + kReadsB>{});
-    int kt = 0;
-    for (; kt + 1 < KT; kt += 2) {
-      stage(kt, sa0, sa1, sb0, sb1);
-      if constexpr (kOne)
-        stage(kt + 1, sa1, sa0, sb1, sb0);
-      else
-        stage(kt + 1, sa1, sa0, sb0, sb1);
+    int slot = 0;
+    for (int kt = 0; kt < KT; ++kt) {
+      const int next = slot + 1 == STAGES ? 0 : slot + 1;
+      const uint32_t cur = ring + slot * kStage, nxt = ring + next * kStage;
+      if constexpr (kOne) {
+        ready(sa0, sb0);
+        phase.template operator()<0, 1, true, false>(sa0, sb0, cur, sa1, sb1, 0, 0);
+        ready(sa1, sb1);
+        turn();
+        phase.template operator()<0, 0, true, true>(sa1, sb1, nxt, sa0, sb0, kt + STAGES, slot);
+      } else {
+        ready(sa0, sb0);
+        phase.template operator()<0, 0, false, false>(sa0, sb0, cur, sa1, sb1, 0, 0);
+        ready(sa0, sb1);
+        phase.template operator()<TN - TB, 1, true, false>(sa0, sb1, cur, sa1, sb0, 0, 0);
+        ready(sa1, sb0);
+        phase.template operator()<0, 1, false, false>(sa1, sb0, cur, sa0, sb1, 0, 0);
+        ready(sa1, sb1);
+        turn();
+        phase.template operator()<TN - TB, 0, true, true>(sa1, sb1, nxt, sa0, sb0, kt + STAGES, slot);
+      }
+      slot = next;
     }
-    if (kt < KT) stage(kt, sa0, sa1, sb0, sb1);
     // the last stage's reads of the one behind it (unused) still write their registers
     wait_lds();
     tie(sa0);

@@ -27,6 +27,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 template <typename T>
 constexpr float kRaise = std::is_same_v<T, f16_t> ? 0x1p14f : 1.0f;
 
+// Stages of a tile's ring: two of 64 KB for the largest, 32 KB each for the next; three for the small ones, whose stages are short.
+template <int BM>
+constexpr int kRing = BM >= 128 ? 2 : 3;
+
 struct LossArgs {
   const uint16_t* x;
   const uint16_t* w;
@@ -110,14 +114,14 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a) {
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, false, false, true, true>;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, false, false, true, true>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
   int tm, tn;
   if (!place(blockIdx.x, (count + BM - 1) / BM, a.tiles_n, tm, tn)) return;
   const int m0 = tm * BM, n0 = tn * BN;
   typename P::Acc acc;
-  P::run(lds, {a.x, a.ldx, a.rows, count - 1, a.dim}, {a.w, a.ldw, nullptr, a.vocab - 1, a.dim}, m0, n0, (a.dim + kBK - 1) / kBK, acc);
+  P::run(lds, {a.x, a.ldx, a.rows, count - 1, a.dim}, {a.w, a.ldw, nullptr, a.vocab - 1, a.dim}, m0, n0, (a.dim + kDepth - 1) / kDepth, acc);
   float2(*joined)[BM] = reinterpret_cast<float2(*)[BM]>(lds);
   const int g = P::lane() >> 4, r = P::lane() & 15, row0 = P::wave_row(), col0 = n0 + P::wave_column() + r;
 #pragma unroll
@@ -222,7 +226,7 @@ __device__ __forceinline__ float loss_factor(const LossArgs& a) {
 // g of a piece: columns first .. last - 1 of the vocabulary, zeros behind them and in the tile's rows that no row with a target is.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, false, false, true, true>;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, false, false, true, true>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
   int tm, tn;
@@ -230,7 +234,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(
   const int m0 = tm * BM, n0 = tn * BN;
   typename P::Acc acc;
   P::run(lds, {a.xc, a.dim, nullptr, count - 1, a.dim}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.vocab - 1 - a.first, a.dim}, m0, n0,
-         (a.dim + kBK - 1) / kBK, acc);
+         (a.dim + kDepth - 1) / kDepth, acc);
   const int g = P::lane() >> 4, r = P::lane() & 15;
   const int row0 = m0 + P::wave_row() + 4 * g, col0 = a.first + n0 + P::wave_column() + r;
   float lse[P::TM][4];
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, false, true, false, true>;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, false, true, false, true>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
   int tm, tn;
@@ -263,7 +267,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const Lo
   const int m0 = tm * BM, n0 = tn * BN, depth = a.last - a.first;
   typename P::Acc acc;
   P::run(lds, {a.g, a.ldg, nullptr, count - 1, depth}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.dim - 1, depth}, m0, n0,
-         (depth + kBK - 1) / kBK, acc);
+         (depth + kDepth - 1) / kDepth, acc);
   const int g = P::lane() >> 4, r = P::lane() & 15;
   const int row0 = m0 + P::wave_row() + 4 * g, col0 = n0 + P::wave_column() + r;
   if (!a.first_piece || !a.last_piece) {
@@ -293,14 +297,14 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const Lo
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, true, true, false, false>;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, true, true, false, false>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
   int tm, tn;
   if (!place(blockIdx.x, static_cast<int>((a.last - a.first + BM - 1) / BM), (a.dim + BN - 1) / BN, tm, tn)) return;
   const int m0 = tm * BM, n0 = tn * BN;
   typename P::Acc acc;
-  P::run(lds, {a.g, a.ldg, nullptr, static_cast<int>(a.ldg) - 1, 0}, {a.xc, a.dim, nullptr, a.dim - 1, 0}, m0, n0, (count + kBK - 1) / kBK, acc);
+  P::run(lds, {a.g, a.ldg, nullptr, static_cast<int>(a.ldg) - 1, 0}, {a.xc, a.dim, nullptr, a.dim - 1, 0}, m0, n0, (count + kDepth - 1) / kDepth, acc);
   const float f = count > 0 ? loss_factor(a) / kRaise<T> : 0.0f;
   P::store(
       lds, [&](int i, int x, int j) { return acc[i][j][x] * f; },
