@@ -141,8 +141,9 @@ struct Feed {
 };
 
 // The BM x BN tile at (m0, n0) of A B^T over k < 64 KT, by WAVES_M x WAVES_N waves. A wave's part begins at row WM (wave / WAVES_N), column
-// WN (wave % WAVES_N); its lane l holds rows 16 i + 4 (l / 16) + x and column 16 j + l % 16 of it in acc[i][j][x]. On return all of the
-// workgroup's waves are past their last use of `lds` (kLds bytes, 1 KB aligned).
+// WN (wave % WAVES_N); its lane l holds row 16 i + l % 16, columns 16 j + 4 (l / 16) + x of it in acc[i][j][x] (the instruction's operands
+// change places: four columns of a row in a lane are what every epilogue here wants). On return all of the workgroup's waves are
+// past their last use of `lds` (kLds bytes, 1 KB aligned).
 // A stage is two steps. Small wave tiles hold two full sets of fragments and take a step in one phase; large ones take it in two, over halves
 // of the B blocks. While a phase's products run the next phase's fragments are read; in the stage's last one, after a barrier behind which
 // the next stage is there and this one is read, the stage STAGES ahead is loaded into this one's place.
@@ -209,7 +210,7 @@ struct Product {
         (
             [&] {
               constexpr int i = M_ / TB, j = M_ % TB;
-              mfma16x<T>(fragment(sa, i), fragment(sb, j), acc[i][J0 + j]);
+              mfma16x<T>(fragment(sb, j), fragment(sa, i), acc[i][J0 + j]);
               constexpr int r0 = mfma16::first(M_, reads, kReadSpan);
               [&]<int... R_>(std::integer_sequence<int, R_...>) {
                 if constexpr (NEXT)
@@ -283,26 +284,29 @@ struct Product {
     __syncthreads();
   }
 
-  // The tile in 16-bit storage, whole 16-byte vectors of 8 columns: each wave hands its part over through its own room in `lds` and calls
-  // put(row, column, vector) with rows and columns of the tile. value(i, x, j): what lane l stores for its acc[i][j][x].
-  template <typename Value, typename Put>
-  __device__ __forceinline__ static void store(unsigned char* lds, Value&& value, Put&& put) {
+  // acc in 16-bit storage as whole 16-byte vectors of 8 columns: each wave hands its part over through its own room in `lds` and calls
+  // put(row, column, vector) with rows and columns of the tile. Chunks of a row are XORed with it: 16 rows' pieces meet in no bank.
+  template <typename Put>
+  __device__ __forceinline__ static void store(unsigned char* lds, const Acc& acc, Put&& put) {
     static_assert(kWaves * WM * WN * 2 <= kLds, "the waves' parts fit in the ring");
+    constexpr int chunks = WN / 8, rows = 64 / chunks;
     const int lane = Product::lane(), g = lane >> 4, r = lane & 15;
-    uint16_t* mine = reinterpret_cast<uint16_t*>(lds + wave() * (WM * WN * 2));
+    unsigned char* mine = lds + wave() * (WM * WN * 2);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) mine[(i * 16 + 4 * g + x) * WN + j * 16 + r] = Io<T>::store(value(i, x, j));
+      for (int j = 0; j < TN; ++j) {
+        const int row = i * 16 + r, chunk = (2 * j + (g >> 1)) ^ (r & (chunks - 1));
+        *reinterpret_cast<u32x2_t*>(mine + row * (WN * 2) + chunk * 16 + (g & 1) * 8) =
+            u32x2_t{store2<T>(acc[i][j][0], acc[i][j][1]), store2<T>(acc[i][j][2], acc[i][j][3])};
+      }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // from lane to lane of one wave, whose accesses run in their order
     __builtin_amdgcn_wave_barrier();
-    constexpr int lanes = WN / 8, rows = 64 / lanes;
 #pragma unroll 4
     for (int at = 0; at < WM; at += rows) {
-      const int row = at + lane / lanes, c = lane % lanes * 8;
-      put(wave_row() + row, wave_column() + c, *reinterpret_cast<const u32x4_t*>(mine + row * WN + c));
+      const int row = at + lane / chunks, c = lane % chunks;
+      put(wave_row() + row, wave_column() + c * 8,
+          *reinterpret_cast<const u32x4_t*>(mine + row * (WN * 2) + ((c ^ (row & 15 & (chunks - 1))) * 16)));
     }
   }
 };

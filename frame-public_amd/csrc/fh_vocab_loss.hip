@@ -22,6 +22,7 @@ namespace {
 using namespace tile;
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
 
 // What g is multiplied by in the storage type.
 template <typename T>
@@ -61,19 +62,42 @@ struct LossArgs {
   int first_piece, last_piece;
 };
 
-// max and sum over the 16 lanes that share rows of a tile
-__device__ __forceinline__ float max16(float v) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+// max and sum over the 4 lanes that share a row of a tile
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
 }
-__device__ __forceinline__ float sum16(float v) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
-  return v;
+__device__ __forceinline__ float row_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
 }
 // A maximum that exponents can be taken against: of a row of -infinity, 0.
 __device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.0f : m; }
+// 2^(z log2 e - from2). Exponents are counted in twos from a `from2` that is kept as it is, so its own rounding changes nothing.
+__device__ __forceinline__ float exp_from(float z, float from2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -from2)); }
+// {from2, sum of 2^(z log2 e - from2)} of two sets of logits. An empty sum (logits of -infinity) is 0 and its from2 says nothing.
+__device__ __forceinline__ float2 add_exponentials(const float2& a, const float2& b) {
+  if (a.y == 0.0f) return b;
+  if (b.y == 0.0f) return a;
+  const float from2 = fmaxf(a.x, b.x);
+  return float2{from2, a.y * __builtin_amdgcn_exp2f(a.x - from2) + b.y * __builtin_amdgcn_exp2f(b.x - from2)};
+}
+
+// Runs f(i, j, x) for the lane's place in acc that is column `target` of row i of the wave's part (columns from `column` on). Few tiles hold the target
+// of any of their rows, so the rows are asked first and the columns only where one answers.
+template <typename P, typename F>
+__device__ __forceinline__ void at_targets(const int (&target)[P::TM], int column, F&& f) {
+#pragma unroll
+  for (int i = 0; i < P::TM; ++i) {
+    const int in = target[i] - column;
+    if (__ballot(in >= 0 && in < P::WN) == 0) continue;
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (in == 16 * j + 4 * (P::lane() >> 4) + x) f(i, j, x);
+  }
+}
 
 // ---- rows with a target ----
 
@@ -123,57 +147,64 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(cons
   typename P::Acc acc;
   P::run(lds, {a.x, a.ldx, a.rows, count - 1, a.dim}, {a.w, a.ldw, nullptr, a.vocab - 1, a.dim}, m0, n0, (a.dim + kDepth - 1) / kDepth, acc);
   float2(*joined)[BM] = reinterpret_cast<float2(*)[BM]>(lds);
-  const int g = P::lane() >> 4, r = P::lane() & 15, row0 = P::wave_row(), col0 = n0 + P::wave_column() + r;
+  const int g = P::lane() >> 4, r = P::lane() & 15, row0 = P::wave_row() + r, column = n0 + P::wave_column();
+  if (n0 + BN > a.vocab) {  // columns that do not exist are tokens of probability zero
 #pragma unroll
-  for (int i = 0; i < P::TM; ++i)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int row = row0 + 16 * i + 4 * g + x, m = m0 + row;
-      const int target = a.targets_c[min(m, count - 1)];
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < P::TN; ++j) {
-        if (col0 + 16 * j < a.vocab) top = fmaxf(top, acc[i][j][x]);
-        if (col0 + 16 * j == target && m < count) a.at_target[m] = acc[i][j][x];
-      }
-      top = max16(top);
-      float sum = 0.0f;
+    for (int i = 0; i < P::TM; ++i)
 #pragma unroll
       for (int j = 0; j < P::TN; ++j)
-        if (col0 + 16 * j < a.vocab) sum += __builtin_amdgcn_exp2f((acc[i][j][x] - origin(top)) * kLog2e);
-      sum = sum16(sum);
-      if (r == 0) joined[P::wave() % WAVES_N][row] = float2{top, sum};
-    }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (column + 16 * j + 4 * g + x >= a.vocab) acc[i][j][x] = -INFINITY;
+  }
+  int target[P::TM];
+#pragma unroll
+  for (int i = 0; i < P::TM; ++i) target[i] = m0 + row0 + 16 * i < count ? a.targets_c[m0 + row0 + 16 * i] : -1;
+  at_targets<P>(target, column, [&](int i, int j, int x) { a.at_target[m0 + row0 + 16 * i] = acc[i][j][x]; });
+#pragma unroll
+  for (int i = 0; i < P::TM; ++i) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) top = fmaxf(top, acc[i][j][x]);
+    const float top2 = origin(row_max(top)) * kLog2e;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum += exp_from(acc[i][j][x], top2);
+    sum = row_sum(sum);
+    if (g == 0) joined[P::wave() % WAVES_N][row0 + 16 * i] = float2{top2, sum};
+  }
   __syncthreads();
   for (int row = threadIdx.x; row < BM; row += P::kThreads) {
     if (m0 + row >= count) break;
-    float top = joined[0][row].x, sum = 0.0f;
-    for (int w = 1; w < WAVES_N; ++w) top = fmaxf(top, joined[w][row].x);
-    for (int w = 0; w < WAVES_N; ++w) sum += joined[w][row].y * __builtin_amdgcn_exp2f((joined[w][row].x - origin(top)) * kLog2e);
-    a.part[static_cast<int64_t>(tn) * a.tokens + m0 + row] = float2{top, sum};
+    float2 both = joined[0][row];
+    for (int w = 1; w < WAVES_N; ++w) both = add_exponentials(both, joined[w][row]);
+    a.part[static_cast<int64_t>(tn) * a.tokens + m0 + row] = both;
   }
 }
 
-// 16 rows per workgroup, 16 threads each a share of the tiles.
+// ROWS rows per workgroup, 256 / ROWS threads each a share of the tiles; the shares are joined in their order.
+template <int ROWS>
 __global__ __launch_bounds__(256) void loss_join_kernel(const LossArgs a) {
-  __shared__ float2 shares[16][16];
-  const int row = threadIdx.x & 15, share = threadIdx.x >> 4;
-  const int count = *a.count, m = static_cast<int>(blockIdx.x) * 16 + row;
-  float top = -INFINITY, sum = 0.0f;
-  if (m < count)
-    for (int t = share; t < a.tiles_n; t += 16) {
-      const float2 p = a.part[static_cast<int64_t>(t) * a.tokens + m];
-      const float both = fmaxf(top, p.x), from = origin(both);
-      sum = sum * __builtin_amdgcn_exp2f((top - from) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - from) * kLog2e);
-      top = both;
-    }
-  shares[share][row] = float2{top, sum};
-  __syncthreads();
-  if (share != 0 || m >= count) return;
-  for (int s = 1; s < 16; ++s) top = fmaxf(top, shares[s][row].x);
-  float all = 0.0f;
-  for (int s = 0; s < 16; ++s) all += shares[s][row].y * __builtin_amdgcn_exp2f((shares[s][row].x - origin(top)) * kLog2e);
-  const float lse = origin(top) + logf(all);
+  __shared__ float2 shares[256 / ROWS][ROWS];
+  constexpr int SHARES = 256 / ROWS;
+  const int row = threadIdx.x % ROWS, share = threadIdx.x / ROWS;
+  const int m = static_cast<int>(blockIdx.x) * ROWS + row;
+  const bool live = m < *a.count;
+  float2 sum{0.0f, 0.0f};
+  if (live)
+    for (int t = share; t < a.tiles_n; t += SHARES) sum = add_exponentials(sum, a.part[static_cast<int64_t>(t) * a.tokens + m]);
+  shares[share][row] = sum;
+#pragma unroll
+  for (int o = SHARES / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (share < o) shares[share][row] = sum = add_exponentials(sum, shares[share + o][row]);
+  }
+  if (share != 0 || !live) return;
+  const float lse = kLn2 * (sum.x + __builtin_amdgcn_logf(sum.y));
   const int t = a.rows[m];
   a.lse[t] = lse;
   a.at_target[m] = lse - a.at_target[m];
@@ -223,6 +254,16 @@ __device__ __forceinline__ float loss_factor(const LossArgs& a) {
   return a.mean ? d / static_cast<float>(*a.count) : d;
 }
 
+template <typename P>
+__device__ __forceinline__ void scale(typename P::Acc& acc, float f) {
+#pragma unroll
+  for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[i][j][x] *= f;
+}
+
 // g of a piece: columns first .. last - 1 of the vocabulary, zeros behind them and in the tile's rows that no row with a target is.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(const LossArgs a) {
@@ -235,26 +276,31 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(
   typename P::Acc acc;
   P::run(lds, {a.xc, a.dim, nullptr, count - 1, a.dim}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.vocab - 1 - a.first, a.dim}, m0, n0,
          (a.dim + kDepth - 1) / kDepth, acc);
-  const int g = P::lane() >> 4, r = P::lane() & 15;
-  const int row0 = m0 + P::wave_row() + 4 * g, col0 = a.first + n0 + P::wave_column() + r;
-  float lse[P::TM][4];
-  int target[P::TM][4];
+  const int row0 = m0 + P::wave_row() + (P::lane() & 15), column = a.first + n0 + P::wave_column();
+  int target[P::TM];
 #pragma unroll
-  for (int i = 0; i < P::TM; ++i)
+  for (int i = 0; i < P::TM; ++i) {
+    const int m = min(row0 + 16 * i, count - 1);
+    const float lse2 = a.lse_c[m] * kLog2e;
+    target[i] = a.targets_c[m];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int m = min(row0 + 16 * i + x, count - 1);
-      lse[i][x] = a.lse_c[m];
-      target[i][x] = a.targets_c[m];
-    }
-  P::store(
-      lds,
-      [&](int i, int x, int j) {
-        const int v = col0 + 16 * j;
-        const float d = __builtin_amdgcn_exp2f((acc[i][j][x] - lse[i][x]) * kLog2e) - (v == target[i][x] ? 1.0f : 0.0f);
-        return row0 + 16 * i + x < count && v < a.last ? d * kRaise<T> : 0.0f;
-      },
-      [&](int row, int c, const u32x4_t& v) { *reinterpret_cast<u32x4_t*>(a.g + static_cast<int64_t>(m0 + row) * a.ldg + n0 + c) = v; });
+    for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[i][j][x] = exp_from(acc[i][j][x], lse2) * kRaise<T>;
+  }
+  at_targets<P>(target, column, [&](int i, int j, int x) { acc[i][j][x] -= kRaise<T>; });
+  if (m0 + BM > count || a.first + n0 + BN > a.last) {
+#pragma unroll
+    for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (row0 + 16 * i >= count || column + 16 * j + 4 * (P::lane() >> 4) + x >= a.last) acc[i][j][x] = 0.0f;
+  }
+  P::store(lds, acc, [&](int row, int c, const u32x4_t& v) {
+    *reinterpret_cast<u32x4_t*>(a.g + static_cast<int64_t>(m0 + row) * a.ldg + n0 + c) = v;
+  });
 }
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
@@ -268,31 +314,25 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const Lo
   typename P::Acc acc;
   P::run(lds, {a.g, a.ldg, nullptr, count - 1, depth}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.dim - 1, depth}, m0, n0,
          (depth + kDepth - 1) / kDepth, acc);
-  const int g = P::lane() >> 4, r = P::lane() & 15;
-  const int row0 = m0 + P::wave_row() + 4 * g, col0 = n0 + P::wave_column() + r;
   if (!a.first_piece || !a.last_piece) {
+    const int row0 = m0 + P::wave_row() + (P::lane() & 15), col0 = n0 + P::wave_column() + 4 * (P::lane() >> 4);
 #pragma unroll
-    for (int i = 0; i < P::TM; ++i)
+    for (int i = 0; i < P::TM; ++i) {
+      if (row0 + 16 * i >= count) continue;
+      f32x4_t* sum = reinterpret_cast<f32x4_t*>(a.dx_sum + static_cast<int64_t>(row0 + 16 * i) * a.dim + col0);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int m = row0 + 16 * i + x;
-        if (m >= count) continue;
-        float* sum = a.dx_sum + static_cast<int64_t>(m) * a.dim + col0;
-#pragma unroll
-        for (int j = 0; j < P::TN; ++j) {
-          if (col0 + 16 * j >= a.dim) continue;
-          if (!a.first_piece) acc[i][j][x] += sum[16 * j];
-          if (!a.last_piece) sum[16 * j] = acc[i][j][x];
-        }
+      for (int j = 0; j < P::TN; ++j) {
+        if (col0 + 16 * j >= a.dim) continue;
+        if (!a.first_piece) acc[i][j] += sum[4 * j];
+        if (!a.last_piece) sum[4 * j] = acc[i][j];
       }
+    }
   }
   if (!a.last_piece) return;
-  const float f = loss_factor(a) / kRaise<T>;
-  P::store(
-      lds, [&](int i, int x, int j) { return acc[i][j][x] * f; },
-      [&](int row, int c, const u32x4_t& v) {
-        if (m0 + row < count && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dx + a.rows[m0 + row] * a.ldx + n0 + c) = v;
-      });
+  scale<P>(acc, loss_factor(a) / kRaise<T>);
+  P::store(lds, acc, [&](int row, int c, const u32x4_t& v) {
+    if (m0 + row < count && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dx + a.rows[m0 + row] * a.ldx + n0 + c) = v;
+  });
 }
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
@@ -305,13 +345,11 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const Lo
   const int m0 = tm * BM, n0 = tn * BN;
   typename P::Acc acc;
   P::run(lds, {a.g, a.ldg, nullptr, static_cast<int>(a.ldg) - 1, 0}, {a.xc, a.dim, nullptr, a.dim - 1, 0}, m0, n0, (count + kDepth - 1) / kDepth, acc);
-  const float f = count > 0 ? loss_factor(a) / kRaise<T> : 0.0f;
-  P::store(
-      lds, [&](int i, int x, int j) { return acc[i][j][x] * f; },
-      [&](int row, int c, const u32x4_t& v) {
-        const int64_t to = a.first + m0 + row;
-        if (to < a.last && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dw + to * a.ldw + n0 + c) = v;
-      });
+  scale<P>(acc, count > 0 ? loss_factor(a) / kRaise<T> : 0.0f);
+  P::store(lds, acc, [&](int row, int c, const u32x4_t& v) {
+    const int64_t to = a.first + m0 + row;
+    if (to < a.last && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dw + to * a.ldw + n0 + c) = v;
+  });
 }
 
 // ---- host ----
@@ -478,7 +516,11 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
       return launch_status("loss_logits_kernel launch");
     });
     if (st != FH_OK) return st;
-    hipLaunchKernelGGL(loss_join_kernel, dim3(static_cast<uint32_t>((g->tokens + 15) / 16)), dim3(256), 0, s, a);
+    // a few rows: a workgroup each (one row of 1,024 tiles: 32 us with 16 threads)
+    if (g->tokens <= 4 * device_cu_count())
+      hipLaunchKernelGGL((loss_join_kernel<1>), dim3(static_cast<uint32_t>(g->tokens)), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((loss_join_kernel<16>), dim3(static_cast<uint32_t>((g->tokens + 15) / 16)), dim3(256), 0, s, a);
     if (fh_status st2 = launch_status("loss_join_kernel launch"); st2 != FH_OK) return st2;
   }
   hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, s, a);

@@ -198,6 +198,16 @@ def test_large_logits(hip, dtype):
     Loss(hip, dtype, 90, 800, 64, std=60.0, learned=False).check()
 
 
+@pytest.mark.parametrize("shift", [-800.0, -150.0, 150.0, 800.0])
+def test_logits_far_from_zero(hip, shift):
+    """Exponentials of the logits themselves are zero or infinite in 32 bits."""
+    say(f"logits around {shift}")
+    p = Loss(hip, BF16, 70, 1000, 64)
+    p.x[:, 0] = synth.to_storage(np.full(1, shift, np.float32), BF16)[0]
+    p.w[:, 0] = 0x3f80  # 1.0
+    p.check()
+
+
 def test_every_logit_alike(hip):
     say("logits all zero: log(vocab), exact thirds")
     p = Loss(hip, BF16, 40, 3, 8)
