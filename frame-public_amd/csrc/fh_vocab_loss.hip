@@ -57,8 +57,9 @@ struct LossArgs {
   float* lse_c;
   uint16_t* g;
   int64_t ldg;
-  float* dx_sum;
+  float* dx_sum;  // [splits][tokens][dim]
   int first, last;  // columns of the piece
+  int splits;       // of a piece's columns in dx' product
   int first_piece, last_piece;
 };
 
@@ -102,36 +103,53 @@ __device__ __forceinline__ void at_targets(const int (&target)[P::TM], int colum
 // ---- rows with a target ----
 
 // By one workgroup: the list of rows with a target, their number and targets; the others' outputs, or (gradients: lse_c) the
-// log-sum-exps.
+// log-sum-exps. 8 rows a thread and turn, read together: 8,192 rows take one turn.
 __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a) {
+  constexpr int EACH = 8;
   __shared__ int waves[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int each = (a.tokens + 1023) / 1024, begin = tid * each, end = min(a.tokens, begin + each);
-  auto has = [&](int t) { return a.targets[t] >= 0 && a.targets[t] < a.vocab; };
-  int n = 0;
-  for (int t = begin; t < end; ++t) n += has(t);
-  int scan = n;
+  int before = 0;  // rows with a target in earlier turns
+  for (int begin = 0; begin < a.tokens; begin += 1024 * EACH) {
+    int target[EACH], n = 0;
+    float lse[EACH];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int up = __shfl_up(scan, o, 64);
-    if (lane >= o) scan += up;
-  }
-  if (lane == 63) waves[wave] = scan;
-  __syncthreads();
-  int at = scan - n;
-  for (int w = 0; w < wave; ++w) at += waves[w];
-  if (tid == 1023) *a.count = at + n;
-  for (int t = begin; t < end; ++t) {
-    if (has(t)) {
-      a.rows[at] = t;
-      a.targets_c[at] = a.targets[t];
-      if (a.lse_c != nullptr) a.lse_c[at] = a.lse[t];
-      ++at;
-    } else if (a.lse_c == nullptr) {
-      a.lse[t] = 0.0f;
-      if (a.row_loss != nullptr) a.row_loss[t] = 0.0f;
+    for (int e = 0; e < EACH; ++e) {
+      const int t = begin + tid * EACH + e;
+      target[e] = t < a.tokens ? a.targets[t] : -1;
+      if (a.lse_c != nullptr) lse[e] = t < a.tokens ? a.lse[t] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) n += target[e] >= 0 && target[e] < a.vocab;
+    int scan = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int lower = __shfl_up(scan, o, 64);
+      if (lane >= o) scan += lower;
+    }
+    if (lane == 63) waves[wave] = scan;
+    __syncthreads();
+    int at = before + scan - n;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) at += waves[w];
+      before += waves[w];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int t = begin + tid * EACH + e;
+      if (target[e] >= 0 && target[e] < a.vocab) {
+        a.rows[at] = t;
+        a.targets_c[at] = target[e];
+        if (a.lse_c != nullptr) a.lse_c[at] = lse[e];
+        ++at;
+      } else if (t < a.tokens && a.lse_c == nullptr) {
+        a.lse[t] = 0.0f;
+        if (a.row_loss != nullptr) a.row_loss[t] = 0.0f;
+      }
     }
   }
+  if (tid == 0) *a.count = before;
 }
 
 // ---- forward ----
@@ -310,29 +328,51 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const Lo
   const int count = *a.count;
   int tm, tn;
   if (!place(blockIdx.x, (count + BM - 1) / BM, (a.dim + BN - 1) / BN, tm, tn)) return;
-  const int m0 = tm * BM, n0 = tn * BN, depth = a.last - a.first;
+  // this split's share of the piece's stages
+  const int stages = (a.last - a.first + kDepth - 1) / kDepth, share = (stages + a.splits - 1) / a.splits;
+  const int k0 = static_cast<int>(blockIdx.y) * share, KT = min(share, stages - k0);
+  const int m0 = tm * BM, n0 = tn * BN, from = a.first + k0 * kDepth, depth = a.last - from;
   typename P::Acc acc;
-  P::run(lds, {a.g, a.ldg, nullptr, count - 1, depth}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.dim - 1, depth}, m0, n0,
-         (depth + kDepth - 1) / kDepth, acc);
-  if (!a.first_piece || !a.last_piece) {
+  P::run(lds, {a.g + k0 * kDepth, a.ldg, nullptr, count - 1, depth}, {a.w + from * a.ldw, a.ldw, nullptr, a.dim - 1, depth}, m0, n0, KT, acc);
+  const bool whole = a.splits == 1 && a.last_piece;
+  if (!a.first_piece || !whole) {
     const int row0 = m0 + P::wave_row() + (P::lane() & 15), col0 = n0 + P::wave_column() + 4 * (P::lane() >> 4);
 #pragma unroll
     for (int i = 0; i < P::TM; ++i) {
       if (row0 + 16 * i >= count) continue;
-      f32x4_t* sum = reinterpret_cast<f32x4_t*>(a.dx_sum + static_cast<int64_t>(row0 + 16 * i) * a.dim + col0);
+      f32x4_t* sum = reinterpret_cast<f32x4_t*>(a.dx_sum + (static_cast<int64_t>(blockIdx.y) * a.tokens + row0 + 16 * i) * a.dim + col0);
 #pragma unroll
       for (int j = 0; j < P::TN; ++j) {
         if (col0 + 16 * j >= a.dim) continue;
         if (!a.first_piece) acc[i][j] += sum[4 * j];
-        if (!a.last_piece) sum[4 * j] = acc[i][j];
+        if (!whole) sum[4 * j] = acc[i][j];
       }
     }
   }
-  if (!a.last_piece) return;
+  if (!whole) return;
   scale<P>(acc, loss_factor(a) / kRaise<T>);
   P::store(lds, acc, [&](int row, int c, const u32x4_t& v) {
     if (m0 + row < count && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dx + a.rows[m0 + row] * a.ldx + n0 + c) = v;
   });
+}
+
+// dx from the splits' sums, in their order: 8 columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void loss_dx_join_kernel(const LossArgs a) {
+  const int vectors = a.dim / 8;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int m = static_cast<int>(at / vectors), c = static_cast<int>(at % vectors) * 8;
+  if (m >= *a.count) return;
+  f32x4_t low{0.0f, 0.0f, 0.0f, 0.0f}, high = low;
+  for (int s = 0; s < a.splits; ++s) {
+    const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.dx_sum + (static_cast<int64_t>(s) * a.tokens + m) * a.dim + c);
+    low += p[0];
+    high += p[1];
+  }
+  const float f = loss_factor(a) / kRaise<T>;
+  *reinterpret_cast<u32x4_t*>(a.dx + a.rows[m] * a.ldx + c) =
+      u32x4_t{store2<T>(low[0] * f, low[1] * f), store2<T>(low[2] * f, low[3] * f), store2<T>(high[0] * f, high[1] * f),
+              store2<T>(high[2] * f, high[3] * f)};
 }
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
@@ -390,15 +430,43 @@ Shape tile_for(int64_t m, int64_t n) {
   if (n >= 128 && tiles(64, 128) >= cus) return {64, 128};
   return {64, 64};
 }
-// launch<BM, BN, WAVES_M, WAVES_N>(workgroups) with the tile of m x n
+// launch<BM, BN, WAVES_M, WAVES_N>(workgroups) with tiles of shape t over m x n
 template <typename F>
-void by_tile(int64_t m, int64_t n, F&& launch) {
-  const Shape t = tile_for(m, n);
+void by_tile(Shape t, int64_t m, int64_t n, F&& launch) {
   const dim3 grid(static_cast<uint32_t>(up(m, t.m) / t.m * (up(n, t.n) / t.n)));
   if (t.m == 256) launch.template operator()<256, 256, 4, 2>(grid);
   else if (t.m == 128) launch.template operator()<128, 128, 2, 4>(grid);
   else if (t.n == 128) launch.template operator()<64, 128, 2, 2>(grid);
   else launch.template operator()<64, 64, 2, 2>(grid);
+}
+
+// dx is small and its sums are long, a piece's columns: where tiles leave CUs idle, the columns are split among `splits` workgroups, whose
+// sums a second launch joins. The cheapest by rounds of workgroups over the CUs, a tile's products over its share of the columns
+// at the rates below, and a stage's worth of waiting at either end.
+struct DxPlan {
+  Shape tile;
+  int splits;
+};
+DxPlan dx_plan(int64_t tokens, int64_t dim, int64_t columns) {
+  const int64_t cus = device_cu_count(), stages = up(columns, 64) / 64;
+  DxPlan best{{64, 64}, 1};
+  double least = 0.0;
+  const struct {
+    Shape t;
+    int together;   // workgroups of a CU
+    double stage;   // us of a stage with so many
+  } kinds[] = {{{256, 256}, 1, 1.7}, {{128, 128}, 2, 1.25}, {{64, 128}, 2, 0.75}, {{64, 64}, 3, 0.6}};
+  for (const auto& k : kinds)
+    for (int splits = 1; splits <= 8; splits *= 2) {
+      const int64_t tiles = up(tokens, k.t.m) / k.t.m * (up(dim, k.t.n) / k.t.n) * splits, share = (stages + splits - 1) / splits;
+      const double rounds = static_cast<double>(up(tiles, cus * k.together) / (cus * k.together));
+      const double us = rounds * (static_cast<double>(share) + 4.0) * k.stage + (splits > 1 ? 4.0 + splits * tokens * dim * 8 / 4e6 : 0.0);
+      if (least == 0.0 || us < least) {
+        least = us;
+        best = {k.t, splits};
+      }
+    }
+  return best;
 }
 
 struct Room {
@@ -430,8 +498,8 @@ struct GradRoom {
   int64_t count, rows, targets, lse, xc, dx_sum, g, bytes;
   int64_t g_rows;
 };
-// with a piece of `columns`
-GradRoom grad_room(const fh_vocab_loss& g, int64_t columns) {
+// with a piece of `columns`, dx' product in `splits`
+GradRoom grad_room(const fh_vocab_loss& g, int64_t columns, int splits) {
   Room r;
   GradRoom f{};
   f.g_rows = up(g.tokens, 256);
@@ -440,17 +508,42 @@ GradRoom grad_room(const fh_vocab_loss& g, int64_t columns) {
   f.targets = r.take(4 * g.tokens);
   f.lse = r.take(4 * g.tokens);
   f.xc = r.take(2 * f.g_rows * g.dim);
-  f.dx_sum = r.take(columns < g.vocab ? 4 * g.tokens * g.dim : 0);
+  f.dx_sum = r.take(columns < g.vocab || splits > 1 ? 4 * splits * g.tokens * g.dim : 0);
   f.g = r.take(2 * f.g_rows * columns);
   f.bytes = r.bytes;
   return f;
 }
-int64_t best_piece(const fh_vocab_loss& g) {
+struct GradPlan {
+  int64_t columns;  // of a piece
+  DxPlan dx;
+};
+GradPlan best_plan(const fh_vocab_loss& g) {
   const int64_t all = up(g.vocab, kLeastPiece), rows = up(std::max<int64_t>(g.tokens, 1), 256);
-  return std::min(all, std::max<int64_t>(kPieceValues / rows / kLeastPiece * kLeastPiece, kLeastPiece));
+  GradPlan p{};
+  p.columns = std::min(all, std::max<int64_t>(kPieceValues / rows / kLeastPiece * kLeastPiece, kLeastPiece));
+  p.dx = dx_plan(g.tokens, g.dim, std::min(p.columns, g.vocab));
+  return p;
 }
-// (one piece needs no sums between pieces)
-int64_t least_room(const fh_vocab_loss& g) { return std::min(grad_room(g, kLeastPiece).bytes, grad_room(g, best_piece(g)).bytes); }
+int64_t best_room(const fh_vocab_loss& g) {
+  const GradPlan p = best_plan(g);
+  return grad_room(g, p.columns, p.dx.splits).bytes;
+}
+// one piece in one split needs no room for sums
+int64_t least_room(const fh_vocab_loss& g) {
+  return std::min({grad_room(g, kLeastPiece, 1).bytes, grad_room(g, best_plan(g).columns, 1).bytes, best_room(g)});
+}
+// The best plan, or what `bytes` have room for: without splits, and then the widest piece that fits.
+GradPlan plan_for(const fh_vocab_loss& g, int64_t bytes) {
+  GradPlan p = best_plan(g);
+  if (bytes >= grad_room(g, p.columns, p.dx.splits).bytes) return p;
+  p.dx = {tile_for(g.tokens, g.dim), 1};
+  if (bytes >= grad_room(g, p.columns, 1).bytes) return p;
+  const GradRoom least = grad_room(g, kLeastPiece, 1);
+  // room beside the sums between pieces, which a piece of the whole vocabulary would not need
+  p.columns = std::min(p.columns, (bytes - least.g) / (2 * least.g_rows) / kLeastPiece * kLeastPiece);
+  if (p.columns >= g.vocab) p.columns = up(g.vocab, kLeastPiece) - kLeastPiece;
+  return p;
+}
 
 LossArgs loss_args(const fh_vocab_loss& g, const void* x, const void* w, const int32_t* targets) {
   LossArgs a{};
@@ -510,7 +603,7 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
   if (fh_status st = launch_status("loss_rows_kernel launch"); st != FH_OK) return st;
   if (g->tokens > 0) {
     const fh_status st = by_type(g->dtype, [&]<typename T>() {
-      by_tile(g->tokens, g->vocab, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+      by_tile(tile_for(g->tokens, g->vocab), g->tokens, g->vocab, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
         hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
       });
       return launch_status("loss_logits_kernel launch");
@@ -529,7 +622,7 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
 
 extern "C" int64_t fh_vocab_loss_grad_workspace(const fh_vocab_loss* g) {
   if (check_loss("fh_vocab_loss_grad_workspace", g) != FH_OK) return -1;
-  return grad_room(*g, best_piece(*g)).bytes;
+  return best_room(*g);
 }
 
 extern "C" int64_t fh_vocab_loss_grad_least(const fh_vocab_loss* g) {
@@ -549,16 +642,10 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
   if ((reinterpret_cast<uintptr_t>(targets) | reinterpret_cast<uintptr_t>(lse)) % 4 != 0 ||
       reinterpret_cast<uintptr_t>(dloss) % dtype_size(g->loss_dtype) != 0)
     return fail(FH_INVALID_ARGUMENT, fn + ": targets, lse and dloss must be aligned to their elements");
-  // the widest piece, up to the best, that the workspace has room for
-  int64_t columns = best_piece(*g);
-  if (workspace_bytes < grad_room(*g, columns).bytes) {
-    const GradRoom least = grad_room(*g, kLeastPiece);
-    if (workspace_bytes < least.bytes) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
-    // room beside the sums between pieces, which a piece of the whole vocabulary would not need
-    columns = std::min(columns, (workspace_bytes - least.g) / (2 * least.g_rows) / kLeastPiece * kLeastPiece);
-    if (columns >= g->vocab) columns = up(g->vocab, kLeastPiece) - kLeastPiece;
-  }
-  const GradRoom room = grad_room(*g, columns);
+  if (workspace_bytes < least_room(*g)) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
+  const GradPlan plan = plan_for(*g, workspace_bytes);
+  const int64_t columns = plan.columns;
+  const GradRoom room = grad_room(*g, columns, plan.dx.splits);
   char* ws = static_cast<char*>(workspace);
   LossArgs a = loss_args(*g, x, w, targets);
   a.lse = const_cast<float*>(lse);
@@ -572,6 +659,7 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
   a.xc = reinterpret_cast<uint16_t*>(ws + room.xc);
   a.dx_sum = reinterpret_cast<float*>(ws + room.dx_sum);
   a.g = reinterpret_cast<uint16_t*>(ws + room.g);
+  a.splits = plan.dx.splits;
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, s, a);
   if (fh_status st = launch_status("loss_rows_kernel launch"); st != FH_OK) return st;
@@ -587,21 +675,26 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
       a.last_piece = a.last == g->vocab;
       a.ldg = up(a.last - a.first, kLeastPiece);
       if (g->tokens > 0) {
-        by_tile(g->tokens, a.ldg, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+        by_tile(tile_for(g->tokens, a.ldg), g->tokens, a.ldg, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
           hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
         });
         if (fh_status st = launch_status("loss_derivative_kernel launch"); st != FH_OK) return st;
         if (dx)
-          by_tile(g->tokens, g->dim, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+          by_tile(plan.dx.tile, g->tokens, g->dim, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+            grid.y = static_cast<uint32_t>(a.splits);
             hipLaunchKernelGGL((loss_dx_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
           });
         if (fh_status st = launch_status("loss_dx_kernel launch"); st != FH_OK) return st;
       }
       if (dw)
-        by_tile(a.last - a.first, g->dim, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
+        by_tile(tile_for(a.last - a.first, g->dim), a.last - a.first, g->dim, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
           hipLaunchKernelGGL((loss_dw_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
         });
       if (fh_status st = launch_status("loss_dw_kernel launch"); st != FH_OK) return st;
+    }
+    if (dx && a.splits > 1 && g->tokens > 0) {
+      hipLaunchKernelGGL((loss_dx_join_kernel<T>), dim3(static_cast<uint32_t>((g->tokens * (g->dim / 8) + 255) / 256)), dim3(256), 0, s, a);
+      return launch_status("loss_dx_join_kernel launch");
     }
     return FH_OK;
   });
