@@ -30,11 +30,11 @@ __device__ const uint4 kZeros = {0, 0, 0, 0};
 
 // depth: elements are zeros from k = depth on (read only where the operand's loads are declared to end unevenly). last: the greatest row
 // that exists; rows behind it are read as it is (column order: chunks of 8 rows that would end behind it end at it), and their products
-// belong to nobody.
+// belong to nobody. ld is less than 2^22.
 struct Operand {
   const uint16_t* p;
   int64_t ld;
-  const int32_t* rows;
+  const int32_t* rows;  // Lie::kListed
   int last, depth;
 };
 
@@ -71,17 +71,25 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 // The swizzle of a row's 16-byte chunks (row order): two rows share the banks' 256 bytes, so rows 2 apart must differ.
 __device__ __forceinline__ int row_swizzle(int row) { return (row >> 1) & 7; }
 
-// One operand's way: R rows of the tile by NW waves' loads, TX blocks of 16 rows read by each wave. UNEVEN: the depth may end inside a stage.
-template <int R, int TX, bool COLUMNS, bool UNEVEN, int NW>
+// How an operand lies: in rows, in rows that a list names, or in columns. UNEVEN: the depth may end inside a stage (one more comparison and
+// select per load: 3 to 7 % of a long product).
+enum class Lie { kRows, kListed, kColumns };
+
+// One operand's way: R rows of the tile by NW waves' loads, TX blocks of 16 rows read by each wave.
+template <int R, int TX, Lie LIE, bool UNEVEN, int NW>
 struct Feed {
+  static constexpr bool COLUMNS = LIE == Lie::kColumns;
   static constexpr int kBytes = R * kDepth * 2;
   static constexpr int kLoads = kBytes / 1024 / NW;  // load instructions per wave and stage
   static constexpr int kChunks = R / 8;              // column order: 16-byte chunks of a row of k
   static_assert(kBytes / 1024 % NW == 0, "a stage's loads split evenly over the waves");
   static_assert(!COLUMNS || (kChunks >= 8 && kChunks <= 64), "rows in [64, 512]");
 
-  const uint16_t* src[kLoads];
-  int64_t step;       // elements from a stage to the next
+  // The lane's place: 32 bits from an address that all lanes share, which a load takes as they are; 64 bits where rows come from a list.
+  const unsigned char* base;
+  const unsigned char* listed[kLoads];
+  uint32_t place[kLoads];
+  int64_t step;       // bytes from a stage to the next
   int first[kLoads];  // the lane's first k in a stage
   int depth;
   int off[COLUMNS ? TX : 2];  // where the lane reads, bytes within a stage: per block, or per step of 32 k
@@ -89,14 +97,17 @@ struct Feed {
   // r0: the tile's first row; mine: the wave's first row in the tile
   __device__ __forceinline__ void init(const Operand& o, int r0, int mine, int wave, int lane) {
     depth = o.depth;
+    const unsigned char* p = reinterpret_cast<const unsigned char*>(o.p);
     if constexpr (COLUMNS) {
-      step = kDepth * o.ld;
+      const int at = min(r0, o.last - 7);
+      base = p + static_cast<int64_t>(at) * 2;
+      step = kDepth * o.ld * 2;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int k = (wave * kLoads + j) * (64 / kChunks) + lane / kChunks;
         const int chunk = (lane % kChunks) ^ b_swizzle16<kChunks>(k);
         first[j] = k;
-        src[j] = o.p + k * o.ld + min(r0 + chunk * 8, o.last - 7);
+        place[j] = static_cast<uint32_t>(k) * static_cast<uint32_t>(o.ld * 2) + static_cast<uint32_t>(min(r0 + chunk * 8, o.last - 7) - at) * 2;
       }
       // lane r = q + 4 e of group g points at k 8 g + e, rows 4 q .. 4 q + 3 of a block; the second read is 4 k further on
       const int g = lane >> 4, q = lane & 3, e = (lane & 15) >> 2, k = 8 * g + e;
@@ -106,13 +117,18 @@ struct Feed {
         off[i] = k * (R * 2) + ((row >> 3) ^ b_swizzle16<kChunks>(k)) * 16 + (row & 7) * 2;
       }
     } else {
-      step = kDepth;
+      const int at = min(r0, o.last);
+      base = LIE == Lie::kListed ? p : p + static_cast<int64_t>(at) * o.ld * 2;
+      step = kDepth * 2;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int in_tile = (wave * kLoads + j) * 8 + (lane >> 3), row = min(r0 + in_tile, o.last);
         const int chunk = (lane & 7) ^ row_swizzle(in_tile);
         first[j] = chunk * 8;
-        src[j] = o.p + static_cast<int64_t>(o.rows != nullptr ? o.rows[row] : row) * o.ld + chunk * 8;
+        if constexpr (LIE == Lie::kListed)
+          listed[j] = p + o.rows[row] * o.ld * 2 + chunk * 16;
+        else
+          place[j] = static_cast<uint32_t>(row - at) * static_cast<uint32_t>(o.ld * 2) + chunk * 16;
       }
       const int row = mine + (lane & 15);
 #pragma unroll
@@ -122,8 +138,8 @@ struct Feed {
   // load instruction J of stage kt to this operand's part of a stage
   template <int J>
   __device__ __forceinline__ void load(int kt, unsigned char* to, int wave) const {
-    const uint16_t* from = src[J] + kt * step;
-    if constexpr (UNEVEN) from = first[J] < depth - kt * kDepth ? from : reinterpret_cast<const uint16_t*>(&kZeros);
+    const unsigned char* from = LIE == Lie::kListed ? listed[J] + kt * step : base + kt * step + place[J];
+    if constexpr (UNEVEN) from = first[J] < depth - kt * kDepth ? from : reinterpret_cast<const unsigned char*>(&kZeros);
     global_to_lds16(from, (FH_LDS void*)(to + (wave * kLoads + J) * 1024));
   }
   // read instruction N of blocks I0, I0 + 1, .. for step H of the stage part at `base`
@@ -147,12 +163,13 @@ struct Feed {
 // A stage is two steps. Small wave tiles hold two full sets of fragments and take a step in one phase; large ones take it in two, over halves
 // of the B blocks. While a phase's products run the next phase's fragments are read; in the stage's last one, after a barrier behind which
 // the next stage is there and this one is read, the stage STAGES ahead is loaded into this one's place.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, bool A_COLUMNS, bool B_COLUMNS, bool A_UNEVEN, bool B_UNEVEN>
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, Lie LIE_A, Lie LIE_B, bool UNEVEN_A, bool UNEVEN_B>
 struct Product {
   static constexpr int kWaves = WAVES_M * WAVES_N, kThreads = kWaves * 64;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 16, TN = WN / 16;
-  using FeedA = Feed<BM, TM, A_COLUMNS, A_UNEVEN, kWaves>;
-  using FeedB = Feed<BN, TN, B_COLUMNS, B_UNEVEN, kWaves>;
+  static constexpr bool A_COLUMNS = LIE_A == Lie::kColumns, B_COLUMNS = LIE_B == Lie::kColumns;
+  using FeedA = Feed<BM, TM, LIE_A, UNEVEN_A, kWaves>;
+  using FeedB = Feed<BN, TN, LIE_B, UNEVEN_B, kWaves>;
   static constexpr int kStage = FeedA::kBytes + FeedB::kBytes, kLds = STAGES * kStage;
   static constexpr int kLoads = FeedA::kLoads + FeedB::kLoads;
   static constexpr bool kOne = (TM + 2 * TN) * 8 + TM * TN * 4 <= 160;

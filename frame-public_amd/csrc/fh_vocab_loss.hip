@@ -154,9 +154,9 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a) {
 
 // ---- forward ----
 
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, false, false, true, true>;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kListed, Lie::kRows, UNEVEN, UNEVEN>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
   int tm, tn;
@@ -283,9 +283,9 @@ __device__ __forceinline__ void scale(typename P::Acc& acc, float f) {
 }
 
 // g of a piece: columns first .. last - 1 of the vocabulary, zeros behind them and in the tile's rows that no row with a target is.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, false, false, true, true>;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kRows, Lie::kRows, UNEVEN, UNEVEN>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
   int tm, tn;
@@ -321,9 +321,9 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(
   });
 }
 
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, false, true, false, true>;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kRows, Lie::kColumns, false, UNEVEN>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
   int tm, tn;
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256) void loss_dx_join_kernel(const LossArgs a) {
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, true, true, false, false>;
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kColumns, Lie::kColumns, false, false>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
   const int count = *a.count;
   int tm, tn;
@@ -413,8 +413,8 @@ fh_status check_loss(const std::string& fn, const fh_vocab_loss* g) {
       up(g->tokens, kTile) / kTile * (up(std::max(g->vocab, g->dim), kLeastPiece) / kTile) > 0x7fffffff)
     return fail(FH_INVALID_ARGUMENT, fn + ": too large");
   for (int64_t ld : {g->x_stride, g->w_stride})
-    if (ld < g->dim || ld % 8 != 0 || ld > (int64_t{1} << 32))
-      return fail(FH_INVALID_ARGUMENT, fn + ": strides must be multiples of 8, dim at least");
+    if (ld < g->dim || ld % 8 != 0 || ld >= (int64_t{1} << 22))
+      return fail(FH_INVALID_ARGUMENT, fn + ": strides must be multiples of 8, at least dim and less than 2^22");
   return FH_OK;
 }
 
@@ -604,7 +604,10 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
   if (g->tokens > 0) {
     const fh_status st = by_type(g->dtype, [&]<typename T>() {
       by_tile(tile_for(g->tokens, g->vocab), g->tokens, g->vocab, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
-        hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
+        if (g->dim % kDepth != 0)
+          hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN, true>), grid, dim3(WM * WN * 64), 0, s, a);
+        else
+          hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN, false>), grid, dim3(WM * WN * 64), 0, s, a);
       });
       return launch_status("loss_logits_kernel launch");
     });
@@ -676,13 +679,19 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
       a.ldg = up(a.last - a.first, kLeastPiece);
       if (g->tokens > 0) {
         by_tile(tile_for(g->tokens, a.ldg), g->tokens, a.ldg, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
-          hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
+          if (g->dim % kDepth != 0)
+            hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN, true>), grid, dim3(WM * WN * 64), 0, s, a);
+          else
+            hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN, false>), grid, dim3(WM * WN * 64), 0, s, a);
         });
         if (fh_status st = launch_status("loss_derivative_kernel launch"); st != FH_OK) return st;
         if (dx)
           by_tile(plan.dx.tile, g->tokens, g->dim, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
             grid.y = static_cast<uint32_t>(a.splits);
-            hipLaunchKernelGGL((loss_dx_kernel<T, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, s, a);
+            if ((a.last - a.first) % kDepth != 0)
+              hipLaunchKernelGGL((loss_dx_kernel<T, BM, BN, WM, WN, true>), grid, dim3(WM * WN * 64), 0, s, a);
+            else
+              hipLaunchKernelGGL((loss_dx_kernel<T, BM, BN, WM, WN, false>), grid, dim3(WM * WN * 64), 0, s, a);
           });
         if (fh_status st = launch_status("loss_dx_kernel launch"); st != FH_OK) return st;
       }
