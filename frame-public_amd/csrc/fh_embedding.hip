@@ -3,10 +3,10 @@
 // Forward: out[t] = scale * table[ids[t]], a copy bound by memory: a wave per 4 KB of a row, 16 bytes per lane and access.
 //
 // Gradient: dtable[v] = base[v] + scale * sum_{t: ids[t] = v} dout[t]. The tokens are sorted by id (stable, so a sum's order is the
-// tokens'), and the sorted list is cut into chunks of kChunk tokens whatever the ids are, so that frequent and rare ids are the same
+// tokens'), and the sorted list is cut into chunks of 8 or 16 tokens whatever the ids are, so that frequent and rare ids are the same
 // work: a wave sums the rows of a chunk id by id, ids that lie within a chunk are finished there, the rest leave fp32 parts that a
-// join adds in their order. No atomics on floats: every sum has one order. Rows that no token names are zeros or base's, written
-// by copies that the sort runs beside.
+// join adds in their order. No atomics on floats: every sum has one order. Rows that no token names are zeros or base's: all rows are
+// written so beside the sort, in the launches that a few workgroups of it would leave the chip idle in, and the sums overwrite theirs.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,21 +23,28 @@ typedef unsigned int u4_t __attribute__((ext_vector_type(4)));
 typedef u4_t u4_any __attribute__((aligned(2)));
 
 constexpr int kRowVectors = 4;  // 16-byte vectors of a row per lane (forward)
-constexpr int kChunk = 16;      // sorted tokens that one wave sums
 
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(typename Io<T>::storage));
 
-// V consecutive elements at p, or the first n of them (rows shorter than a vector).
+// A vector of consecutive elements at p, or the first n of them (rows shorter than a vector) and zeros.
+template <typename T>
+__device__ __forceinline__ uint4 load_bits(const typename Io<T>::storage* p, int n) {
+  if (n >= kVec<T>) {
+    const u4_t w = *reinterpret_cast<const u4_any*>(p);
+    return uint4{w[0], w[1], w[2], w[3]};
+  }
+  typename Io<T>::storage e[kVec<T>] = {};
+#pragma unroll
+  for (int x = 0; x < kVec<T>; ++x)
+    if (x < n) e[x] = p[x];
+  uint4 w;
+  __builtin_memcpy(&w, e, 16);
+  return w;
+}
 template <typename T, int V>
 __device__ __forceinline__ void load_elems(const typename Io<T>::storage* p, int n, float (&v)[V]) {
-  if (n >= V) {
-    const u4_t w = *reinterpret_cast<const u4_any*>(p);
-    unpack_vec<T>(uint4{w[0], w[1], w[2], w[3]}, v);
-  } else {
-#pragma unroll
-    for (int x = 0; x < V; ++x) v[x] = x < n ? Io<T>::load(p[x]) : 0.0f;
-  }
+  unpack_vec<T>(load_bits<T>(p, n), v);
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_elems(typename Io<T>::storage* p, int n, const float (&v)[V]) {
@@ -61,11 +68,11 @@ struct EmbedArgs {
   int tokens, vocab, dim;
   uint32_t blocks;  // of columns that one wave holds, in a row
   float scale;
-  // gradient: the tokens sorted by id, and the parts of ids that cross chunks [chunks][2][dim]
+  // gradient: the tokens sorted by id, and the parts of ids that cross chunks [chunks][2][part_ld], whole vectors
   uint32_t* keys;
   uint32_t* order;
   float* part;
-  int chunks;
+  int chunks, part_ld;  // chunks of CHUNK tokens
 };
 
 template <typename T>
@@ -99,7 +106,42 @@ __global__ __launch_bounds__(256) void embedding_kernel(const EmbedArgs a) {
 // ---- sorting the tokens by id: least significant digits first, stable ----
 
 constexpr int kSortThreads = 256, kSortItems = 8, kSortTile = kSortThreads * kSortItems, kSortWaves = kSortThreads / 64;
+// tokens that one workgroup sorts: 16,384 in 40 us, which base's writing hides; 32,768 in 140 (registers), where several workgroups take 55
+constexpr int kSortAlone = 16 * 1024;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
+
+// What a launch of the sort writes beside it: base's values, or zeros, in all of dtable; past the caches, which the sums want (33,000 tokens,
+// 131,072 x 4,096: 364 us in all, 398 through them).
+struct BaseArgs {
+  const void* base;
+  void* dtable;
+  int64_t end;         // in units of `size` bytes
+  int size;            // 16, or the elements' own where something is not aligned to 16
+};
+template <typename E>
+__device__ __forceinline__ void copy_base(const BaseArgs& a, int64_t at, int64_t step) {
+  const E* from = static_cast<const E*>(a.base);
+  E* to = static_cast<E*>(a.dtable);
+  if (from == nullptr) {
+    for (int64_t i = at; i < a.end; i += step) __builtin_nontemporal_store(E{}, to + i);
+    return;
+  }
+  for (int64_t i = at; i < a.end; i += 4 * step) {
+    E v[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[x] = from[min(i + x * step, a.end - 1)];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (i + x * step < a.end) __builtin_nontemporal_store(v[x], to + i + x * step);
+  }
+}
+// By workgroup `group` of `groups`.
+__device__ __forceinline__ void write_base(const BaseArgs& a, int group, int groups) {
+  const int64_t at = static_cast<int64_t>(group) * blockDim.x + threadIdx.x, step = static_cast<int64_t>(groups) * blockDim.x;
+  if (a.size == 16) copy_base<u4_t>(a, at, step);
+  else if (a.size == 4) copy_base<uint32_t>(a, at, step);
+  else copy_base<uint16_t>(a, at, step);
+}
 
 struct SortArgs {
   const int32_t* ids;        // the first pass reads the ids; those outside the vocabulary sort behind all others, as `vocab`
@@ -133,21 +175,38 @@ __device__ __forceinline__ void hand_over() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// SCATTER false: how many tokens of the tile have each digit. true: each token to its place.
-template <bool SCATTER>
-__global__ __launch_bounds__(kSortThreads) void sort_tile_kernel(const SortArgs a) {
+// How many tokens of the tile have each digit (integers: the additions' order changes nothing).
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortArgs a, const BaseArgs base) {
+  __shared__ uint32_t bins[kMaxBins];
+  if (static_cast<int>(blockIdx.x) >= a.tiles) return write_base(base, static_cast<int>(blockIdx.x) - a.tiles, static_cast<int>(gridDim.x) - a.tiles);
+  const int tid = threadIdx.x, nbins = 1 << a.bits, first = static_cast<int>(blockIdx.x) * kSortTile + tid;
+  uint32_t key[kSortItems];
+#pragma unroll
+  for (int j = 0; j < kSortItems; ++j) key[j] = first + j * kSortThreads < a.tokens ? sort_key(a, first + j * kSortThreads) : 0;
+  for (int b = tid; b < nbins; b += kSortThreads) bins[b] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kSortItems; ++j)
+    if (first + j * kSortThreads < a.tokens) atomicAdd(&bins[(key[j] >> a.shift) & (nbins - 1)], 1u);
+  __syncthreads();
+  for (int b = tid; b < nbins; b += kSortThreads) a.counts[b * a.tiles + blockIdx.x] = bins[b];
+}
+
+// Each token of the tile to its place.
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortArgs a) {
   __shared__ uint32_t bins[kSortWaves][kMaxBins];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int nbins = 1 << a.bits;
-  for (int b = tid; b < kSortWaves * kMaxBins; b += kSortThreads) (&bins[0][0])[b] = 0;
-  __syncthreads();
   const int first = static_cast<int>(blockIdx.x) * kSortTile + wave * (kSortTile / kSortWaves);
-  uint32_t key[kSortItems], rank[kSortItems];
+  uint32_t key[kSortItems], order[kSortItems], rank[kSortItems];
 #pragma unroll
   for (int j = 0; j < kSortItems; ++j) {
     const int i = first + j * 64 + lane;
     key[j] = i < a.tokens ? sort_key(a, i) : 0;
+    order[j] = a.order_in != nullptr && i < a.tokens ? a.order_in[i] : static_cast<uint32_t>(i);
   }
+  for (int b = tid; b < kSortWaves * kMaxBins; b += kSortThreads) (&bins[0][0])[b] = 0;
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < kSortItems; ++j) {
     const bool there = first + j * 64 + lane < a.tokens;
@@ -163,25 +222,20 @@ __global__ __launch_bounds__(kSortThreads) void sort_tile_kernel(const SortArgs 
   }
   __syncthreads();
   for (int b = tid; b < nbins; b += kSortThreads) {
-    uint32_t sum = 0;
+    uint32_t at = a.counts[b * a.tiles + blockIdx.x];
     for (int w = 0; w < kSortWaves; ++w) {
       const uint32_t n = bins[w][b];
-      if (SCATTER) bins[w][b] = sum;
-      sum += n;
+      bins[w][b] = at;
+      at += n;
     }
-    if (!SCATTER) a.counts[b * a.tiles + blockIdx.x] = sum;
   }
-  if constexpr (SCATTER) {
-    __syncthreads();
+  __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
-      const int i = first + j * 64 + lane;
-      if (i >= a.tokens) continue;
-      const uint32_t digit = (key[j] >> a.shift) & (nbins - 1);
-      const uint32_t to = a.counts[digit * a.tiles + blockIdx.x] + bins[wave][digit] + rank[j];
-      a.keys_out[to] = key[j];
-      a.order_out[to] = a.order_in != nullptr ? a.order_in[i] : static_cast<uint32_t>(i);
-    }
+  for (int j = 0; j < kSortItems; ++j) {
+    if (first + j * 64 + lane >= a.tokens) continue;
+    const uint32_t to = bins[wave][(key[j] >> a.shift) & (nbins - 1)] + rank[j];
+    a.keys_out[to] = key[j];
+    a.order_out[to] = order[j];
   }
 }
 
@@ -192,29 +246,28 @@ __global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts, int n
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) carry = 0;
   __syncthreads();
-  for (int at = 0; at < n; at += 4096) {
-    uint32_t v[4], sum = 0;
+  constexpr int EACH = 16;
+  for (int at = 0; at < n; at += 1024 * EACH) {
+    uint32_t v[EACH], sum = 0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int i = at + tid * 4 + x;
-      v[x] = i < n ? counts[i] : 0;
-      sum += v[x];
-    }
+    for (int x = 0; x < EACH; ++x) v[x] = at + tid * EACH + x < n ? counts[at + tid * EACH + x] : 0;
+#pragma unroll
+    for (int x = 0; x < EACH; ++x) sum += v[x];
     uint32_t scan = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t up = __shfl_up(scan, o, 64);
-      if (lane >= o) scan += up;
+      const uint32_t lower = __shfl_up(scan, o, 64);
+      if (lane >= o) scan += lower;
     }
     if (lane == 63) waves[wave] = scan;
     __syncthreads();
-    uint32_t before = carry;
-    for (int w = 0; w < wave; ++w) before += waves[w];
-    uint32_t run = before + scan - sum;
+    uint32_t run = carry + scan - sum;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int i = at + tid * 4 + x;
-      if (i < n) counts[i] = run;
+    for (int w = 0; w < 16; ++w)
+      if (w < wave) run += waves[w];
+#pragma unroll
+    for (int x = 0; x < EACH; ++x) {
+      if (at + tid * EACH + x < n) counts[at + tid * EACH + x] = run;
       run += v[x];
     }
     __syncthreads();
@@ -223,14 +276,93 @@ __global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts, int n
   }
 }
 
-// ---- dtable ----
-
-// base, or zeros, in every row; the sums overwrite the named ones. In elements of one size or 16 bytes.
-template <typename E>
-__global__ __launch_bounds__(256) void embedding_base_kernel(const E* base, E* dtable, int64_t n) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) dtable[i] = base != nullptr ? base[i] : E{};
+// The whole sort by one workgroup, ITEMS * 1024 tokens at most (fewer than 2^16: tokens and places in 16 bits), which go through LDS between the
+// passes, keys first, then the tokens.
+template <int ITEMS>
+__global__ __launch_bounds__(1024) void sort_all_kernel(const SortArgs a, int passes, const BaseArgs base) {
+  __shared__ uint32_t moved[ITEMS * 1024];
+  __shared__ uint16_t bins[16][kMaxBins];
+  __shared__ uint32_t sums[16];
+  if (blockIdx.x > 0) return write_base(base, static_cast<int>(blockIdx.x) - 1, static_cast<int>(gridDim.x) - 1);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nbins = 1 << a.bits, first = wave * ITEMS * 64 + lane;
+  uint32_t key[ITEMS], state[ITEMS];  // state: the token, and above it its rank, then its place
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const int i = first + j * 64;
+    state[j] = i;
+    key[j] = i < a.tokens ? sort_key(a, i) : 0;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * a.bits;
+    for (int b = tid; b < 16 * kMaxBins / 2; b += 1024) reinterpret_cast<uint32_t*>(&bins[0][0])[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const bool there = first + j * 64 < a.tokens;
+      const uint32_t digit = (key[j] >> shift) & (nbins - 1);
+      const uint64_t same = same_digit(digit, a.bits, __ballot(there));
+      const uint64_t below = same & ((1ull << lane) - 1);
+      const uint32_t seen = bins[wave][digit];
+      hand_over();
+      if (there && below == 0) bins[wave][digit] = static_cast<uint16_t>(seen + __popcll(same));
+      hand_over();
+      state[j] = (state[j] & 0xffffu) | ((seen + __popcll(below)) << 16);
+      __builtin_amdgcn_sched_barrier(0);  // one item's ballots at a time: the registers
+    }
+    __syncthreads();
+    // where each wave's share of each digit begins
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) sum += tid < nbins ? bins[w][tid] : 0;
+    uint32_t scan = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t lower = __shfl_up(scan, o, 64);
+      if (lane >= o) scan += lower;
+    }
+    if (lane == 63) sums[wave] = scan;
+    __syncthreads();
+    uint32_t at = scan - sum;
+#pragma unroll
+    for (int w = 0; w < 16; ++w)
+      if (w < wave) at += sums[w];
+    if (tid < nbins) {
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        const uint32_t n = bins[w][tid];
+        bins[w][tid] = static_cast<uint16_t>(at);
+        at += n;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      if (first + j * 64 >= a.tokens) continue;
+      const uint32_t to = bins[wave][(key[j] >> shift) & (nbins - 1)] + (state[j] >> 16);
+      state[j] = (state[j] & 0xffffu) | (to << 16);
+      moved[to] = key[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) key[j] = first + j * 64 < a.tokens ? moved[first + j * 64] : 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (first + j * 64 < a.tokens) moved[state[j] >> 16] = state[j] & 0xffffu;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) state[j] = first + j * 64 < a.tokens ? moved[first + j * 64] : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const int i = first + j * 64;
+    if (i >= a.tokens) continue;
+    a.keys_out[i] = key[j];
+    a.order_out[i] = state[j] & 0xffffu;
+  }
 }
+
+// ---- dtable ----
 
 // dtable[id] columns c .. <- base + scale * sum
 template <typename T>
@@ -247,9 +379,15 @@ __device__ __forceinline__ void finish_row(const EmbedArgs& a, uint32_t id, int 
   store_elems<T, V>(static_cast<S*>(a.out) + at, a.dim - c, sum);
 }
 
+// Columns c .. of a chunk's part: of the id that begins in it and goes on, or of the one that began earlier.
+template <int V>
+__device__ __forceinline__ float4* part_at(const EmbedArgs& a, int chunk, bool begins, int c) {
+  return reinterpret_cast<float4*>(a.part + (static_cast<int64_t>(chunk) * 2 + (begins ? 1 : 0)) * a.part_ld + c);
+}
+
 // A wave sums the rows of chunk `chunk` of the sorted tokens, 64 vectors of columns wide. An id's sum is finished if all of its tokens
 // lie in the chunk; otherwise it is a part: [0] of an id that began in an earlier chunk, [1] of one that begins here.
-template <typename T>
+template <typename T, int CHUNK>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const EmbedArgs a) {
   using S = typename Io<T>::storage;
   constexpr int V = kVec<T>;
@@ -258,41 +396,42 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const EmbedArgs a) {
   const int chunk = static_cast<int>(work / a.blocks);
   const int c = (static_cast<int>(work % a.blocks) * 64 + lane) * V;
   if (chunk >= a.chunks) return;
-  const int first = chunk * kChunk, n = min(kChunk, a.tokens - first);
-  // lane i: token i of the chunk; lane 16 the one behind the chunk, lane 17 the one before it
-  const int at = lane == kChunk + 1 ? first - 1 : first + min(lane, kChunk);
+  const int first = chunk * CHUNK, n = min(CHUNK, a.tokens - first);
+  // lane i: token i of the chunk; lane CHUNK the one behind the chunk, the next the one before it
+  const int at = lane == CHUNK + 1 ? first - 1 : first + min(lane, CHUNK);
   const uint32_t none = 0xffffffffu;
   const uint32_t mine = at >= 0 && at < a.tokens ? a.keys[at] : none;
   const uint32_t token = lane < n ? a.order[first + lane] : 0;
-  const uint32_t before = __builtin_amdgcn_readlane(mine, kChunk + 1);
-  float row[kChunk][V];
+  const uint32_t before = __builtin_amdgcn_readlane(mine, CHUNK + 1);
+  uint4 row[CHUNK];  // as it is stored
 #pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
+  for (int i = 0; i < CHUNK; ++i) {
     const uint32_t key = __builtin_amdgcn_readlane(mine, i);
     const int64_t t = __builtin_amdgcn_readlane(token, i);
-    if (i < n && key < static_cast<uint32_t>(a.vocab) && c < a.dim)
-      load_elems<T, V>(static_cast<const S*>(a.in) + t * a.ld + c, a.dim - c, row[i]);
+    row[i] = i < n && key < static_cast<uint32_t>(a.vocab) && c < a.dim ? load_bits<T>(static_cast<const S*>(a.in) + t * a.ld + c, a.dim - c)
+                                                                      : uint4{0, 0, 0, 0};
   }
   float sum[V];
 #pragma unroll
   for (int x = 0; x < V; ++x) sum[x] = 0.0f;
   bool began_here = __builtin_amdgcn_readlane(mine, 0) != before;
 #pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
+  for (int i = 0; i < CHUNK; ++i) {
     const uint32_t key = __builtin_amdgcn_readlane(mine, i);
     if (i >= n || key >= static_cast<uint32_t>(a.vocab)) break;
+    float v[V];
+    unpack_vec<T>(row[i], v);
 #pragma unroll
-    for (int x = 0; x < V; ++x) sum[x] += row[i][x];
+    for (int x = 0; x < V; ++x) sum[x] += v[x];
     const bool ends = __builtin_amdgcn_readlane(mine, i + 1) != key;
-    if (!ends && i + 1 < kChunk) continue;
+    if (!ends && i + 1 < CHUNK) continue;
     if (c < a.dim) {
       if (ends && began_here) {
         finish_row<T>(a, key, c, sum);
       } else {
-        float* p = a.part + (static_cast<int64_t>(chunk) * 2 + (began_here ? 1 : 0)) * a.dim + c;
+        float4* p = part_at<V>(a, chunk, began_here, c);
 #pragma unroll
-        for (int x = 0; x < V; ++x)
-          if (c + x < a.dim) p[x] = sum[x];
+        for (int x = 0; x < V / 4; ++x) p[x] = float4{sum[4 * x], sum[4 * x + 1], sum[4 * x + 2], sum[4 * x + 3]};
       }
     }
 #pragma unroll
@@ -301,43 +440,84 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const EmbedArgs a) {
   }
 }
 
-// The parts of an id that begins in chunk `chunk` and goes on behind it, in the chunks' order: each of the workgroup's four waves adds a
-// run of them, the runs are added in LDS. Workgroups of other chunks end at once.
+// sum += parts first .. last - 1 of the id that begins in chunk `chunk`, in their order; the loads of eight at a time
 template <typename T>
-__global__ __launch_bounds__(256) void embedding_join_kernel(const EmbedArgs a) {
-  constexpr int V = kVec<T>;
-  __shared__ float runs[4][64][V];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int chunk = static_cast<int>(blockIdx.x / a.blocks);
-  const int c = static_cast<int>((blockIdx.x % a.blocks) * 64 + lane) * V;
-  const int behind = (chunk + 1) * kChunk;  // the first token behind the chunk (there is one: the last chunk has no workgroup)
-  const uint32_t key = a.keys[behind];
-  if (key != a.keys[behind - 1] || key >= static_cast<uint32_t>(a.vocab)) return;
-  const int first = chunk * kChunk;
-  if (first > 0 && a.keys[first - 1] == key) return;  // began earlier
-  int low = behind + 1, high = a.tokens;              // the first token with a greater id
-  while (low < high) {
-    const int mid = low + (high - low) / 2;
-    if (a.keys[mid] > key) high = mid; else low = mid + 1;
+__device__ __forceinline__ void add_parts(const EmbedArgs& a, int chunk, int first, int last, int c, float (&sum)[kVec<T>]) {
+  constexpr int V = kVec<T>, AHEAD = 8;
+  for (int p = first; p < last; p += AHEAD) {
+    float4 v[AHEAD][V / 4];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int at = min(p + i, last - 1);
+#pragma unroll
+      for (int x = 0; x < V / 4; ++x) v[i][x] = part_at<V>(a, chunk + at, at == 0, c)[x];
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (p + i >= last) break;
+#pragma unroll
+      for (int x = 0; x < V / 4; ++x) {
+        sum[4 * x] += v[i][x].x;
+        sum[4 * x + 1] += v[i][x].y;
+        sum[4 * x + 2] += v[i][x].z;
+        sum[4 * x + 3] += v[i][x].w;
+      }
+    }
   }
-  const int parts = (low - 1) / kChunk - chunk + 1, each = (parts + 3) / 4;
+}
+
+// The parts of ids that go on behind the chunk they begin in. Each of the workgroup's four waves looks at one chunk; few parts are added by
+// the wave itself, many by the four waves together, each a run of them.
+template <typename T, int CHUNK>
+__global__ __launch_bounds__(256) void embedding_join_kernel(const EmbedArgs a) {
+  constexpr int V = kVec<T>, FEW = 8;
+  __shared__ float runs[4][64][V];
+  __shared__ int many[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int group = static_cast<int>(blockIdx.x / a.blocks) * 4;
+  const int c = static_cast<int>((blockIdx.x % a.blocks) * 64 + lane) * V;
+  const int chunk = group + wave, behind = (chunk + 1) * CHUNK;  // the first token behind the chunk
+  uint32_t key = 0;
+  int parts = 0;
+  if (behind < a.tokens) {
+    key = a.keys[behind];
+    const uint32_t last = a.keys[behind - 1], before = chunk > 0 ? a.keys[chunk * CHUNK - 1] : 0xffffffffu;
+    if (key == last && key != before && key < static_cast<uint32_t>(a.vocab)) {
+      int low = behind + 1, high = a.tokens;  // the first token with a greater id lies there: 64 looks at a time
+      while (low < high) {
+        const int step = (high - low + 63) / 64, at = low + lane * step;
+        const int upto = __popcll(__ballot(at < high && a.keys[min(at, high - 1)] <= key));
+        high = min(low + upto * step, high);
+        low = upto == 0 ? high : low + (upto - 1) * step + 1;
+      }
+      parts = (low - 1) / CHUNK - chunk + 1;
+    }
+  }
   float sum[V];
 #pragma unroll
   for (int x = 0; x < V; ++x) sum[x] = 0.0f;
-  if (c < a.dim)
-    for (int p = wave * each; p < min(parts, (wave + 1) * each); ++p) {
-      const float* q = a.part + (static_cast<int64_t>(chunk + p) * 2 + (p == 0 ? 1 : 0)) * a.dim + c;
-#pragma unroll
-      for (int x = 0; x < V; ++x)
-        if (c + x < a.dim) sum[x] += q[x];
-    }
-#pragma unroll
-  for (int x = 0; x < V; ++x) runs[wave][lane][x] = sum[x];
+  if (parts > 0 && parts <= FEW && c < a.dim) {
+    add_parts<T>(a, chunk, 0, parts, c, sum);
+    finish_row<T>(a, key, c, sum);
+  }
+  if (lane == 0) many[wave] = parts > FEW ? parts : 0;
   __syncthreads();
-  if (wave != 0 || c >= a.dim) return;
+  for (int w = 0; w < 4; ++w) {
+    const int all = many[w], each = (all + 3) / 4;
+    if (all == 0) continue;
 #pragma unroll
-  for (int x = 0; x < V; ++x) sum[x] = ((runs[0][lane][x] + runs[1][lane][x]) + runs[2][lane][x]) + runs[3][lane][x];
-  finish_row<T>(a, key, c, sum);
+    for (int x = 0; x < V; ++x) sum[x] = 0.0f;
+    if (c < a.dim) add_parts<T>(a, group + w, wave * each, min(all, (wave + 1) * each), c, sum);
+#pragma unroll
+    for (int x = 0; x < V; ++x) runs[wave][lane][x] = sum[x];
+    __syncthreads();
+    if (wave == w && c < a.dim) {
+#pragma unroll
+      for (int x = 0; x < V; ++x) sum[x] = ((runs[0][lane][x] + runs[1][lane][x]) + runs[2][lane][x]) + runs[3][lane][x];
+      finish_row<T>(a, key, c, sum);
+    }
+    __syncthreads();
+  }
 }
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
@@ -361,6 +541,7 @@ bool misaligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr
 struct GradPlan {
   int64_t tiles, chunks, passes, bits;
   int64_t list, counts, part, bytes;  // bytes of one list, offsets
+  int64_t part_ld, chunk;
 };
 GradPlan grad_plan(const fh_token_embedding& g) {
   GradPlan p{};
@@ -369,11 +550,16 @@ GradPlan grad_plan(const fh_token_embedding& g) {
   p.passes = (key_bits + kMaxBits - 1) / kMaxBits;
   p.bits = (key_bits + p.passes - 1) / p.passes;
   p.tiles = (g.tokens + kSortTile - 1) / kSortTile;
-  p.chunks = (g.tokens + kChunk - 1) / kChunk;
+  // as long chunks as give every CU 16 waves of 1 KB of a row (4,096 tokens of 1,024 bf16: 13.8 us for sums and join with 8, 17.7 with 16;
+  // 32,768 of 4,096: 153 with 8, 137 with 16)
+  const int64_t blocks = (g.dim * dtype_size(g.dtype) + 1023) / 1024;
+  p.chunk = (g.tokens + 15) / 16 * blocks >= 16 * device_cu_count() ? 16 : 8;
+  p.chunks = (g.tokens + p.chunk - 1) / p.chunk;
   p.list = (g.tokens * 4 + 15) / 16 * 16;
   p.counts = 4 * p.list;
   p.part = p.counts + (p.tiles * kMaxBins * 4 + 15) / 16 * 16;
-  p.bytes = p.part + p.chunks * 2 * g.dim * 4;
+  p.part_ld = (g.dim + 7) / 8 * 8;
+  p.bytes = p.part + p.chunks * 2 * p.part_ld * 4;
   return p;
 }
 
@@ -426,42 +612,61 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   if (workspace_bytes < p.bytes) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
   hipStream_t s = static_cast<hipStream_t>(stream);
 
-  if (base != dtable) {
-    const int64_t bytes = g->vocab * g->dim * esz;
-    const bool wide = bytes % 16 == 0 && !misaligned(base, 16) && !misaligned(dtable, 16);
-    const int64_t n = wide ? bytes / 16 : bytes / esz;
-    const dim3 grid(static_cast<uint32_t>(std::min<int64_t>((n + 255) / 256, 8 * device_cu_count())));
-    if (wide)
-      hipLaunchKernelGGL((embedding_base_kernel<uint4>), grid, dim3(256), 0, s, static_cast<const uint4*>(base), static_cast<uint4*>(dtable), n);
-    else if (esz == 4)
-      hipLaunchKernelGGL((embedding_base_kernel<uint32_t>), grid, dim3(256), 0, s, static_cast<const uint32_t*>(base), static_cast<uint32_t*>(dtable), n);
-    else
-      hipLaunchKernelGGL((embedding_base_kernel<uint16_t>), grid, dim3(256), 0, s, static_cast<const uint16_t*>(base), static_cast<uint16_t*>(dtable), n);
-    if (fh_status st = launch_status("embedding_base_kernel launch"); st != FH_OK) return st;
-  }
-  if (g->tokens == 0) return FH_OK;
+  // base (or zeros), beside the sort: beside its first launch, where it takes more than one (shares of 180 MB each of six launches: 256 us, 169 in one)
+  const int64_t bytes = g->vocab * g->dim * esz;
+  BaseArgs share{};
+  share.base = base;
+  share.dtable = dtable;
+  share.size = bytes % 16 == 0 && !misaligned(base, 16) && !misaligned(dtable, 16) ? 16 : static_cast<int>(esz);
+  share.end = base == dtable ? 0 : bytes / share.size;
+  const bool alone = g->tokens <= kSortAlone;  // one workgroup sorts
+  // workgroups of `threads` that write base: as many as run at once beside `busy`, so that none waits for a second round
+  auto sharers = [&](int64_t threads, int64_t of_a_cu, int64_t busy) {
+    return static_cast<uint32_t>(std::min<int64_t>((share.end + threads - 1) / threads, of_a_cu * device_cu_count() - busy));
+  };
 
   char* ws = static_cast<char*>(workspace);
   auto list = [&](int i) { return reinterpret_cast<uint32_t*>(ws + i * p.list); };
   SortArgs sort{};
   sort.ids = ids;
-  sort.counts = reinterpret_cast<uint32_t*>(ws + p.counts);
   sort.tokens = static_cast<int>(g->tokens);
   sort.vocab = static_cast<int>(g->vocab);
-  sort.tiles = static_cast<int>(p.tiles);
   sort.bits = static_cast<int>(p.bits);
-  for (int pass = 0; pass < p.passes; ++pass) {
-    sort.shift = pass * sort.bits;
-    sort.keys_out = list(2 * (pass & 1));
-    sort.order_out = list(2 * (pass & 1) + 1);
-    hipLaunchKernelGGL((sort_tile_kernel<false>), dim3(static_cast<uint32_t>(p.tiles)), dim3(kSortThreads), 0, s, sort);
-    if (fh_status st = launch_status("sort_tile_kernel launch"); st != FH_OK) return st;
-    hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, s, sort.counts, static_cast<int>(p.tiles << p.bits));
-    if (fh_status st = launch_status("sort_scan_kernel launch"); st != FH_OK) return st;
-    hipLaunchKernelGGL((sort_tile_kernel<true>), dim3(static_cast<uint32_t>(p.tiles)), dim3(kSortThreads), 0, s, sort);
-    if (fh_status st = launch_status("sort_tile_kernel launch"); st != FH_OK) return st;
-    sort.keys_in = sort.keys_out;
-    sort.order_in = sort.order_out;
+  if (g->tokens == 0) {
+    if (share.end == 0) return FH_OK;
+    hipLaunchKernelGGL(sort_count_kernel, dim3(sharers(kSortThreads, 8, 0)), dim3(kSortThreads), 0, s, sort, share);
+    return launch_status("sort_count_kernel launch");
+  }
+  if (alone) {
+    sort.keys_out = list(0);
+    sort.order_out = list(1);
+    const int passes = static_cast<int>(p.passes);
+    const dim3 grid(1 + sharers(1024, 1, 1));
+    if (g->tokens <= 1024)
+      hipLaunchKernelGGL((sort_all_kernel<1>), grid, dim3(1024), 0, s, sort, passes, share);
+    else if (g->tokens <= 4096)
+      hipLaunchKernelGGL((sort_all_kernel<4>), grid, dim3(1024), 0, s, sort, passes, share);
+    else
+      hipLaunchKernelGGL((sort_all_kernel<16>), grid, dim3(1024), 0, s, sort, passes, share);
+    if (fh_status st = launch_status("sort_all_kernel launch"); st != FH_OK) return st;
+  } else {
+    sort.counts = reinterpret_cast<uint32_t*>(ws + p.counts);
+    sort.tiles = static_cast<int>(p.tiles);
+    const uint32_t tiles = static_cast<uint32_t>(p.tiles);
+    for (int pass = 0; pass < p.passes; ++pass) {
+      sort.shift = pass * sort.bits;
+      sort.keys_out = list(2 * (pass & 1));
+      sort.order_out = list(2 * (pass & 1) + 1);
+      const uint32_t groups = pass == 0 ? sharers(kSortThreads, 8, 0) : 0;
+      hipLaunchKernelGGL(sort_count_kernel, dim3(tiles + groups), dim3(kSortThreads), 0, s, sort, share);
+      if (fh_status st = launch_status("sort_count_kernel launch"); st != FH_OK) return st;
+      hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, s, sort.counts, static_cast<int>(p.tiles << p.bits));
+      if (fh_status st = launch_status("sort_scan_kernel launch"); st != FH_OK) return st;
+      hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles), dim3(kSortThreads), 0, s, sort);
+      if (fh_status st = launch_status("sort_scatter_kernel launch"); st != FH_OK) return st;
+      sort.keys_in = sort.keys_out;
+      sort.order_in = sort.order_out;
+    }
   }
 
   EmbedArgs a{};
@@ -477,14 +682,16 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   a.order = sort.order_out;
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.chunks = static_cast<int>(p.chunks);
+  a.part_ld = static_cast<int>(p.part_ld);
   const int64_t width = 64 * 16 / esz;
   a.blocks = static_cast<uint32_t>((g->dim + width - 1) / width);
-  auto launch = [&]<typename T>() {
-    hipLaunchKernelGGL((embedding_sum_kernel<T>), dim3(static_cast<uint32_t>((p.chunks * a.blocks + 3) / 4)), dim3(256), 0, s, a);
+  auto launch = [&]<typename T, int CHUNK>() {
+    hipLaunchKernelGGL((embedding_sum_kernel<T, CHUNK>), dim3(static_cast<uint32_t>((p.chunks * a.blocks + 3) / 4)), dim3(256), 0, s, a);
     if (fh_status st = launch_status("embedding_sum_kernel launch"); st != FH_OK || p.chunks == 1) return st;
-    hipLaunchKernelGGL((embedding_join_kernel<T>), dim3(static_cast<uint32_t>((p.chunks - 1) * a.blocks)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((embedding_join_kernel<T, CHUNK>), dim3(static_cast<uint32_t>((p.chunks + 3) / 4 * a.blocks)), dim3(256), 0, s, a);
     return launch_status("embedding_join_kernel launch");
   };
-  if (g->dtype == FH_F32) return launch.template operator()<float>();
-  return g->dtype == FH_F16 ? launch.template operator()<f16_t>() : launch.template operator()<bf16_t>();
+  auto by_chunk = [&]<typename T>() { return p.chunk == 16 ? launch.template operator()<T, 16>() : launch.template operator()<T, 8>(); };
+  if (g->dtype == FH_F32) return by_chunk.template operator()<float>();
+  return g->dtype == FH_F16 ? by_chunk.template operator()<f16_t>() : by_chunk.template operator()<bf16_t>();
 }
