@@ -110,37 +110,24 @@ constexpr int kSortThreads = 256, kSortItems = 8, kSortTile = kSortThreads * kSo
 constexpr int kSortAlone = 16 * 1024;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 
-// What a launch of the sort writes beside it: base's values, or zeros, in all of dtable; past the caches, which the sums want (33,000 tokens,
-// 131,072 x 4,096: 364 us in all, 398 through them).
+// What a launch of the sort writes beside it: base's values, or zeros, in all of dtable. One store per thread, past the caches, which the
+// sums want (131,072 x 4,096 bf16 and one token: 177 us; a loop over the table in as many threads as run at once 225, four stores per
+// thread 218, through the caches 200 and 60 us more for the sums).
 struct BaseArgs {
   const void* base;
   void* dtable;
-  int64_t end;         // in units of `size` bytes
-  int size;            // 16, or the elements' own where something is not aligned to 16
+  int64_t end;  // in units of `size` bytes
+  int size;     // 16, or the elements' own where something is not aligned to 16
 };
 template <typename E>
-__device__ __forceinline__ void copy_base(const BaseArgs& a, int64_t at, int64_t step) {
-  const E* from = static_cast<const E*>(a.base);
-  E* to = static_cast<E*>(a.dtable);
-  if (from == nullptr) {
-    for (int64_t i = at; i < a.end; i += step) __builtin_nontemporal_store(E{}, to + i);
-    return;
-  }
-  for (int64_t i = at; i < a.end; i += 4 * step) {
-    E v[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) v[x] = from[min(i + x * step, a.end - 1)];
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (i + x * step < a.end) __builtin_nontemporal_store(v[x], to + i + x * step);
-  }
+__device__ __forceinline__ void copy_base(const BaseArgs& a, int64_t at) {
+  if (at < a.end) __builtin_nontemporal_store(a.base != nullptr ? static_cast<const E*>(a.base)[at] : E{}, static_cast<E*>(a.dtable) + at);
 }
-// By workgroup `group` of `groups`.
-__device__ __forceinline__ void write_base(const BaseArgs& a, int group, int groups) {
-  const int64_t at = static_cast<int64_t>(group) * blockDim.x + threadIdx.x, step = static_cast<int64_t>(groups) * blockDim.x;
-  if (a.size == 16) copy_base<u4_t>(a, at, step);
-  else if (a.size == 4) copy_base<uint32_t>(a, at, step);
-  else copy_base<uint16_t>(a, at, step);
+__device__ __forceinline__ void write_base(const BaseArgs& a, int group) {
+  const int64_t at = static_cast<int64_t>(group) * blockDim.x + threadIdx.x;
+  if (a.size == 16) copy_base<u4_t>(a, at);
+  else if (a.size == 4) copy_base<uint32_t>(a, at);
+  else copy_base<uint16_t>(a, at);
 }
 
 struct SortArgs {
@@ -178,7 +165,7 @@ __device__ __forceinline__ void hand_over() {
 // How many tokens of the tile have each digit (integers: the additions' order changes nothing).
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortArgs a, const BaseArgs base) {
   __shared__ uint32_t bins[kMaxBins];
-  if (static_cast<int>(blockIdx.x) >= a.tiles) return write_base(base, static_cast<int>(blockIdx.x) - a.tiles, static_cast<int>(gridDim.x) - a.tiles);
+  if (static_cast<int>(blockIdx.x) >= a.tiles) return write_base(base, static_cast<int>(blockIdx.x) - a.tiles);
   const int tid = threadIdx.x, nbins = 1 << a.bits, first = static_cast<int>(blockIdx.x) * kSortTile + tid;
   uint32_t key[kSortItems];
 #pragma unroll
@@ -283,7 +270,7 @@ __global__ __launch_bounds__(1024) void sort_all_kernel(const SortArgs a, int pa
   __shared__ uint32_t moved[ITEMS * 1024];
   __shared__ uint16_t bins[16][kMaxBins];
   __shared__ uint32_t sums[16];
-  if (blockIdx.x > 0) return write_base(base, static_cast<int>(blockIdx.x) - 1, static_cast<int>(gridDim.x) - 1);
+  if (blockIdx.x > 0) return write_base(base, static_cast<int>(blockIdx.x) - 1);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nbins = 1 << a.bits, first = wave * ITEMS * 64 + lane;
   uint32_t key[ITEMS], state[ITEMS];  // state: the token, and above it its rank, then its place
 #pragma unroll
@@ -527,7 +514,8 @@ fh_status check_embedding(const std::string& fn, const fh_token_embedding* g) {
   if (!is_supported_float(g->dtype)) return fail(FH_UNIMPLEMENTED, fn + ": dtype must be f32, f16 or bf16");
   if (g->tokens < 0 || g->vocab < 1 || g->dim < 1) return fail(FH_INVALID_ARGUMENT, fn + ": bad tokens, vocab or dim");
   // the grids' and the sort's indexes are 32-bit
-  if (g->vocab > 0x7ffffffe || g->dim > (1 << 20) || g->tokens > (1 << 28) || g->tokens * ((g->dim + 63) / 64) > kMaxGrid)
+  if (g->vocab > 0x7ffffffe || g->dim > (1 << 20) || g->tokens > (1 << 28) || g->tokens * ((g->dim + 63) / 64) > kMaxGrid ||
+      g->vocab * g->dim > (int64_t{1} << 38))
     return fail(FH_INVALID_ARGUMENT, fn + ": too large");
   if (g->row_stride < g->dim) return fail(FH_INVALID_ARGUMENT, fn + ": row_stride is less than dim");
   if (g->row_stride > (int64_t{1} << 40)) return fail(FH_INVALID_ARGUMENT, fn + ": too large");
@@ -612,7 +600,7 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   if (workspace_bytes < p.bytes) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
   hipStream_t s = static_cast<hipStream_t>(stream);
 
-  // base (or zeros), beside the sort: beside its first launch, where it takes more than one (shares of 180 MB each of six launches: 256 us, 169 in one)
+  // base (or zeros), beside the sort: beside its first launch, where it takes more than one (shares beside each of six: slower than one after the other)
   const int64_t bytes = g->vocab * g->dim * esz;
   BaseArgs share{};
   share.base = base;
@@ -620,10 +608,8 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   share.size = bytes % 16 == 0 && !misaligned(base, 16) && !misaligned(dtable, 16) ? 16 : static_cast<int>(esz);
   share.end = base == dtable ? 0 : bytes / share.size;
   const bool alone = g->tokens <= kSortAlone;  // one workgroup sorts
-  // workgroups of `threads` that write base: as many as run at once beside `busy`, so that none waits for a second round
-  auto sharers = [&](int64_t threads, int64_t of_a_cu, int64_t busy) {
-    return static_cast<uint32_t>(std::min<int64_t>((share.end + threads - 1) / threads, of_a_cu * device_cu_count() - busy));
-  };
+  // workgroups of `threads` that write base
+  auto sharers = [&](int64_t threads) { return static_cast<uint32_t>((share.end + threads - 1) / threads); };
 
   char* ws = static_cast<char*>(workspace);
   auto list = [&](int i) { return reinterpret_cast<uint32_t*>(ws + i * p.list); };
@@ -634,14 +620,14 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   sort.bits = static_cast<int>(p.bits);
   if (g->tokens == 0) {
     if (share.end == 0) return FH_OK;
-    hipLaunchKernelGGL(sort_count_kernel, dim3(sharers(kSortThreads, 8, 0)), dim3(kSortThreads), 0, s, sort, share);
+    hipLaunchKernelGGL(sort_count_kernel, dim3(sharers(kSortThreads)), dim3(kSortThreads), 0, s, sort, share);
     return launch_status("sort_count_kernel launch");
   }
   if (alone) {
     sort.keys_out = list(0);
     sort.order_out = list(1);
     const int passes = static_cast<int>(p.passes);
-    const dim3 grid(1 + sharers(1024, 1, 1));
+    const dim3 grid(1 + sharers(1024));
     if (g->tokens <= 1024)
       hipLaunchKernelGGL((sort_all_kernel<1>), grid, dim3(1024), 0, s, sort, passes, share);
     else if (g->tokens <= 4096)
@@ -657,7 +643,7 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
       sort.shift = pass * sort.bits;
       sort.keys_out = list(2 * (pass & 1));
       sort.order_out = list(2 * (pass & 1) + 1);
-      const uint32_t groups = pass == 0 ? sharers(kSortThreads, 8, 0) : 0;
+      const uint32_t groups = pass == 0 ? sharers(kSortThreads) : 0;
       hipLaunchKernelGGL(sort_count_kernel, dim3(tiles + groups), dim3(kSortThreads), 0, s, sort, share);
       if (fh_status st = launch_status("sort_count_kernel launch"); st != FH_OK) return st;
       hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, s, sort.counts, static_cast<int>(p.tiles << p.bits));

@@ -29,7 +29,7 @@ def loss(**over):
     (dict(dtype=1), UNIMPLEMENTED), (dict(dtype=6), UNIMPLEMENTED), (dict(tokens=-1), INVALID), (dict(vocab=0), INVALID),
     (dict(vocab=2 ** 31), INVALID), (dict(dim=0), INVALID), (dict(dim=2 ** 21, row_stride=2 ** 21), INVALID),
     (dict(tokens=2 ** 29), INVALID), (dict(tokens=2 ** 28, dim=2 ** 20, row_stride=2 ** 20), INVALID), (dict(row_stride=63), INVALID),
-    (dict(row_stride=2 ** 41), INVALID), (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID),
+    (dict(row_stride=2 ** 41), INVALID), (dict(vocab=2 ** 30, dim=512, row_stride=512), INVALID), (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID),
 ], ids=str)
 def test_embedding_sizes_are_refused(over, code):
     lib, r = abi.lib(), ctypes.byref(table(**over))
