@@ -121,6 +121,14 @@ class Graph:
         return self.op("packed_attention", [q, k, v, cu_seqlens], q.shape,
                        {"heads": int(heads), "kv_heads": int(kv_heads), "causal": bool(causal), "scale": float(scale)})
 
+    def embedding(self, table, ids, scale=1.0):
+        """Rows of table [vocab, dim] by int32 ids, times scale; zeros for ids outside the vocabulary."""
+        return self.op("embedding", [table, ids], (ids.shape[0], table.shape[1]), {"scale": float(scale)})
+
+    def vocab_loss(self, x, w, targets, mean=True):
+        """Softmax cross entropy of x w^T against int32 targets, one value; rows whose target is outside the vocabulary do not count."""
+        return self.op("vocab_loss", [x, w, targets], (), {"mean": bool(mean)})
+
     def layer_norm(self, x, g, b, eps=1e-5):
         return self.op("layer_norm", [x, g, b], x.shape, {"eps": float(eps)})
 
@@ -398,23 +406,46 @@ def transformer_block(batch=8, seq=512, d_model=1024, heads=16, ffn=4096, dtype=
     return g, shapes
 
 
+def _decoder_shapes(d_model, heads, kv_heads, ffn):
+    """Parameters of a decoder layer: ln1_g, ln1_b, wq, wk, wv, wo, ln2_g, ln2_b, w1, w2."""
+    kv = kv_heads * (d_model // heads)
+    return [(d_model,), (d_model,), (d_model, d_model), (d_model, kv), (d_model, kv), (d_model, d_model), (d_model,), (d_model,),
+            (d_model, ffn), (ffn, d_model)]
+
+
+def _decoder_layer(g, x, cu, params, heads, kv_heads):
+    ln1_g, ln1_b, wq, wk, wv, wo, ln2_g, ln2_b, w1, w2 = params
+    h1 = g.layer_norm(x, ln1_g, ln1_b)
+    q, k, v = (g.matmul(h1, w) for w in (wq, wk, wv))
+    h = g.add(g.matmul(g.packed_attention(q, k, v, cu, heads, kv_heads), wo), x)
+    return g.add(g.matmul(g.gelu(g.matmul(g.layer_norm(h, ln2_g, ln2_b), w1)), w2), h)
+
+
+def language_model(tokens, batch, vocab, d_model=1024, heads=16, kv_heads=4, ffn=4096, layers=1, tied=True, dtype=BF16, device="hip"):
+    """A language model's loss on `batch` sequences packed in `tokens` rows: embedding, decoder layers, a final layer norm, vocab_loss. Inputs:
+    ids (int32 [tokens]), cu_seqlens (int32 [batch + 1]), targets (int32 [tokens], -1 where none), then the parameters: the table
+    [vocab, d_model], the layers', the last norm's two, and (not tied) an output table. Returns the graph and the parameters' shapes."""
+    g = Graph(device)
+    ids, cu, targets = g.input(I32, (tokens,)), g.input(I32, (batch + 1,)), g.input(I32, (tokens,))
+    layer = _decoder_shapes(d_model, heads, kv_heads, ffn)
+    shapes = [(vocab, d_model)] + layer * layers + [(d_model,), (d_model,)] + ([] if tied else [(vocab, d_model)])
+    p = [g.input(dtype, s) for s in shapes]
+    x = g.embedding(p[0], ids)
+    for i in range(layers):
+        x = _decoder_layer(g, x, cu, p[1 + i * len(layer):1 + (i + 1) * len(layer)], heads, kv_heads)
+    norm = 1 + layers * len(layer)
+    g.output(g.vocab_loss(g.layer_norm(x, p[norm], p[norm + 1]), p[0] if tied else p[-1], targets))
+    return g, shapes
+
+
 def decoder_block(tokens, batch, d_model=1024, heads=16, kv_heads=4, ffn=4096, dtype=BF16, device="hip", train=False):
     """The pre-LN block with causal attention over packed sequences and grouped heads: `batch` sequences of any lengths in
     `tokens` rows, given by the second input, cu_seqlens (int32 [batch + 1]). Returns the graph and the parameters' shapes;
     train=True adds a target input after them and outputs mse_loss(y, target)."""
     g = Graph(device)
-    dh = d_model // heads
     x, cu = g.input(dtype, (tokens, d_model)), g.input(I32, (batch + 1,))
-    names = ["ln1_g", "ln1_b", "wq", "wk", "wv", "wo", "ln2_g", "ln2_b", "w1", "w2"]
-    shapes = [(d_model,), (d_model,), (d_model, d_model), (d_model, kv_heads * dh), (d_model, kv_heads * dh),
-              (d_model, d_model), (d_model,), (d_model,), (d_model, ffn), (ffn, d_model)]
-    p = {n: g.input(dtype, s) for n, s in zip(names, shapes)}
-    h1 = g.layer_norm(x, p["ln1_g"], p["ln1_b"])
-    q, k, v = (g.matmul(h1, p[w]) for w in ("wq", "wk", "wv"))
-    attn = g.packed_attention(q, k, v, cu, heads, kv_heads)
-    h = g.add(g.matmul(attn, p["wo"]), x)
-    h2 = g.layer_norm(h, p["ln2_g"], p["ln2_b"])
-    y = g.add(g.matmul(g.gelu(g.matmul(h2, p["w1"])), p["w2"]), h)
+    shapes = _decoder_shapes(d_model, heads, kv_heads, ffn)
+    y = _decoder_layer(g, x, cu, [g.input(dtype, s) for s in shapes], heads, kv_heads)
     g.output(g.mse_loss(y, g.input(dtype, (tokens, d_model))) if train else y)
     return g, shapes
 

@@ -228,6 +228,13 @@ inline constexpr std::string_view kPackedAttentionOp = "hip_packed_attention_int
 // packed_attention_grad_internal with the forward's lse: (q, k, v, cu_seqlens, y, lse, gy) -> gq, gk, gv, workspace.
 inline constexpr std::string_view kPackedAttentionGradOp = "hip_packed_attention_grad_internal";
 
+// embedding_grad_internal with a planned workspace, and (three inputs) on top of another gradient of the table:
+// (gy, ids[, base]) -> gtable, workspace.
+inline constexpr std::string_view kEmbeddingGradOp = "hip_embedding_grad_internal";
+// vocab_loss(x, w, targets) -> loss, lse [tokens] fp32, workspace; its gradient reads lse: (x, w, targets, lse, gy) -> gx, gw, workspace.
+inline constexpr std::string_view kVocabLossOp = "hip_vocab_loss_internal";
+inline constexpr std::string_view kVocabLossGradOp = "hip_vocab_loss_grad_internal";
+
 // The graph HipBackend::compile plans for `graph` (already through the pass pipeline): attention, epilogue
 // (opt_level >= 1) and channels-last conv lowering applied to a copy. Host-only; used by compile and by
 // frame_hip_lowered_text.

@@ -1414,6 +1414,110 @@ Status lower_packed_attention(ir::Graph& g) {
   return Status::ok();
 }
 
+// The two ends of a language model get their workspaces planned: embedding_grad_internal, vocab_loss and the vocab_loss_grad_internal whose
+// forward the graph holds (which hands it the rows' log-sum-exps) become their internal forms, at every opt level. At opt_level >= 1 an add
+// of an embedding's gradient to another gradient of the same table (tied weights) goes into the former, which is then summed and
+// rounded once. Types that the kernels do not take stay as they are and are named when the step runs.
+Status lower_language_ends(ir::Graph& g, int32_t opt_level) {
+  auto sixteen = [](const ir::Value* v) {
+    const DTypeCode d = v->type().dtype.code();
+    return d == DTypeCode::kBFloat16 || d == DTypeCode::kFloat16;
+  };
+  auto loss_of = [&](const ir::Node* n) -> const ir::Node* {
+    if (n->op() != "vocab_loss_grad_internal" || n->inputs().size() != 5 || !sixteen(n->inputs()[0])) return nullptr;
+    const ir::Node* f = n->inputs()[3]->producer();
+    if (f == nullptr || f->op() != "vocab_loss" || f->attrs() != n->attrs()) return nullptr;
+    for (size_t i = 0; i < 3; ++i)
+      if (f->inputs()[i] != n->inputs()[i]) return nullptr;
+    return f;
+  };
+  auto is_embedding_grad = [](const ir::Node* n) {
+    return n != nullptr && n->op() == "embedding_grad_internal" && n->inputs().size() == 2 && n->outputs().size() == 1;
+  };
+  std::unordered_map<const ir::Value*, int> uses;
+  bool any = false;
+  for (const ir::Node* n : g.topological_order()) {
+    for (const ir::Value* v : n->inputs()) ++uses[v];
+    any = any || is_embedding_grad(n) || (n->op() == "vocab_loss" && n->inputs().size() == 3 && sixteen(n->inputs()[0]));
+  }
+  if (!any) return Status::ok();
+  for (const ir::Value* v : g.outputs()) ++uses[v];
+  // add -> the operand that is an embedding's gradient and nothing else's; those gradients
+  std::unordered_map<const ir::Node*, size_t> sums;
+  std::unordered_set<const ir::Node*> folded;
+  if (opt_level >= 1)
+    for (const ir::Node* n : g.topological_order()) {
+      if (n->op() != "add" || n->inputs().size() != 2 || n->inputs()[0] == n->inputs()[1]) continue;
+      for (size_t i = 0; i < 2 && sums.count(n) == 0; ++i)
+        if (is_embedding_grad(n->inputs()[i]->producer()) && uses[n->inputs()[i]] == 1 && n->inputs()[1 - i]->type().dtype == n->inputs()[i]->type().dtype) {
+          sums.emplace(n, i);
+          folded.insert(n->inputs()[i]->producer());
+        }
+    }
+
+  auto scratch = [](const ir::Value* like, int64_t bytes) {  // (a geometry that the kernels refuse is named when the step runs)
+    ir::TensorType t = like->type();
+    t.dtype = DType::of<float>();
+    t.shape = Shape({(std::max<int64_t>(bytes, 4) + 3) / 4});
+    return t;
+  };
+  std::unordered_map<const ir::Value*, ir::Value*> map;
+  std::unordered_map<const ir::Node*, ir::Value*> lse;
+  ir::Graph out{std::string(g.name())};
+  for (const ir::Node* n : g.topological_order()) {
+    if (n->op() == ir::kGraphInputOp) {
+      Result<ir::Value*> v = out.add_graph_input(n->outputs()[0].type());
+      if (!v.is_ok()) return v.status();
+      map[&n->outputs()[0]] = v.value();
+      continue;
+    }
+    if (folded.count(n)) continue;  // stands where the add did
+    const ir::Node* source = n;     // whose inputs and attributes
+    std::vector<ir::Value*> ins;
+    std::vector<ir::TensorType> types;
+    for (const ir::Value& o : n->outputs()) types.push_back(o.type());
+    const auto sum = sums.find(n);
+    if (sum != sums.end()) source = n->inputs()[sum->second]->producer();
+    for (const ir::Value* v : source->inputs()) ins.push_back(map.at(v));
+    std::string op(source->op());
+    const bool loss = n->op() == "vocab_loss" && n->inputs().size() == 3 && sixteen(n->inputs()[0]);
+    if (is_embedding_grad(source)) {
+      op = std::string(kEmbeddingGradOp);
+      if (sum != sums.end()) ins.push_back(map.at(n->inputs()[1 - sum->second]));
+      const Shape& table = source->outputs()[0].type().shape;
+      fh_token_embedding e{};
+      e.dtype = static_cast<int32_t>(source->inputs()[0]->type().dtype.code());
+      e.tokens = source->inputs()[0]->type().shape.dim(0);
+      e.vocab = table.dim(0);
+      e.dim = e.row_stride = table.dim(1);
+      types.push_back(scratch(source->inputs()[0], fh_embedding_grad_workspace(&e)));
+    } else if (const ir::Node* f = loss_of(n); loss || f != nullptr) {
+      const Shape &x = n->inputs()[0]->type().shape, &w = n->inputs()[1]->type().shape;
+      fh_vocab_loss l{};
+      l.dtype = l.loss_dtype = static_cast<int32_t>(n->inputs()[0]->type().dtype.code());
+      l.mean = *n->attr<bool>("mean") ? 1 : 0;
+      l.tokens = x.dim(0);
+      l.vocab = w.dim(0);
+      l.dim = l.x_stride = l.w_stride = x.dim(1);
+      op = std::string(loss ? kVocabLossOp : kVocabLossGradOp);
+      if (loss) {
+        types.push_back(scratch(n->inputs()[0], 4 * l.tokens));
+      } else {
+        ins[3] = lse.at(f);
+      }
+      types.push_back(scratch(n->inputs()[0], loss ? fh_vocab_loss_workspace(&l) : fh_vocab_loss_grad_workspace(&l)));
+    }
+    Result<ir::Node*> c = out.create_node(std::move(op), std::move(ins), std::move(types));
+    if (!c.is_ok()) return c.status();
+    for (const auto& [k, v] : source->attrs()) c.value()->set_attr(k, v);
+    for (size_t i = 0; i < n->outputs().size(); ++i) map[&n->outputs()[i]] = c.value()->output(static_cast<int32_t>(i));
+    if (loss) lse[n] = c.value()->output(1);
+  }
+  for (const ir::Value* o : g.outputs()) FRAME_RETURN_IF_ERROR(out.mark_output(map.at(o)));
+  g = std::move(out);
+  return Status::ok();
+}
+
 // Replaces every matched attention decomposition by one kAttentionOp node. Nodes of a decomposition whose
 // results are also used outside it (or are graph outputs) keep the decomposition as it is. The graph is rebuilt in
 // topological order without the nodes the rewrite leaves unused (the shared scale constant among them).
@@ -2076,6 +2180,7 @@ Result<ir::Graph> lower_for_hip(const ir::Graph& graph, int32_t opt_level) {
   Result<ir::Graph> source = ir::clone_graph(graph);
   if (!source.is_ok()) return source.status();
   FRAME_RETURN_IF_ERROR(lower_packed_attention(source.value()));
+  FRAME_RETURN_IF_ERROR(lower_language_ends(source.value(), opt_level));
   if (opt_level >= 1) FRAME_RETURN_IF_ERROR(lower_attention_grads(source.value()));
   Result<ir::Graph> work = lower_matmul_grads(source.value(), opt_level);
   if (!work.is_ok()) return work.status();

@@ -731,6 +731,171 @@ Status packed_attention_grad_kernel(KernelContext& ctx) {
   return Status::ok();
 }
 
+// ---- token embedding, and the loss over the vocabulary ----
+
+// Scratch of a node that is launched by itself; compiled graphs plan theirs.
+class Scratch {
+ public:
+  Scratch() = default;
+  Scratch(const Scratch&) = delete;
+  Scratch& operator=(const Scratch&) = delete;
+  ~Scratch() {
+    if (ptr_ != nullptr) allocator_->deallocate(ptr_);  // kernels queued on the stream may still use it: the allocator waits for them
+  }
+  Status take(const KernelContext& ctx, int64_t bytes) {
+    Result<hal::Backend*> b = hal::BackendRegistry::instance().get(kHipBackendName);
+    if (!b.is_ok()) return b.status();
+    allocator_ = b.value()->allocator(ctx.device);
+    if (allocator_ == nullptr) return Status::make(ErrorCode::kInternal, "no allocator of the node's device");
+    Result<void*> p = allocator_->allocate(static_cast<size_t>(std::max<int64_t>(bytes, 4)), 256);
+    if (!p.is_ok()) return p.status();
+    ptr_ = p.value();
+    return Status::ok();
+  }
+  void* get() const { return ptr_; }
+
+ private:
+  hal::Allocator* allocator_ = nullptr;
+  void* ptr_ = nullptr;
+};
+
+int64_t tensor_bytes(const Tensor& t) { return t.numel() * static_cast<int64_t>(elem_bytes(t)); }
+
+Status embedding_geometry(const KernelContext& ctx, const std::string& op, const Tensor& table, const Tensor& ids, const Tensor& rows,
+                          fh_token_embedding& g) {
+  const auto* scale = attr<double>(ctx, "scale");
+  if (scale == nullptr) return invalid(op, "missing attribute 'scale'");
+  if (table.shape().rank() != 2 || ids.shape().rank() != 1 || !same_elem_type(ids, DType::of<std::int32_t>()))
+    return invalid(op, "expects a table [vocab, dim] and ids int32 [tokens]");
+  if (rows.shape() != Shape({ids.shape().dim(0), table.shape().dim(1)}) || !same_elem_type(rows, table))
+    return invalid(op, "rows must be [tokens, dim] in the table's type");
+  Result<int32_t> dt = float_code(op, table.dtype());
+  if (!dt.is_ok()) return dt.status();
+  g.dtype = dt.value();
+  g.tokens = ids.shape().dim(0);
+  g.vocab = table.shape().dim(0);
+  g.dim = g.row_stride = table.shape().dim(1);
+  g.scale = static_cast<float>(*scale);
+  return Status::ok();
+}
+
+Status embedding_kernel(KernelContext& ctx) {
+  const std::string op = "embedding";
+  FRAME_RETURN_IF_ERROR(arity(ctx, op, 2, 1));
+  fh_token_embedding g{};
+  FRAME_RETURN_IF_ERROR(embedding_geometry(ctx, op, ctx.inputs[0], ctx.inputs[1], ctx.outputs[0], g));
+  FRAME_HIP_RETURN_IF_ERROR(fh_embedding_fwd(&g, ctx.inputs[0].raw_data(), static_cast<const int32_t*>(ctx.inputs[1].raw_data()),
+                                             ctx.outputs[0].raw_data(), stream_handle(ctx)),
+                            "op '" + op + "' (hip)");
+  return Status::ok();
+}
+
+// Planned: the compiled graph's form, with a workspace as the second output and perhaps a base as the third input.
+template <bool Planned>
+Status embedding_grad_kernel(KernelContext& ctx) {
+  const std::string op(Planned ? kEmbeddingGradOp : "embedding_grad_internal");
+  const bool on_base = Planned && ctx.inputs.size() == 3;
+  FRAME_RETURN_IF_ERROR(arity(ctx, op, on_base ? 3 : 2, Planned ? 2 : 1));
+  Tensor& gtable = ctx.outputs[0];
+  fh_token_embedding g{};
+  FRAME_RETURN_IF_ERROR(embedding_geometry(ctx, op, gtable, ctx.inputs[1], ctx.inputs[0], g));
+  if (on_base && !alike(ctx.inputs[2], gtable)) return invalid(op, "the base must be of the table's shape and type");
+  Scratch own;
+  const int64_t need = fh_embedding_grad_workspace(&g);
+  if (!Planned && need > 0) FRAME_RETURN_IF_ERROR(own.take(ctx, need));
+  FRAME_HIP_RETURN_IF_ERROR(
+      fh_embedding_grad(&g, ctx.inputs[0].raw_data(), static_cast<const int32_t*>(ctx.inputs[1].raw_data()),
+                        on_base ? ctx.inputs[2].raw_data() : nullptr, gtable.raw_data(), Planned ? ctx.outputs[1].raw_data() : own.get(),
+                        Planned ? tensor_bytes(ctx.outputs[1]) : need, stream_handle(ctx)),
+      "op '" + op + "' (hip)");
+  return Status::ok();
+}
+
+Status loss_geometry(const KernelContext& ctx, const std::string& op, fh_vocab_loss& g) {
+  const auto* mean = attr<bool>(ctx, "mean");
+  if (mean == nullptr) return invalid(op, "missing attribute 'mean'");
+  const Tensor &x = ctx.inputs[0], &w = ctx.inputs[1], &t = ctx.inputs[2];
+  if (x.shape().rank() != 2 || w.shape().rank() != 2 || x.shape().dim(1) != w.shape().dim(1) || !same_elem_type(x, w))
+    return invalid(op, "expects x [tokens, dim] and w [vocab, dim] of one type");
+  if (!same_elem_type(t, DType::of<std::int32_t>()) || t.shape() != Shape({x.shape().dim(0)}))
+    return invalid(op, "expects targets int32 [tokens]");
+  Result<int32_t> dt = float_code(op, x.dtype());
+  if (!dt.is_ok()) return dt.status();
+  g.dtype = g.loss_dtype = dt.value();
+  g.mean = *mean ? 1 : 0;
+  g.tokens = x.shape().dim(0);
+  g.vocab = w.shape().dim(0);
+  g.dim = g.x_stride = g.w_stride = x.shape().dim(1);
+  return Status::ok();
+}
+
+Status loss_forward(const KernelContext& ctx, const std::string& op, const fh_vocab_loss& g, void* loss, float* lse, void* workspace,
+                    int64_t bytes) {
+  FRAME_HIP_RETURN_IF_ERROR(fh_vocab_loss_fwd(&g, ctx.inputs[0].raw_data(), ctx.inputs[1].raw_data(),
+                                              static_cast<const int32_t*>(ctx.inputs[2].raw_data()), loss, nullptr, lse, workspace, bytes,
+                                              stream_handle(ctx)),
+                            "op '" + op + "' (hip)");
+  return Status::ok();
+}
+
+// Planned: the compiled graph's form, whose second output a gradient reads and whose third is a workspace.
+template <bool Planned>
+Status vocab_loss_kernel(KernelContext& ctx) {
+  const std::string op(Planned ? kVocabLossOp : "vocab_loss");
+  FRAME_RETURN_IF_ERROR(arity(ctx, op, 3, Planned ? 3 : 1));
+  fh_vocab_loss g{};
+  FRAME_RETURN_IF_ERROR(loss_geometry(ctx, op, g));
+  if (ctx.outputs[0].numel() != 1 || !same_elem_type(ctx.outputs[0], ctx.inputs[0])) return invalid(op, "the loss must be one value of x's type");
+  if constexpr (Planned) {
+    if (tensor_bytes(ctx.outputs[1]) < 4 * g.tokens) return invalid(op, "lse must be fp32 [tokens]");
+    return loss_forward(ctx, op, g, ctx.outputs[0].raw_data(), static_cast<float*>(ctx.outputs[1].raw_data()), ctx.outputs[2].raw_data(),
+                        tensor_bytes(ctx.outputs[2]));
+  } else {
+    Scratch lse, workspace;
+    const int64_t need = fh_vocab_loss_workspace(&g);
+    FRAME_RETURN_IF_ERROR(lse.take(ctx, 4 * g.tokens));
+    FRAME_RETURN_IF_ERROR(workspace.take(ctx, need));
+    return loss_forward(ctx, op, g, ctx.outputs[0].raw_data(), static_cast<float*>(lse.get()), workspace.get(), need);
+  }
+}
+
+// Planned: inputs x, w, targets, lse, gy and a workspace as the third output. Otherwise (a node launched by itself) x, w, targets, y, gy: the
+// log-sum-exps are formed again.
+template <bool Planned>
+Status vocab_loss_grad_kernel(KernelContext& ctx) {
+  const std::string op(Planned ? kVocabLossGradOp : "vocab_loss_grad_internal");
+  FRAME_RETURN_IF_ERROR(arity(ctx, op, 5, Planned ? 3 : 2));
+  fh_vocab_loss g{};
+  FRAME_RETURN_IF_ERROR(loss_geometry(ctx, op, g));
+  const Tensor& gy = ctx.inputs[4];
+  if (gy.numel() != 1 || !same_elem_type(gy, ctx.inputs[0])) return invalid(op, "gy must be one value of x's type");
+  for (size_t i = 0; i < 2; ++i)
+    if (!alike(ctx.outputs[i], ctx.inputs[i])) return invalid(op, "gx and gw must be of x's and w's shape and type");
+  Scratch formed, workspace;
+  const float* lse = nullptr;
+  void* ws = nullptr;
+  int64_t room = 0;
+  if constexpr (Planned) {
+    if (tensor_bytes(ctx.inputs[3]) < 4 * g.tokens) return invalid(op, "lse must be fp32 [tokens]");
+    lse = static_cast<const float*>(ctx.inputs[3].raw_data());
+    ws = ctx.outputs[2].raw_data();
+    room = tensor_bytes(ctx.outputs[2]);
+  } else {
+    room = std::max(fh_vocab_loss_grad_workspace(&g), fh_vocab_loss_workspace(&g));
+    FRAME_RETURN_IF_ERROR(formed.take(ctx, 4 * g.tokens + 4));  // and the loss behind them, formed again too
+    FRAME_RETURN_IF_ERROR(workspace.take(ctx, room));
+    ws = workspace.get();
+    float* to = static_cast<float*>(formed.get());
+    FRAME_RETURN_IF_ERROR(loss_forward(ctx, op, g, to + g.tokens, to, ws, room));
+    lse = to;
+  }
+  FRAME_HIP_RETURN_IF_ERROR(
+      fh_vocab_loss_grad(&g, ctx.inputs[0].raw_data(), ctx.inputs[1].raw_data(), static_cast<const int32_t*>(ctx.inputs[2].raw_data()), lse,
+                         gy.raw_data(), ctx.outputs[0].raw_data(), ctx.outputs[1].raw_data(), ws, room, stream_handle(ctx)),
+      "op '" + op + "' (hip)");
+  return Status::ok();
+}
+
 Status layer_norm_kernel(KernelContext& ctx) {
   FRAME_RETURN_IF_ERROR(arity(ctx, "layer_norm", 3, 1));
   FRAME_RETURN_IF_ERROR(same_dtype(ctx, "layer_norm"));
@@ -1239,6 +1404,13 @@ FRAME_REGISTER_KERNEL("packed_attention", kHipBackendName, &packed_attention_ker
 FRAME_REGISTER_KERNEL(kPackedAttentionOp, kHipBackendName, &packed_attention_kernel<true>);
 FRAME_REGISTER_KERNEL("packed_attention_grad_internal", kHipBackendName, &packed_attention_grad_kernel<false>);
 FRAME_REGISTER_KERNEL(kPackedAttentionGradOp, kHipBackendName, &packed_attention_grad_kernel<true>);
+FRAME_REGISTER_KERNEL("embedding", kHipBackendName, &embedding_kernel);
+FRAME_REGISTER_KERNEL("embedding_grad_internal", kHipBackendName, &embedding_grad_kernel<false>);
+FRAME_REGISTER_KERNEL(kEmbeddingGradOp, kHipBackendName, &embedding_grad_kernel<true>);
+FRAME_REGISTER_KERNEL("vocab_loss", kHipBackendName, &vocab_loss_kernel<false>);
+FRAME_REGISTER_KERNEL(kVocabLossOp, kHipBackendName, &vocab_loss_kernel<true>);
+FRAME_REGISTER_KERNEL("vocab_loss_grad_internal", kHipBackendName, &vocab_loss_grad_kernel<false>);
+FRAME_REGISTER_KERNEL(kVocabLossGradOp, kHipBackendName, &vocab_loss_grad_kernel<true>);
 FRAME_REGISTER_KERNEL("layer_norm", kHipBackendName, &layer_norm_kernel);
 FRAME_REGISTER_KERNEL("max_pool2d", kHipBackendName, &pool_kernel<0>);
 FRAME_REGISTER_KERNEL("avg_pool2d", kHipBackendName, &pool_kernel<1>);

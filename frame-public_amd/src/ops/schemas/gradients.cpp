@@ -9,7 +9,7 @@
 //   reshape / transpose / slice / concat gradients   src/ops/schemas/shape.cpp:60-410
 //   softmax / layer_norm gradients and their row-statistics helpers   src/ops/schemas/sequence.cpp:255-615
 //   sigmoid / tanh / rsqrt gradients   src/ops/schemas/elementwise.cpp:401-660
-// gelu, packed_attention and their gradient ops are this build's own (the reference has neither).
+// gelu, packed_attention, embedding, vocab_loss and their gradient ops are this build's own (the reference has none of them).
 // Only first-order gradients are registered: the gradient-only ops carry no GradientFn here, so differentiating
 // a training graph a second time reports kUnimplemented naming the op.
 #include "gradients.h"
@@ -517,6 +517,61 @@ Result<ir::Graph> packed_attention_gradient(const NodeContext& c) {
                                pick(c, {"heads", "kv_heads", "causal", "scale"})));
 }
 
+Shapes infer_embedding_grad(const NodeContext& c) {
+  const std::string op = "embedding_grad_internal";
+  if (c.input_types.size() != 2) return bad(op, "expects 2 inputs, got " + std::to_string(c.input_types.size()));
+  Result<Shape> table = static_shape_attr(c, op, "table_shape");
+  if (!table.is_ok()) return table.status();
+  Shapes y = infer_as("embedding", {with_shape(c.input_types[0], table.value()), c.input_types[1]}, c.attrs);
+  if (!y.is_ok()) return bad(op, std::string(y.status().message()));
+  if (!(y.value()[0] == c.input_types[0].shape))
+    return bad(op, "requires gy to be " + y.value()[0].to_string() + ", got " + c.input_types[0].shape.to_string());
+  return std::vector<Shape>{table.value()};
+}
+
+// ids, an integer input, have no gradient.
+Result<ir::Graph> embedding_gradient(const NodeContext& c) {
+  FRAME_RETURN_IF_ERROR(expect(c, 2, "2 inputs (table, ids)"));
+  Micro m("embedding_gradient");
+  Fwd f = forward_inputs(m, c);
+  AttrMap attrs = pick(c, {"scale"});
+  attrs.emplace("table_shape", c.input_types[0].shape);
+  return m.finish({m.op("embedding_grad_internal", {f.gy, f.x[1]}, attrs)});
+}
+
+Status vocab_loss_inputs(const NodeContext& c) {
+  const std::string op(c.op);
+  const auto &x = c.input_types[0], &w = c.input_types[1], &t = c.input_types[2];
+  if (c.attr<bool>("mean") == nullptr) return bad(op, "is missing required attribute 'mean' (bool)");
+  if (x.shape.rank() != 2 || w.shape.rank() != 2) return bad(op, "requires x [tokens, dim] and w [vocab, dim] to be rank-2");
+  FRAME_RETURN_IF_ERROR(same_dtype(op, x, w, "x", "w"));
+  if (x.shape.dim(1) != w.shape.dim(1))
+    return bad(op, "requires x and w of the same second dimension, got " + x.shape.to_string() + " and " + w.shape.to_string());
+  if (!(t.dtype == DType(DTypeCode::kInt32)) || !(t.shape == Shape({x.shape.dim(0)})))
+    return bad(op, "requires targets to be int32 [tokens], got '" + std::string(t.dtype.name()) + "' " + t.shape.to_string());
+  return Status::ok();
+}
+
+Shapes infer_vocab_loss_grad(const NodeContext& c) {
+  const std::string op = "vocab_loss_grad_internal";
+  if (c.input_types.size() != 5) return bad(op, "expects 5 inputs, got " + std::to_string(c.input_types.size()));
+  FRAME_RETURN_IF_ERROR(vocab_loss_inputs(c));
+  for (size_t i = 3; i < 5; ++i) {
+    FRAME_RETURN_IF_ERROR(same_dtype(op, c.input_types[0], c.input_types[i], "x", i == 3 ? "y" : "gy"));
+    if (c.input_types[i].shape.rank() != 0 && c.input_types[i].shape.numel() != 1)
+      return bad(op, "requires y and gy to be scalar (rank 0 or numel==1), got " + c.input_types[i].shape.to_string());
+  }
+  return std::vector<Shape>{c.input_types[0].shape, c.input_types[1].shape};
+}
+
+// One node for both gradients; targets, an integer input, have none.
+Result<ir::Graph> vocab_loss_gradient(const NodeContext& c) {
+  FRAME_RETURN_IF_ERROR(expect(c, 3, "3 inputs (x, w, targets)"));
+  Micro m("vocab_loss_gradient");
+  Fwd f = forward_inputs(m, c);
+  return m.finish(m.op_outputs("vocab_loss_grad_internal", {f.x[0], f.x[1], f.x[2], f.y, f.gy}, 2, pick(c, {"mean"})));
+}
+
 // layer_norm (reference: src/ops/schemas/sequence.cpp:479-615): mean / variance / rsqrt recomputed from x, then
 // gx = r * ((a - mean(a)) - xhat * mean(a * xhat)) with a = gamma * gy; ggamma = sum(gy * xhat, axis 0);
 // gbeta = sum(gy, axis 0).
@@ -771,6 +826,25 @@ FRAME_REGISTER_OP("packed_attention_grad_internal")
     .output("gv", "gradient w.r.t. v")
     .output("stats", "scratch of two fp32 values per (row, head), [tokens, 4 * heads] in 16-bit elements")
     .shape_infer(&fs::infer_packed_attention_grad);
+
+FRAME_REGISTER_OP("embedding_grad_internal")
+    .input("gy", "upstream gradient of embedding's output")
+    .input("ids", "embedding's ids")
+    .attr("scale", AttrType::kDouble, true)
+    .attr("table_shape", AttrType::kShape, true)
+    .output("gtable", "gradient w.r.t. the table: scale times the sum of gy's rows per id")
+    .shape_infer(&fs::infer_embedding_grad);
+
+FRAME_REGISTER_OP("vocab_loss_grad_internal")
+    .input("x", "vocab_loss' inputs")
+    .input("w", "")
+    .input("targets", "")
+    .input("y", "its output")
+    .input("gy", "upstream gradient of y")
+    .attr("mean", AttrType::kBool, true)
+    .output("gx", "gradient w.r.t. x; rows without a target are zeros")
+    .output("gw", "gradient w.r.t. w")
+    .shape_infer(&fs::infer_vocab_loss_grad);
 
 FRAME_REGISTER_OP("gelu_grad_internal")
     .input("x", "gelu's original input")

@@ -29,6 +29,12 @@ Result<ir::Graph> rsqrt_gradient(const NodeContext& ctx);
 Result<ir::Graph> gelu_gradient(const NodeContext& ctx);
 Result<ir::Graph> packed_attention_gradient(const NodeContext& ctx);
 
+Result<ir::Graph> embedding_gradient(const NodeContext& ctx);
+Result<ir::Graph> vocab_loss_gradient(const NodeContext& ctx);
+
+// What is wrong with vocab_loss' first three inputs (x, w, targets) and attributes; its gradient op takes the same.
+Status vocab_loss_inputs(const NodeContext& ctx);
+
 // The output shape of packed_attention on the context's first four inputs (q, k, v, cu_seqlens) and attributes, or what is wrong
 // with them; its gradient op takes the same.
 Result<std::vector<Shape>> packed_attention_shapes(const NodeContext& ctx);

@@ -11,6 +11,9 @@
 // elementwise and fusable so operator_fusion can merge bias-add + gelu into one fused group.
 // packed_attention has none either: attention over sequences of different lengths in one tensor's rows, with grouped heads and an
 // optional causal mask, as one op (the reference unrolls attention of one length per batch and head, src/nn/layers.cpp:1014-1080).
+// Nor have embedding (rows of a table by int32 ids) and vocab_loss (softmax cross entropy of x w^T against int32 targets, the logits never
+// a tensor of the graph), the two ends of a language model: the reference has no op that reads integers.
+#include <cmath>
 #include <cstdint>
 #include <numeric>
 #include <string>
@@ -276,6 +279,24 @@ Shapes infer_packed_attention(const NodeContext& c) {
   return frame::ops::schemas::packed_attention_shapes(c);
 }
 
+Shapes infer_embedding(const NodeContext& c) {
+  FRAME_RETURN_IF_ERROR(expect_inputs(c, 2));
+  const auto &table = c.input_types[0], &ids = c.input_types[1];
+  const double* scale = c.attr<double>("scale");
+  if (scale == nullptr || !std::isfinite(*scale)) return bad("embedding", "requires a finite attribute 'scale' (double)");
+  if (table.shape.rank() != 2 || table.shape.dim(0) < 1 || table.shape.dim(1) < 1)
+    return bad("embedding", "requires table to be rank-2 [vocab, dim], got " + table.shape.to_string());
+  if (!(ids.dtype == DType(frame::DTypeCode::kInt32)) || ids.shape.rank() != 1)
+    return bad("embedding", "requires ids to be int32 rank-1 [tokens], got '" + std::string(ids.dtype.name()) + "' " + ids.shape.to_string());
+  return std::vector<Shape>{Shape({ids.shape.dim(0), table.shape.dim(1)})};
+}
+
+Shapes infer_vocab_loss(const NodeContext& c) {
+  FRAME_RETURN_IF_ERROR(expect_inputs(c, 3));
+  FRAME_RETURN_IF_ERROR(frame::ops::schemas::vocab_loss_inputs(c));
+  return std::vector<Shape>{Shape()};
+}
+
 Shapes infer_fused(const NodeContext& c) {
   if (c.input_types.empty()) return bad("fused_elementwise_internal", "expects at least 1 input, got 0");
   if (c.attrs == nullptr) return bad("fused_elementwise_internal", "requires non-null attrs");
@@ -371,6 +392,23 @@ FRAME_REGISTER_OP("packed_attention")
     .output("out", "softmax(scale q k^T) v per sequence and head; rows outside the sequences are zeros")
     .shape_infer(&infer_packed_attention)
     .gradient(&frame::ops::schemas::packed_attention_gradient);
+
+FRAME_REGISTER_OP("embedding")
+    .input("table", "rank-2 [vocab, dim]")
+    .input("ids", "int32 rank-1 [tokens]; one outside [0, vocab) names no row")
+    .attr("scale", AttrType::kDouble, true)
+    .output("out", "[tokens, dim]: scale * table[ids[t]], zeros where ids[t] names no row")
+    .shape_infer(&infer_embedding)
+    .gradient(&frame::ops::schemas::embedding_gradient);
+
+FRAME_REGISTER_OP("vocab_loss")
+    .input("x", "rank-2 [tokens, dim]")
+    .input("w", "rank-2 [vocab, dim]")
+    .input("targets", "int32 rank-1 [tokens]; a row whose target is outside [0, vocab) does not count")
+    .attr("mean", AttrType::kBool, true)
+    .output("out", "scalar: softmax cross entropy of x w^T against the targets, the rows' mean or sum; 0 where no row counts")
+    .shape_infer(&infer_vocab_loss)
+    .gradient(&frame::ops::schemas::vocab_loss_gradient);
 
 FRAME_REGISTER_OP("layer_norm")
     .input("x", "rank-2 [N, D]")

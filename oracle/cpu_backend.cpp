@@ -328,6 +328,33 @@ Status packed_attention_kernel(ops::KernelContext& c) {
             "packed_attention");
 }
 
+Status embedding_kernel(ops::KernelContext& c) {
+  const Shape& table = c.inputs[0].shape();
+  return rc(oracle_embedding(dcode(c.outputs[0].dtype()), c.inputs[0].raw_data(), static_cast<const int32_t*>(c.inputs[1].raw_data()),
+                             c.outputs[0].raw_data(), c.inputs[1].numel(), table.dim(0), table.dim(1), *attr<double>(c, "scale")),
+            "embedding");
+}
+Status embedding_grad_kernel(ops::KernelContext& c) {
+  const Shape& table = c.outputs[0].shape();
+  return rc(oracle_embedding_grad(dcode(c.outputs[0].dtype()), c.inputs[0].raw_data(), static_cast<const int32_t*>(c.inputs[1].raw_data()),
+                                  c.outputs[0].raw_data(), c.inputs[1].numel(), table.dim(0), table.dim(1), *attr<double>(c, "scale")),
+            "embedding_grad");
+}
+// vocab_loss (inputs x, w, targets) and its gradients (.., y, gy)
+template <bool Grad>
+Status vocab_loss_kernel(ops::KernelContext& c) {
+  const Shape &x = c.inputs[0].shape(), &w = c.inputs[1].shape();
+  const auto* targets = static_cast<const int32_t*>(c.inputs[2].raw_data());
+  const int dt = dcode(c.outputs[0].dtype()), mean = *attr<bool>(c, "mean") ? 1 : 0;
+  if (Grad)
+    return rc(oracle_vocab_loss_grad(dt, c.inputs[0].raw_data(), c.inputs[1].raw_data(), targets, c.inputs[4].raw_data(),
+                                     c.outputs[0].raw_data(), c.outputs[1].raw_data(), x.dim(0), w.dim(0), x.dim(1), mean),
+              "vocab_loss_grad");
+  return rc(oracle_vocab_loss(dt, c.inputs[0].raw_data(), c.inputs[1].raw_data(), targets, c.outputs[0].raw_data(), x.dim(0), w.dim(0),
+                              x.dim(1), mean),
+            "vocab_loss");
+}
+
 }  // namespace oracle_cpu
 
 FRAME_REGISTER_BACKEND(frame::kCpuBackendName, oracle_cpu::CpuBackend);
@@ -361,6 +388,10 @@ FRAME_REGISTER_KERNEL("max_pool2d_grad_internal", frame::kCpuBackendName, &oracl
 FRAME_REGISTER_KERNEL("avg_pool2d_grad_internal", frame::kCpuBackendName, &oracle_cpu::pool_grad_kernel<1>);
 FRAME_REGISTER_KERNEL("sum", frame::kCpuBackendName, &oracle_cpu::sum_kernel);
 FRAME_REGISTER_KERNEL("sum_grad_internal", frame::kCpuBackendName, &oracle_cpu::sum_grad_kernel);
+FRAME_REGISTER_KERNEL("embedding", frame::kCpuBackendName, &oracle_cpu::embedding_kernel);
+FRAME_REGISTER_KERNEL("embedding_grad_internal", frame::kCpuBackendName, &oracle_cpu::embedding_grad_kernel);
+FRAME_REGISTER_KERNEL("vocab_loss", frame::kCpuBackendName, &oracle_cpu::vocab_loss_kernel<false>);
+FRAME_REGISTER_KERNEL("vocab_loss_grad_internal", frame::kCpuBackendName, &oracle_cpu::vocab_loss_kernel<true>);
 FRAME_REGISTER_KERNEL("packed_attention", frame::kCpuBackendName, &oracle_cpu::packed_attention_kernel<false>);
 FRAME_REGISTER_KERNEL("packed_attention_grad_internal", frame::kCpuBackendName, &oracle_cpu::packed_attention_kernel<true>);
 FRAME_REGISTER_KERNEL("mse_loss", frame::kCpuBackendName, &oracle_cpu::mse_loss_kernel);

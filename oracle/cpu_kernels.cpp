@@ -817,4 +817,95 @@ int oracle_mse_loss_grad(int dtype, const void* pred, const void* target, const 
   });
 }
 
+int oracle_embedding(int dtype, const void* table, const int32_t* ids, void* out, int64_t tokens, int64_t vocab, int64_t dim, double scale) {
+  return with_dtype(dtype, [&](auto d0) {
+    using D = decltype(d0);
+    using S = typename D::S;
+    for (int64_t t = 0; t < tokens; ++t)
+      for (int64_t c = 0; c < dim; ++c)
+        static_cast<S*>(out)[t * dim + c] =
+            ids[t] >= 0 && ids[t] < vocab ? D::st(static_cast<float>(static_cast<double>(D::ld(static_cast<const S*>(table)[ids[t] * dim + c])) * scale))
+                                          : D::st(0.0f);
+    return 0;
+  });
+}
+
+int oracle_embedding_grad(int dtype, const void* gy, const int32_t* ids, void* gtable, int64_t tokens, int64_t vocab, int64_t dim, double scale) {
+  return with_dtype(dtype, [&](auto d0) {
+    using D = decltype(d0);
+    using S = typename D::S;
+    std::vector<double> sum(static_cast<size_t>(vocab * dim), 0.0);
+    for (int64_t t = 0; t < tokens; ++t)
+      if (ids[t] >= 0 && ids[t] < vocab)
+        for (int64_t c = 0; c < dim; ++c)
+          sum[static_cast<size_t>(ids[t] * dim + c)] += static_cast<double>(D::ld(static_cast<const S*>(gy)[t * dim + c])) * scale;
+    for (int64_t i = 0; i < vocab * dim; ++i) static_cast<S*>(gtable)[i] = D::st(static_cast<float>(sum[static_cast<size_t>(i)]));
+    return 0;
+  });
+}
+
+}  // extern "C"
+
+namespace {
+// Per row with a target: its number, its softmax over the vocabulary and its loss; returns how many there are.
+template <typename D, typename Fn>
+int64_t loss_rows(const typename D::S* X, const typename D::S* W, const int32_t* targets, int64_t tokens, int64_t vocab, int64_t dim, Fn&& fn) {
+  int64_t count = 0;
+  std::vector<double> p(static_cast<size_t>(vocab));
+  for (int64_t t = 0; t < tokens; ++t) {
+    if (targets[t] < 0 || targets[t] >= vocab) continue;
+    ++count;
+    double top = -std::numeric_limits<double>::infinity(), sum = 0.0;
+    for (int64_t v = 0; v < vocab; ++v) {
+      double z = 0.0;
+      for (int64_t c = 0; c < dim; ++c) z += static_cast<double>(D::ld(X[t * dim + c])) * static_cast<double>(D::ld(W[v * dim + c]));
+      p[static_cast<size_t>(v)] = z;
+      top = std::max(top, z);
+    }
+    for (double z : p) sum += std::exp(z - top);
+    const double lse = top + std::log(sum), loss = lse - p[static_cast<size_t>(targets[t])];
+    for (double& z : p) z = std::exp(z - lse);
+    fn(t, p, loss);
+  }
+  return count;
+}
+}  // namespace
+
+extern "C" {
+
+int oracle_vocab_loss(int dtype, const void* x, const void* w, const int32_t* targets, void* loss, int64_t tokens, int64_t vocab, int64_t dim,
+                      int mean) {
+  return with_dtype(dtype, [&](auto d0) {
+    using D = decltype(d0);
+    using S = typename D::S;
+    double sum = 0.0;
+    const int64_t count = loss_rows<D>(static_cast<const S*>(x), static_cast<const S*>(w), targets, tokens, vocab, dim,
+                                       [&](int64_t, const std::vector<double>&, double l) { sum += l; });
+    static_cast<S*>(loss)[0] = D::st(static_cast<float>(mean && count > 0 ? sum / static_cast<double>(count) : sum));
+    return 0;
+  });
+}
+
+int oracle_vocab_loss_grad(int dtype, const void* x, const void* w, const int32_t* targets, const void* gy, void* gx, void* gw, int64_t tokens,
+                           int64_t vocab, int64_t dim, int mean) {
+  return with_dtype(dtype, [&](auto d0) {
+    using D = decltype(d0);
+    using S = typename D::S;
+    const S *X = static_cast<const S*>(x), *W = static_cast<const S*>(w);
+    std::vector<double> dx(static_cast<size_t>(tokens * dim), 0.0), dw(static_cast<size_t>(vocab * dim), 0.0);
+    const int64_t count = loss_rows<D>(X, W, targets, tokens, vocab, dim, [&](int64_t t, std::vector<double>& p, double) {
+      p[static_cast<size_t>(targets[t])] -= 1.0;
+      for (int64_t v = 0; v < vocab; ++v)
+        for (int64_t c = 0; c < dim; ++c) {
+          dx[static_cast<size_t>(t * dim + c)] += p[static_cast<size_t>(v)] * static_cast<double>(D::ld(W[v * dim + c]));
+          dw[static_cast<size_t>(v * dim + c)] += p[static_cast<size_t>(v)] * static_cast<double>(D::ld(X[t * dim + c]));
+        }
+    });
+    const double f = count == 0 ? 0.0 : static_cast<double>(D::ld(static_cast<const S*>(gy)[0])) / (mean ? static_cast<double>(count) : 1.0);
+    for (int64_t i = 0; i < tokens * dim; ++i) static_cast<S*>(gx)[i] = D::st(static_cast<float>(count == 0 ? 0.0 : f * dx[static_cast<size_t>(i)]));
+    for (int64_t i = 0; i < vocab * dim; ++i) static_cast<S*>(gw)[i] = D::st(static_cast<float>(count == 0 ? 0.0 : f * dw[static_cast<size_t>(i)]));
+    return 0;
+  });
+}
+
 }  // extern "C"

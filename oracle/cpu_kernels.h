@@ -105,6 +105,15 @@ int oracle_packed_attention_grad(int dtype, const void* q, const void* k, const 
                                  void* dk, void* dv, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dh,
                                  int causal, double scale);
 
+/* embedding, vocab_loss and their gradients (no reference counterpart), in double with one rounding at the end; ids and targets outside
+ * [0, vocab) name nothing. The loss is one value of dtype; no row with a target: 0, and gradients of zeros. */
+int oracle_embedding(int dtype, const void* table, const int32_t* ids, void* out, int64_t tokens, int64_t vocab, int64_t dim, double scale);
+int oracle_embedding_grad(int dtype, const void* gy, const int32_t* ids, void* gtable, int64_t tokens, int64_t vocab, int64_t dim, double scale);
+int oracle_vocab_loss(int dtype, const void* x, const void* w, const int32_t* targets, void* loss, int64_t tokens, int64_t vocab, int64_t dim,
+                      int mean);
+int oracle_vocab_loss_grad(int dtype, const void* x, const void* w, const int32_t* targets, const void* gy, void* gx, void* gw, int64_t tokens,
+                           int64_t vocab, int64_t dim, int mean);
+
 #ifdef __cplusplus
 }
 #endif
