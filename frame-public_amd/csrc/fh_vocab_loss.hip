@@ -102,54 +102,54 @@ __device__ __forceinline__ void at_targets(const int (&target)[P::TM], int colum
 
 // ---- rows with a target ----
 
-// By one workgroup: the list of rows with a target, their number and targets; the others' outputs, or (gradients: lse_c) the
-// log-sum-exps. 8 rows a thread and turn, read together: 8,192 rows take one turn.
-__global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a) {
-  constexpr int EACH = 8;
+// The list of rows with a target, their number and targets; the others' outputs, or (gradients: lse_c) the log-sum-exps. Workgroup b takes
+// the b'th run of `each` rows and counts the targets before it by itself: it reads them once more instead of waiting for the others
+// (8,192 rows: 6 us; one workgroup that reads its rows once 13, and 20 with the log-sum-exps).
+__global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a, int each) {
   __shared__ int waves[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int before = 0;  // rows with a target in earlier turns
-  for (int begin = 0; begin < a.tokens; begin += 1024 * EACH) {
-    int target[EACH], n = 0;
-    float lse[EACH];
+  const int begin = static_cast<int>(blockIdx.x) * each, end = min(a.tokens, begin + each);
+  auto counts = [&](int target) { return target >= 0 && target < a.vocab; };
+  // the workgroup's sum of n, to all
+  auto total = [&](int n) {
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int t = begin + tid * EACH + e;
-      target[e] = t < a.tokens ? a.targets[t] : -1;
-      if (a.lse_c != nullptr) lse[e] = t < a.tokens ? a.lse[t] : 0.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) n += target[e] >= 0 && target[e] < a.vocab;
-    int scan = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int lower = __shfl_up(scan, o, 64);
-      if (lane >= o) scan += lower;
-    }
-    if (lane == 63) waves[wave] = scan;
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    if (lane == 0) waves[wave] = n;
     __syncthreads();
-    int at = before + scan - n;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) sum += waves[w];
+    __syncthreads();
+    return sum;
+  };
+  int n = 0;
+#pragma unroll 8
+  for (int t = tid; t < begin; t += 1024) n += counts(a.targets[t]);
+  int before = begin > 0 ? total(n) : 0;
+  for (int at = begin; at < end; at += 1024) {
+    const int t = at + tid;
+    const int target = t < end ? a.targets[t] : -1;
+    const bool mine = counts(target);
+    const uint64_t mask = __ballot(mine);
+    if (lane == 0) waves[wave] = __popcll(mask);
+    __syncthreads();
+    int to = before + __popcll(mask & ((1ull << lane) - 1));
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
-      if (w < wave) at += waves[w];
+      if (w < wave) to += waves[w];
       before += waves[w];
     }
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int t = begin + tid * EACH + e;
-      if (target[e] >= 0 && target[e] < a.vocab) {
-        a.rows[at] = t;
-        a.targets_c[at] = target[e];
-        if (a.lse_c != nullptr) a.lse_c[at] = lse[e];
-        ++at;
-      } else if (t < a.tokens && a.lse_c == nullptr) {
-        a.lse[t] = 0.0f;
-        if (a.row_loss != nullptr) a.row_loss[t] = 0.0f;
-      }
+    if (mine) {
+      a.rows[to] = t;
+      a.targets_c[to] = target;
+      if (a.lse_c != nullptr) a.lse_c[to] = a.lse[t];
+    } else if (t < end && a.lse_c == nullptr) {
+      a.lse[t] = 0.0f;
+      if (a.row_loss != nullptr) a.row_loss[t] = 0.0f;
     }
   }
-  if (tid == 0) *a.count = before;
+  if (blockIdx.x + 1 == gridDim.x && tid == 0) *a.count = before;
 }
 
 // ---- forward ----
@@ -299,12 +299,12 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(
 #pragma unroll
   for (int i = 0; i < P::TM; ++i) {
     const int m = min(row0 + 16 * i, count - 1);
-    const float lse2 = a.lse_c[m] * kLog2e;
+    const float lse = a.lse_c[m];
     target[i] = a.targets_c[m];
 #pragma unroll
     for (int j = 0; j < P::TN; ++j)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) acc[i][j][x] = exp_from(acc[i][j][x], lse2) * kRaise<T>;
+      for (int x = 0; x < 4; ++x) acc[i][j][x] = __builtin_amdgcn_exp2f((acc[i][j][x] - lse) * kLog2e) * kRaise<T>;
   }
   at_targets<P>(target, column, [&](int i, int j, int x) { acc[i][j][x] -= kRaise<T>; });
   if (m0 + BM > count || a.first + n0 + BN > a.last) {
@@ -397,6 +397,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const Lo
 constexpr int kTile = 64;  // the smallest tile's rows and columns
 constexpr int kLeastPiece = 256;
 constexpr int64_t kPieceValues = int64_t{1} << 26;  // of g: 128 MB (3,686 rows of 131,072 columns: 9.64 ms; 256 MB 9.68, 512 MB 9.56)
+constexpr int64_t kMostPieceValues = int64_t{1} << 28;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -520,7 +521,10 @@ struct GradPlan {
 GradPlan best_plan(const fh_vocab_loss& g) {
   const int64_t all = up(g.vocab, kLeastPiece), rows = up(std::max<int64_t>(g.tokens, 1), 256);
   GradPlan p{};
-  p.columns = std::min(all, std::max<int64_t>(kPieceValues / rows / kLeastPiece * kLeastPiece, kLeastPiece));
+  // at least as many columns as give every CU one of dw's largest tiles (8,192 rows of 131,072 x 512: 3.48 ms, 3.84 by kPieceValues alone)
+  const int64_t round = up(up(device_cu_count() * 65536, g.dim) / g.dim, kLeastPiece);
+  const int64_t columns = std::min(std::max(kPieceValues / rows, round), kMostPieceValues / rows) / kLeastPiece * kLeastPiece;
+  p.columns = std::min(all, std::max<int64_t>(columns, kLeastPiece));
   p.dx = dx_plan(g.tokens, g.dim, std::min(p.columns, g.vocab));
   return p;
 }
@@ -558,6 +562,13 @@ LossArgs loss_args(const fh_vocab_loss& g, const void* x, const void* w, const i
   a.mean = g.mean;
   a.loss_dtype = g.loss_dtype;
   return a;
+}
+
+fh_status list_rows(const LossArgs& a, hipStream_t stream) {
+  // at most 64 workgroups: what they count again stays few times the rows
+  const int each = static_cast<int>(std::max<int64_t>(up((a.tokens + 63) / 64, 1024), 1024));
+  hipLaunchKernelGGL(loss_rows_kernel, dim3(static_cast<uint32_t>(std::max(1, (a.tokens + each - 1) / each))), dim3(1024), 0, stream, a, each);
+  return launch_status("loss_rows_kernel launch");
 }
 
 template <typename F>
@@ -599,8 +610,7 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
   a.targets_c = reinterpret_cast<int32_t*>(ws + room.targets);
   a.tiles_n = static_cast<int>(room.tiles_n);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, s, a);
-  if (fh_status st = launch_status("loss_rows_kernel launch"); st != FH_OK) return st;
+  if (fh_status st = list_rows(a, s); st != FH_OK) return st;
   if (g->tokens > 0) {
     const fh_status st = by_type(g->dtype, [&]<typename T>() {
       by_tile(tile_for(g->tokens, g->vocab), g->tokens, g->vocab, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
@@ -664,8 +674,7 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
   a.g = reinterpret_cast<uint16_t*>(ws + room.g);
   a.splits = plan.dx.splits;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(loss_rows_kernel, dim3(1), dim3(1024), 0, s, a);
-  if (fh_status st = launch_status("loss_rows_kernel launch"); st != FH_OK) return st;
+  if (fh_status st = list_rows(a, s); st != FH_OK) return st;
   if (g->tokens > 0) {
     hipLaunchKernelGGL(loss_gather_kernel, dim3(static_cast<uint32_t>(up(g->tokens, 64) / 4)), dim3(256), 0, s, a);
     if (fh_status st = launch_status("loss_gather_kernel launch"); st != FH_OK) return st;
