@@ -1414,8 +1414,9 @@ Status lower_packed_attention(ir::Graph& g) {
   return Status::ok();
 }
 
-// The two ends of a language model get their workspaces planned: embedding_grad_internal, vocab_loss and the vocab_loss_grad_internal whose
-// forward the graph holds (which hands it the rows' log-sum-exps) become their internal forms, at every opt level. At opt_level >= 1 an add
+// The two ends of a language model get their workspaces planned: embedding_grad_internal, vocab_loss and vocab_loss_grad_internal become
+// their internal forms, at every opt level; the forward hands the last one the rows' log-sum-exps (one that the graph does not hold is
+// added for them). At opt_level >= 1 an add
 // of an embedding's gradient to another gradient of the same table (tied weights) goes into the former, which is then summed and
 // rounded once. Types that the kernels do not take stay as they are and are named when the step runs.
 Status lower_language_ends(ir::Graph& g, int32_t opt_level) {
@@ -1423,8 +1424,11 @@ Status lower_language_ends(ir::Graph& g, int32_t opt_level) {
     const DTypeCode d = v->type().dtype.code();
     return d == DTypeCode::kBFloat16 || d == DTypeCode::kFloat16;
   };
+  auto is_loss = [&](const ir::Node* n) { return n->op() == "vocab_loss" && n->inputs().size() == 3 && sixteen(n->inputs()[0]); };
+  auto is_loss_grad = [&](const ir::Node* n) {
+    return n->op() == "vocab_loss_grad_internal" && n->inputs().size() == 5 && sixteen(n->inputs()[0]);
+  };
   auto loss_of = [&](const ir::Node* n) -> const ir::Node* {
-    if (n->op() != "vocab_loss_grad_internal" || n->inputs().size() != 5 || !sixteen(n->inputs()[0])) return nullptr;
     const ir::Node* f = n->inputs()[3]->producer();
     if (f == nullptr || f->op() != "vocab_loss" || f->attrs() != n->attrs()) return nullptr;
     for (size_t i = 0; i < 3; ++i)
@@ -1438,7 +1442,7 @@ Status lower_language_ends(ir::Graph& g, int32_t opt_level) {
   bool any = false;
   for (const ir::Node* n : g.topological_order()) {
     for (const ir::Value* v : n->inputs()) ++uses[v];
-    any = any || is_embedding_grad(n) || (n->op() == "vocab_loss" && n->inputs().size() == 3 && sixteen(n->inputs()[0]));
+    any = any || is_embedding_grad(n) || is_loss(n) || is_loss_grad(n);
   }
   if (!any) return Status::ok();
   for (const ir::Value* v : g.outputs()) ++uses[v];
@@ -1480,7 +1484,6 @@ Status lower_language_ends(ir::Graph& g, int32_t opt_level) {
     if (sum != sums.end()) source = n->inputs()[sum->second]->producer();
     for (const ir::Value* v : source->inputs()) ins.push_back(map.at(v));
     std::string op(source->op());
-    const bool loss = n->op() == "vocab_loss" && n->inputs().size() == 3 && sixteen(n->inputs()[0]);
     if (is_embedding_grad(source)) {
       op = std::string(kEmbeddingGradOp);
       if (sum != sums.end()) ins.push_back(map.at(n->inputs()[1 - sum->second]));
@@ -1491,7 +1494,7 @@ Status lower_language_ends(ir::Graph& g, int32_t opt_level) {
       e.vocab = table.dim(0);
       e.dim = e.row_stride = table.dim(1);
       types.push_back(scratch(source->inputs()[0], fh_embedding_grad_workspace(&e)));
-    } else if (const ir::Node* f = loss_of(n); loss || f != nullptr) {
+    } else if (is_loss(n) || is_loss_grad(n)) {
       const Shape &x = n->inputs()[0]->type().shape, &w = n->inputs()[1]->type().shape;
       fh_vocab_loss l{};
       l.dtype = l.loss_dtype = static_cast<int32_t>(n->inputs()[0]->type().dtype.code());
@@ -1499,19 +1502,29 @@ Status lower_language_ends(ir::Graph& g, int32_t opt_level) {
       l.tokens = x.dim(0);
       l.vocab = w.dim(0);
       l.dim = l.x_stride = l.w_stride = x.dim(1);
-      op = std::string(loss ? kVocabLossOp : kVocabLossGradOp);
-      if (loss) {
-        types.push_back(scratch(n->inputs()[0], 4 * l.tokens));
+      const ir::TensorType rows = scratch(n->inputs()[0], 4 * l.tokens), room = scratch(n->inputs()[0], fh_vocab_loss_workspace(&l));
+      if (is_loss(n)) {
+        op = std::string(kVocabLossOp);
+        types.push_back(rows);
+        types.push_back(room);
       } else {
-        ins[3] = lse.at(f);
+        op = std::string(kVocabLossGradOp);
+        if (const ir::Node* f = loss_of(n); f != nullptr) {
+          ins[3] = lse.at(f);
+        } else {
+          Result<ir::Node*> forward = out.create_node(std::string(kVocabLossOp), {ins[0], ins[1], ins[2]}, {ins[3]->type(), rows, room});
+          if (!forward.is_ok()) return forward.status();
+          for (const auto& [k, v] : n->attrs()) forward.value()->set_attr(k, v);
+          ins[3] = forward.value()->output(1);
+        }
+        types.push_back(scratch(n->inputs()[0], fh_vocab_loss_grad_workspace(&l)));
       }
-      types.push_back(scratch(n->inputs()[0], loss ? fh_vocab_loss_workspace(&l) : fh_vocab_loss_grad_workspace(&l)));
     }
     Result<ir::Node*> c = out.create_node(std::move(op), std::move(ins), std::move(types));
     if (!c.is_ok()) return c.status();
     for (const auto& [k, v] : source->attrs()) c.value()->set_attr(k, v);
     for (size_t i = 0; i < n->outputs().size(); ++i) map[&n->outputs()[i]] = c.value()->output(static_cast<int32_t>(i));
-    if (loss) lse[n] = c.value()->output(1);
+    if (is_loss(n)) lse[n] = c.value()->output(1);
   }
   for (const ir::Value* o : g.outputs()) FRAME_RETURN_IF_ERROR(out.mark_output(map.at(o)));
   g = std::move(out);

@@ -55,6 +55,17 @@ def test_hip_plans_workspaces_and_hands_the_gradient_the_rows_log_sum_exps(opt):
     assert low.count(" hip_embedding_grad_internal(") == 1 and " embedding_grad_internal(" not in low
 
 
+GRADIENT_ALONE = ("%0 = graph_input() : bfloat16[40,64]@hip:0\n%1 = graph_input() : bfloat16[90,64]@hip:0\n%2 = graph_input() : int32[40]@hip:0\n"
+                  "%3 = graph_input() : bfloat16[]@hip:0\n%4 = graph_input() : bfloat16[]@hip:0\n"
+                  "%5, %6 = vocab_loss_grad_internal(%0, %1, %2, %3, %4) {mean=true} : bfloat16[40,64]@hip:0, bfloat16[90,64]@hip:0\n"
+                  "graph_output(%5)\ngraph_output(%6)\n")
+
+
+def test_hip_forms_the_log_sum_exps_of_a_gradient_without_its_forward():
+    low = host.hip_lowered(GRADIENT_ALONE, 1)
+    assert low.count(" hip_vocab_loss_internal(") == 1 and low.count(" hip_vocab_loss_grad_internal(") == 1 and "float32[40]" in low
+
+
 def test_hip_sums_a_tied_tables_gradients_in_one():
     back = lg.backward(lg.tied_graph(BF16, 300, 1000, 64, device="hip"), [0])
     assert back.count(" add(") == 1

@@ -7,6 +7,7 @@ import language_graphs as lg
 import language_ref as ref
 import oracle_lib as orc
 from frame_hip import graphs, host, synth
+from test_cpu_language_graph import GRADIENT_ALONE
 from tolerance import assert_deep_lowp
 
 pytestmark = pytest.mark.gpu
@@ -76,6 +77,15 @@ def test_loss_nodes_launched_by_themselves(case):
     lg.check_loss([loss, *grads], ins, dtype, mean)
 
 
+def test_a_compiled_gradient_without_its_forward():
+    say("vocab_loss gradient compiled by itself")
+    ins = lg.loss_inputs(BF16, 40, 90, 64)
+    zero, one = (synth.to_storage(np.full((), v, np.float32), BF16).reshape(()) for v in (0.0, 1.0))
+    grads = host.compile(GRADIENT_ALONE, "hip", 1).run(ins + [zero, one])
+    (loss,) = host.compile(lg.loss_graph(BF16, 40, 90, 64, device="hip"), "hip", 1).run(ins)
+    lg.check_loss([loss, *grads], ins, BF16, True)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_embedding_nodes_launched_by_themselves(dtype):
     say(f"embedding eager dtype={dtype}")
@@ -133,15 +143,24 @@ def test_language_model_training_step(tied):
         assert_deep_lowp(got[1 + i], want[1 + i], exact[1 + i], BF16, mean_slack=1.75, max_slack=3.0, what=f"gradient {i} {shapes[i]}")
 
 
-def test_language_model_step_repeated():
-    """The training step's executable run again and again on one stream gives the same bits, between eager work of the same ops."""
-    say("language model step repeated")
+def test_language_model_step_replayed(monkeypatch):
+    """The training step captured on its second run and replayed: other tokens, targets and parameters in the same tensors, eager work of the
+    same ops and host synchronisation between the replays; every run equals a fresh eager one bit for bit."""
+    say("language model step captured and replayed")
+    monkeypatch.setenv("FRAME_HIP_GRAPHS", "1")  # replay is opt-in; restored however the test ends
     tokens, vocab, d, cu = 96, 130, 64, [0, 40, 96]
     g, shapes = graphs.language_model(tokens, 2, vocab, d_model=d, heads=1, kv_heads=1, ffn=128, device="hip")
-    ins = lg.model_inputs(shapes, cu, tokens, vocab, BF16)
-    exe = host.compile(lg.backward(g, list(range(3, 3 + len(shapes)))), "hip", 1)
-    first = exe.run(ins)
+    text = lg.backward(g, list(range(3, 3 + len(shapes))))
+    exe, stream = host.compile(text, "hip", 1), host.Stream("hip")
+    ins, outs = exe.upload_inputs(lg.model_inputs(shapes, cu, tokens, vocab, BF16)), exe.alloc_outputs()
     small = lg.loss_inputs(BF16, 50, 70, 64)
-    for _ in range(4):
+    for run in range(6):
+        values = lg.model_inputs(shapes, cu, tokens, vocab, BF16, seed=901 + 50 * run)
+        for t, a in zip(ins, values):
+            host.check(host.lib().frame_tensor_upload(t.handle, np.ascontiguousarray(a).ctypes.data, a.nbytes))
+        exe.run_tensors(ins, outs, stream)  # eager, capture and launch, then replays
         eager("vocab_loss", "mean=true", small, [BF16, BF16, graphs.I32], [()])
-        assert all(np.array_equal(a, b) for a, b in zip(first, exe.run(ins)))
+        stream.synchronize()
+        want = host.compile(text, "hip", 1).run(values)  # a fresh executable: eager
+        for i, (a, b) in enumerate(zip(outs, want)):
+            assert np.array_equal(a.numpy(), b), f"run {run}, output {i}"
