@@ -110,21 +110,21 @@ constexpr int kSortThreads = 256, kSortItems = 8, kSortTile = kSortThreads * kSo
 constexpr int kSortAlone = 16 * 1024;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 
-// What a launch of the sort writes beside it: base's values, or zeros, in all of dtable. One store per thread, past the caches, which the
+// What a launch of the sort writes beside it: base's values, or zeros, in a share of dtable. One store per thread, past the caches, which the
 // sums want (131,072 x 4,096 bf16 and one token: 177 us; a loop over the table in as many threads as run at once 225, four stores per
 // thread 218, through the caches 200 and 60 us more for the sums).
 struct BaseArgs {
   const void* base;
   void* dtable;
-  int64_t end;  // in units of `size` bytes
-  int size;     // 16, or the elements' own where something is not aligned to 16
+  int64_t begin, end;  // in units of `size` bytes
+  int size;            // 16, or the elements' own where something is not aligned to 16
 };
 template <typename E>
 __device__ __forceinline__ void copy_base(const BaseArgs& a, int64_t at) {
   if (at < a.end) __builtin_nontemporal_store(a.base != nullptr ? static_cast<const E*>(a.base)[at] : E{}, static_cast<E*>(a.dtable) + at);
 }
 __device__ __forceinline__ void write_base(const BaseArgs& a, int group) {
-  const int64_t at = static_cast<int64_t>(group) * blockDim.x + threadIdx.x;
+  const int64_t at = a.begin + static_cast<int64_t>(group) * blockDim.x + threadIdx.x;
   if (a.size == 16) copy_base<u4_t>(a, at);
   else if (a.size == 4) copy_base<uint32_t>(a, at);
   else copy_base<uint16_t>(a, at);
@@ -180,8 +180,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortArgs
 }
 
 // Each token of the tile to its place.
-__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortArgs a) {
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortArgs a, const BaseArgs base) {
   __shared__ uint32_t bins[kSortWaves][kMaxBins];
+  if (static_cast<int>(blockIdx.x) >= a.tiles) return write_base(base, static_cast<int>(blockIdx.x) - a.tiles);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int nbins = 1 << a.bits;
   const int first = static_cast<int>(blockIdx.x) * kSortTile + wave * (kSortTile / kSortWaves);
@@ -227,9 +228,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortAr
 }
 
 // counts -> where each digit of each tile begins, by one workgroup.
-__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts, int n) {
+__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts, int n, const BaseArgs base) {
   __shared__ uint32_t waves[16];
   __shared__ uint32_t carry;
+  if (blockIdx.x > 0) return write_base(base, static_cast<int>(blockIdx.x) - 1);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) carry = 0;
   __syncthreads();
@@ -600,16 +602,22 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   if (workspace_bytes < p.bytes) return fail(FH_INVALID_ARGUMENT, fn + ": workspace too small");
   hipStream_t s = static_cast<hipStream_t>(stream);
 
-  // base (or zeros), beside the sort: beside its first launch, where it takes more than one (shares beside each of six: slower than one after the other)
+  // base (or zeros), in equal shares beside the sort's launches (32,768 tokens of 131,072 x 4,096: 283 us in all, 302 beside the first alone)
   const int64_t bytes = g->vocab * g->dim * esz;
   BaseArgs share{};
   share.base = base;
   share.dtable = dtable;
   share.size = bytes % 16 == 0 && !misaligned(base, 16) && !misaligned(dtable, 16) ? 16 : static_cast<int>(esz);
-  share.end = base == dtable ? 0 : bytes / share.size;
+  const int64_t units = base == dtable ? 0 : bytes / share.size;
   const bool alone = g->tokens <= kSortAlone;  // one workgroup sorts
-  // workgroups of `threads` that write base
-  auto sharers = [&](int64_t threads) { return static_cast<uint32_t>((share.end + threads - 1) / threads); };
+  const int64_t launches = alone ? 1 : 3 * p.passes;
+  int64_t launched = 0;
+  // the next share, and how many workgroups of `threads` write it
+  auto sharers = [&](int64_t threads) {
+    share.begin = units * launched / launches;
+    share.end = units * ++launched / launches;
+    return static_cast<uint32_t>((share.end - share.begin + threads - 1) / threads);
+  };
 
   char* ws = static_cast<char*>(workspace);
   auto list = [&](int i) { return reinterpret_cast<uint32_t*>(ws + i * p.list); };
@@ -619,8 +627,9 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   sort.vocab = static_cast<int>(g->vocab);
   sort.bits = static_cast<int>(p.bits);
   if (g->tokens == 0) {
-    if (share.end == 0) return FH_OK;
-    hipLaunchKernelGGL(sort_count_kernel, dim3(sharers(kSortThreads)), dim3(kSortThreads), 0, s, sort, share);
+    const uint32_t groups = sharers(kSortThreads);
+    if (groups == 0) return FH_OK;
+    hipLaunchKernelGGL(sort_count_kernel, dim3(groups), dim3(kSortThreads), 0, s, sort, share);
     return launch_status("sort_count_kernel launch");
   }
   if (alone) {
@@ -643,12 +652,14 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
       sort.shift = pass * sort.bits;
       sort.keys_out = list(2 * (pass & 1));
       sort.order_out = list(2 * (pass & 1) + 1);
-      const uint32_t groups = pass == 0 ? sharers(kSortThreads) : 0;
+      uint32_t groups = sharers(kSortThreads);
       hipLaunchKernelGGL(sort_count_kernel, dim3(tiles + groups), dim3(kSortThreads), 0, s, sort, share);
       if (fh_status st = launch_status("sort_count_kernel launch"); st != FH_OK) return st;
-      hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, s, sort.counts, static_cast<int>(p.tiles << p.bits));
+      groups = sharers(1024);
+      hipLaunchKernelGGL(sort_scan_kernel, dim3(1 + groups), dim3(1024), 0, s, sort.counts, static_cast<int>(p.tiles << p.bits), share);
       if (fh_status st = launch_status("sort_scan_kernel launch"); st != FH_OK) return st;
-      hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles), dim3(kSortThreads), 0, s, sort);
+      groups = sharers(kSortThreads);
+      hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles + groups), dim3(kSortThreads), 0, s, sort, share);
       if (fh_status st = launch_status("sort_scatter_kernel launch"); st != FH_OK) return st;
       sort.keys_in = sort.keys_out;
       sort.order_in = sort.order_out;

@@ -152,18 +152,72 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(const LossArgs a, int e
   if (blockIdx.x + 1 == gridDim.x && tid == 0) *a.count = before;
 }
 
+// The same list for up to MOST rows, by every workgroup for itself in LDS, which saves a launch; returns the rows' number. The workgroup that
+// is `first` also writes what loss_rows_kernel writes.
+template <int MOST>
+struct FewRows {
+  int32_t rows[MOST], targets[MOST];
+  int waves[16];
+};
+template <int THREADS, int MOST>
+__device__ __forceinline__ int list_few_rows(const LossArgs& a, FewRows<MOST>& few, bool first) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int count = 0;
+  for (int at = 0; at < a.tokens; at += THREADS) {
+    const int t = at + static_cast<int>(threadIdx.x);
+    const int target = t < a.tokens ? a.targets[t] : -1;
+    const bool mine = target >= 0 && target < a.vocab;
+    const uint64_t mask = __ballot(mine);
+    if (lane == 0) few.waves[wave] = __popcll(mask);
+    __syncthreads();
+    int to = count + __popcll(mask & ((1ull << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) to += few.waves[w];
+      count += few.waves[w];
+    }
+    if (mine) {
+      few.rows[to] = t;
+      few.targets[to] = target;
+    }
+    __syncthreads();
+    if (!first) continue;
+    if (mine) {
+      a.rows[to] = t;
+      a.targets_c[to] = target;
+      if (a.lse_c != nullptr) a.lse_c[to] = a.lse[t];
+    } else if (t < a.tokens && a.lse_c == nullptr) {
+      a.lse[t] = 0.0f;
+      if (a.row_loss != nullptr) a.row_loss[t] = 0.0f;
+    }
+  }
+  if (first && threadIdx.x == 0) *a.count = count;
+  return count;
+}
+
 // ---- forward ----
 
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN>
+constexpr int kFewRows = 64;
+// FEW: up to kFewRows rows, which the workgroups list themselves.
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN, bool FEW>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(const LossArgs a) {
   using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kListed, Lie::kRows, UNEVEN, UNEVEN>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
-  const int count = *a.count;
+  __shared__ FewRows<FEW ? kFewRows : 1> few;
+  int count;
+  const int32_t *rows = a.rows, *targets = a.targets_c;
+  if constexpr (FEW) {
+    count = list_few_rows<P::kThreads>(a, few, blockIdx.x == 0);
+    rows = few.rows;
+    targets = few.targets;
+  } else {
+    count = *a.count;
+  }
   int tm, tn;
   if (!place(blockIdx.x, (count + BM - 1) / BM, a.tiles_n, tm, tn)) return;
   const int m0 = tm * BM, n0 = tn * BN;
   typename P::Acc acc;
-  P::run(lds, {a.x, a.ldx, a.rows, count - 1, a.dim}, {a.w, a.ldw, nullptr, a.vocab - 1, a.dim}, m0, n0, (a.dim + kDepth - 1) / kDepth, acc);
+  P::run(lds, {a.x, a.ldx, rows, count - 1, a.dim}, {a.w, a.ldw, nullptr, a.vocab - 1, a.dim}, m0, n0, (a.dim + kDepth - 1) / kDepth, acc);
   float2(*joined)[BM] = reinterpret_cast<float2(*)[BM]>(lds);
   const int g = P::lane() >> 4, r = P::lane() & 15, row0 = P::wave_row() + r, column = n0 + P::wave_column();
   if (n0 + BN > a.vocab) {  // columns that do not exist are tokens of probability zero
@@ -177,7 +231,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(cons
   }
   int target[P::TM];
 #pragma unroll
-  for (int i = 0; i < P::TM; ++i) target[i] = m0 + row0 + 16 * i < count ? a.targets_c[m0 + row0 + 16 * i] : -1;
+  for (int i = 0; i < P::TM; ++i) target[i] = m0 + row0 + 16 * i < count ? targets[m0 + row0 + 16 * i] : -1;
   at_targets<P>(target, column, [&](int i, int j, int x) { a.at_target[m0 + row0 + 16 * i] = acc[i][j][x]; });
 #pragma unroll
   for (int i = 0; i < P::TM; ++i) {
@@ -204,29 +258,57 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(cons
   }
 }
 
-// ROWS rows per workgroup, 256 / ROWS threads each a share of the tiles; the shares are joined in their order.
-template <int ROWS>
-__global__ __launch_bounds__(256) void loss_join_kernel(const LossArgs a) {
-  __shared__ float2 shares[256 / ROWS][ROWS];
-  constexpr int SHARES = 256 / ROWS;
-  const int row = threadIdx.x % ROWS, share = threadIdx.x / ROWS;
+__device__ __forceinline__ void store_loss(const LossArgs& a, double sum, int count) {
+  const float loss = static_cast<float>(a.mean && count > 0 ? sum / count : sum);
+  if (a.loss_dtype == FH_F32) *static_cast<float*>(a.loss) = loss;
+  if (a.loss_dtype == FH_BF16) *static_cast<uint16_t*>(a.loss) = Io<bf16_t>::store(loss);
+  if (a.loss_dtype == FH_F16) *static_cast<uint16_t*>(a.loss) = Io<f16_t>::store(loss);
+}
+
+// ROWS rows per workgroup, THREADS / ROWS threads each a share of the tiles, eight of them at a time; the shares are joined in their
+// order. ALL: the only workgroup, which forms the loss as well.
+template <int ROWS, int THREADS, bool ALL>
+__global__ __launch_bounds__(THREADS) void loss_join_kernel(const LossArgs a) {
+  constexpr int SHARES = THREADS / ROWS, AHEAD = 8;
+  __shared__ float2 shares[SHARES][ROWS];
+  __shared__ float losses[ROWS];
+  const int row = threadIdx.x % ROWS, share = threadIdx.x / ROWS, count = *a.count;
   const int m = static_cast<int>(blockIdx.x) * ROWS + row;
-  const bool live = m < *a.count;
+  const bool live = m < count;
   float2 sum{0.0f, 0.0f};
   if (live)
-    for (int t = share; t < a.tiles_n; t += SHARES) sum = add_exponentials(sum, a.part[static_cast<int64_t>(t) * a.tokens + m]);
+    for (int first = share; first < a.tiles_n; first += AHEAD * SHARES) {
+      float2 p[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) p[i] = a.part[static_cast<int64_t>(min(first + i * SHARES, a.tiles_n - 1)) * a.tokens + m];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (first + i * SHARES < a.tiles_n) sum = add_exponentials(sum, p[i]);
+    }
   shares[share][row] = sum;
 #pragma unroll
   for (int o = SHARES / 2; o > 0; o >>= 1) {
     __syncthreads();
     if (share < o) shares[share][row] = sum = add_exponentials(sum, shares[share + o][row]);
   }
-  if (share != 0 || !live) return;
-  const float lse = kLn2 * (sum.x + __builtin_amdgcn_logf(sum.y));
-  const int t = a.rows[m];
-  a.lse[t] = lse;
-  a.at_target[m] = lse - a.at_target[m];
-  if (a.row_loss != nullptr) a.row_loss[t] = a.at_target[m];
+  float loss = 0.0f;
+  if (share == 0 && live) {
+    const float lse = kLn2 * (sum.x + __builtin_amdgcn_logf(sum.y));
+    const int t = a.rows[m];
+    a.lse[t] = lse;
+    loss = lse - a.at_target[m];
+    a.at_target[m] = loss;
+    if (a.row_loss != nullptr) a.row_loss[t] = loss;
+  }
+  if constexpr (ALL) {
+    if (share == 0) losses[row] = loss;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double all = 0.0;
+      for (int r = 0; r < ROWS; ++r) all += losses[r];
+      store_loss(a, all, count);
+    }
+  }
 }
 
 // The loss, by one workgroup: the rows' losses in one order, in double.
@@ -241,23 +323,30 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const LossArgs a) {
     if (tid < o) shares[tid] += shares[tid + o];
     __syncthreads();
   }
-  if (tid != 0) return;
-  const float loss = static_cast<float>(a.mean && count > 0 ? shares[0] / count : shares[0]);
-  if (a.loss_dtype == FH_F32) *static_cast<float*>(a.loss) = loss;
-  if (a.loss_dtype == FH_BF16) *static_cast<uint16_t*>(a.loss) = Io<bf16_t>::store(loss);
-  if (a.loss_dtype == FH_F16) *static_cast<uint16_t*>(a.loss) = Io<f16_t>::store(loss);
+  if (tid == 0) store_loss(a, shares[0], count);
 }
 
 // ---- gradients ----
 
+constexpr int kGatherFew = 1024;
 // A wave per row: xc's row m is x's row rows[m]; rows behind the last, up to a multiple of 64, are zeros (dw sums over them); dx's rows
-// without a target are zeros.
+// without a target are zeros. FEW: up to kGatherFew rows, which the workgroups list themselves.
+template <bool FEW>
 __global__ __launch_bounds__(256) void loss_gather_kernel(const LossArgs a) {
+  __shared__ FewRows<FEW ? kGatherFew : 1> few;
   const int lane = threadIdx.x & 63, t = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int count = *a.count, end = (count + 63) / 64 * 64;
+  int count;
+  const int32_t* rows = a.rows;
+  if constexpr (FEW) {
+    count = list_few_rows<256>(a, few, blockIdx.x == 0);
+    rows = few.rows;
+  } else {
+    count = *a.count;
+  }
+  const int end = (count + 63) / 64 * 64;
   const u32x4_t zeros{0, 0, 0, 0};
   if (t < end) {
-    const uint16_t* from = t < count ? a.x + a.rows[t] * a.ldx : nullptr;
+    const uint16_t* from = t < count ? a.x + rows[t] * a.ldx : nullptr;
     for (int c = lane * 8; c < a.dim; c += 512)
       *reinterpret_cast<u32x4_t*>(a.xc + static_cast<int64_t>(t) * a.dim + c) = from != nullptr ? *reinterpret_cast<const u32x4_t*>(from + c) : zeros;
   }
@@ -610,23 +699,34 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
   a.targets_c = reinterpret_cast<int32_t*>(ws + room.targets);
   a.tiles_n = static_cast<int>(room.tiles_n);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (fh_status st = list_rows(a, s); st != FH_OK) return st;
+  const bool few = g->tokens > 0 && g->tokens <= kFewRows;  // (then tiles have 64 rows)
+  if (!few)
+    if (fh_status st = list_rows(a, s); st != FH_OK) return st;
   if (g->tokens > 0) {
     const fh_status st = by_type(g->dtype, [&]<typename T>() {
       by_tile(tile_for(g->tokens, g->vocab), g->tokens, g->vocab, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
-        if (g->dim % kDepth != 0)
-          hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN, true>), grid, dim3(WM * WN * 64), 0, s, a);
-        else
-          hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN, false>), grid, dim3(WM * WN * 64), 0, s, a);
+        auto go = [&]<bool UNEVEN, bool FEW>() {
+          hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN, UNEVEN, FEW>), grid, dim3(WM * WN * 64), 0, s, a);
+        };
+        const bool uneven = g->dim % kDepth != 0;
+        if constexpr (BM == 64) {
+          if (few) return uneven ? go.template operator()<true, true>() : go.template operator()<false, true>();
+        }
+        uneven ? go.template operator()<true, false>() : go.template operator()<false, false>();
       });
       return launch_status("loss_logits_kernel launch");
     });
     if (st != FH_OK) return st;
-    // a few rows: a workgroup each (one row of 1,024 tiles: 32 us with 16 threads)
+    // up to 16 rows by one workgroup, which sums them too (16 rows of 5,000 x 512: 14 us in all, 17 with the sum's launch); a few: a workgroup
+    // each (one row of 1,024 tiles by 16 threads: 32 us)
+    if (g->tokens <= 16) {
+      hipLaunchKernelGGL((loss_join_kernel<16, 1024, true>), dim3(1), dim3(1024), 0, s, a);
+      return launch_status("loss_join_kernel launch");
+    }
     if (g->tokens <= 4 * device_cu_count())
-      hipLaunchKernelGGL((loss_join_kernel<1>), dim3(static_cast<uint32_t>(g->tokens)), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((loss_join_kernel<1, 256, false>), dim3(static_cast<uint32_t>(g->tokens)), dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((loss_join_kernel<16>), dim3(static_cast<uint32_t>((g->tokens + 15) / 16)), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((loss_join_kernel<16, 256, false>), dim3(static_cast<uint32_t>((g->tokens + 15) / 16)), dim3(256), 0, s, a);
     if (fh_status st2 = launch_status("loss_join_kernel launch"); st2 != FH_OK) return st2;
   }
   hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, s, a);
@@ -674,9 +774,15 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
   a.g = reinterpret_cast<uint16_t*>(ws + room.g);
   a.splits = plan.dx.splits;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (fh_status st = list_rows(a, s); st != FH_OK) return st;
+  const dim3 gather(static_cast<uint32_t>(up(g->tokens, 64) / 4));
+  const bool few = g->tokens > 0 && g->tokens <= kGatherFew;
+  if (!few)
+    if (fh_status st = list_rows(a, s); st != FH_OK) return st;
   if (g->tokens > 0) {
-    hipLaunchKernelGGL(loss_gather_kernel, dim3(static_cast<uint32_t>(up(g->tokens, 64) / 4)), dim3(256), 0, s, a);
+    if (few)
+      hipLaunchKernelGGL((loss_gather_kernel<true>), gather, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((loss_gather_kernel<false>), gather, dim3(256), 0, s, a);
     if (fh_status st = launch_status("loss_gather_kernel launch"); st != FH_OK) return st;
   }
   return by_type(g->dtype, [&]<typename T>() {

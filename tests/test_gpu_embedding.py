@@ -135,6 +135,32 @@ def test_gradient_runs(hip, pattern, tokens):
     assert np.array_equal(e.backward(dout).astype(np.float64), want)
 
 
+@pytest.mark.parametrize("tokens", [1024, 1025, 4096, 4097, 16384, 16385])
+def test_gradient_where_another_sort_takes_over(hip, tokens):
+    say(f"embedding gradient, {tokens} tokens of 700 ids")
+    vocab, dim = 700, 16
+    ids = text_ids(tokens, vocab, 17, 0.1)
+    e = Embedding(hip, F32, tokens, vocab, dim, ids)
+    dout = np.random.default_rng(2).integers(-8, 9, (tokens, dim)).astype(np.float32)
+    want = np.zeros((vocab, dim))
+    named = (ids >= 0) & (ids < vocab)
+    np.add.at(want, ids[named], dout[named].astype(np.float64))
+    assert np.array_equal(e.backward(dout).astype(np.float64), want)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 510, 511, 512, 513, 262143, 262144])
+def test_gradient_of_any_number_of_digits(hip, vocab):
+    """The ids outside the vocabulary sort behind all others: their key is the vocabulary's size, which may need one bit more."""
+    say(f"embedding gradient, {vocab} ids")
+    tokens, dim = 3000, 8
+    ids = np.random.default_rng(vocab).integers(0, vocab, tokens).astype(np.int32)
+    ids[::7], ids[1], ids[-1] = -1, vocab - 1, vocab - 1
+    dout = np.random.default_rng(2).integers(-8, 9, (tokens, dim)).astype(np.float32)
+    want = np.zeros((vocab, dim))
+    np.add.at(want, ids[ids >= 0], dout[ids >= 0].astype(np.float64))
+    assert np.array_equal(Embedding(hip, F32, tokens, vocab, dim, ids).backward(dout).astype(np.float64), want)
+
+
 def test_many_tokens_and_a_large_vocabulary(hip):
     say("70,000 tokens of 300,000 ids")
     tokens, vocab, dim = 70000, 300000, 8

@@ -116,6 +116,9 @@ SHAPES = [  # tokens, vocab, dim, share of rows without a target, mean, pad
     # the larger tiles: of logits, of dx and dw, of both, and few rows of many columns
     (2048, 8197, 40, 0.1, 1, 0), (2100, 2051, 6152, 0.3, 1, 0), (300, 11003, 24, 0.0, 1, 0), (800, 900, 5000, 0.0, 1, 0),
     (60, 40000, 16, 0.0, 1, 0), (5, 70, 33000, 0.0, 1, 0),
+    # where another kernel takes over: the joins' rows, the rows that workgroups list themselves, runs of the list
+    (16, 300, 24, 0.3, 1, 0), (17, 300, 24, 0.3, 1, 0), (64, 300, 24, 0.3, 1, 0), (1024, 130, 24, 0.3, 1, 0), (1025, 130, 24, 0.3, 1, 0),
+    (2049, 70, 16, 0.5, 0, 0),
 ]
 
 
