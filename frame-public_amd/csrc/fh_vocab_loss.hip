@@ -1,13 +1,22 @@
 // Softmax cross entropy over a vocabulary without keeping the logits (fh_vocab_loss_fwd) and its gradients (fh_vocab_loss_grad).
 //
 // With z = x w^T, lse = log sum_v exp z and one target per row:
-//   forward:   row_loss = lse - z[target]; a tile of logits leaves the maximum and the sum of its exponentials per row, which a second
-//              kernel joins over the tiles of the vocabulary.
+//   forward:   row_loss = lse - z[target]; a tile of logits leaves per row its maximum and the sum of its exponentials, which a second
+//              kernel joins over the tiles of the vocabulary, in their order.
 //   gradients: with g = exp(z - lse) - [v = target], dx = f g w and dw = f g^T x, f = dloss (/ count for the mean): a piece of
 //              the vocabulary at a time, whose logits are formed again, whose g is kept in the storage type (f16: times 2^14, so that
 //              probabilities down to 2^-28 keep their bits) and read by both products. f is left to the products' results.
 // Rows without a target are taken out first: a list of the others stands for x's rows (forward), or they are copied together (gradients,
-// where rows are also summed over, and what such rows hold must not reach the sums).
+// where rows are also summed over, and what such rows hold must not reach the sums). Their number is on the device alone: grids are made
+// for all rows, and workgroups without work end at once.
+//
+// Measured (bf16; two cards, which differ by 6 % under this load):
+//   7,373 rows of 131,072 x 4,096:  loss 5.82 to 6.15 ms, 1,290 to 1,360 TFLOP/s (a plain product of these sizes by the vendor's library
+//                                   5.48 ms). The matrix unit is busy for 75 % of the cycles at 1.75 GHz of 2.4: the board's power.
+//   3,686 rows of the same:         gradients 9.33 to 10.2 ms, 1,160 to 1,270 TFLOP/s over three products; per piece of 16,384 columns
+//                                   derivatives 422 us, dx 422, dw 411 (busy for 71, 71 and 67 % of the cycles).
+//   4,096 rows of 32,768 x 1,024:   231 to 259 us and 730 to 805. Short products: 4 us of a tile's 31 are its beginning and end.
+//   1 row of 131,072 x 4,096:       182 us, 5.9 TB/s: the bytes of w (64 x 128 tiles, two stages ahead).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -49,11 +58,11 @@ struct LossArgs {
   int* count;        // rows with a target
   int32_t* rows;     // which they are, in their order
   float* at_target;  // their target's logit
-  float2* part;      // [column tiles][tokens]: maximum, sum of exp(z - maximum)
+  int32_t* targets_c;  // and their targets
+  float2* part;        // [column tiles][tokens]: from2, sum of 2^(z log2 e - from2)
   int tiles_n;
-  // gradients: the rows with a target copied together, their targets and log-sum-exps, a piece of g, fp32 sums of dx over the pieces
+  // gradients: the rows with a target copied together, their log-sum-exps, a piece of g, fp32 sums of dx over the pieces
   uint16_t* xc;
-  int32_t* targets_c;
   float* lse_c;
   uint16_t* g;
   int64_t ldg;
@@ -197,8 +206,8 @@ __device__ __forceinline__ int list_few_rows(const LossArgs& a, FewRows<MOST>& f
 
 // ---- forward ----
 
+// FEW: up to kFewRows rows, which the workgroups list themselves (16 rows of 5,000 x 512: 10 us in all, 14 with a launch for the list).
 constexpr int kFewRows = 64;
-// FEW: up to kFewRows rows, which the workgroups list themselves.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN, bool FEW>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(const LossArgs a) {
   using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kListed, Lie::kRows, UNEVEN, UNEVEN>;
@@ -328,9 +337,10 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const LossArgs a) {
 
 // ---- gradients ----
 
-constexpr int kGatherFew = 1024;
 // A wave per row: xc's row m is x's row rows[m]; rows behind the last, up to a multiple of 64, are zeros (dw sums over them); dx's rows
-// without a target are zeros. FEW: up to kGatherFew rows, which the workgroups list themselves.
+// without a target are zeros. FEW: up to kGatherFew rows, which the workgroups list themselves (1,024 rows of 5,000 x 512: 51 us in all,
+// 57 for one row more and a launch for the list).
+constexpr int kGatherFew = 1024;
 template <bool FEW>
 __global__ __launch_bounds__(256) void loss_gather_kernel(const LossArgs a) {
   __shared__ FewRows<FEW ? kGatherFew : 1> few;
@@ -508,7 +518,9 @@ fh_status check_loss(const std::string& fn, const fh_vocab_loss* g) {
   return FH_OK;
 }
 
-// The tile of a product of m rows and n columns: the largest that gives (nearly) every CU a workgroup, as in fh_gemm16.hip.
+// The tile of a product of m rows and n columns: the largest that gives (nearly) every CU a workgroup, as in fh_gemm16.hip (loss of 8,192
+// rows of 131,072 x 512: 1,106 us in 256 x 256 tiles, 1,451 in 128 x 128; 400 rows of 131,072 x 1,024: 136 and 173; dw of 512 rows of
+// 131,072 x 4,096, eight stages a tile: 6 % of the whole call slower in 128 x 128, 19 % in 64 x 128).
 struct Shape {
   int m, n;
 };
@@ -532,7 +544,8 @@ void by_tile(Shape t, int64_t m, int64_t n, F&& launch) {
 
 // dx is small and its sums are long, a piece's columns: where tiles leave CUs idle, the columns are split among `splits` workgroups, whose
 // sums a second launch joins. The cheapest by rounds of workgroups over the CUs, a tile's products over its share of the columns
-// at the rates below, and a stage's worth of waiting at either end.
+// at the rates below, and a stage's worth of waiting at either end (4,096 rows of 32,768 x 1,024: dx 445 us in 128 x 128 tiles, 276 and 16
+// for the join in four splits of 256 x 256; 333 of 5,003 x 1,000: 23, and 10 and 5).
 struct DxPlan {
   Shape tile;
   int splits;

@@ -422,14 +422,16 @@ fh_status fh_embedding_fwd(const fh_token_embedding* geom, const void* table, co
 
 /* dtable[v] = base[v] + scale * sum of dout[t] over the tokens with ids[t] = v, in fp32, rounded once; base NULL is zeros. base may be
  * dtable itself: then rows that no token names are left as they are. The table's other gradient (tied weights: fh_vocab_loss_grad's dw)
- * goes in that way. Deterministic: a sum's order depends on the ids alone. */
+ * goes in that way. Nothing else may overlap. Deterministic: a sum's order depends on the ids and the sizes alone. */
 int64_t fh_embedding_grad_workspace(const fh_token_embedding* geom);
 fh_status fh_embedding_grad(const fh_token_embedding* geom, const void* dout, const int32_t* ids, const void* base, void* dtable,
                             void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Softmax cross entropy of the logits x w^T against one target per row, without keeping the logits: x [tokens, dim], w [vocab, dim]
  * (the embedding's table where they are tied), rows x_stride and w_stride elements apart. Rows without a target (see above) do not count:
- * no work is done for them. bf16 / f16, dim and strides multiples of 8, tensors 16-byte aligned, no output may overlap an input. */
+ * no work is done for them. What is not finite reaches the rows that meet it, a row's NaN its loss, its dx and all of dw; a logit of -infinity
+ * is a probability of 0, one of +infinity makes its row NaN. bf16 / f16, dim and strides multiples of 8, strides less than 2^22, tensors
+ * 16-byte aligned, no output may overlap an input. A workspace, here and above, serves one call at a time. */
 typedef struct fh_vocab_loss {
   int32_t dtype;      /* of x, w, dx and dw: FH_BF16 or FH_F16 */
   int32_t loss_dtype; /* of the loss and of its gradient, one value each: FH_F32 or dtype */
