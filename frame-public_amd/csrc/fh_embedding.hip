@@ -513,14 +513,14 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const EmbedArgs a) 
   }
 }
 
-constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int64_t kMaxUnits = int64_t{1} << 31;  // that one launch writes beside the sort
 
 fh_status check_embedding(const std::string& fn, const fh_token_embedding* g) {
   if (g == nullptr) return fail(FH_INVALID_ARGUMENT, fn + ": null geometry");
   if (!is_supported_float(g->dtype)) return fail(FH_UNIMPLEMENTED, fn + ": dtype must be f32, f16 or bf16");
   if (g->tokens < 0 || g->vocab < 1 || g->dim < 1) return fail(FH_INVALID_ARGUMENT, fn + ": bad tokens, vocab or dim");
-  // the grids' and the sort's indexes are 32-bit
-  if (g->vocab > 0x7ffffffe || g->dim > (1 << 20) || g->tokens > (1 << 28) || g->tokens * ((g->dim + 63) / 64) > kMaxGrid ||
+  // a launch has fewer than 2^32 threads: 2^26 waves (of 1,024 columns or more of a token; the gradient's have fewer)
+  if (g->vocab > 0x7ffffffe || g->dim > (1 << 20) || g->tokens > (1 << 25) || g->tokens * ((g->dim + 1023) / 1024) >= (1 << 26) ||
       g->vocab * g->dim > (int64_t{1} << 38))
     return fail(FH_INVALID_ARGUMENT, fn + ": too large");
   if (g->row_stride < g->dim) return fail(FH_INVALID_ARGUMENT, fn + ": row_stride is less than dim");
@@ -614,7 +614,7 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   share.size = bytes % 16 == 0 && !misaligned(base, 16) && !misaligned(dtable, 16) ? 16 : static_cast<int>(esz);
   const int64_t units = base == dtable ? 0 : bytes / share.size;
   const bool alone = g->tokens <= kSortAlone;  // one workgroup sorts
-  const int64_t launches = alone ? 1 : 3 * p.passes;
+  const int64_t sorts = alone ? 1 : 3 * p.passes, before = units / kMaxUnits, launches = before + sorts;
   int64_t launched = 0;
   // the next share, and how many workgroups of `threads` write it
   auto sharers = [&](int64_t threads) {
@@ -630,6 +630,10 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
   sort.tokens = static_cast<int>(g->tokens);
   sort.vocab = static_cast<int>(g->vocab);
   sort.bits = static_cast<int>(p.bits);
+  for (int64_t i = 0; i < before; ++i) {  // what would be too many threads beside the sort is written before it
+    hipLaunchKernelGGL(sort_count_kernel, dim3(sharers(kSortThreads)), dim3(kSortThreads), 0, s, sort, share);
+    if (fh_status st = launch_status("sort_count_kernel launch"); st != FH_OK) return st;
+  }
   if (g->tokens == 0) {
     const uint32_t groups = sharers(kSortThreads);
     if (groups == 0) return FH_OK;

@@ -493,7 +493,6 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const Lo
 
 // ---- host ----
 
-constexpr int kTile = 64;  // the smallest tile's rows and columns
 constexpr int kLeastPiece = 256;
 constexpr int64_t kPieceValues = int64_t{1} << 26;  // of g: 128 MB (3,686 rows of 131,072 columns: 9.64 ms; 256 MB 9.68, 512 MB 9.56)
 constexpr int64_t kMostPieceValues = int64_t{1} << 28;
@@ -508,9 +507,10 @@ fh_status check_loss(const std::string& fn, const fh_vocab_loss* g) {
   if (g->mean != 0 && g->mean != 1) return fail(FH_INVALID_ARGUMENT, fn + ": mean must be 0 or 1");
   if (g->tokens < 0 || g->vocab < 1 || g->dim < 8) return fail(FH_INVALID_ARGUMENT, fn + ": bad tokens, vocab or dim");
   if (g->dim % 8 != 0) return fail(FH_UNIMPLEMENTED, fn + ": dim must be a multiple of 8");
-  // tiles are counted in 32 bits
-  if (g->tokens > (1 << 24) || g->vocab > (1 << 24) || g->dim > (1 << 20) ||
-      up(g->tokens, kTile) / kTile * (up(std::max(g->vocab, g->dim), kLeastPiece) / kTile) > 0x7fffffff)
+  // a launch has fewer than 2^32 threads: 2^22 of the largest tiles, of 512 threads (smaller ones are taken where these are few)
+  auto tiles = [](int64_t m, int64_t n) { return up(m, 256) / 256 * (up(n, 256) / 256); };
+  if (g->tokens > (1 << 24) || g->vocab > (1 << 24) || g->dim > (1 << 20) || tiles(g->tokens, std::max(g->vocab, g->dim)) > (1 << 22) ||
+      tiles(g->vocab, g->dim) > (1 << 22))
     return fail(FH_INVALID_ARGUMENT, fn + ": too large");
   for (int64_t ld : {g->x_stride, g->w_stride})
     if (ld < g->dim || ld % 8 != 0 || ld >= (int64_t{1} << 22))

@@ -237,6 +237,36 @@ def test_table_past_32_bits(hip):
     assert (near == 0x3f80).all()
 
 
+def test_table_of_more_elements_than_a_launch_writes(hip):
+    """Elements that are written one by one (the table begins behind 2 bytes), more than 2^31 of them: in two launches."""
+    vocab, dim, tokens = 2 ** 21 + 5, 1029, 5
+    say(f"table of {vocab * dim} elements behind 2 bytes")
+    ids = np.array([1, vocab - 1, 1, vocab // 2, -1], np.int32)
+    lib = hip.lib()
+    dout = synth.tensor(27, (tokens, dim), BF16, "normal")
+    table = hip.DeviceBuffer((vocab * dim + 8) * 2)
+    hip.check(lib.fh_fill(table.value, 2, 0x3f80, vocab * dim + 8, None))
+    g = hip.TokenEmbedding(dtype=BF16, tokens=tokens, vocab=vocab, dim=dim, row_stride=dim, scale=1.0)
+    need = lib.fh_embedding_grad_workspace(ctypes.byref(g))
+    ws, dev_ids, dev_dout = hip.DeviceBuffer(need), hip.to_device(ids), hip.to_device(dout)
+    hip.check(lib.fh_embedding_grad(ctypes.byref(g), dev_dout.value, dev_ids.value, None, table.value + 2, ws.value, need, None))
+    hip.check(lib.fh_device_synchronize())
+
+    def elements(first, n):
+        got = np.empty(n, np.uint16)
+        hip.check(lib.fh_memcpy(got.ctypes.data, table.value + 2 + first * 2, got.nbytes, hip.D2H, None))
+        return got
+
+    assert elements(-1, 1)[0] == 0x3f80 and (elements(vocab * dim, 7) == 0x3f80).all(), "written outside the tensor"
+    named = {1: ref.values(dout[0], BF16) + ref.values(dout[2], BF16), vocab - 1: ref.values(dout[1], BF16), vocab // 2: ref.values(dout[3], BF16)}
+    middle = vocab * dim // 2 // dim  # where the second launch takes over
+    rows = {0, 2, middle - 1, middle, middle + 1, 2 ** 31 // dim - 1, 2 ** 31 // dim, 2 ** 31 // dim + 1, vocab - 2}
+    rows |= set(np.random.default_rng(28).integers(0, vocab, 200).tolist())
+    for v in sorted(rows | set(named)):
+        want = named.get(v, np.zeros(dim))
+        ref.check(ref.values(elements(v * dim, dim), BF16), want, ref.rounded(want, 0.0, BF16), f"row {v}")
+
+
 def test_captured_and_replayed(hip):
     say("embedding and its gradient captured, ids changed between the replays")
     tokens, vocab, dim = 700, 90, 136
