@@ -7,10 +7,11 @@
 // work: a wave sums the rows of a chunk id by id, ids that lie within a chunk are finished there, the rest leave fp32 parts that a
 // join adds in their order. No atomics on floats: every sum has one order. Rows that no token names are zeros or base's: all rows are
 // written so beside the sort, in the launches that a few workgroups of it would leave the chip idle in, and the sums overwrite theirs.
+// Few tokens need no sort: an id's first token looks for the others and sums them, in one launch.
 //
 // Measured: forward, 8,192 tokens of 131,072 x 4,096 bf16: 21.8 us, 5.1 TB/s; 64 tokens of 1,024: 6.7 (the call). Gradient: 32,768 tokens of
 // 131,072 x 4,096 bf16: 283 us (sort and zeros 208, sums 58, join 16) for 1.3 GB that must move (256 at a copy's rate; named rows are
-// written twice); 4,096 of 32,768 x 1,024 on a base 34 us (20, 8 and 5); 301 of 5,003 x 333 f32 15 us: three dependent launches.
+// written twice); 4,096 of 32,768 x 1,024 on a base 34 us (20, 8 and 5); 301 of 5,003 x 333 f32 7.3 us, about what any call takes.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -513,6 +514,96 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const EmbedArgs a) 
   }
 }
 
+// ---- few tokens: no sort ----
+
+// Taken for up to 1,024 tokens whose workgroups are 4,096 at most and write at most 2^22 units (us, with this kernel and with the sort's three
+// launches; bf16 unless said): 301 of 5,003 x 333 f32: 7.3, 15.4; 64 of 32,768 x 1,024: 14.8, 18 (on another base 24, 30; in place 6.8, 15);
+// 512 of 131,072 x 4,096 in place: 12, 18 (1,000, 8,000 workgroups: 25, 18); 512 tokens of one id: 19, 22; 1,000: 34, 27, but 1,000 as
+// frequent as words on a base 26, 32 and of 50,257 x 64 f32 7.4, 15. 2^26 units of 131,072 x 4,096: 228, 185 (every workgroup reads the ids).
+constexpr int kFew = 1024, kFewGroups = 4096, kFewThreads = 256, kFewWaves = kFewThreads / 64;
+constexpr int64_t kFewUnits = int64_t{1} << 22;
+
+// One launch. The first `groups` workgroups: each looks for its token's id among all; the id's first token sums the rows of all of them, 64
+// vectors of columns wide, many rows by four waves, each a run of them. The others write base or zeros, `row_units` units a row, in the
+// rows that no token names. Tokens: EACH * kFewThreads at most.
+template <typename T, int EACH>
+__global__ __launch_bounds__(kFewThreads) void embedding_few_kernel(const EmbedArgs a, const BaseArgs base, uint32_t groups, uint32_t row_units) {
+  using S = typename Io<T>::storage;
+  constexpr int V = kVec<T>, AHEAD = 16;
+  __shared__ float runs[kFewWaves][64][V];
+  __shared__ uint16_t list[EACH * kFewThreads];
+  __shared__ int counts[EACH * kFewWaves];
+  __shared__ uint8_t named[kFewThreads];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int ids[EACH];
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) ids[j] = j * kFewThreads + tid < a.tokens ? a.ids[j * kFewThreads + tid] : -1;
+  if (blockIdx.x >= groups) {
+    const int64_t at = base.begin + static_cast<int64_t>(blockIdx.x - groups) * kFewThreads, row = at / row_units;
+    named[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < EACH; ++j)  // the workgroup's units lie in as many rows as it has threads at most
+      if (ids[j] - row >= 0 && ids[j] - row < kFewThreads) named[ids[j] - row] = 1;
+    __syncthreads();
+    if (named[(static_cast<uint32_t>(at - row * row_units) + tid) / row_units]) return;
+    return write_base(base, static_cast<int>(blockIdx.x - groups));
+  }
+  const int token = static_cast<int>(blockIdx.x / a.blocks);
+  const int c = (static_cast<int>(blockIdx.x % a.blocks) * 64 + lane) * V;
+  const int id = a.ids[token];
+  if (id < 0 || id >= a.vocab) return;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const uint64_t all = __ballot(ids[j] == id);
+    if (lane == 0) counts[j * kFewWaves + wave] = __popcll(all);
+  }
+  __syncthreads();
+  int n = 0;  // tokens of the id
+#pragma unroll
+  for (int i = 0; i < EACH * kFewWaves; ++i) {
+    const int j = i / kFewWaves;
+    const uint64_t all = __ballot(ids[j] == id);
+    if (i % kFewWaves == wave && ids[j] == id)
+      list[n + __popcll(all & ((1ull << lane) - 1))] = static_cast<uint16_t>(j * kFewThreads + tid);
+    n += __builtin_amdgcn_readfirstlane(counts[i]);
+  }
+  __syncthreads();
+  if (list[0] != token) return;
+  // the list's run that this wave sums
+  const int each = n <= AHEAD ? n : (n + kFewWaves - 1) / kFewWaves, first = wave * each, last = min(n, first + each);
+  float sum[V];
+#pragma unroll
+  for (int x = 0; x < V; ++x) sum[x] = 0.0f;
+  for (int p = first; p < last; p += AHEAD) {
+    const int mine = list[min(p + (lane & (AHEAD - 1)), last - 1)];
+    uint4 row[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int64_t t = __builtin_amdgcn_readlane(mine, i);
+      row[i] = p + i < last && c < a.dim ? load_bits<T>(static_cast<const S*>(a.in) + t * a.ld + c, a.dim - c) : uint4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      float v[V];
+      unpack_vec<T>(row[i], v);
+#pragma unroll
+      for (int x = 0; x < V; ++x) sum[x] = p + i < last ? sum[x] + v[x] : sum[x];
+    }
+  }
+  if (n > AHEAD) {
+#pragma unroll
+    for (int x = 0; x < V; ++x) runs[wave][lane][x] = sum[x];
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+      sum[x] = runs[0][lane][x];
+      for (int w = 1; w < kFewWaves; ++w) sum[x] += runs[w][lane][x];
+    }
+  }
+  if (wave == 0 && c < a.dim) finish_row<T>(a, id, c, sum);
+}
+
 constexpr int64_t kMaxUnits = int64_t{1} << 31;  // that one launch writes beside the sort
 
 fh_status check_embedding(const std::string& fn, const fh_token_embedding* g) {
@@ -623,6 +714,39 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
     return static_cast<uint32_t>((share.end - share.begin + threads - 1) / threads);
   };
 
+  EmbedArgs a{};
+  a.in = dout;
+  a.base = base;
+  a.out = dtable;
+  a.ids = ids;
+  a.ld = g->row_stride;
+  a.tokens = static_cast<int>(g->tokens);
+  a.vocab = static_cast<int>(g->vocab);
+  a.dim = static_cast<int>(g->dim);
+  a.scale = g->scale;
+  const int64_t width = 64 * 16 / esz;
+  a.blocks = static_cast<uint32_t>((g->dim + width - 1) / width);
+
+  if (g->tokens > 0 && g->tokens <= kFew && g->tokens * a.blocks <= kFewGroups) {
+    // a row is a whole number of units here
+    BaseArgs rest = share;
+    rest.size = g->dim * esz % 16 == 0 && !misaligned(base, 16) && !misaligned(dtable, 16) ? 16 : static_cast<int>(esz);
+    rest.end = base == dtable ? 0 : bytes / rest.size;
+    auto launch = [&]<typename T, int EACH>() {
+      const uint32_t row_units = static_cast<uint32_t>(g->dim * esz / rest.size), groups = static_cast<uint32_t>(g->tokens * a.blocks);
+      const dim3 grid(groups + static_cast<uint32_t>((rest.end + kFewThreads - 1) / kFewThreads));
+      hipLaunchKernelGGL((embedding_few_kernel<T, EACH>), grid, dim3(kFewThreads), 0, s, a, rest, groups, row_units);
+      return launch_status("embedding_few_kernel launch");
+    };
+    auto by_tokens = [&]<typename T>() {
+      return g->tokens <= kFew / 2 ? launch.template operator()<T, kFew / kFewThreads / 2>() : launch.template operator()<T, kFew / kFewThreads>();
+    };
+    if (rest.end <= kFewUnits) {
+      if (g->dtype == FH_F32) return by_tokens.template operator()<float>();
+      return g->dtype == FH_F16 ? by_tokens.template operator()<f16_t>() : by_tokens.template operator()<bf16_t>();
+    }
+  }
+
   char* ws = static_cast<char*>(workspace);
   auto list = [&](int i) { return reinterpret_cast<uint32_t*>(ws + i * p.list); };
   SortArgs sort{};
@@ -674,22 +798,11 @@ extern "C" fh_status fh_embedding_grad(const fh_token_embedding* g, const void* 
     }
   }
 
-  EmbedArgs a{};
-  a.in = dout;
-  a.base = base;
-  a.out = dtable;
-  a.ld = g->row_stride;
-  a.tokens = static_cast<int>(g->tokens);
-  a.vocab = static_cast<int>(g->vocab);
-  a.dim = static_cast<int>(g->dim);
-  a.scale = g->scale;
   a.keys = sort.keys_out;
   a.order = sort.order_out;
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.chunks = static_cast<int>(p.chunks);
   a.part_ld = static_cast<int>(p.part_ld);
-  const int64_t width = 64 * 16 / esz;
-  a.blocks = static_cast<uint32_t>((g->dim + width - 1) / width);
   auto launch = [&]<typename T, int CHUNK>() {
     hipLaunchKernelGGL((embedding_sum_kernel<T, CHUNK>), dim3(static_cast<uint32_t>((p.chunks * a.blocks + 3) / 4)), dim3(256), 0, s, a);
     if (fh_status st = launch_status("embedding_sum_kernel launch"); st != FH_OK || p.chunks == 1) return st;

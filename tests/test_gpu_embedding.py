@@ -148,6 +148,37 @@ def test_gradient_where_another_sort_takes_over(hip, tokens):
     assert np.array_equal(e.backward(dout).astype(np.float64), want)
 
 
+@pytest.mark.parametrize("dim,shift", [(1, 0), (8, 0), (24, 1), (333, 0), (1200, 0), (2056, 0)])
+@pytest.mark.parametrize("tokens", [255, 256, 257, 511, 512, 513, 700, 1023, 1024, 1025])
+def test_gradient_of_few_tokens(hip, tokens, dim, shift):
+    """The first, the last and an id of most tokens; rows shorter and longer than what a workgroup writes, some of them not whole vectors."""
+    say(f"embedding gradient, {tokens} tokens of 600 x {dim}, {shift} elements behind 16 bytes")
+    vocab, rng = 600, np.random.default_rng(tokens)
+    ids = np.where(rng.random(tokens) < 0.6, 77, rng.integers(-1, vocab + 1, tokens)).astype(np.int32)
+    ids[0], ids[-1], ids[5] = vocab - 1, 0, vocab - 1
+    e = Embedding(hip, F32, tokens, vocab, dim, ids, shift=shift)
+    dout = rng.integers(-8, 9, (tokens, dim)).astype(np.float32)
+    base = rng.integers(-8, 9, (vocab, dim)).astype(np.float32)
+    want = np.zeros((vocab, dim))
+    named = (ids >= 0) & (ids < vocab)
+    np.add.at(want, ids[named], dout[named].astype(np.float64))
+    assert np.array_equal(e.backward(dout).astype(np.float64), want)
+    assert np.array_equal(e.backward(dout, base).astype(np.float64), want + base)
+    assert np.array_equal(e.backward(dout, base, True).astype(np.float64), want + base)
+
+
+@pytest.mark.parametrize("vocab", [8192, 8193])
+def test_gradient_where_the_writing_takes_longer_than_a_sort(hip, vocab):
+    say(f"embedding gradient, 40 tokens of {vocab} x 2,048 f32")
+    dim, rng = 2048, np.random.default_rng(3)
+    ids = rng.integers(0, vocab, 40).astype(np.int32)
+    ids[3], ids[7] = vocab - 1, ids[30]
+    dout = rng.integers(-8, 9, (40, dim)).astype(np.float32)
+    want = np.zeros((vocab, dim), np.float32)
+    np.add.at(want, ids, dout)
+    assert np.array_equal(Embedding(hip, F32, 40, vocab, dim, ids).backward(dout), want)
+
+
 @pytest.mark.parametrize("vocab", [1, 2, 510, 511, 512, 513, 262143, 262144])
 def test_gradient_of_any_number_of_digits(hip, vocab):
     """The ids outside the vocabulary sort behind all others: their key is the vocabulary's size, which may need one bit more."""
