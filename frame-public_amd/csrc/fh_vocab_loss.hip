@@ -420,16 +420,18 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(
   });
 }
 
+// A tile of dx: one split's share of a piece.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN>
-__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kRows, Lie::kColumns, false, UNEVEN>;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
+using DxProduct = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kRows, Lie::kColumns, false, UNEVEN>;
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN>
+__device__ __forceinline__ void dx_tile(const LossArgs& a, unsigned char* lds, uint32_t block, int split) {
+  using P = DxProduct<T, BM, BN, WAVES_M, WAVES_N, UNEVEN>;
   const int count = *a.count;
   int tm, tn;
-  if (!place(blockIdx.x, (count + BM - 1) / BM, (a.dim + BN - 1) / BN, tm, tn)) return;
+  if (!place(block, (count + BM - 1) / BM, (a.dim + BN - 1) / BN, tm, tn)) return;
   // this split's share of the piece's stages
   const int stages = (a.last - a.first + kDepth - 1) / kDepth, share = (stages + a.splits - 1) / a.splits;
-  const int k0 = static_cast<int>(blockIdx.y) * share, KT = min(share, stages - k0);
+  const int k0 = split * share, KT = min(share, stages - k0);
   const int m0 = tm * BM, n0 = tn * BN, from = a.first + k0 * kDepth, depth = a.last - from;
   typename P::Acc acc;
   P::run(lds, {a.g + k0 * kDepth, a.ldg, nullptr, count - 1, depth}, {a.w + from * a.ldw, a.ldw, nullptr, a.dim - 1, depth}, m0, n0, KT, acc);
@@ -439,7 +441,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const Lo
 #pragma unroll
     for (int i = 0; i < P::TM; ++i) {
       if (row0 + 16 * i >= count) continue;
-      f32x4_t* sum = reinterpret_cast<f32x4_t*>(a.dx_sum + (static_cast<int64_t>(blockIdx.y) * a.tokens + row0 + 16 * i) * a.dim + col0);
+      f32x4_t* sum = reinterpret_cast<f32x4_t*>(a.dx_sum + (static_cast<int64_t>(split) * a.tokens + row0 + 16 * i) * a.dim + col0);
 #pragma unroll
       for (int j = 0; j < P::TN; ++j) {
         if (col0 + 16 * j >= a.dim) continue;
@@ -453,6 +455,11 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const Lo
   P::store(lds, acc, [&](int row, int c, const u32x4_t& v) {
     if (m0 + row < count && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dx + a.rows[m0 + row] * a.ldx + n0 + c) = v;
   });
+}
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dx_kernel(const LossArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[DxProduct<T, BM, BN, WAVES_M, WAVES_N, UNEVEN>::kLds];
+  dx_tile<T, BM, BN, WAVES_M, WAVES_N, UNEVEN>(a, lds, blockIdx.x, static_cast<int>(blockIdx.y));
 }
 
 // dx from the splits' sums, in their order: 8 columns a thread.
@@ -474,13 +481,15 @@ __global__ __launch_bounds__(256) void loss_dx_join_kernel(const LossArgs a) {
               store2<T>(high[2] * f, high[3] * f)};
 }
 
+// A tile of dw.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kColumns, Lie::kColumns, false, false>;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
+using DwProduct = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kColumns, Lie::kColumns, false, false>;
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+__device__ __forceinline__ void dw_tile(const LossArgs& a, unsigned char* lds, uint32_t block) {
+  using P = DwProduct<T, BM, BN, WAVES_M, WAVES_N>;
   const int count = *a.count;
   int tm, tn;
-  if (!place(blockIdx.x, static_cast<int>((a.last - a.first + BM - 1) / BM), (a.dim + BN - 1) / BN, tm, tn)) return;
+  if (!place(block, static_cast<int>((a.last - a.first + BM - 1) / BM), (a.dim + BN - 1) / BN, tm, tn)) return;
   const int m0 = tm * BM, n0 = tn * BN;
   typename P::Acc acc;
   P::run(lds, {a.g, a.ldg, nullptr, static_cast<int>(a.ldg) - 1, 0}, {a.xc, a.dim, nullptr, a.dim - 1, 0}, m0, n0, (count + kDepth - 1) / kDepth, acc);
@@ -489,6 +498,22 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const Lo
     const int64_t to = a.first + m0 + row;
     if (to < a.last && n0 + c < a.dim) *reinterpret_cast<u32x4_t*>(a.dw + to * a.ldw + n0 + c) = v;
   });
+}
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_dw_kernel(const LossArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[DwProduct<T, BM, BN, WAVES_M, WAVES_N>::kLds];
+  dw_tile<T, BM, BN, WAVES_M, WAVES_N>(a, lds, blockIdx.x);
+}
+
+// Both in one launch, where either is small: `dx_tiles` workgroups for each of dx' splits, then dw's.
+template <typename T, bool UNEVEN>
+__global__ __launch_bounds__(256) void loss_products_kernel(const LossArgs a, uint32_t dx_tiles) {
+  using X = DxProduct<T, 64, 64, 2, 2, UNEVEN>;
+  using W = DwProduct<T, 64, 64, 2, 2>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[X::kLds > W::kLds ? X::kLds : W::kLds];
+  const uint32_t of_dx = dx_tiles * static_cast<uint32_t>(a.splits);
+  if (blockIdx.x < of_dx) dx_tile<T, 64, 64, 2, 2, UNEVEN>(a, lds, blockIdx.x % dx_tiles, static_cast<int>(blockIdx.x / dx_tiles));
+  else dw_tile<T, 64, 64, 2, 2>(a, lds, blockIdx.x - of_dx);
 }
 
 // ---- host ----
@@ -571,6 +596,11 @@ DxPlan dx_plan(int64_t tokens, int64_t dim, int64_t columns) {
     }
   return best;
 }
+
+// Where dx takes the smallest tiles and dw has few of them, 8 per CU, one launch does both in those tiles (both gradients, us, two launches
+// before: 16 rows of 5,000 x 512 23.6 and 19.4, 333 of 5,003 x 1,000 43 and 40, 1,000 of 5,000 x 512 50.6 and 45.5, at the limit 512 of
+// 8,192 x 1,024 59.6 and 59.3). Behind it dw's larger tiles gain.
+constexpr int64_t kTogether = 8;
 
 struct Room {
   int64_t bytes = 0;
@@ -798,6 +828,10 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
       hipLaunchKernelGGL((loss_gather_kernel<false>), gather, dim3(256), 0, s, a);
     if (fh_status st = launch_status("loss_gather_kernel launch"); st != FH_OK) return st;
   }
+  auto together = [&](const LossArgs& p) {
+    return dx && dw && plan.dx.tile.m == 64 && plan.dx.tile.n == 64 &&
+           up(p.last - p.first, 64) / 64 * (up(g->dim, 64) / 64) <= kTogether * device_cu_count();
+  };
   return by_type(g->dtype, [&]<typename T>() {
     for (int64_t first = 0; first < g->vocab; first += columns) {
       a.first = static_cast<int>(first);
@@ -813,6 +847,16 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
             hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN, false>), grid, dim3(WM * WN * 64), 0, s, a);
         });
         if (fh_status st = launch_status("loss_derivative_kernel launch"); st != FH_OK) return st;
+        if (together(a)) {
+          const uint32_t dx_tiles = static_cast<uint32_t>(up(g->tokens, 64) / 64 * (up(g->dim, 64) / 64));
+          const dim3 grid(dx_tiles * static_cast<uint32_t>(a.splits) + static_cast<uint32_t>(up(a.last - a.first, 64) / 64 * (up(g->dim, 64) / 64)));
+          if ((a.last - a.first) % kDepth != 0)
+            hipLaunchKernelGGL((loss_products_kernel<T, true>), grid, dim3(256), 0, s, a, dx_tiles);
+          else
+            hipLaunchKernelGGL((loss_products_kernel<T, false>), grid, dim3(256), 0, s, a, dx_tiles);
+          if (fh_status st = launch_status("loss_products_kernel launch"); st != FH_OK) return st;
+          continue;
+        }
         if (dx)
           by_tile(plan.dx.tile, g->tokens, g->dim, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
             grid.y = static_cast<uint32_t>(a.splits);
