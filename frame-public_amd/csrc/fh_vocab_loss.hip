@@ -320,7 +320,8 @@ __global__ __launch_bounds__(THREADS) void loss_join_kernel(const LossArgs a) {
   }
 }
 
-// The loss, by one workgroup: the rows' losses in one order, in double.
+// The loss, by one workgroup: the rows' losses in one order, in double. (By the join's workgroup that is through last: 1,000 rows of 5,000 x 512
+// 39 us in all, 22 with this launch: every workgroup has to write its caches back.)
 __global__ __launch_bounds__(1024) void loss_sum_kernel(const LossArgs a) {
   __shared__ double shares[1024];
   const int tid = threadIdx.x, count = *a.count;
@@ -341,19 +342,8 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const LossArgs a) {
 // without a target are zeros. FEW: up to kGatherFew rows, which the workgroups list themselves (1,024 rows of 5,000 x 512: 51 us in all,
 // 57 for one row more and a launch for the list).
 constexpr int kGatherFew = 1024;
-template <bool FEW>
-__global__ __launch_bounds__(256) void loss_gather_kernel(const LossArgs a) {
-  __shared__ FewRows<FEW ? kGatherFew : 1> few;
-  const int lane = threadIdx.x & 63, t = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  int count;
-  const int32_t* rows = a.rows;
-  if constexpr (FEW) {
-    count = list_few_rows<256>(a, few, blockIdx.x == 0);
-    rows = few.rows;
-  } else {
-    count = *a.count;
-  }
-  const int end = (count + 63) / 64 * 64;
+__device__ __forceinline__ void gather_row(const LossArgs& a, const int32_t* rows, int count, int t) {
+  const int lane = threadIdx.x & 63, end = (count + 63) / 64 * 64;
   const u32x4_t zeros{0, 0, 0, 0};
   if (t < end) {
     const uint16_t* from = t < count ? a.x + rows[t] * a.ldx : nullptr;
@@ -362,6 +352,17 @@ __global__ __launch_bounds__(256) void loss_gather_kernel(const LossArgs a) {
   }
   if (a.dx != nullptr && t < a.tokens && !(a.targets[t] >= 0 && a.targets[t] < a.vocab))
     for (int c = lane * 8; c < a.dim; c += 512) *reinterpret_cast<u32x4_t*>(a.dx + t * a.ldx + c) = zeros;
+}
+template <bool FEW>
+__global__ __launch_bounds__(256) void loss_gather_kernel(const LossArgs a) {
+  __shared__ FewRows<FEW ? kGatherFew : 1> few;
+  const int t = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if constexpr (FEW) {
+    const int count = list_few_rows<256>(a, few, blockIdx.x == 0);
+    gather_row(a, few.rows, count, t);
+  } else {
+    gather_row(a, a.rows, *a.count, t);
+  }
 }
 
 __device__ __forceinline__ float loss_factor(const LossArgs& a) {
@@ -382,24 +383,36 @@ __device__ __forceinline__ void scale(typename P::Acc& acc, float f) {
 }
 
 // g of a piece: columns first .. last - 1 of the vocabulary, zeros behind them and in the tile's rows that no row with a target is.
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN>
-__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(const LossArgs a) {
-  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kRows, Lie::kRows, UNEVEN, UNEVEN>;
+// FEW: up to kDerivativeFew rows, which the workgroups list themselves and read where they are; the first `gathers` workgroups do what
+// loss_gather_kernel does.
+// A launch less: both gradients of 16 rows of 5,000 x 512 19.4 us before, 16.7 now, of 333 of 5,003 x 1,000 40 and 37, of 512 of 2,048 x 2,048
+// 39 and 34. (512 rows: three workgroups' tiles and lists still fit a CU.)
+constexpr int kDerivativeFew = 512;
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN, bool FEW>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(const LossArgs a, uint32_t gathers) {
+  using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, FEW ? Lie::kListed : Lie::kRows, Lie::kRows, UNEVEN, UNEVEN>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
-  const int count = *a.count;
+  __shared__ FewRows<FEW ? kDerivativeFew : 1> few;
+  int count;
+  if constexpr (FEW) {
+    count = list_few_rows<P::kThreads>(a, few, blockIdx.x == 0);
+    if (blockIdx.x < gathers) return gather_row(a, few.rows, count, static_cast<int>(blockIdx.x) * (P::kThreads / 64) + (threadIdx.x >> 6));
+  } else {
+    count = *a.count;
+  }
   int tm, tn;
-  if (!place(blockIdx.x, (count + BM - 1) / BM, static_cast<int>(a.ldg / BN), tm, tn)) return;
+  if (!place(blockIdx.x - gathers, (count + BM - 1) / BM, static_cast<int>(a.ldg / BN), tm, tn)) return;
   const int m0 = tm * BM, n0 = tn * BN;
   typename P::Acc acc;
-  P::run(lds, {a.xc, a.dim, nullptr, count - 1, a.dim}, {a.w + a.first * a.ldw, a.ldw, nullptr, a.vocab - 1 - a.first, a.dim}, m0, n0,
-         (a.dim + kDepth - 1) / kDepth, acc);
+  P::run(lds, {FEW ? a.x : a.xc, FEW ? a.ldx : a.dim, FEW ? few.rows : nullptr, count - 1, a.dim},
+         {a.w + a.first * a.ldw, a.ldw, nullptr, a.vocab - 1 - a.first, a.dim}, m0, n0, (a.dim + kDepth - 1) / kDepth, acc);
   const int row0 = m0 + P::wave_row() + (P::lane() & 15), column = a.first + n0 + P::wave_column();
   int target[P::TM];
 #pragma unroll
   for (int i = 0; i < P::TM; ++i) {
     const int m = min(row0 + 16 * i, count - 1);
-    const float lse = a.lse_c[m];
-    target[i] = a.targets_c[m];
+    const float lse = FEW ? a.lse[few.rows[m]] : a.lse_c[m];
+    target[i] = FEW ? few.targets[m] : a.targets_c[m];
 #pragma unroll
     for (int j = 0; j < P::TN; ++j)
 #pragma unroll
@@ -817,15 +830,16 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
   a.g = reinterpret_cast<uint16_t*>(ws + room.g);
   a.splits = plan.dx.splits;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 gather(static_cast<uint32_t>(up(g->tokens, 64) / 4));
+  const uint32_t gathers = static_cast<uint32_t>(up(g->tokens, 64) / 4);  // of four rows
   const bool few = g->tokens > 0 && g->tokens <= kGatherFew;
+  const bool fewer = few && g->tokens <= kDerivativeFew && tile_for(g->tokens, std::min(up(g->vocab, kLeastPiece), columns)).m == 64;
   if (!few)
     if (fh_status st = list_rows(a, s); st != FH_OK) return st;
-  if (g->tokens > 0) {
+  if (g->tokens > 0 && !fewer) {
     if (few)
-      hipLaunchKernelGGL((loss_gather_kernel<true>), gather, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((loss_gather_kernel<true>), dim3(gathers), dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((loss_gather_kernel<false>), gather, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((loss_gather_kernel<false>), dim3(gathers), dim3(256), 0, s, a);
     if (fh_status st = launch_status("loss_gather_kernel launch"); st != FH_OK) return st;
   }
   auto together = [&](const LossArgs& p) {
@@ -841,10 +855,15 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
       a.ldg = up(a.last - a.first, kLeastPiece);
       if (g->tokens > 0) {
         by_tile(tile_for(g->tokens, a.ldg), g->tokens, a.ldg, [&]<int BM, int BN, int WM, int WN>(dim3 grid) {
-          if (g->dim % kDepth != 0)
-            hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN, true>), grid, dim3(WM * WN * 64), 0, s, a);
-          else
-            hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN, false>), grid, dim3(WM * WN * 64), 0, s, a);
+          auto go = [&]<bool UNEVEN, bool FEW>() {
+            if (FEW) grid.x += gathers;
+            hipLaunchKernelGGL((loss_derivative_kernel<T, BM, BN, WM, WN, UNEVEN, FEW>), grid, dim3(WM * WN * 64), 0, s, a, FEW ? gathers : 0);
+          };
+          const bool uneven = g->dim % kDepth != 0;
+          if constexpr (BM == 64) {
+            if (fewer && first == 0) return uneven ? go.template operator()<true, true>() : go.template operator()<false, true>();
+          }
+          uneven ? go.template operator()<true, false>() : go.template operator()<false, false>();
         });
         if (fh_status st = launch_status("loss_derivative_kernel launch"); st != FH_OK) return st;
         if (together(a)) {

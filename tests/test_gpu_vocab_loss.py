@@ -136,6 +136,15 @@ def test_pieces_of_the_vocabulary(hip, columns):
     Loss(hip, BF16, 300, 2003, 136, 0.2).check(1.0, columns)
 
 
+@pytest.mark.parametrize("columns", [None, 256])
+@pytest.mark.parametrize("shape", [(511, 900, 72, 0.4, 1, 8), (512, 900, 64, 0.4, 0, 0), (513, 900, 72, 0.4, 1, 0), (20, 8192, 1024, 0.2, 1, 0),
+                                   (20, 8193, 1024, 0.2, 1, 0), (512, 700, 64, 2.0, 1, 0)], ids=str)
+def test_where_fewer_launches_take_over(hip, shape, columns):
+    say(f"rows listed beside the derivatives, both gradients in one launch: {shape}, pieces of {columns} columns")
+    tokens, vocab, dim, outside, mean, pad = shape
+    Loss(hip, BF16, tokens, vocab, dim, outside, mean, pad).check(1.5, columns)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_loss_in_the_tensors_type(hip, dtype):
     say(f"loss and its gradient as one value of dtype {dtype}")
