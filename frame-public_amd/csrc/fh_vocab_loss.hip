@@ -16,6 +16,7 @@
 //   3,686 rows of the same:         gradients 9.33 to 10.2 ms, 1,160 to 1,270 TFLOP/s over three products; per piece of 16,384 columns
 //                                   derivatives 422 us, dx 422, dw 411 (busy for 71, 71 and 67 % of the cycles).
 //   4,096 rows of 32,768 x 1,024:   231 to 259 us and 730 to 805. Short products: 4 us of a tile's 31 are its beginning and end.
+//   333 rows of 5,003 x 1,000, f16: gradients 35 us: three dependent launches (derivatives 14, products 20, dx' join 5).
 //   1 row of 131,072 x 4,096:       182 us, 5.9 TB/s: the bytes of w (64 x 128 tiles, two stages ahead).
 #include <hip/hip_runtime.h>
 
@@ -206,8 +207,9 @@ __device__ __forceinline__ int list_few_rows(const LossArgs& a, FewRows<MOST>& f
 
 // ---- forward ----
 
-// FEW: up to kFewRows rows, which the workgroups list themselves (16 rows of 5,000 x 512: 10 us in all, 14 with a launch for the list).
-constexpr int kFewRows = 64;
+// FEW: up to kFewRows rows, which the workgroups list themselves (us, with a launch for the list before: 16 rows of 5,000 x 512 14 and 10, 333 of
+// 50,261 x 1,000 42 and 40, 500 of 32,768 x 256 23.4 and 21.2; the same from 80 us on). Three of the smallest tiles and their lists still fit a CU.
+constexpr int kFewRows = 512;
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN, bool FEW>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(const LossArgs a) {
   using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, Lie::kListed, Lie::kRows, UNEVEN, UNEVEN>;
@@ -383,16 +385,15 @@ __device__ __forceinline__ void scale(typename P::Acc& acc, float f) {
 }
 
 // g of a piece: columns first .. last - 1 of the vocabulary, zeros behind them and in the tile's rows that no row with a target is.
-// FEW: up to kDerivativeFew rows, which the workgroups list themselves and read where they are; the first `gathers` workgroups do what
+// FEW: up to kFewRows rows, which the workgroups list themselves and read where they are; the first `gathers` workgroups do what
 // loss_gather_kernel does.
-// A launch less: both gradients of 16 rows of 5,000 x 512 19.4 us before, 16.7 now, of 333 of 5,003 x 1,000 40 and 37, of 512 of 2,048 x 2,048
-// 39 and 34. (512 rows: three workgroups' tiles and lists still fit a CU.)
-constexpr int kDerivativeFew = 512;
+// A launch less: both gradients of 16 rows of 5,000 x 512 19.4 us before, 16.7 now, of 333 of 5,003 x 1,000 40 and 35, of 512 of 2,048 x 2,048
+// 39 and 34.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool UNEVEN, bool FEW>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_derivative_kernel(const LossArgs a, uint32_t gathers) {
   using P = Product<T, BM, BN, WAVES_M, WAVES_N, kRing<BM>, FEW ? Lie::kListed : Lie::kRows, Lie::kRows, UNEVEN, UNEVEN>;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[P::kLds];
-  __shared__ FewRows<FEW ? kDerivativeFew : 1> few;
+  __shared__ FewRows<FEW ? kFewRows : 1> few;
   int count;
   if constexpr (FEW) {
     count = list_few_rows<P::kThreads>(a, few, blockIdx.x == 0);
@@ -755,7 +756,7 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
   a.targets_c = reinterpret_cast<int32_t*>(ws + room.targets);
   a.tiles_n = static_cast<int>(room.tiles_n);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool few = g->tokens > 0 && g->tokens <= kFewRows;  // (then tiles have 64 rows)
+  const bool few = g->tokens > 0 && g->tokens <= kFewRows;
   if (!few)
     if (fh_status st = list_rows(a, s); st != FH_OK) return st;
   if (g->tokens > 0) {
@@ -765,9 +766,7 @@ extern "C" fh_status fh_vocab_loss_fwd(const fh_vocab_loss* g, const void* x, co
           hipLaunchKernelGGL((loss_logits_kernel<T, BM, BN, WM, WN, UNEVEN, FEW>), grid, dim3(WM * WN * 64), 0, s, a);
         };
         const bool uneven = g->dim % kDepth != 0;
-        if constexpr (BM == 64) {
-          if (few) return uneven ? go.template operator()<true, true>() : go.template operator()<false, true>();
-        }
+        if (few) return uneven ? go.template operator()<true, true>() : go.template operator()<false, true>();
         uneven ? go.template operator()<true, false>() : go.template operator()<false, false>();
       });
       return launch_status("loss_logits_kernel launch");
@@ -832,7 +831,7 @@ extern "C" fh_status fh_vocab_loss_grad(const fh_vocab_loss* g, const void* x, c
   hipStream_t s = static_cast<hipStream_t>(stream);
   const uint32_t gathers = static_cast<uint32_t>(up(g->tokens, 64) / 4);  // of four rows
   const bool few = g->tokens > 0 && g->tokens <= kGatherFew;
-  const bool fewer = few && g->tokens <= kDerivativeFew && tile_for(g->tokens, std::min(up(g->vocab, kLeastPiece), columns)).m == 64;
+  const bool fewer = few && g->tokens <= kFewRows && tile_for(g->tokens, std::min(up(g->vocab, kLeastPiece), columns)).m == 64;
   if (!few)
     if (fh_status st = list_rows(a, s); st != FH_OK) return st;
   if (g->tokens > 0 && !fewer) {

@@ -77,13 +77,13 @@ def test_loss_sizes_are_refused(over, code):
     assert lib.fh_vocab_loss_grad(r, *[P] * 8, 1 << 50, None) == code
 
 
-@pytest.mark.parametrize("make,over", [
-    (table, dict(tokens=2 ** 25 + 1)), (table, dict(tokens=2 ** 25, dim=2048, row_stride=2048)),
-    (loss, dict(tokens=2 ** 24, vocab=2 ** 18)), (loss, dict(vocab=2 ** 24, dim=2 ** 17, x_stride=2 ** 17, w_stride=2 ** 17)),
+@pytest.mark.parametrize("what,over", [
+    ("table", dict(tokens=2 ** 25 + 1)), ("table", dict(tokens=2 ** 25, dim=2048, row_stride=2048)),
+    ("loss", dict(tokens=2 ** 24, vocab=2 ** 18)), ("loss", dict(vocab=2 ** 24, dim=2 ** 17, x_stride=2 ** 17, w_stride=2 ** 17)),
 ], ids=str)
-def test_launches_of_2_to_the_32_threads_are_refused(make, over):
-    lib, r = abi.lib(), ctypes.byref(make(**over))
-    if make is table:
+def test_launches_of_2_to_the_32_threads_are_refused(what, over):
+    lib, r = abi.lib(), ctypes.byref(table(**over) if what == "table" else loss(**over))
+    if what == "table":
         assert lib.fh_embedding_fwd(r, P, P, P, None) == INVALID and lib.fh_embedding_grad_workspace(r) == -1
     else:
         assert lib.fh_vocab_loss_workspace(r) == -1 and lib.fh_vocab_loss_grad_workspace(r) == -1
