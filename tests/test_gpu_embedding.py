@@ -298,10 +298,11 @@ def test_table_of_more_elements_than_a_launch_writes(hip):
         ref.check(ref.values(elements(v * dim, dim), BF16), want, ref.rounded(want, 0.0, BF16), f"row {v}")
 
 
-def test_captured_and_replayed(hip):
+@pytest.mark.parametrize("tokens", [700, 3000, 20000])
+def test_captured_and_replayed(hip, tokens):
     say("embedding and its gradient captured, ids changed between the replays")
-    tokens, vocab, dim = 700, 90, 136
-    lib, e = hip.lib(), Embedding(hip, BF16, 700, 90, 136, text_ids(700, 90, 8, 0.1))
+    vocab, dim = 90, 136
+    lib, e = hip.lib(), Embedding(hip, BF16, tokens, vocab, dim, text_ids(tokens, vocab, 8, 0.1))
     table, dout = synth.tensor(21, (vocab, dim), BF16, "normal"), synth.tensor(22, (tokens, dim), BF16, "normal")
     g = e.geom()
     need = lib.fh_embedding_grad_workspace(ctypes.byref(g))

@@ -268,15 +268,16 @@ def test_deterministic(hip):
         assert np.array_equal(a, b)
 
 
-def test_captured_and_replayed(hip):
+@pytest.mark.parametrize("n", [300, 1100])
+def test_captured_and_replayed(hip, n):
     say("loss and gradients captured, targets changed between the replays")
-    p = Loss(hip, BF16, 300, 1300, 136, 0.2)
+    p = Loss(hip, BF16, n, 1300, 136, 0.2)
     p.x[~p.counted] = 0
     lib, g = hip.lib(), p.geom()
     r = ctypes.byref(g)
     need, need_grad = lib.fh_vocab_loss_workspace(r), lib.fh_vocab_loss_grad_workspace(r)
     x, w, t, d = p.up(p.x), p.up(p.w), hip.to_device(p.targets), p.scalar(1.0)
-    loss, lse, dx, dw = p.scalar(0.0), hip.DeviceBuffer(1200), p.up(p.x), p.up(p.w)
+    loss, lse, dx, dw = p.scalar(0.0), hip.DeviceBuffer(4 * n), p.up(p.x), p.up(p.w)
     ws, stream, graph = hip.DeviceBuffer(max(need, need_grad)), hip.Stream(), ctypes.c_void_p()
     hip.check(lib.fh_device_synchronize())
     hip.check(lib.fh_graph_begin_capture(stream.ptr))
@@ -285,16 +286,16 @@ def test_captured_and_replayed(hip):
     hip.check(lib.fh_graph_end_capture(stream.ptr, 1, ctypes.byref(graph)))
     rng = np.random.default_rng(9)
     for replay in range(4):
-        p.targets = np.where(rng.random(300) < 0.3 * replay, -1, rng.integers(0, 1300, 300)).astype(np.int32)
+        p.targets = np.where(rng.random(n) < 0.3 * replay, -1, rng.integers(0, 1300, n)).astype(np.int32)
         p.counted = p.targets >= 0
         t.upload(p.targets)
         hip.check(lib.fh_graph_launch(graph, stream.ptr))
         stream.synchronize()
         want = p.forward()
         assert loss.download((1,), np.float32)[0] == np.float32(want[0]), replay
-        assert np.array_equal(lse.download((300,), np.float32), want[2]), replay
+        assert np.array_equal(lse.download((n,), np.float32), want[2]), replay
         want = p.backward(want[2])
-        assert np.array_equal(p.down(dx, 300), want[0]) and np.array_equal(p.down(dw, 1300), want[1]), replay
+        assert np.array_equal(p.down(dx, n), want[0]) and np.array_equal(p.down(dw, 1300), want[1]), replay
     hip.check(lib.fh_graph_destroy(graph))
 
 
