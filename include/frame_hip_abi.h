@@ -422,7 +422,8 @@ fh_status fh_embedding_fwd(const fh_token_embedding* geom, const void* table, co
 
 /* dtable[v] = base[v] + scale * sum of dout[t] over the tokens with ids[t] = v, in fp32, rounded once; base NULL is zeros. base may be
  * dtable itself: then rows that no token names are left as they are. The table's other gradient (tied weights: fh_vocab_loss_grad's dw)
- * goes in that way. Nothing else may overlap. Deterministic: a sum's order depends on the ids and the sizes alone. */
+ * goes in that way. Nothing else may overlap. Deterministic: a sum's order depends on the ids, the sizes, on
+ * whether dtable and base are aligned to 16 bytes and on whether they are one, never on timing. */
 int64_t fh_embedding_grad_workspace(const fh_token_embedding* geom);
 fh_status fh_embedding_grad(const fh_token_embedding* geom, const void* dout, const int32_t* ids, const void* base, void* dtable,
                             void* workspace, int64_t workspace_bytes, void* stream);
