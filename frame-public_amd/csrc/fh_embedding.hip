@@ -10,7 +10,7 @@
 // Few tokens need no sort: an id's first token looks for the others and sums them, in one launch.
 //
 // Measured: forward, 8,192 tokens of 131,072 x 4,096 bf16: 21.8 us, 5.1 TB/s; 64 tokens of 1,024: 6.7 (the call). Gradient: 32,768 tokens of
-// 131,072 x 4,096 bf16: 283 us (sort and zeros 208, sums 58, join 16) for 1.3 GB that must move (256 at a copy's rate; named rows are
+// 131,072 x 4,096 bf16: 283 to 306 us (sort and zeros 208, sums 58, join 16) for 1.3 GB that must move (256 at a copy's rate; named rows are
 // written twice); 4,096 of 32,768 x 1,024 on a base 34 us (20, 8 and 5); 301 of 5,003 x 333 f32 7.3 us, about what any call takes.
 #include <hip/hip_runtime.h>
 
