@@ -1418,25 +1418,27 @@ Status lower_packed_attention(ir::Graph& g) {
 // their internal forms, at every opt level; the forward hands the last one the rows' log-sum-exps (one that the graph does not hold is
 // added for them). At opt_level >= 1 an add
 // of an embedding's gradient to another gradient of the same table (tied weights) goes into the former, which is then summed and
-// rounded once. Types that the kernels do not take stay as they are and are named when the step runs.
+// rounded once. Nodes of types that the kernels do not take, or of other ranks or attributes, stay as they are and are named when the step runs.
 Status lower_language_ends(ir::Graph& g, int32_t opt_level) {
-  auto sixteen = [](const ir::Value* v) {
-    const DTypeCode d = v->type().dtype.code();
-    return d == DTypeCode::kBFloat16 || d == DTypeCode::kFloat16;
+  // Backend::compile also takes graphs that no pass has verified: of a node, only what is read here is asked for.
+  auto matrix = [](const ir::Value* v) { return v->type().shape.rank() == 2; };
+  auto is_loss_like = [&](const ir::Node* n, const char* op, size_t inputs, size_t outputs) {
+    if (n->op() != op || n->inputs().size() != inputs || n->outputs().size() != outputs || n->attr<bool>("mean") == nullptr) return false;
+    const DTypeCode d = n->inputs()[0]->type().dtype.code();
+    return (d == DTypeCode::kBFloat16 || d == DTypeCode::kFloat16) && matrix(n->inputs()[0]) && matrix(n->inputs()[1]);
   };
-  auto is_loss = [&](const ir::Node* n) { return n->op() == "vocab_loss" && n->inputs().size() == 3 && sixteen(n->inputs()[0]); };
-  auto is_loss_grad = [&](const ir::Node* n) {
-    return n->op() == "vocab_loss_grad_internal" && n->inputs().size() == 5 && sixteen(n->inputs()[0]);
-  };
+  auto is_loss = [&](const ir::Node* n) { return is_loss_like(n, "vocab_loss", 3, 1); };
+  auto is_loss_grad = [&](const ir::Node* n) { return is_loss_like(n, "vocab_loss_grad_internal", 5, 2); };
   auto loss_of = [&](const ir::Node* n) -> const ir::Node* {
     const ir::Node* f = n->inputs()[3]->producer();
-    if (f == nullptr || f->op() != "vocab_loss" || f->attrs() != n->attrs()) return nullptr;
+    if (f == nullptr || !is_loss(f) || f->attrs() != n->attrs()) return nullptr;
     for (size_t i = 0; i < 3; ++i)
       if (f->inputs()[i] != n->inputs()[i]) return nullptr;
     return f;
   };
-  auto is_embedding_grad = [](const ir::Node* n) {
-    return n != nullptr && n->op() == "embedding_grad_internal" && n->inputs().size() == 2 && n->outputs().size() == 1;
+  auto is_embedding_grad = [&](const ir::Node* n) {
+    return n != nullptr && n->op() == "embedding_grad_internal" && n->inputs().size() == 2 && n->outputs().size() == 1 && matrix(n->inputs()[0]) &&
+           matrix(&n->outputs()[0]);
   };
   std::unordered_map<const ir::Value*, int> uses;
   bool any = false;
