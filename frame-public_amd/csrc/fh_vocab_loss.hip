@@ -60,7 +60,7 @@ struct LossArgs {
   int32_t* rows;     // which they are, in their order
   float* at_target;  // their target's logit
   int32_t* targets_c;  // and their targets
-  float2* part;        // [column tiles][tokens]: from2, sum of 2^(z log2 e - from2)
+  float2* part;        // [column tiles][tokens]: from, sum of exp(z - from)
   int tiles_n;
   // gradients: the rows with a target copied together, their log-sum-exps, a piece of g, fp32 sums of dx over the pieces
   uint16_t* xc;
@@ -84,14 +84,16 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 // A maximum that exponents can be taken against: of a row of -infinity, 0.
 __device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.0f : m; }
-// 2^(z log2 e - from2). Exponents are counted in twos from a `from2` that is kept as it is, so its own rounding changes nothing.
-__device__ __forceinline__ float exp_from(float z, float from2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, -from2)); }
-// {from2, sum of 2^(z log2 e - from2)} of two sets of logits. An empty sum (logits of -infinity) is 0 and its from2 says nothing.
+// exp(z - from). The difference is formed first: of logits near their maximum it is exact, however large they are, and a row's largest counts as
+// exactly 1. (z log2 e - from log2 e in one fused operation saves one of three per logit, and is off by the rounding of from log2 e: a
+// probability too large for the row's log-sum-exp at a few hundred, infinite or zero from logits of 2^32 on.)
+__device__ __forceinline__ float exp_from(float z, float from) { return __builtin_amdgcn_exp2f((z - from) * kLog2e); }
+// {from, sum of exp(z - from)} of two sets of logits. An empty sum (logits of -infinity) is 0 and its from says nothing.
 __device__ __forceinline__ float2 add_exponentials(const float2& a, const float2& b) {
   if (a.y == 0.0f) return b;
   if (b.y == 0.0f) return a;
-  const float from2 = fmaxf(a.x, b.x);
-  return float2{from2, a.y * __builtin_amdgcn_exp2f(a.x - from2) + b.y * __builtin_amdgcn_exp2f(b.x - from2)};
+  const float from = fmaxf(a.x, b.x);
+  return float2{from, a.y * exp_from(a.x, from) + b.y * exp_from(b.x, from)};
 }
 
 // Runs f(i, j, x) for the lane's place in acc that is column `target` of row i of the wave's part (columns from `column` on). Few tiles hold the target
@@ -251,14 +253,14 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(cons
     for (int j = 0; j < P::TN; ++j)
 #pragma unroll
       for (int x = 0; x < 4; ++x) top = fmaxf(top, acc[i][j][x]);
-    const float top2 = origin(row_max(top)) * kLog2e;
+    const float from = origin(row_max(top));
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < P::TN; ++j)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) sum += exp_from(acc[i][j][x], top2);
+      for (int x = 0; x < 4; ++x) sum += exp_from(acc[i][j][x], from);
     sum = row_sum(sum);
-    if (g == 0) joined[P::wave() % WAVES_N][row0 + 16 * i] = float2{top2, sum};
+    if (g == 0) joined[P::wave() % WAVES_N][row0 + 16 * i] = float2{from, sum};
   }
   __syncthreads();
   for (int row = threadIdx.x; row < BM; row += P::kThreads) {
@@ -304,7 +306,8 @@ __global__ __launch_bounds__(THREADS) void loss_join_kernel(const LossArgs a) {
   }
   float loss = 0.0f;
   if (share == 0 && live) {
-    const float lse = kLn2 * (sum.x + __builtin_amdgcn_logf(sum.y));
+    // not less than the row's largest logit: the sum is 1 at least
+    const float lse = sum.x + kLn2 * __builtin_amdgcn_logf(sum.y);
     const int t = a.rows[m];
     a.lse[t] = lse;
     loss = lse - a.at_target[m];
