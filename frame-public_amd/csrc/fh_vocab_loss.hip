@@ -307,10 +307,11 @@ __global__ __launch_bounds__(THREADS) void loss_join_kernel(const LossArgs a) {
   float loss = 0.0f;
   if (share == 0 && live) {
     // not less than the row's largest logit: the sum is 1 at least
-    const float lse = sum.x + kLn2 * __builtin_amdgcn_logf(sum.y);
+    const float above = kLn2 * __builtin_amdgcn_logf(sum.y);
     const int t = a.rows[m];
-    a.lse[t] = lse;
-    loss = lse - a.at_target[m];
+    a.lse[t] = sum.x + above;
+    // not lse - the target's logit: what lse lost to rounding can be more than a confident row's whole loss
+    loss = (sum.x - a.at_target[m]) + above;
     a.at_target[m] = loss;
     if (a.row_loss != nullptr) a.row_loss[t] = loss;
   }

@@ -82,3 +82,21 @@ def test_a_probability_is_at_most_one(hip, shape, shift):
     want = np.expm1(z[first, 0] - exact[first])
     # a probability's error is its exponent's, by the log-sum-exp's; two roundings follow
     ref.check(d, want, 1.02 * (2.0 ** -24 * np.abs(exact[first]) + 2.0 ** -16) + 2.1 * ref.U[p.dtype] * np.abs(want) + 2.0 ** -20, "derivative")
+
+
+@pytest.mark.parametrize("shape", [(5, 300), (90, 1000), (700, 1500), (2048, 9000)], ids=str)
+@pytest.mark.parametrize("shift", SHIFTS)
+def test_losses_of_confident_rows(hip, shape, shift):
+    """Losses of 1e-9 to 1e-3, as exact around logits of hundreds as around zero. Off by the sum's roundings, 64 of at most 2^-24 (32 in a lane, the
+    rest in joins) and the logarithm's 2^-22, and relative to themselves by their exponents' (products of up to 60 rounded three times)."""
+    say(f"losses of confident rows, shift {shift}, {shape}")
+    p, z, _ = confident(hip, F16 if shift == 30000.0 else BF16, *shape, shift)
+    loss, row, _ = p.forward()
+    n, z, target = p.counted.sum(), z[p.counted], p.targets[p.counted]
+    d = z - z[np.arange(n), target][:, None]
+    d[np.arange(n), target] = -np.inf
+    want = np.log1p(np.exp(d).sum(1))
+    tol = 68 * 2.0 ** -24 + 2.0 ** -18 * want
+    assert (row >= 0).all() and np.median(want) < 1e-5
+    ref.check(row[p.counted].astype(np.float64), want, tol, "row_loss")
+    assert abs(loss - want.mean()) <= tol.mean() + 2.0 ** -23 * want.mean()
