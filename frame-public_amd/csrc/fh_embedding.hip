@@ -3,15 +3,18 @@
 // Forward: out[t] = scale * table[ids[t]], a copy bound by memory: a wave per 4 KB of a row, 16 bytes per lane and access.
 //
 // Gradient: dtable[v] = base[v] + scale * sum_{t: ids[t] = v} dout[t]. The tokens are sorted by id (stable, so a sum's order is the
-// tokens'), and the sorted list is cut into chunks of 8 or 16 tokens whatever the ids are, so that frequent and rare ids are the same
-// work: a wave sums the rows of a chunk id by id, ids that lie within a chunk are finished there, the rest leave fp32 parts that a
-// join adds in their order. No atomics on floats: every sum has one order. Rows that no token names are zeros or base's: all rows are
+// tokens'), and the sorted list is cut into chunks of 8 or 16 tokens whatever the ids are, so that the sums of frequent and rare ids are the
+// same work: a wave sums the rows of a chunk id by id, ids that lie within a chunk are finished there, the rest leave fp32 parts that a
+// join adds in their order, an id's by one workgroup per 64 vectors of columns (16 bytes each): the join's time grows with the most frequent id. No
+// atomics on floats: every sum has one order. Rows that no token names are zeros or base's: all rows are
 // written so beside the sort, in the launches that a few workgroups of it would leave the chip idle in, and the sums overwrite theirs.
 // Few tokens need no sort: an id's first token looks for the others and sums them, in one launch.
 //
 // Measured: forward, 8,192 tokens of 131,072 x 4,096 bf16: 21.8 us, 5.1 TB/s; 64 tokens of 1,024: 6.7 (the call). Gradient: 32,768 tokens of
-// 131,072 x 4,096 bf16: 283 to 306 us (sort and zeros 208, sums 58, join 16) for 1.3 GB that must move (256 at a copy's rate; named rows are
-// written twice); 4,096 of 32,768 x 1,024 on a base 34 us (20, 8 and 5); 301 of 5,003 x 333 f32 7.3 us, about what any call takes.
+// 131,072 x 4,096 bf16: 283 to 306 us (sort and zeros 207, sums 57, join 16) for 0.24 GB that must be read and 1.07 written (194 at 6.3 and 6.9
+// TB/s, the rates of reads and writes alone; named rows are written twice); 4,096 of 32,768 x 1,024 on a base 34 us (20, 8 and 6); 301 of 5,003 x
+// 333 f32 7 us, about what any call takes. Tokens of a table of 32,768 x 1,024 bf16 in place, as frequent as words, half of them one id, all of them:
+// 4,096 24, 41 and 56 us; 32,768 72, 135 and 201; 131,072 185, 431 and 699.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
