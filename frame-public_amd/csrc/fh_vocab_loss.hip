@@ -1,8 +1,9 @@
 // Softmax cross entropy over a vocabulary without keeping the logits (fh_vocab_loss_fwd) and its gradients (fh_vocab_loss_grad).
 //
 // With z = x w^T, lse = log sum_v exp z and one target per row:
-//   forward:   row_loss = lse - z[target]; a tile of logits leaves per row its maximum and the sum of its exponentials, which a second
-//              kernel joins over the tiles of the vocabulary, in their order.
+//   forward:   a tile of logits leaves per row the maximum and the sum of exponentials of all but the target's, which a second kernel joins over
+//              the tiles of the vocabulary, in their order; with o = log of that sum, row_loss = log(1 + exp(o - z[target])): however small a
+//              confident row's loss is, it keeps its bits, which lse - z[target] loses, and 1 + a small sum as well.
 //   gradients: with g = exp(z - lse) - [v = target], dx = f g w and dw = f g^T x, f = dloss (/ count for the mean): a piece of
 //              the vocabulary at a time, whose logits are formed again, whose g is kept in the storage type (f16: times 2^14, so that
 //              probabilities down to 2^-28 keep their bits) and read by both products. f is left to the products' results.
@@ -247,7 +248,10 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void loss_logits_kernel(cons
   int target[P::TM];
 #pragma unroll
   for (int i = 0; i < P::TM; ++i) target[i] = m0 + row0 + 16 * i < count ? targets[m0 + row0 + 16 * i] : -1;
-  at_targets<P>(target, column, [&](int i, int j, int x) { a.at_target[m0 + row0 + 16 * i] = acc[i][j][x]; });
+  at_targets<P>(target, column, [&](int i, int j, int x) {
+    a.at_target[m0 + row0 + 16 * i] = acc[i][j][x];
+    acc[i][j][x] = -INFINITY;  // the sums are the other tokens'
+  });
 #pragma unroll
   for (int i = 0; i < P::TM; ++i) {
     float top = -INFINITY;
@@ -308,12 +312,15 @@ __global__ __launch_bounds__(THREADS) void loss_join_kernel(const LossArgs a) {
   }
   float loss = 0.0f;
   if (share == 0 && live) {
-    // not less than the row's largest logit: the sum is 1 at least
-    const float above = kLn2 * __builtin_amdgcn_logf(sum.y);
+    // d: the others' log-sum-exp less the target's logit (a logit of +infinity has no distance). Neither result is below what it is added to, so
+    // lse is not less than any logit: the others' sum, with their largest, is 1 at least.
+    const float z = a.at_target[m], above = kLn2 * __builtin_amdgcn_logf(sum.y);
+    const float d = z == INFINITY ? NAN : (sum.x - z) + above;
+    const float more = log1pf(expf(-fabsf(d)));
+    const bool none = sum.y == 0.0f && z == -INFINITY;  // no token has a probability
     const int t = a.rows[m];
-    a.lse[t] = sum.x + above;
-    // not lse - the target's logit: what lse lost to rounding can be more than a confident row's whole loss
-    loss = (sum.x - a.at_target[m]) + above;
+    a.lse[t] = none ? -INFINITY : (d > 0.0f ? sum.x + above : z) + more;
+    loss = fmaxf(d, 0.0f) + more;
     a.at_target[m] = loss;
     if (a.row_loss != nullptr) a.row_loss[t] = loss;
   }

@@ -441,7 +441,8 @@ typedef struct fh_vocab_loss {
 } fh_vocab_loss;
 
 /* lse[t] = log sum_v exp(x[t] . w[v]), row_loss[t] = lse[t] - x[t] . w[target[t]] (both fp32, 0 for rows without a target; row_loss
- * may be NULL; it is formed before lse is rounded, and is not negative), and the loss. The gradients read lse: its rounding, |lse| 2^-24, is the least that their probabilities are off by, relative
+ * may be NULL; it is formed from the other tokens' sum, before lse is rounded: not negative, and small ones keep
+ * their bits), and the loss. The gradients read lse: its rounding, |lse| 2^-24, is the least that their probabilities are off by, relative
  * to themselves; lse is not less than its row's largest logit, so none is above 1. */
 int64_t fh_vocab_loss_workspace(const fh_vocab_loss* geom);
 fh_status fh_vocab_loss_fwd(const fh_vocab_loss* geom, const void* x, const void* w, const int32_t* targets, void* loss, float* row_loss,

@@ -100,3 +100,38 @@ def test_losses_of_confident_rows(hip, shape, shift):
     assert (row >= 0).all() and np.median(want) < 1e-5
     ref.check(row[p.counted].astype(np.float64), want, tol, "row_loss")
     assert abs(loss - want.mean()) <= tol.mean() + 2.0 ** -23 * want.mean()
+
+
+@pytest.mark.parametrize("shape", [(5, 300), (90, 1000), (700, 1500), (2048, 9000)], ids=str)
+@pytest.mark.parametrize("shift", SHIFTS)
+def test_losses_of_confident_rows_keep_their_bits(hip, shape, shift):
+    """The same to a part of themselves: the other tokens' exponents (up to 30, three roundings), their sum's logarithm (up to 13) and its
+    distance from the target's logit (up to 33) are off by less than 2^-16 in all, 256 roundings of one."""
+    say(f"losses of confident rows to their last bits, shift {shift}, {shape}")
+    p, z, _ = confident(hip, F16 if shift == 30000.0 else BF16, *shape, shift)
+    loss, row, _ = p.forward()
+    n, z, target = p.counted.sum(), z[p.counted], p.targets[p.counted]
+    d = z - z[np.arange(n), target][:, None]
+    d[np.arange(n), target] = -np.inf
+    want = np.log1p(np.exp(d).sum(1))
+    ref.check(row[p.counted].astype(np.float64), want, 2.0 ** -16 * want, "row_loss")
+    assert abs(loss - want.mean()) <= (2.0 ** -16 + 2.0 ** -23) * want.mean()
+
+
+def test_a_target_of_infinite_logit(hip):
+    """+infinity makes its row NaN whoever's it is; a target of -infinity has an infinite loss; the only token has a loss of 0."""
+    say("the target's logit is infinite; a vocabulary of one")
+    p = Loss(hip, BF16, 20, 300, 64)
+    p.x[:, 0], p.w[:, 0] = 0, 0
+    lse0 = p.forward()[2]
+    p.x[:, 0] = 0x3f80  # 1.0
+    p.targets[:] = np.where(np.arange(20) < 10, 7, 8)
+    p.w[7, 0] = 0xff80  # -infinity
+    _, row, lse = p.forward()
+    assert (row[:10] == np.inf).all() and np.isfinite(row[10:]).all() and np.isfinite(lse).all() and (lse <= lse0).all()
+    p.w[7, 0] = 0x7f80  # +infinity
+    _, row, lse = p.forward()
+    assert np.isnan(row).all() and np.isnan(lse).all()
+    q = Loss(hip, BF16, 20, 1, 64)
+    _, row, lse = q.forward()
+    assert (row == 0).all() and np.isfinite(lse).all()
