@@ -63,7 +63,7 @@ struct LossArgs {
   int32_t* rows;     // which they are, in their order
   float* at_target;  // their target's logit
   int32_t* targets_c;  // and their targets
-  float2* part;        // [column tiles][tokens]: from, sum of exp(z - from)
+  float2* part;        // [column tiles][tokens]: from, sum of exp(z - from) over all but the target
   int tiles_n;
   // gradients: the rows with a target copied together, their log-sum-exps, a piece of g, fp32 sums of dx over the pieces
   uint16_t* xc;
