@@ -12,11 +12,11 @@
 // for all rows, and workgroups without work end at once.
 //
 // Measured (bf16; two cards, which differ by 6 % under this load):
-//   7,373 rows of 131,072 x 4,096:  loss 5.84 to 6.15 ms, 1,290 to 1,360 TFLOP/s (a plain product of these sizes by the vendor's library
+//   7,373 rows of 131,072 x 4,096:  loss 5.75 to 6.15 ms, 1,290 to 1,380 TFLOP/s (a plain product of these sizes by the vendor's library
 //                                   5.48 ms). The matrix unit is busy for 75 % of the cycles at 1.75 GHz of 2.4: the board's power.
 //   3,686 rows of the same:         gradients 9.33 to 10.2 ms, 1,160 to 1,270 TFLOP/s over three products; per piece of 16,384 columns
 //                                   derivatives 411 us, dx 409, dw 399 (busy for 71, 71 and 67 % of the cycles).
-//   4,096 rows of 32,768 x 1,024:   236 to 259 us and 730 to 805. Short products: 4 us of a tile's 31 are its beginning and end. Within the first
+//   4,096 rows of 32,768 x 1,024:   225 to 259 us and 730 to 805. Short products: 4 us of a tile's 31 are its beginning and end. Within the first
 //                                   10 ms of such calls one card took 246, then 302, then 243 us for the logits: its power regulation.
 //   333 rows of 5,003 x 1,000, f16: gradients 35 us: three dependent launches (traced, where none overlaps the next, 38: derivatives 13, products
 //                                   20, dx' join 5). A derivative tile waits 0.8 us for each of its 16 stages: few tiles are on a CU to hide it.
